@@ -8,6 +8,7 @@ through ``libcandle_moe_b200.so`` (include/candle_moe.h).  There is no CPU path:
 library is missing, every call raises.
 
 Extensions beyond the reference API: ``topk_softmax`` (allocating, optional renormalisation),
+``route_experts`` / ``route_experts_backward`` (general routing and its gradient),
 ``route_prep`` (the sort/align step on its own), ``fused_moe`` (status-checked, optional
 caller workspace), ``workspace_size``, ``device_error_bits``, ``set_gemm_path`` /
 ``last_gemm_path``.
@@ -61,6 +62,13 @@ def lib() -> ctypes.CDLL:
         L.moe_topk_softmax_v2.restype = ctypes.c_int
         L.moe_router_project_topk.argtypes = [P, P, I64, I32, I32, I32, I32, U32, P, P, P, P, P]
         L.moe_router_project_topk.restype = ctypes.c_int
+        F32 = ctypes.c_float
+        L.moe_route_experts.argtypes = [P, U32, I64, P, I64, I32, I32, I32, I32, I32, I32, I32, F32,
+                                        P, P, P]
+        L.moe_route_experts.restype = ctypes.c_int
+        L.moe_route_experts_backward.argtypes = [P, P, U32, I64, P, P, I64, I32, I32, I32, I32, F32,
+                                                 P, P]
+        L.moe_route_experts_backward.restype = ctypes.c_int
         L.moe_route_prep.argtypes = [P, P, I64, I32, I32, P, P, P, P]
         L.moe_route_prep.restype = ctypes.c_int
         L.moe_fused_workspace_size.argtypes = [I64, I32, I32, I32, I32, U32, U32]
@@ -253,6 +261,109 @@ def router_project_topk(hidden: torch.Tensor, gate_proj: torch.Tensor, top_k: in
     if st != MOE_OK:
         raise MoeError(st, "moe_router_project_topk")
     return (w, idx, src, logits) if return_logits else (w, idx, src)
+
+
+class Scoring(enum.IntEnum):
+    """Score of an expert in route_experts."""
+    Softmax = 0
+    Sigmoid = 1
+
+
+class GroupScore(enum.IntEnum):
+    """Worth of a group in route_experts: its largest key, or the sum of its two largest
+    score + bias."""
+    Max = 0
+    Top2 = 1
+
+
+def _need_rows(t: torch.Tensor, name: str):
+    # rows may lie apart (a slice of a wider projection), a row itself may not
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be rank 2, got {tuple(t.shape)}")
+    if t.numel() and ((t.shape[1] > 1 and t.stride(1) != 1) or
+                      (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
+        raise ValueError(f"{name} must have contiguous rows that do not overlap")
+
+
+def _need_same_device(dev: torch.device, *named):
+    for t, n in named:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{n} must be on {dev}, got {t.device}")
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def route_experts(logits: torch.Tensor, top_k: int, scoring: Scoring = Scoring.Softmax,
+                  bias: Optional[torch.Tensor] = None, num_groups: int = 1, topk_groups: int = 1,
+                  group_score: GroupScore = GroupScore.Max, renormalize: bool = False,
+                  scaling: float = 1.0):
+    """General routing: softmax or sigmoid scores, a balance bias [E] f32 added to them for the
+    picks only, the best topk_groups of num_groups groups, the top_k picks, weights optionally
+    divided by their sum and times `scaling` (see include/candle_moe.h for every detail).
+
+    logits [T,E] f32/f16/bf16, E <= 512; rows may be strided.  Returns (weights [T,k] f32, indices
+    [T,k] int32); a slot without an available expert (logit -inf or NaN) holds index E and
+    weight 0, which the expert calls skip."""
+    _need_cuda(logits, "logits")
+    _need_rows(logits, "logits")
+    T, E = logits.shape
+    dev = logits.device
+    if bias is not None:
+        _need_cuda(bias, "bias")
+        _need_contig(bias, "bias")
+        if bias.dtype != torch.float32 or tuple(bias.shape) != (E,):
+            raise ValueError(f"bias must be a float32 tensor of shape ({E},)")
+        _need_same_device(dev, (bias, "bias"))
+    w = torch.empty((T, max(top_k, 0)), dtype=torch.float32, device=dev)
+    idx = torch.empty((T, max(top_k, 0)), dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        st = lib().moe_route_experts(_ptr(logits), fused_moe_internal_dtype(logits.dtype),
+                                     _row_stride(logits), _ptr(bias), T, E, top_k, int(scoring),
+                                     num_groups, topk_groups, int(group_score), int(renormalize),
+                                     scaling, _ptr(w), _ptr(idx), _stream(dev))
+    if st != MOE_OK:
+        raise MoeError(st, "moe_route_experts")
+    return w, idx
+
+
+def route_experts_backward(grad_weights: torch.Tensor, logits: torch.Tensor,
+                           weights: torch.Tensor, indices: torch.Tensor,
+                           scoring: Scoring = Scoring.Softmax, renormalize: bool = False,
+                           scaling: float = 1.0) -> torch.Tensor:
+    """Gradient of route_experts' weights with respect to the logits: [T,E] in their dtype.
+    grad_weights [T,k] f32; logits, scoring, renormalize and scaling as given to route_experts,
+    weights and indices as it returned them.  The picks are constants; the bias has no
+    gradient."""
+    for t, n in ((grad_weights, "grad_weights"), (logits, "logits"), (weights, "weights"),
+                 (indices, "indices")):
+        _need_cuda(t, n)
+    _need_rows(logits, "logits")
+    T, E = logits.shape
+    dev = logits.device
+    if indices.dim() != 2 or indices.shape[0] != T:
+        raise ValueError(f"indices must be [{T}, k], got {tuple(indices.shape)}")
+    if indices.dtype not in _INDEX_DTYPES:
+        raise TypeError("indices must be int32 or uint32")
+    for t, n in ((grad_weights, "grad_weights"), (weights, "weights")):
+        if t.dtype != torch.float32:
+            raise TypeError(f"{n} must be float32")
+        if t.shape != indices.shape:
+            raise ValueError(f"{n} must be {tuple(indices.shape)}, got {tuple(t.shape)}")
+    for t, n in ((grad_weights, "grad_weights"), (weights, "weights"), (indices, "indices")):
+        _need_contig(t, n)
+    _need_same_device(dev, (grad_weights, "grad_weights"), (weights, "weights"),
+                      (indices, "indices"))
+    grad = torch.empty((T, E), dtype=logits.dtype, device=dev)
+    with torch.cuda.device(dev):
+        st = lib().moe_route_experts_backward(
+            _ptr(grad_weights), _ptr(logits), fused_moe_internal_dtype(logits.dtype),
+            _row_stride(logits), _ptr(weights), _ptr(indices), T, E, indices.shape[1],
+            int(scoring), int(renormalize), scaling, _ptr(grad), _stream(dev))
+    if st != MOE_OK:
+        raise MoeError(st, "moe_route_experts_backward")
+    return grad
 
 
 # ---------------------------------------------------------------------------------------------

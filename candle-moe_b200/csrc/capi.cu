@@ -14,6 +14,7 @@
 #include <climits>
 #include <cstdint>
 #include <cstring>
+#include <limits>
 #include <mutex>
 #include <vector>
 
@@ -655,6 +656,84 @@ CMOE_API int moe_router_project_topk(const void* input, const void* gate_proj,
   const int grid = static_cast<int>(tiles < sms ? tiles : sms);
   if (launch_router_project(static_cast<int>(dtype), num_experts, mx, mw, p, grid,
                             static_cast<cudaStream_t>(stream)) != 0)
+    return MOE_ERR_UNSUPPORTED;
+  ++g_launches;
+  return finish(MOE_OK);
+}
+
+CMOE_API int moe_route_experts(const void* logits, uint32_t dtype, int64_t logits_stride,
+                               const float* bias, int64_t num_tokens, int32_t num_experts,
+                               int32_t topk, int32_t scoring, int32_t num_groups,
+                               int32_t topk_groups, int32_t group_score, int32_t renormalize,
+                               float scaling, float* topk_weights, int32_t* topk_indices,
+                               void* stream) {
+  if (dtype > 2 || num_tokens < 0 || num_experts <= 0 || topk <= 0 || logits_stride < num_experts ||
+      scoring < 0 || scoring > 1 || group_score < 0 || group_score > 1 || num_groups <= 0 ||
+      num_experts % num_groups != 0 || topk_groups <= 0 || topk_groups > num_groups ||
+      topk > topk_groups * (num_experts / num_groups) || !(scaling > 0.f) ||
+      scaling > std::numeric_limits<float>::max())
+    return MOE_ERR_INVALID_ARG;
+  if (num_experts > kRouteMaxExperts || num_groups > kRouteMaxGroups || topk > kRouteMaxK)
+    return MOE_ERR_UNSUPPORTED;
+  if (num_tokens == 0) return MOE_OK;
+  if (!logits || !topk_weights || !topk_indices) return MOE_ERR_INVALID_ARG;
+  DeviceState* ds = nullptr;
+  int st = current_device_state(&ds);
+  if (st != MOE_OK) return st;
+  RouteExpertsParams p;
+  p.logits = logits;
+  p.bias = bias;
+  p.weights = topk_weights;
+  p.indices = topk_indices;
+  p.num_tokens = num_tokens;
+  p.stride = logits_stride;
+  p.E = num_experts;
+  p.k = topk;
+  p.scoring = scoring;
+  p.num_groups = num_groups;
+  p.topk_groups = topk_groups;
+  p.group_score = group_score;
+  p.renormalize = renormalize;
+  p.scaling = scaling;
+  if (launch_route_experts(static_cast<int>(dtype), p, ds->num_sms,
+                           static_cast<cudaStream_t>(stream)) != 0)
+    return MOE_ERR_UNSUPPORTED;
+  ++g_launches;
+  return finish(MOE_OK);
+}
+
+CMOE_API int moe_route_experts_backward(const float* grad_weights, const void* logits,
+                                        uint32_t dtype, int64_t logits_stride,
+                                        const float* topk_weights, const int32_t* topk_indices,
+                                        int64_t num_tokens, int32_t num_experts, int32_t topk,
+                                        int32_t scoring, int32_t renormalize, float scaling,
+                                        void* grad_logits, void* stream) {
+  if (dtype > 2 || num_tokens < 0 || num_experts <= 0 || topk <= 0 || topk > num_experts ||
+      logits_stride < num_experts || scoring < 0 || scoring > 1 || !(scaling > 0.f) ||
+      scaling > std::numeric_limits<float>::max())
+    return MOE_ERR_INVALID_ARG;
+  if (num_experts > kRouteMaxExperts || topk > kRouteMaxK) return MOE_ERR_UNSUPPORTED;
+  if (num_tokens == 0) return MOE_OK;
+  if (!grad_weights || !logits || !topk_weights || !topk_indices || !grad_logits)
+    return MOE_ERR_INVALID_ARG;
+  DeviceState* ds = nullptr;
+  int st = current_device_state(&ds);
+  if (st != MOE_OK) return st;
+  RouteExpertsBackwardParams p;
+  p.grad_weights = grad_weights;
+  p.logits = logits;
+  p.weights = topk_weights;
+  p.indices = topk_indices;
+  p.grad_logits = grad_logits;
+  p.num_tokens = num_tokens;
+  p.stride = logits_stride;
+  p.E = num_experts;
+  p.k = topk;
+  p.scoring = scoring;
+  p.renormalize = renormalize;
+  p.scaling = scaling;
+  if (launch_route_experts_backward(static_cast<int>(dtype), p, ds->num_sms,
+                                    static_cast<cudaStream_t>(stream)) != 0)
     return MOE_ERR_UNSUPPORTED;
   ++g_launches;
   return finish(MOE_OK);

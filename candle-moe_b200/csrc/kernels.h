@@ -30,6 +30,33 @@ bool router_project_set_attributes();
 int launch_router_project(int dtype, int E, const CUtensorMap& x, const CUtensorMap& w,
                           const RouterProjParams& p, int grid, cudaStream_t s);
 
+// ---- route_experts.cu (R2: general routing and its gradient) ---------------------------------
+constexpr int kRouteMaxExperts = 512;
+constexpr int kRouteMaxGroups = 32;
+constexpr int kRouteMaxK = 32;
+struct RouteExpertsParams {
+  const void* logits;   // rows of E values, `stride` elements apart
+  const float* bias;    // [E] or null
+  float* weights;       // [T, k]
+  int32_t* indices;     // [T, k]
+  int64_t num_tokens, stride;
+  int E, k, scoring, num_groups, topk_groups, group_score, renormalize;
+  float scaling;
+};
+struct RouteExpertsBackwardParams {
+  const float* grad_weights;  // [T, k]
+  const void* logits;         // rows of E values, `stride` elements apart
+  const float* weights;       // [T, k], the forward call's
+  const int32_t* indices;     // [T, k], the forward call's
+  void* grad_logits;          // [T, E]
+  int64_t num_tokens, stride;
+  int E, k, scoring, renormalize;
+  float scaling;
+};
+int launch_route_experts(int dtype, const RouteExpertsParams& p, int num_sms, cudaStream_t s);
+int launch_route_experts_backward(int dtype, const RouteExpertsBackwardParams& p, int num_sms,
+                                  cudaStream_t s);
+
 // ---- route_prep.cu ---------------------------------------------------------------------------
 size_t route_prep_scratch_bytes(int64_t rows, int E);
 int route_prep_max_experts();

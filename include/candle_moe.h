@@ -109,6 +109,54 @@ int moe_router_project_topk(const void* input, const void* gate_proj, int64_t nu
                             void* stream);
 
 /*
+ * General expert routing (no counterpart in the reference, whose router is topk_softmax): softmax
+ * or sigmoid scores, a balance bias that steers the picks only, groups of experts of which the
+ * best stay open, top-k picks and optionally renormalised weights.
+ *   logits        num_tokens rows of num_experts values of `dtype`, logits_stride elements apart
+ *                 (>= num_experts).  An expert whose logit is -inf or NaN is unavailable to that
+ *                 token: it stays out of the softmax and is never picked.  +inf is a valid logit
+ *                 for sigmoid scores only (softmax weights become NaN).
+ *   bias          [num_experts] f32 or NULL: picks are made by score + bias, weights by the score
+ *                 alone (NULL: picks by the logits, which order the scores).  A bias of -inf or
+ *                 NaN makes the expert unavailable.
+ *   scoring       MOE_SCORING_SOFTMAX or MOE_SCORING_SIGMOID
+ *   num_groups    consecutive groups of num_experts / num_groups experts (1: no groups), of which
+ *                 the topk_groups with the largest value stay open: the largest key of the group
+ *                 (MOE_GROUP_MAX) or the sum of its two largest score + bias (MOE_GROUP_TOP2)
+ *   topk_weights  [num_tokens, topk] f32 out: scaling * score, divided by the sum of the token's
+ *                 picked scores with renormalize (0 where that sum is 0)
+ *   topk_indices  [num_tokens, topk] i32 out, by descending key; every tie goes to the lower id,
+ *                 decided on scores in 64 bits.  A slot for which no available expert is left
+ *                 holds num_experts (which moe_fused_v2 and the other expert calls skip) and
+ *                 weight 0.
+ * Any num_experts <= 512, num_groups <= 32 (a divisor of num_experts), topk <= 32 and <= the open
+ * groups' experts; scaling positive and finite.
+ */
+#define MOE_SCORING_SOFTMAX 0
+#define MOE_SCORING_SIGMOID 1
+#define MOE_GROUP_MAX 0
+#define MOE_GROUP_TOP2 1
+int moe_route_experts(const void* logits, uint32_t dtype, int64_t logits_stride,
+                      const float* bias, int64_t num_tokens, int32_t num_experts, int32_t topk,
+                      int32_t scoring, int32_t num_groups, int32_t topk_groups,
+                      int32_t group_score, int32_t renormalize, float scaling,
+                      float* topk_weights, int32_t* topk_indices, void* stream);
+
+/*
+ * Gradient of moe_route_experts' weights with respect to the logits.  grad_weights [num_tokens,
+ * topk] f32; logits, topk_weights, topk_indices, scoring, renormalize and scaling as in (and from)
+ * the forward call; grad_logits [num_tokens, num_experts] of `dtype`, contiguous, written whole.
+ * The picks are constants and the bias has no gradient.  Slots with ids outside [0, num_experts)
+ * contribute nothing, an id that a token holds twice contributes both.  Deterministic.
+ */
+int moe_route_experts_backward(const float* grad_weights, const void* logits, uint32_t dtype,
+                               int64_t logits_stride, const float* topk_weights,
+                               const int32_t* topk_indices, int64_t num_tokens,
+                               int32_t num_experts, int32_t topk, int32_t scoring,
+                               int32_t renormalize, float scaling, void* grad_logits,
+                               void* stream);
+
+/*
  * Sort / align step on its own.  Replaces launch_preprocessing (kernels/preprocessing.cuh:253-313),
  * which the reference runs inside fused_moe without exporting it.
  *   expert_offsets    [num_experts + 2] i32 out: exclusive prefix of per-expert row counts,
