@@ -10,7 +10,8 @@ library is missing, every call raises.
 Extensions beyond the reference API: ``topk_softmax`` (allocating, optional renormalisation),
 ``route_experts`` / ``route_experts_backward`` (general routing and its gradient),
 ``route_prep`` (the sort/align step on its own), ``fused_moe`` (status-checked, optional
-caller workspace), ``workspace_size``, ``device_error_bits``, ``set_gemm_path`` /
+caller workspace), ``fused_moe_int4`` / ``Int4Experts`` / ``quantize_int4`` (experts in 4 bits),
+``workspace_size``, ``device_error_bits``, ``set_gemm_path`` /
 ``last_gemm_path``.
 """
 from __future__ import annotations
@@ -107,6 +108,17 @@ def lib() -> ctypes.CDLL:
         L.moe_phase_timing.restype = ctypes.c_int
         L.moe_phase_times.argtypes = [P, P]
         L.moe_phase_times.restype = ctypes.c_int
+        L.moe_int4_packed_size.argtypes = [I32, I32, I32, I32, U32, I32]
+        L.moe_int4_packed_size.restype = SZ
+        L.moe_int4_quantize.argtypes = [P, I32, I32, I32, I32, U32, P, P, P, P]
+        L.moe_int4_quantize.restype = ctypes.c_int
+        L.moe_int4_pack.argtypes = [P, P, P, I32, I32, I32, I32, U32, P, P]
+        L.moe_int4_pack.restype = ctypes.c_int
+        L.moe_fused_int4_workspace_size.argtypes = [I64, I32, I32, I32, I32]
+        L.moe_fused_int4_workspace_size.restype = SZ
+        L.moe_fused_int4.argtypes = [P, P, P, P, P, P, P, I64, I32, I32, I32, I32, I32, U32, I32,
+                                     I32, P, SZ, P]
+        L.moe_fused_int4.restype = ctypes.c_int
         U8P = ctypes.POINTER(ctypes.c_uint8)
         L.moe_peer_alloc.argtypes = [SZ, ctypes.POINTER(ctypes.c_void_p), U8P]
         L.moe_peer_alloc.restype = ctypes.c_int
@@ -641,6 +653,165 @@ def fused_moe_scatter(input, gate_weights, up_weights, down_weights, routing_wei
     return out
 
 
+class Int4Weights:
+    """A weight matrix [E,K,N] (K the reduction) in 4 bits: W[e,k,n] = (q - zero) * scale, one
+    scale (and zero point) per group of group_size consecutive k and column.
+
+    q [E,K/2,N] uint8 (low nibble: even k, high nibble: k + 1); scales [E,K/group_size,N] f16 or
+    bf16, the type of the activations; zeros like scales, uint8 in 0..15, or None (8
+    everywhere).  group_size 32, 64 or 128; K and N multiples of 64."""
+
+    def __init__(self, q: torch.Tensor, scales: torch.Tensor,
+                 zeros: Optional[torch.Tensor] = None, group_size: int = 128):
+        if q.dim() != 3 or q.dtype != torch.uint8:
+            raise TypeError("q must be a rank-3 uint8 tensor")
+        E, half, N = q.shape
+        K = 2 * half
+        if group_size not in (32, 64, 128):
+            raise ValueError(f"group_size must be 32, 64 or 128, got {group_size}")
+        if E == 0 or K == 0 or N == 0 or K % 64 or N % 64 or K % group_size:
+            raise ValueError(f"K ({K}) and N ({N}) must be multiples of 64 and K of the group size "
+                             f"{group_size}")
+        if scales.dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError("scales must be float16 or bfloat16")
+        if tuple(scales.shape) != (E, K // group_size, N):
+            raise ValueError(f"scales must be {(E, K // group_size, N)}, got {tuple(scales.shape)}")
+        if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape):
+            raise ValueError(f"zeros must be a uint8 tensor of shape {tuple(scales.shape)}")
+        for t, n in ((q, "q"), (scales, "scales"), (zeros, "zeros")):
+            if t is not None:
+                _need_cuda(t, n)
+                _need_contig(t, n)
+        _need_same_device(q.device, (scales, "scales"), (zeros, "zeros"))
+        self.q, self.scales, self.zeros, self.group_size = q, scales, zeros, group_size
+        self.shape = (E, K, N)
+
+    def _pack(self) -> torch.Tensor:
+        E, K, N = self.shape
+        dt = fused_moe_internal_dtype(self.scales.dtype)
+        size = int(lib().moe_int4_packed_size(E, K, N, self.group_size, dt,
+                                              int(self.zeros is not None)))
+        out = torch.empty((size,), dtype=torch.uint8, device=self.q.device)
+        with torch.cuda.device(self.q.device):
+            st = lib().moe_int4_pack(_ptr(self.q), _ptr(self.scales), _ptr(self.zeros), E, K, N,
+                                     self.group_size, dt, _ptr(out), _stream(self.q.device))
+        if st != MOE_OK:
+            raise MoeError(st, "moe_int4_pack")
+        return out
+
+
+def quantize_int4(weights: torch.Tensor, group_size: int = 128,
+                  symmetric: bool = True) -> Int4Weights:
+    """Int4Weights of f16/bf16 weights [E,K,N]; symmetric: zero point 8, else one per group (see
+    include/candle_moe.h for the rule)."""
+    _need_cuda(weights, "weights")
+    _need_contig(weights, "weights")
+    if weights.dim() != 3 or weights.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError("weights must be a rank-3 float16 or bfloat16 tensor")
+    if group_size not in (32, 64, 128) or weights.shape[1] % group_size:
+        raise ValueError(f"group_size must be 32, 64 or 128 and divide K, got {group_size}")
+    E, K, N = weights.shape
+    dev = weights.device
+    q = torch.empty((E, K // 2, N), dtype=torch.uint8, device=dev)
+    scales = torch.empty((E, K // group_size, N), dtype=weights.dtype, device=dev)
+    zeros = None if symmetric else torch.empty(scales.shape, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        st = lib().moe_int4_quantize(_ptr(weights), E, K, N, group_size,
+                                     fused_moe_internal_dtype(weights.dtype), _ptr(q),
+                                     _ptr(scales), _ptr(zeros), _stream(dev))
+    if st != MOE_OK:
+        raise MoeError(st, "moe_int4_quantize")
+    return Int4Weights(q, scales, zeros, group_size)
+
+
+class Int4Experts:
+    """The experts' matrices in the layout the 4-bit kernels read, packed once: gate and up
+    [E,H,I], down [E,I,H] as Int4Weights; up None: two-matrix experts, act(x.gate).down (for
+    Nomic weights [E,H,I] the second matrix goes in transposed)."""
+
+    def __init__(self, gate: Int4Weights, up: Optional[Int4Weights], down: Int4Weights):
+        E, H, I = gate.shape
+        if up is not None and up.shape != gate.shape:
+            raise ValueError(f"up must be {gate.shape}, got {up.shape}")
+        if down.shape != (E, I, H):
+            raise ValueError(f"down must be {(E, I, H)}, got {down.shape}")
+        mats = [m for m in (gate, up, down) if m is not None]
+        if any(m.group_size != gate.group_size or m.scales.dtype != gate.scales.dtype or
+               (m.zeros is None) != (gate.zeros is None) or m.q.device != gate.q.device
+               for m in mats):
+            raise ValueError("the matrices must share group size, scale type, zero points and "
+                             "device")
+        self.num_experts, self.hidden_dim, self.intermediate_dim = E, H, I
+        self.group_size, self.dtype = gate.group_size, gate.scales.dtype
+        self.has_zeros, self.device = gate.zeros is not None, gate.q.device
+        self.gate, self.down = gate._pack(), down._pack()
+        self.up = None if up is None else up._pack()
+
+    @classmethod
+    def quantize(cls, gate_weights: torch.Tensor, up_weights: Optional[torch.Tensor],
+                 down_weights: torch.Tensor, group_size: int = 128, symmetric: bool = True):
+        """From f16/bf16 gate and up [E,H,I] (up may be None) and down [E,I,H]."""
+        return cls(*[None if w is None else quantize_int4(w, group_size, symmetric)
+                     for w in (gate_weights, up_weights, down_weights)])
+
+
+def int4_workspace_size(num_tokens: int, hidden_dim: int, intermediate_dim: int,
+                        num_experts: int, top_k: int) -> int:
+    return int(lib().moe_fused_int4_workspace_size(num_tokens, hidden_dim, intermediate_dim,
+                                                   num_experts, top_k))
+
+
+def fused_moe_int4(input: torch.Tensor, experts: Int4Experts, routing_weights: torch.Tensor,
+                   expert_indices: torch.Tensor, activation: int = Activation.Silu,
+                   out: Optional[torch.Tensor] = None,
+                   workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """fused_moe on 4-bit experts: input [T,H] of the experts' type, routing_weights [T,k] f32,
+    expert_indices [T,k] int32/uint32 (ids >= E are skipped).  workspace: uint8, at least
+    int4_workspace_size() bytes, 256-byte aligned, optional."""
+    if input.dim() != 2 or routing_weights.dim() != 2 or expert_indices.dim() != 2:
+        raise ValueError("input, routing_weights and expert_indices must be rank 2")
+    T, H = input.shape
+    k = expert_indices.shape[1]
+    if H != experts.hidden_dim:
+        raise ValueError(f"Hidden dimension mismatch (expected {experts.hidden_dim}, got {H})")
+    if expert_indices.shape[0] != T or routing_weights.shape[0] != T:
+        raise ValueError("Number of tokens mismatch")
+    if routing_weights.shape[1] != k:
+        raise ValueError("Number of selected experts mismatch")
+    if input.dtype != experts.dtype:
+        raise TypeError(f"input must have the experts' dtype {experts.dtype}, got {input.dtype}")
+    if routing_weights.dtype != torch.float32:
+        raise TypeError("routing_weights must be float32")
+    if expert_indices.dtype not in _INDEX_DTYPES:
+        raise TypeError("expert_indices must be int32 or uint32")
+    tensors = [(input, "input"), (routing_weights, "routing_weights"),
+               (expert_indices, "expert_indices")]
+    if out is not None:
+        if tuple(out.shape) != (T, H) or out.dtype != input.dtype:
+            raise ValueError(f"out must be {(T, H)} of {input.dtype}")
+        tensors.append((out, "out"))
+    if workspace is not None:
+        tensors.append((workspace, "workspace"))
+    for t, n in tensors:
+        _need_cuda(t, n)
+        _need_contig(t, n)
+    dev = experts.device
+    _need_same_device(dev, *tensors)
+    if out is None:
+        out = torch.empty((T, H), dtype=input.dtype, device=dev)
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    with torch.cuda.device(dev):
+        st = lib().moe_fused_int4(_ptr(input), _ptr(experts.gate), _ptr(experts.up),
+                                  _ptr(experts.down), _ptr(routing_weights), _ptr(expert_indices),
+                                  _ptr(out), T, H, experts.intermediate_dim, experts.num_experts,
+                                  k, int(activation), fused_moe_internal_dtype(input.dtype),
+                                  experts.group_size, int(experts.has_zeros), _ptr(workspace),
+                                  ws_bytes, _stream(dev))
+    if st != MOE_OK:
+        raise MoeError(st, "moe_fused_int4")
+    return out
+
+
 class FusedMoE:
     """src/lib.rs:244-335."""
 
@@ -684,6 +855,16 @@ class FusedMoE:
         return fused_moe(input, gate_weights, up_weights, down_weights, routing_weights,
                          expert_indices, self.num_experts, self.num_selected_experts,
                          self.activation.to_int(), moe_type)
+
+    def forward_int4(self, input: torch.Tensor, experts: Int4Experts,
+                     routing_weights: torch.Tensor, expert_indices: torch.Tensor) -> torch.Tensor:
+        """forward with the experts' weights in 4 bits (the moe_type follows from the experts):
+        input [T,H] in the experts' dtype, the rest as forward."""
+        if experts.num_experts != self.num_experts:
+            raise ValueError("Number of experts mismatch")
+        if expert_indices.dim() == 2 and expert_indices.shape[1] != self.num_selected_experts:
+            raise ValueError("Number of selected experts mismatch")
+        return fused_moe_int4(input, experts, routing_weights, expert_indices, self.activation)
 
 
 class SparseMoeBlock:

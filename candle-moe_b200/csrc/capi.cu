@@ -963,6 +963,192 @@ CMOE_API int moe_fused_v2(const void* input, const void* gate_weights, const voi
                     workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
+// ---- 4-bit expert weights --------------------------------------------------------------------
+
+namespace cmoe {
+namespace {
+
+// MOE_OK, or why a [E, K, N] matrix with groups of G cannot be held in 4 bits.
+int int4_shape_status(int64_t E, int64_t K, int64_t N, int32_t G, uint32_t dtype) {
+  if (E <= 0 || K <= 0 || N <= 0 || dtype > 2) return MOE_ERR_INVALID_ARG;
+  if (G != 32 && G != 64 && G != 128) return MOE_ERR_INVALID_ARG;
+  if (K % G != 0) return MOE_ERR_INVALID_ARG;
+  if (dtype == kF32 || K % 64 != 0 || N % 64 != 0) return MOE_ERR_UNSUPPORTED;
+  return MOE_OK;
+}
+
+Int4Layout int4_layout(int64_t E, int64_t K, int64_t N, int32_t G, bool zeros) {
+  Int4Layout L;
+  L.scales = align256(static_cast<size_t>(E * K * N / 2));
+  L.zeros = L.scales + align256(static_cast<size_t>(E * (K / G) * N) * 2);
+  L.total = L.zeros + (zeros ? align256(static_cast<size_t>(E * (K / G) * N)) : 0);
+  return L;
+}
+
+struct Int4WsLayout {
+  size_t offsets, chunk_prefix, sorted_token, sorted_flat, sorted_w, prep_scratch, inter, slots,
+      total;
+};
+
+Int4WsLayout int4_ws_layout(int64_t T, int H, int I, int E, int k) {
+  const int64_t rows = T * k;
+  Int4WsLayout L;
+  size_t o = 0;
+  L.offsets = o;       o += align256(sizeof(int32_t) * (E + 2));
+  L.chunk_prefix = o;  o += align256(sizeof(int32_t) * (E + 1));
+  L.sorted_token = o;  o += align256(sizeof(int32_t) * rows);
+  L.sorted_flat = o;   o += align256(sizeof(int32_t) * rows);
+  L.sorted_w = o;      o += align256(sizeof(float) * rows);
+  L.prep_scratch = o;  o += align256(route_prep_scratch_bytes(rows, E));
+  L.inter = o;         o += align256(2 * static_cast<size_t>(rows) * I);
+  L.slots = o;         o += align256(4 * static_cast<size_t>(rows) * H);
+  L.total = o;
+  return L;
+}
+
+}  // namespace
+}  // namespace cmoe
+
+CMOE_API size_t moe_int4_packed_size(int32_t num_experts, int32_t k_dim, int32_t n_dim,
+                                     int32_t group_size, uint32_t dtype, int32_t has_zeros) {
+  if (int4_shape_status(num_experts, k_dim, n_dim, group_size, dtype) != MOE_OK) return 0;
+  return int4_layout(num_experts, k_dim, n_dim, group_size, has_zeros != 0).total;
+}
+
+CMOE_API int moe_int4_quantize(const void* weights, int32_t num_experts, int32_t k_dim,
+                               int32_t n_dim, int32_t group_size, uint32_t dtype, uint8_t* q,
+                               void* scales, uint8_t* zeros, void* stream) {
+  const int shape = int4_shape_status(num_experts, k_dim, n_dim, group_size, dtype);
+  if (shape != MOE_OK) return shape;
+  if (!weights || !q || !scales) return MOE_ERR_INVALID_ARG;
+  DeviceState* ds = nullptr;
+  int st = current_device_state(&ds);
+  if (st != MOE_OK) return st;
+  launch_int4_quantize(static_cast<int>(dtype), weights, num_experts, k_dim, n_dim, group_size,
+                       zeros == nullptr, q, scales, zeros, ds->num_sms,
+                       static_cast<cudaStream_t>(stream));
+  ++g_launches;
+  return finish(MOE_OK);
+}
+
+CMOE_API int moe_int4_pack(const uint8_t* q, const void* scales, const uint8_t* zeros,
+                           int32_t num_experts, int32_t k_dim, int32_t n_dim, int32_t group_size,
+                           uint32_t dtype, void* packed, void* stream) {
+  const int shape = int4_shape_status(num_experts, k_dim, n_dim, group_size, dtype);
+  if (shape != MOE_OK) return shape;
+  if (!q || !scales || !packed || (reinterpret_cast<uintptr_t>(packed) & 255u) != 0)
+    return MOE_ERR_INVALID_ARG;
+  DeviceState* ds = nullptr;
+  int st = current_device_state(&ds);
+  if (st != MOE_OK) return st;
+  g_launches += launch_int4_pack(
+      static_cast<int>(dtype), q, scales, zeros, num_experts, k_dim, n_dim, group_size,
+      int4_layout(num_experts, k_dim, n_dim, group_size, zeros != nullptr), packed, ds->num_sms,
+      static_cast<cudaStream_t>(stream));
+  return finish(MOE_OK);
+}
+
+CMOE_API size_t moe_fused_int4_workspace_size(int64_t num_tokens, int32_t hidden_dim,
+                                              int32_t intermediate_dim, int32_t num_experts,
+                                              int32_t topk) {
+  if (num_tokens <= 0 || hidden_dim <= 0 || intermediate_dim <= 0 || num_experts <= 0 ||
+      topk <= 0 || num_tokens > INT32_MAX / topk)
+    return 0;
+  return int4_ws_layout(num_tokens, hidden_dim, intermediate_dim, num_experts, topk).total;
+}
+
+CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const void* up_packed,
+                            const void* down_packed, const float* routing_weights,
+                            const uint32_t* expert_indices, void* output, int64_t num_tokens,
+                            int32_t hidden_dim, int32_t intermediate_dim, int32_t num_experts,
+                            int32_t topk, int32_t activation_type, uint32_t dtype,
+                            int32_t group_size, int32_t has_zeros, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  const int H = hidden_dim, I = intermediate_dim, E = num_experts;
+  if (num_tokens < 0 || topk <= 0) return MOE_ERR_INVALID_ARG;
+  int st = int4_shape_status(E, H, I, group_size, dtype);
+  if (st == MOE_OK) st = int4_shape_status(E, I, H, group_size, dtype);
+  if (st != MOE_OK) return st;
+  if (num_tokens == 0) return MOE_OK;
+  if (!input || !gate_packed || !down_packed || !routing_weights || !expert_indices || !output)
+    return MOE_ERR_INVALID_ARG;
+  if (E > route_prep_max_experts() || num_tokens > INT32_MAX / topk) return MOE_ERR_UNSUPPORTED;
+  if (!aligned16(input) || !aligned16(gate_packed) || (up_packed && !aligned16(up_packed)) ||
+      !aligned16(down_packed))
+    return MOE_ERR_UNSUPPORTED;
+  DeviceState* ds = nullptr;
+  st = current_device_state(&ds);
+  if (st != MOE_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const Int4WsLayout L = int4_ws_layout(num_tokens, H, I, E, topk);
+  char* ws = static_cast<char*>(workspace);
+  const bool owned = ws == nullptr;
+  if (owned) {
+    void* p = nullptr;
+    if (cudaMallocFromPoolAsync(&p, L.total, ds->pool, s) != cudaSuccess) {
+      cudaGetLastError();
+      return MOE_ERR_NO_MEMORY;
+    }
+    ws = static_cast<char*>(p);
+  } else if (workspace_bytes < L.total || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0) {
+    return MOE_ERR_WORKSPACE;
+  }
+  const int64_t rows = num_tokens * topk;
+  const int chunk = int4_chunk_rows(rows, E);
+  Int4Params g1 = {}, g2 = {};
+  const Int4Layout l1 = int4_layout(E, H, I, group_size, has_zeros != 0);
+  const Int4Layout l2 = int4_layout(E, I, H, group_size, has_zeros != 0);
+  auto matrix = [&](Int4Params& p, int m, const void* packed, const Int4Layout& l) {
+    const char* b = static_cast<const char*>(packed);
+    p.w[m] = b;
+    p.scale[m] = b + l.scales;
+    p.zero[m] = has_zeros ? reinterpret_cast<const uint8_t*>(b + l.zeros) : nullptr;
+  };
+  matrix(g1, 0, gate_packed, l1);
+  if (up_packed) matrix(g1, 1, up_packed, l1);
+  matrix(g2, 0, down_packed, l2);
+  g1.x = input;
+  g1.out = ws + L.inter;
+  g1.offsets = reinterpret_cast<int32_t*>(ws + L.offsets);
+  g1.chunk_prefix = reinterpret_cast<int32_t*>(ws + L.chunk_prefix);
+  g1.sorted_token = reinterpret_cast<int32_t*>(ws + L.sorted_token);
+  g1.sorted_flat = reinterpret_cast<int32_t*>(ws + L.sorted_flat);
+  g1.sorted_w = reinterpret_cast<float*>(ws + L.sorted_w);
+  g1.N = I;
+  g1.K = H;
+  g1.G = group_size;
+  g1.E = E;
+  g1.act = activation_type;
+  g2.x = ws + L.inter;
+  g2.out = ws + L.slots;
+  g2.offsets = g1.offsets;
+  g2.chunk_prefix = g1.chunk_prefix;
+  g2.sorted_token = g1.sorted_token;
+  g2.sorted_flat = g1.sorted_flat;
+  g2.sorted_w = g1.sorted_w;
+  g2.N = H;
+  g2.K = I;
+  g2.G = group_size;
+  g2.E = E;
+  g2.act = activation_type;
+  if (launch_route_prep(expert_indices, routing_weights, num_tokens, topk, E, chunk,
+                        reinterpret_cast<int32_t*>(ws + L.offsets),
+                        reinterpret_cast<int32_t*>(ws + L.chunk_prefix),
+                        reinterpret_cast<int32_t*>(ws + L.sorted_token),
+                        reinterpret_cast<float*>(ws + L.sorted_w),
+                        reinterpret_cast<int32_t*>(ws + L.sorted_flat), ws + L.prep_scratch,
+                        s) != 0)
+    st = MOE_ERR_CUDA;
+  if (st == MOE_OK) {
+    int64_t n = route_prep_scratch_bytes(rows, E) ? 3 : 1;
+    n += launch_int4_ffn(static_cast<int>(dtype), chunk, g1, g2, expert_indices, num_tokens, topk,
+                         output, ds->num_sms, s);
+    g_launches += n;
+  }
+  if (owned) cudaFreeAsync(ws, s);
+  return finish(st);
+}
+
 CMOE_API int moe_fused_scatter(const void* input, const void* gate_weights,
                                const void* up_weights, const void* down_weights,
                                const float* routing_weights, const uint32_t* expert_indices,

@@ -261,6 +261,45 @@ int moe_fused_v2(const void* input, const void* gate_weights, const void* up_wei
                  size_t workspace_bytes, void* stream);
 
 /*
+ * Expert weights in 4 bits with group scales (no counterpart in the reference).  A matrix
+ * W [num_experts, k_dim, n_dim] (k_dim the reduction; gate and up: hidden -> intermediate, down:
+ * intermediate -> hidden) is
+ *     W[e,k,n] = (q[e,k,n] - zero[e,k/group_size,n]) * scale[e,k/group_size,n]
+ *   q       [num_experts, k_dim/2, n_dim] u8: the low nibble is even k, the high nibble k + 1
+ *   scales  [num_experts, k_dim/group_size, n_dim] of `dtype` (0 f16, 1 bf16: the activations')
+ *   zeros   the same shape, u8 in 0..15, or NULL: 8 everywhere
+ * group_size 32, 64 or 128, a divisor of k_dim; k_dim and n_dim multiples of 64 (else
+ * MOE_ERR_UNSUPPORTED).
+ *
+ * moe_int4_quantize: q and scales (and zeros, when not NULL) of f16/bf16 weights, per group and
+ *   column: without zeros scale = max|w| / 7, q = round(w / scale) + 8; with zeros scale =
+ *   (max(w, 0) - min(w, 0)) / 15, zero = round(-min(w, 0) / scale), q = round(w / scale) + zero;
+ *   scale rounded to `dtype` first, round half to even, q and zero clamped to 0..15.
+ * moe_int4_packed_size / moe_int4_pack: size of, and copy into, the layout the kernels read
+ *   (packed: 256-byte aligned); done once per set of weights, for the activations' dtype.
+ * moe_fused_int4: moe_fused_v2 on packed weights, f16/bf16.  up_packed NULL: out = sum_j w
+ *   act(x.Gate).Down (the Nomic form; its second matrix packed as [E, I, H]).  has_zeros tells
+ *   whether all matrices were packed with zeros.  workspace as moe_fused_v2, of
+ *   moe_fused_int4_workspace_size() bytes.
+ */
+size_t moe_int4_packed_size(int32_t num_experts, int32_t k_dim, int32_t n_dim, int32_t group_size,
+                            uint32_t dtype, int32_t has_zeros);
+int moe_int4_quantize(const void* weights, int32_t num_experts, int32_t k_dim, int32_t n_dim,
+                      int32_t group_size, uint32_t dtype, uint8_t* q, void* scales, uint8_t* zeros,
+                      void* stream);
+int moe_int4_pack(const uint8_t* q, const void* scales, const uint8_t* zeros, int32_t num_experts,
+                  int32_t k_dim, int32_t n_dim, int32_t group_size, uint32_t dtype, void* packed,
+                  void* stream);
+size_t moe_fused_int4_workspace_size(int64_t num_tokens, int32_t hidden_dim,
+                                     int32_t intermediate_dim, int32_t num_experts, int32_t topk);
+int moe_fused_int4(const void* input, const void* gate_packed, const void* up_packed,
+                   const void* down_packed, const float* routing_weights,
+                   const uint32_t* expert_indices, void* output, int64_t num_tokens,
+                   int32_t hidden_dim, int32_t intermediate_dim, int32_t num_experts, int32_t topk,
+                   int32_t activation_type, uint32_t dtype, int32_t group_size, int32_t has_zeros,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * The expert computation of fused_moe without the combine: the weighted contribution
  * w[t,j] * y_{e(t,j)}(x_t) of every routed (t, j) (ids >= num_experts skipped) is written,
  * rounded to `dtype`, to row out_row[t*topk + j] of `output` ([rows, hidden_dim]; the rows of
