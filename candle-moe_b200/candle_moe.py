@@ -16,6 +16,7 @@ caller workspace), ``fused_moe_int4`` / ``Int4Experts`` / ``quantize_int4`` (exp
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import enum
 import os
@@ -288,6 +289,22 @@ class GroupScore(enum.IntEnum):
     Top2 = 1
 
 
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on(dev: torch.device):
+    """Context with `dev` current; nothing to enter (and no time spent) when it already is."""
+    return _NO_GUARD if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _raw_stream(dev: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _addr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
 def _need_rows(t: torch.Tensor, name: str):
     # rows may lie apart (a slice of a wider projection), a row itself may not
     if t.dim() != 2:
@@ -330,11 +347,11 @@ def route_experts(logits: torch.Tensor, top_k: int, scoring: Scoring = Scoring.S
         _need_same_device(dev, (bias, "bias"))
     w = torch.empty((T, max(top_k, 0)), dtype=torch.float32, device=dev)
     idx = torch.empty((T, max(top_k, 0)), dtype=torch.int32, device=dev)
-    with torch.cuda.device(dev):
-        st = lib().moe_route_experts(_ptr(logits), fused_moe_internal_dtype(logits.dtype),
-                                     _row_stride(logits), _ptr(bias), T, E, top_k, int(scoring),
+    with _on(dev):
+        st = lib().moe_route_experts(_addr(logits), fused_moe_internal_dtype(logits.dtype),
+                                     _row_stride(logits), _addr(bias), T, E, top_k, int(scoring),
                                      num_groups, topk_groups, int(group_score), int(renormalize),
-                                     scaling, _ptr(w), _ptr(idx), _stream(dev))
+                                     scaling, _addr(w), _addr(idx), _raw_stream(dev))
     if st != MOE_OK:
         raise MoeError(st, "moe_route_experts")
     return w, idx
@@ -368,11 +385,11 @@ def route_experts_backward(grad_weights: torch.Tensor, logits: torch.Tensor,
     _need_same_device(dev, (grad_weights, "grad_weights"), (weights, "weights"),
                       (indices, "indices"))
     grad = torch.empty((T, E), dtype=logits.dtype, device=dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         st = lib().moe_route_experts_backward(
-            _ptr(grad_weights), _ptr(logits), fused_moe_internal_dtype(logits.dtype),
-            _row_stride(logits), _ptr(weights), _ptr(indices), T, E, indices.shape[1],
-            int(scoring), int(renormalize), scaling, _ptr(grad), _stream(dev))
+            _addr(grad_weights), _addr(logits), fused_moe_internal_dtype(logits.dtype),
+            _row_stride(logits), _addr(weights), _addr(indices), T, E, indices.shape[1],
+            int(scoring), int(renormalize), scaling, _addr(grad), _raw_stream(dev))
     if st != MOE_OK:
         raise MoeError(st, "moe_route_experts_backward")
     return grad
@@ -800,13 +817,13 @@ def fused_moe_int4(input: torch.Tensor, experts: Int4Experts, routing_weights: t
     if out is None:
         out = torch.empty((T, H), dtype=input.dtype, device=dev)
     ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    with torch.cuda.device(dev):
-        st = lib().moe_fused_int4(_ptr(input), _ptr(experts.gate), _ptr(experts.up),
-                                  _ptr(experts.down), _ptr(routing_weights), _ptr(expert_indices),
-                                  _ptr(out), T, H, experts.intermediate_dim, experts.num_experts,
+    with _on(dev):
+        st = lib().moe_fused_int4(_addr(input), _addr(experts.gate), _addr(experts.up),
+                                  _addr(experts.down), _addr(routing_weights), _addr(expert_indices),
+                                  _addr(out), T, H, experts.intermediate_dim, experts.num_experts,
                                   k, int(activation), fused_moe_internal_dtype(input.dtype),
-                                  experts.group_size, int(experts.has_zeros), _ptr(workspace),
-                                  ws_bytes, _stream(dev))
+                                  experts.group_size, int(experts.has_zeros), _addr(workspace),
+                                  ws_bytes, _raw_stream(dev))
     if st != MOE_OK:
         raise MoeError(st, "moe_fused_int4")
     return out

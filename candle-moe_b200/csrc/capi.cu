@@ -1006,6 +1006,13 @@ Int4WsLayout int4_ws_layout(int64_t T, int H, int I, int E, int k) {
   return L;
 }
 
+// Calls of many rows expand the weights to 16 bits once and run the grouped GEMMs on them: the
+// expansion moves 2.5 bytes a weight and is paid once, where the packed kernels unpack a weight
+// again for every chunk of rows.
+bool int4_expands(int64_t T, int H, int I, int E, int k) {
+  return H % 128 == 0 && I % 128 == 0 && E <= sm100_max_experts() && T * k >= 64 * E;
+}
+
 }  // namespace
 }  // namespace cmoe
 
@@ -1054,7 +1061,15 @@ CMOE_API size_t moe_fused_int4_workspace_size(int64_t num_tokens, int32_t hidden
   if (num_tokens <= 0 || hidden_dim <= 0 || intermediate_dim <= 0 || num_experts <= 0 ||
       topk <= 0 || num_tokens > INT32_MAX / topk)
     return 0;
-  return int4_ws_layout(num_tokens, hidden_dim, intermediate_dim, num_experts, topk).total;
+  size_t n = int4_ws_layout(num_tokens, hidden_dim, intermediate_dim, num_experts, topk).total;
+  if (int4_expands(num_tokens, hidden_dim, intermediate_dim, num_experts, topk)) {
+    const size_t matrix =
+        align256(2 * static_cast<size_t>(num_experts) * hidden_dim * intermediate_dim);
+    n = std::max(n, 3 * matrix + moe_fused_workspace_size(num_tokens, hidden_dim,
+                                                          intermediate_dim, num_experts, topk, 0,
+                                                          kBF16));
+  }
+  return n;
 }
 
 CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const void* up_packed,
@@ -1081,16 +1096,17 @@ CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const vo
   if (st != MOE_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const Int4WsLayout L = int4_ws_layout(num_tokens, H, I, E, topk);
+  const size_t need = moe_fused_int4_workspace_size(num_tokens, H, I, E, topk);
   char* ws = static_cast<char*>(workspace);
   const bool owned = ws == nullptr;
   if (owned) {
     void* p = nullptr;
-    if (cudaMallocFromPoolAsync(&p, L.total, ds->pool, s) != cudaSuccess) {
+    if (cudaMallocFromPoolAsync(&p, need, ds->pool, s) != cudaSuccess) {
       cudaGetLastError();
       return MOE_ERR_NO_MEMORY;
     }
     ws = static_cast<char*>(p);
-  } else if (workspace_bytes < L.total || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0) {
+  } else if (workspace_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0) {
     return MOE_ERR_WORKSPACE;
   }
   const int64_t rows = num_tokens * topk;
@@ -1107,6 +1123,24 @@ CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const vo
   matrix(g1, 0, gate_packed, l1);
   if (up_packed) matrix(g1, 1, up_packed, l1);
   matrix(g2, 0, down_packed, l2);
+  if (int4_expands(num_tokens, H, I, E, topk) && aligned16(output)) {
+    // two-matrix experts: the grouped GEMMs read the second matrix as [E, H, I]
+    const size_t size = align256(2 * static_cast<size_t>(E) * H * I);
+    const int dt = static_cast<int>(dtype);
+    launch_int4_expand(dt, g1.w[0], g1.scale[0], g1.zero[0], E, H, I, group_size, false, ws, s);
+    if (up_packed)
+      launch_int4_expand(dt, g1.w[1], g1.scale[1], g1.zero[1], E, H, I, group_size, false,
+                         ws + size, s);
+    char* down = ws + (up_packed ? 2 : 1) * size;
+    launch_int4_expand(dt, g2.w[0], g2.scale[0], g2.zero[0], E, I, H, group_size, !up_packed, down,
+                       s);
+    g_launches += up_packed ? 3 : 2;
+    st = fused_impl(input, ws, up_packed ? ws + size : down, up_packed ? down : nullptr,
+                    routing_weights, expert_indices, output, num_tokens, H, I, E, topk,
+                    activation_type, up_packed ? 0 : 1, dtype, ws + 3 * size, need - 3 * size, s);
+    if (owned) cudaFreeAsync(ws, s);
+    return finish(st);
+  }
   g1.x = input;
   g1.out = ws + L.inter;
   g1.offsets = reinterpret_cast<int32_t*>(ws + L.offsets);

@@ -188,6 +188,9 @@ int launch_int4_quantize(int dtype, const void* w, int E, int K, int N, int G, i
 int launch_int4_pack(int dtype, const uint8_t* q, const void* scales, const uint8_t* zeros, int E,
                      int K, int N, int G, const Int4Layout& L, void* packed, int num_sms,
                      cudaStream_t s);
+// out [E,K,N], or [E,N,K] with trans, in 16 bits; N a multiple of 128.
+void launch_int4_expand(int dtype, const void* w, const void* scale, const uint8_t* zero, int E,
+                        int K, int N, int G, bool trans, void* out, cudaStream_t s);
 int launch_int4_ffn(int dtype, int chunk_rows, const Int4Params& g1, const Int4Params& g2,
                     const uint32_t* idx, int64_t num_tokens, int k, void* out, int num_sms,
                     cudaStream_t s);

@@ -155,6 +155,69 @@ __global__ void int4_pack_groups_kernel(const V* __restrict__ in, int E, int KG,
   }
 }
 
+// ---- weights back in 16 bits (for calls of many rows) --------------------------------------------
+
+template <typename T> struct Pair;
+template <> struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
+template <> struct Pair<__half> { using type = __half2; };
+
+// One CTA per (expert, 64 k, 128 n): a warp takes 16 n (one packed tile), the rows leave through
+// shared memory in 256-byte (out [E,K,N]) or 128-byte (kTrans: out [E,N,K]) pieces.  q - z is
+// exact, the product with the scale is rounded once.
+template <typename T, bool kTrans>
+__global__ void __launch_bounds__(256)
+    int4_expand_kernel(const uint4* __restrict__ w, const T* __restrict__ scale,
+                       const uint8_t* __restrict__ zero, int K, int N, int G, T* __restrict__ out) {
+  using T2 = typename Pair<T>::type;
+  constexpr int kCols = kTrans ? 64 : 128;
+  constexpr int kPitch = kCols + 8;
+  __shared__ alignas(16) T buf[(kTrans ? 128 : 64) * kPitch];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+  const int nb = N / 128, kb = K / 64, kg = K / G;
+  const int nblk = blockIdx.x % nb;
+  const int b = (blockIdx.x / nb) % kb;
+  const int64_t e = blockIdx.x / nb / kb;
+  const int64_t tile = e * (N / 16) + nblk * 8 + warp;
+  const uint4 q = __ldcs(w + (tile * kb + b) * 32 + lane);
+  const uint32_t word[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int64_t gi = ((tile * kg + (64 * b + 32 * h) / G) * 8 + gid) * 2;
+    T2 sc[2], off[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      sc[r].x = sc[r].y = scale[gi + r];
+      off[r].x = off[r].y =
+          Elem<T>::from_f(16.f + (zero ? static_cast<float>(zero[gi + r]) : 8.f));
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        const uint32_t u = nib_pair<T>(word[2 * h + s], f);
+        const T2 v = __hmul2(__hsub2(*reinterpret_cast<const T2*>(&u), off[f & 1]), sc[f & 1]);
+        const int n = 16 * warp + gid + 8 * (f & 1);
+        const int k = 32 * h + 8 * tig + 4 * s + 2 * (f >> 1);
+        if (kTrans) {
+          *reinterpret_cast<T2*>(buf + n * kPitch + k) = v;
+        } else {
+          buf[k * kPitch + n] = v.x;
+          buf[(k + 1) * kPitch + n] = v.y;
+        }
+      }
+  }
+  __syncthreads();
+  constexpr int kVecs = kCols / 8;
+  const int64_t row0 = kTrans ? e * N + nblk * 128 : e * K + b * 64;
+  const int ld = kTrans ? K : N, col0 = kTrans ? b * 64 : nblk * 128;
+#pragma unroll
+  for (int i = threadIdx.x; i < 128 * 64 / 8; i += 256) {
+    const int r = i / kVecs, c = (i % kVecs) * 8;
+    *reinterpret_cast<uint4*>(out + (row0 + r) * ld + col0 + c) =
+        *reinterpret_cast<const uint4*>(buf + r * kPitch + c);
+  }
+}
+
 // ---- the products ------------------------------------------------------------------------------
 
 constexpr int kWarps = 8;
@@ -320,7 +383,27 @@ void launch_ffn(int nt, const Int4Params& g1, const Int4Params& g2, const uint32
       static_cast<const float*>(g2.out), idx, T_, k, g2.N, g2.E, static_cast<T*>(out));
 }
 
+template <typename T>
+void expand(const void* w, const void* scale, const uint8_t* zero, int E, int K, int N, int G,
+            bool trans, void* out, cudaStream_t s) {
+  const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(E) * (K / 64) * (N / 128));
+  if (trans)
+    int4_expand_kernel<T, true><<<grid, 256, 0, s>>>(static_cast<const uint4*>(w),
+                                                     static_cast<const T*>(scale), zero, K, N, G,
+                                                     static_cast<T*>(out));
+  else
+    int4_expand_kernel<T, false><<<grid, 256, 0, s>>>(static_cast<const uint4*>(w),
+                                                      static_cast<const T*>(scale), zero, K, N, G,
+                                                      static_cast<T*>(out));
+}
+
 }  // namespace
+
+void launch_int4_expand(int dtype, const void* w, const void* scale, const uint8_t* zero, int E,
+                        int K, int N, int G, bool trans, void* out, cudaStream_t s) {
+  if (dtype == kBF16) expand<__nv_bfloat16>(w, scale, zero, E, K, N, G, trans, out, s);
+  else expand<__half>(w, scale, zero, E, K, N, G, trans, out, s);
+}
 
 int int4_chunk_rows(int64_t rows, int E) {
   const int64_t per = rows / E;

@@ -198,3 +198,14 @@ def test_refusals():
     odd = torch.empty(4 * 128 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(4, 128)
     with pytest.raises(cm.MoeError):
         cm.fused_moe_int4(odd, ex, w, idx)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("T,E,k,H,I,G", [(300, 4, 2, 256, 384, 64), (129, 1, 1, 128, 256, 128),
+                                         (517, 7, 3, 384, 128, 32)])
+def test_many_rows(T, E, k, H, I, G, dtype, zeros):
+    """Calls whose weights are expanded to 16 bits (the bound counts those roundings)."""
+    for nomic in (False, True):
+        x, mats, w, idx = make(T + E, T, E, k, H, I, G, dtype, zeros, nomic, skip=0.1)
+        run(x, mats, w, idx, cm.Activation.Gelu if nomic else cm.Activation.Silu, rounded=True)
