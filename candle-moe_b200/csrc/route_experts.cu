@@ -11,7 +11,8 @@
 //   w_j   = c r_j / sum_i r_i  or  c r_j,  with r_j the picked s (a zero sum gives zeros)
 //
 // The picks compare scores, and two scores that differ in their 9th digit have to come out in
-// the order of their true values, so the keys are held in 64 bits.
+// the order of their true values: a 32-bit comparison that its rounding errors could have
+// turned is made again in 64 bits.
 //
 // Backward, with g the gradient of w:
 //   dr_j = c (g_j - sum_i g_i r_i / R) / R  (R = sum r)   or   c g_j
@@ -27,7 +28,9 @@ namespace cmoe {
 
 namespace {
 
-constexpr int kWarps = 4;  // rows of a block, one per warp
+constexpr int kWarps = 4;      // rows of a block, one per warp
+constexpr int kFastWarps = 8;  // the same for route_experts_kernel
+constexpr int kMaxCand = 64;   // candidates it ranks
 
 __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
@@ -58,166 +61,485 @@ __device__ __forceinline__ void warp_best(double& v, int& id) {
   }
 }
 
+// NaN logits count as -inf.
+template <typename T> __device__ __forceinline__ float logit_of(const T* l, int e) {
+  const float x = Elem<T>::to_f(l[e]);
+  return x == x ? x : -CUDART_INF_F;
+}
+
+// Doubles of scratch per warp of route_row64.
+__host__ __device__ __forceinline__ int row64_scratch(int E) { return E + kRouteMaxGroups; }
+
+// One row by one warp with 64-bit keys, any shape: key and value (the groups') in scratch.
+// Leaves the pick of slot `lane` (id E: none) and its score.
 template <typename T>
-__global__ void __launch_bounds__(kWarps * 32) route_experts_kernel(RouteExpertsParams p) {
-  extern __shared__ double smem_d[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  double* key = smem_d + warp * (2 * p.E + kRouteMaxGroups);
-  double* sum_key = key + p.E;  // s + b, for the sums of two
-  double* value = sum_key + p.E;
+__device__ __noinline__ void route_row64(const RouteExpertsParams& p, int64_t row, double* key,
+                                         float& mine, int& mine_id) {
+  const int lane = threadIdx.x & 31;
+  double* value = key + p.E;
   const int per = p.E / p.num_groups;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + warp; row < p.num_tokens;
-       row += static_cast<int64_t>(gridDim.x) * kWarps) {
-    const T* l = static_cast<const T*>(p.logits) + row * p.stride;
-    auto logit = [&](int e) {
-      const float x = Elem<T>::to_f(l[e]);
-      return x == x ? x : -CUDART_INF_F;
-    };
-    float m = -CUDART_INF_F;
-    for (int e = lane; e < p.E; e += 32) m = fmaxf(m, logit(e));
-    m = warp_max(m);
-    double total = 0.0;
-    if (p.scoring == 0) {
-      for (int e = lane; e < p.E; e += 32) {
-        const float x = logit(e);
-        if (x > -CUDART_INF_F) total += exp(static_cast<double>(x) - static_cast<double>(m));
-      }
-      total = warp_sum(total);
-    }
-    auto score = [&](float x) -> double {
-      if (!(x > -CUDART_INF_F)) return 0.0;
-      if (p.scoring == 0) return exp(static_cast<double>(x) - static_cast<double>(m)) / total;
-      return 1.0 / (1.0 + exp(-static_cast<double>(x)));
-    };
+  const T* l = static_cast<const T*>(p.logits) + row * p.stride;
+  float m = -CUDART_INF_F;
+  for (int e = lane; e < p.E; e += 32) m = fmaxf(m, logit_of(l, e));
+  m = warp_max(m);
+  double total = 0.0;
+  if (p.scoring == 0) {
     for (int e = lane; e < p.E; e += 32) {
-      const float x = logit(e);
-      double s = -CUDART_INF, k = -CUDART_INF;
+      const float x = logit_of(l, e);
+      if (x > -CUDART_INF_F) total += exp(static_cast<double>(x) - static_cast<double>(m));
+    }
+    total = warp_sum(total);
+  }
+  auto score = [&](float x) -> double {
+    if (!(x > -CUDART_INF_F)) return 0.0;
+    if (p.scoring == 0) return exp(static_cast<double>(x) - static_cast<double>(m)) / total;
+    return 1.0 / (1.0 + exp(-static_cast<double>(x)));
+  };
+  // keys; sums: of score + bias (for the groups' sums of two)
+  auto fill = [&](bool sums) {
+    for (int e = lane; e < p.E; e += 32) {
+      const float x = logit_of(l, e);
+      double k = -CUDART_INF;
       if (x > -CUDART_INF_F) {
-        s = score(x) + (p.bias ? static_cast<double>(p.bias[e]) : 0.0);
-        if (!(s > -CUDART_INF)) s = -CUDART_INF;  // a bias of -inf or NaN shuts the expert off
-        k = p.bias ? s : static_cast<double>(x);
+        k = (p.bias || sums) ? score(x) + (p.bias ? static_cast<double>(p.bias[e]) : 0.0)
+                             : static_cast<double>(x);
+        if (!(k > -CUDART_INF)) k = -CUDART_INF;  // a bias of -inf or NaN shuts the expert off
       }
       key[e] = k;
-      sum_key[e] = s;
     }
     __syncwarp();
-    if (p.num_groups > 1) {
-      for (int g = lane; g < p.num_groups; g += 32) {
-        double a = -CUDART_INF, b = -CUDART_INF;
-        const double* from = p.group_score == 0 ? key : sum_key;
-        for (int i = 0; i < per; ++i) {
-          const double v = from[g * per + i];
-          if (v > a) {
-            b = a;
-            a = v;
-          } else if (v > b) {
-            b = v;
-          }
+  };
+  unsigned open = 0xffffffffu;
+  if (p.num_groups > 1) {
+    const bool top2 = p.group_score != 0;
+    fill(top2);
+    for (int g = lane; g < p.num_groups; g += 32) {
+      double a = -CUDART_INF, b = -CUDART_INF;
+      for (int i = 0; i < per; ++i) {
+        const double v = key[g * per + i];
+        if (v > a) {
+          b = a;
+          a = v;
+        } else if (v > b) {
+          b = v;
         }
-        value[g] = (p.group_score == 0 || !(b > -CUDART_INF)) ? a : a + b;
       }
-      __syncwarp();
-      unsigned open = 0;
-      for (int i = 0; i < p.topk_groups; ++i) {
-        double v = -CUDART_INF;
-        int id = 0x7fffffff;
-        if (lane < p.num_groups && !((open >> lane) & 1u)) {
-          v = value[lane];
-          id = lane;
-        }
-        warp_best(v, id);
-        if (!(v > -CUDART_INF)) break;
-        open |= 1u << id;
-      }
-      for (int e = lane; e < p.E; e += 32)
-        if (!((open >> (e / per)) & 1u)) key[e] = -CUDART_INF;
-      __syncwarp();
+      value[g] = (!top2 || !(b > -CUDART_INF)) ? a : a + b;
     }
-    float mine = 0.f;  // the pick of slot `lane`
-    int mine_id = p.E;
-    for (int j = 0; j < p.k; ++j) {
+    __syncwarp();
+    open = 0;
+    for (int i = 0; i < p.topk_groups; ++i) {
       double v = -CUDART_INF;
       int id = 0x7fffffff;
-      for (int e = lane; e < p.E; e += 32)
-        if (key[e] > v) {
-          v = key[e];
-          id = e;
-        }
+      if (lane < p.num_groups && !((open >> lane) & 1u)) {
+        v = value[lane];
+        id = lane;
+      }
       warp_best(v, id);
       if (!(v > -CUDART_INF)) break;
-      if (lane == j) {
-        mine = static_cast<float>(score(logit(id)));
-        mine_id = id;
+      open |= 1u << id;
+    }
+  }
+  fill(false);
+  if (p.num_groups > 1) {
+    for (int e = lane; e < p.E; e += 32)
+      if (!((open >> (e / per)) & 1u)) key[e] = -CUDART_INF;
+    __syncwarp();
+  }
+  mine = 0.f;
+  mine_id = p.E;
+  for (int j = 0; j < p.k; ++j) {
+    double v = -CUDART_INF;
+    int id = 0x7fffffff;
+    for (int e = lane; e < p.E; e += 32)
+      if (key[e] > v) {
+        v = key[e];
+        id = e;
       }
-      if (id % 32 == lane) key[id] = -CUDART_INF;
-      __syncwarp();
+    warp_best(v, id);
+    if (!(v > -CUDART_INF)) break;
+    if (lane == j) {
+      mine = static_cast<float>(score(logit_of(l, id)));
+      mine_id = id;
     }
-    if (p.renormalize) {
-      const float r = warp_sum(mine);
-      mine = r > 0.f ? mine / r : mine;
-    }
-    if (lane < p.k) {
-      p.weights[row * p.k + lane] = mine * p.scaling;
-      p.indices[row * p.k + lane] = mine_id;
-    }
+    if (id % 32 == lane) key[id] = -CUDART_INF;
     __syncwarp();
   }
 }
 
+// Writes the row's k slots from the pick that each lane holds (slot `lane`).
+__device__ __forceinline__ void store_row(const RouteExpertsParams& p, int64_t row, float r,
+                                          int id) {
+  const int lane = threadIdx.x & 31;
+  if (p.renormalize) {
+    const float sum = warp_sum(r);
+    r = sum > 0.f ? r / sum : r;
+  }
+  if (lane < p.k) {
+    p.weights[row * p.k + lane] = r * p.scaling;
+    p.indices[row * p.k + lane] = id;
+  }
+}
+
+// Every row in 64 bits: shapes whose rows do not fit the registers of the kernel below.
 template <typename T>
-__global__ void __launch_bounds__(kWarps * 32)
-    route_experts_backward_kernel(RouteExpertsBackwardParams p) {
-  extern __shared__ float smem_f[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float* ds = smem_f + warp * p.E;
+__global__ void __launch_bounds__(kWarps * 32) route_experts64_kernel(RouteExpertsParams p) {
+  extern __shared__ double smem_d[];
+  const int warp = threadIdx.x >> 5;
+  double* key = smem_d + warp * row64_scratch(p.E);
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + warp; row < p.num_tokens;
        row += static_cast<int64_t>(gridDim.x) * kWarps) {
+    float r;
+    int id;
+    route_row64<T>(p, row, key, r, id);
+    store_row(p, row, r, id);
+    __syncwarp();
+  }
+}
+
+__device__ __forceinline__ float redux_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// One row per warp, 32-bit keys in registers.  Lane l holds `bs` <= VPT consecutive experts (of one
+// group: lpg = 32 / num_groups lanes per group), so lane order is expert order.
+//
+// Picks: the k-th largest of the 32 lane maxima (k rounds of a warp maximum) is a lower bound of
+// the k-th largest key, so the keys at or above it -- a few more than k -- are the only
+// candidates; they are compacted into shared memory in expert order, one per lane (two with
+// more than 32), and each counts the candidates before it: that count is its slot.  No round
+// depends on the one before, as k warp argmax rounds would.
+//
+// Keys that are logits are exact.  With a bias the key s + b is off by at most `delta`; two
+// candidates nearer than 2 delta that are not the same numbers, or two groups nearer than their
+// sums' error, send the row to route_row64, which decides in 64 bits (one row in some hundreds).
+// delta: a sigmoid is off by under 4 half-steps of 1 plus the sum's own rounding; a softmax score
+// by (expf 2 ulp, l - m: |l - m| 2^-24, 21 additions, one division, averaged over the row under
+// 4e-6) of the largest score.
+template <typename T, int VPT, bool kBias, bool kGroups>
+__global__ void __launch_bounds__(kFastWarps * 32)
+    route_experts_kernel(RouteExpertsParams p, int bs, int lpg, int vec) {
+  extern __shared__ double smem_d[];
+  __shared__ alignas(16) float s_key[kFastWarps][kMaxCand];
+  __shared__ uint16_t s_id[kFastWarps][kMaxCand];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float kNone = -CUDART_INF_F;
+  float* ck = s_key[warp];
+  uint16_t* cid = s_id[warp];
+  const int per = p.E / p.num_groups;
+  // this lane's experts: [e0, e0 + n)
+  const int g = kGroups ? lane / lpg : 0;
+  int e0 = kGroups ? g * per + (lane % lpg) * bs : lane * bs;
+  int n = min(bs, (kGroups ? (g + 1) * per : p.E) - e0);
+  if (kGroups && g >= p.num_groups) n = 0;
+  n = max(n, 0);
+  if (n == 0) e0 = 0;
+  float b[kBias ? VPT : 1];
+  if (kBias) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) b[i] = i < n ? __ldg(p.bias + e0 + i) : 0.f;
+  }
+  const bool sums = kGroups && p.group_score != 0;
+  const bool need_total = p.scoring == 0 && (kBias || sums || !p.renormalize);
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kFastWarps + warp; row < p.num_tokens;
+       row += static_cast<int64_t>(gridDim.x) * kFastWarps) {
     const T* l = static_cast<const T*>(p.logits) + row * p.stride;
-    T* out = static_cast<T*>(p.grad_logits) + row * p.E;
-    auto logit = [&](int e) {
-      const float x = Elem<T>::to_f(l[e]);
-      return x == x ? x : -CUDART_INF_F;
-    };
-    float m = -CUDART_INF_F, total = 0.f;
-    if (p.scoring == 0) {
-      for (int e = lane; e < p.E; e += 32) m = fmaxf(m, logit(e));
-      m = warp_max(m);
-      for (int e = lane; e < p.E; e += 32)
-        if (logit(e) > -CUDART_INF_F) total += expf(logit(e) - m);
-      total = warp_sum(total);
+    float v[VPT];
+    if (vec) {  // n is 0 or bs, and bs a multiple of 16 bytes
+      constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+      for (int c = 0; c < (VPT + kPer - 1) / kPer; ++c) {
+        alignas(16) T q[kPer];
+        if (c * kPer < n)
+          *reinterpret_cast<uint4*>(q) = __ldg(reinterpret_cast<const uint4*>(l + e0) + c);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (c * kPer + i < VPT) v[c * kPer + i] = c * kPer < n ? Elem<T>::to_f(q[i]) : kNone;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) v[i] = i < n ? Elem<T>::to_f(l[e0 + i]) : kNone;
     }
-    auto score = [&](float x) -> float {
-      if (!(x > -CUDART_INF_F)) return 0.f;
-      return p.scoring == 0 ? expf(x - m) / total : 1.f / (1.f + expf(-x));
-    };
-    for (int e = lane; e < p.E; e += 32) ds[e] = 0.f;
-    float g = 0.f, r = 0.f;
-    int id = p.E;
-    if (lane < p.k) {
-      id = p.indices[row * p.k + lane];
-      if (id >= 0 && id < p.E) {
-        g = p.grad_weights[row * p.k + lane] * p.scaling;
-        r = score(logit(id));
-      } else {
-        id = p.E;
+    float m = kNone;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      v[i] = v[i] == v[i] ? v[i] : kNone;
+      m = fmaxf(m, v[i]);
+    }
+    const float lane_max = m;
+    float total = 1.f, delta = 0.f;
+    if (p.scoring == 0) {
+      m = redux_max(m);
+      if (need_total) {
+        total = 0.f;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+          if (v[i] > kNone) total += expf(v[i] - m);
+        total = warp_sum(total);
       }
     }
-    float dr = g;
-    if (p.renormalize) {
-      const float R = warp_sum(r);
-      dr = R > 0.f ? (g - warp_sum(g * (r / R))) / R : 0.f;
+    const float inv = 1.f / total;
+    auto score = [&](float x) -> float {
+      return p.scoring == 0 ? expf(x - m) * inv : 1.f / (1.f + expf(-x));
+    };
+    bool unsure = false;
+    float top = lane_max;
+    float group_value = kNone, magnitude = 0.f;
+    if (kBias || sums) {
+      float a = kNone, a2 = kNone;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        float x = kNone;
+        if (v[i] > kNone) {
+          x = score(v[i]) + (kBias ? b[i] : 0.f);
+          x = x == x ? x : kNone;
+        }
+        if (kBias) v[i] = x;
+        a2 = fmaxf(a2, fminf(a, x));
+        a = fmaxf(a, x);
+      }
+      if (kBias) top = a;
+      // score(m) = 1 / total is the largest softmax score
+      delta = p.scoring == 0 ? 6e-6f * inv : 4e-7f;
+      if (sums) {
+        group_value = a;
+        float second = a2;
+        for (int o = 1; o < lpg; ++o) {  // the other lanes of the group, in turn
+          const int from = g * lpg + (lane - g * lpg + o) % lpg;
+          const float oa = __shfl_sync(0xffffffffu, a, from & 31);
+          const float o2 = __shfl_sync(0xffffffffu, a2, from & 31);
+          second = fmaxf(fmaxf(second, o2), fminf(group_value, oa));
+          group_value = fmaxf(group_value, oa);
+        }
+        if (group_value > kNone) magnitude = fabsf(group_value);
+        if (second > kNone) {
+          magnitude = fmaxf(magnitude, fabsf(second));
+          group_value += second;
+        }
+      }
     }
-    const float D = p.scoring == 0 ? (p.renormalize ? 0.f : warp_sum(dr * r)) : 0.f;
-    __syncwarp();
-    for (int j = 0; j < p.k; ++j) {  // in slot order: one id twice adds up, always the same way
-      if (lane == j && id < p.E) ds[id] += dr;
+    if (kGroups) {
+      if (!sums) {
+        group_value = top;
+        for (int o = 1; o < lpg; ++o)
+          group_value = fmaxf(group_value, __shfl_sync(0xffffffffu, top,
+                                                       (g * lpg + (lane - g * lpg + o) % lpg) & 31));
+        magnitude = fabsf(group_value);
+      }
+      if (g >= p.num_groups) group_value = kNone;
+      // a group's place among the groups, and whether the 32-bit values may mislead about it
+      const bool exact = !kBias && !sums;
+      const float slack = exact ? -1.f : 4.f * delta + 5e-7f * magnitude;
+      int place = 0;
+      for (int o = 0; o < p.num_groups; ++o) {
+        const float ov = __shfl_sync(0xffffffffu, group_value, o * lpg);
+        place += ov > group_value || (ov == group_value && o < g);
+        unsure |= o != g && fabsf(ov - group_value) <= slack;
+      }
+      unsure = unsure && group_value > kNone;
+      if (!(place < p.topk_groups)) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) v[i] = kNone;
+        top = kNone;
+      }
+    }
+    // lower bound of the k-th largest key
+    float t = kNone, cur = top, best = kNone;
+    for (int j = 0; j < p.k; ++j) {
+      t = redux_max(cur);
+      if (j == 0) best = t;
+      if (!(t > kNone)) break;
+      cur = cur == t ? kNone : cur;
+    }
+    if (kBias) {
+      delta += 1.2e-7f * fmaxf(fabsf(best), t > kNone ? fabsf(t) : 0.f);
+      t -= 4.f * delta;
+    }
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) mine += v[i] >= t && v[i] > kNone;
+    int before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += up;
+    }
+    const int count = __shfl_sync(0xffffffffu, before, 31);
+    before -= mine;
+    float r = 0.f;
+    int id = p.E;
+    if (count <= kMaxCand) {
+      ck[lane] = kNone;
+      ck[lane + 32] = kNone;
       __syncwarp();
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        if (v[i] >= t && v[i] > kNone) {
+          ck[before] = v[i];
+          cid[before] = static_cast<uint16_t>(e0 + i);
+          ++before;
+        }
+      __syncwarp();
+      int place[2] = {0, 0};
+      const float key[2] = {ck[lane], ck[lane + 32]};
+      const int halves = count > 32 ? 2 : 1;
+      for (int i = 0; i < count; i += 4) {
+        const float4 o4 = *reinterpret_cast<const float4*>(ck + i);
+        const float o[4] = {o4.x, o4.y, o4.z, o4.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (h == halves) break;
+            const int at = lane + 32 * h;
+            place[h] += o[q] > key[h] || (o[q] == key[h] && i + q < at);
+            if (kBias && i + q != at && at < count && fabsf(o[q] - key[h]) <= 2.f * delta) {
+              // the same numbers tie for certain
+              const int x = cid[i + q], y = cid[at];
+              unsure |= Elem<T>::to_f(l[x]) != Elem<T>::to_f(l[y]) || p.bias[x] != p.bias[y];
+            }
+          }
+        }
+      }
+      __syncwarp();
+      // slot `place` takes this candidate: through shared memory to the lane of that slot
+      const int ids[2] = {lane < count ? cid[lane] : 0, lane + 32 < count ? cid[lane + 32] : 0};
+      __syncwarp();
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (lane + 32 * h < count && place[h] < p.k) cid[place[h]] = static_cast<uint16_t>(ids[h]);
+      __syncwarp();
+      if (lane < p.k && lane < count) {
+        id = cid[lane];
+        r = score(logit_of(l, id));
+      }
+    } else if (kBias) {
+      unsure = true;
+    } else {
+      // many equal keys: k warp argmax rounds
+      for (int j = 0; j < p.k; ++j) {
+        float x = kNone;
+        int at = 0;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+          if (v[i] > x) {
+            x = v[i];
+            at = i;
+          }
+        const float w = redux_max(x);
+        const int first = __ffs(__ballot_sync(0xffffffffu, x == w)) - 1;
+        const int pick = __shfl_sync(0xffffffffu, e0 + at, first);
+        if (lane == first) {
+#pragma unroll
+          for (int i = 0; i < VPT; ++i)
+            if (i == at) v[i] = kNone;
+        }
+        if (lane == j) {
+          id = pick;
+          r = score(logit_of(l, id));
+        }
+      }
     }
-    for (int e = lane; e < p.E; e += 32) {
-      const float s = score(logit(e));
-      const float d = p.scoring == 0 ? s * (ds[e] - D) : ds[e] * s * (1.f - s);
-      out[e] = Elem<T>::from_f(d);
+    if ((kBias || sums) && __any_sync(0xffffffffu, unsure))
+      route_row64<T>(p, row, smem_d + warp * row64_scratch(p.E), r, id);
+    store_row(p, row, r, id);
+    __syncwarp();
+  }
+}
+
+// One row per warp; the row is put together in shared memory (zero except at the picks) and leaves
+// in 16-byte stores.  kDense (softmax weights that are not renormalised): every expert has a
+// gradient, so the logits are read whole; else at most the picks' logits are, since
+//     softmax, renormalised:  dl_j = w_j (g_j - G),            G = sum_i g_i w_i / c
+//     sigmoid:                dl_j = w_j (g_j - G) (1 - s_j),  G = 0 unless renormalised
+// The kernel is bound by the T*E gradients it writes.
+template <typename T, bool kDense>
+__global__ void __launch_bounds__(kFastWarps * 32)
+    route_experts_backward_kernel(RouteExpertsBackwardParams p, int vec) {
+  extern __shared__ float smem_f[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kPer = 16 / sizeof(T);
+  const int pitch = (p.E + 7) & ~7;
+  float* ds = smem_f + warp * pitch;
+  for (int e = lane; e < pitch; e += 32) ds[e] = 0.f;
+  __syncwarp();
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kFastWarps;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kFastWarps + warp;
+  // the next row's picks are loaded while this row is written
+  float gn = 0.f, wn = 0.f;
+  int idn = -1;
+  auto load = [&](int64_t r) {
+    if (r < p.num_tokens && lane < p.k) {
+      gn = __ldcs(p.grad_weights + r * p.k + lane);
+      wn = __ldcs(p.weights + r * p.k + lane);
+      idn = __ldcs(p.indices + r * p.k + lane);
     }
+  };
+  load(row);
+  for (; row < p.num_tokens; row += stride) {
+    const T* l = static_cast<const T*>(p.logits) + row * p.stride;
+    T* out = static_cast<T*>(p.grad_logits) + row * p.E;
+    const bool ok = lane < p.k && idn >= 0 && idn < p.E;
+    const int id = ok ? idn : 0;
+    const float g = ok ? gn : 0.f, w = ok ? wn : 0.f;
+    load(row + stride);
+    const float gw = g * w;
+    float d = gw, D = 0.f;
+    if (kDense) {
+      D = warp_sum(gw);
+      d = g * p.scaling;
+    } else {
+      if (p.renormalize) d = w * (g - warp_sum(gw) / p.scaling);
+      if (p.scoring != 0 && ok) {
+        const float x = logit_of(l, id);
+        d *= 1.f / (1.f + expf(x));
+      }
+    }
+    // one id twice in a row adds up in slot order
+    const unsigned peers = __match_any_sync(0xffffffffu, ok ? id : -1 - lane);
+    const bool twice = ok && (peers & (peers - 1)) != 0;
+    if (!__any_sync(0xffffffffu, twice)) {
+      if (ok) ds[id] = d;
+    } else {
+      for (int j = 0; j < p.k; ++j) {
+        if (lane == j && ok) ds[id] += d;
+        __syncwarp();
+      }
+    }
+    __syncwarp();
+    if (kDense) {
+      float m = -CUDART_INF_F, total = 0.f;
+      for (int e = lane; e < p.E; e += 32) m = fmaxf(m, logit_of(l, e));
+      m = warp_max(m);
+      for (int e = lane; e < p.E; e += 32) {
+        const float x = logit_of(l, e);
+        if (x > -CUDART_INF_F) total += expf(x - m);
+      }
+      const float inv = 1.f / warp_sum(total);
+      for (int e = lane; e < p.E; e += 32) {
+        const float x = logit_of(l, e);
+        out[e] = Elem<T>::from_f(x > -CUDART_INF_F ? expf(x - m) * inv * (ds[e] - D) : 0.f);
+      }
+    } else if (vec) {
+      for (int e = lane * kPer; e < p.E; e += 32 * kPer) {
+        alignas(16) T q[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; i += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(ds + e + i);
+          q[i] = Elem<T>::from_f(f.x);
+          q[i + 1] = Elem<T>::from_f(f.y);
+          q[i + 2] = Elem<T>::from_f(f.z);
+          q[i + 3] = Elem<T>::from_f(f.w);
+        }
+        __stcs(reinterpret_cast<uint4*>(out + e), *reinterpret_cast<const uint4*>(q));
+      }
+    } else {
+      for (int e = lane; e < p.E; e += 32) out[e] = Elem<T>::from_f(ds[e]);
+    }
+    __syncwarp();
+    if (ok) ds[id] = 0.f;
     __syncwarp();
   }
 }
@@ -229,25 +551,79 @@ int blocks_for(int64_t rows, int num_sms) {
 
 }  // namespace
 
+namespace {
+
+template <typename T, int VPT>
+void launch_fast(const RouteExpertsParams& p, int bs, int lpg, int vec, int num_sms,
+                 cudaStream_t s) {
+  const int64_t blocks = (p.num_tokens + kFastWarps - 1) / kFastWarps;
+  const int64_t cap = static_cast<int64_t>(num_sms) * 8;  // 64 warps on an SM
+  const unsigned grid = static_cast<unsigned>(blocks < cap ? blocks : cap);
+  const bool groups = p.num_groups > 1;
+  const bool may64 = p.bias || (groups && p.group_score != 0);
+  const size_t smem = may64 ? sizeof(double) * kFastWarps * row64_scratch(p.E) : 0;
+  if (p.bias) {
+    if (groups)
+      route_experts_kernel<T, VPT, true, true><<<grid, kFastWarps * 32, smem, s>>>(p, bs, lpg, vec);
+    else
+      route_experts_kernel<T, VPT, true, false><<<grid, kFastWarps * 32, smem, s>>>(p, bs, lpg, vec);
+  } else {
+    if (groups)
+      route_experts_kernel<T, VPT, false, true><<<grid, kFastWarps * 32, smem, s>>>(p, bs, lpg, vec);
+    else
+      route_experts_kernel<T, VPT, false, false><<<grid, kFastWarps * 32, smem, s>>>(p, bs, lpg, vec);
+  }
+}
+
+template <typename T>
+void launch_route(const RouteExpertsParams& p, int num_sms, cudaStream_t s) {
+  const int lpg = 32 / p.num_groups;
+  const int per = p.E / p.num_groups;
+  const int bs = (per + lpg - 1) / lpg;
+  const int vec = (bs * sizeof(T)) % 16 == 0 && per % bs == 0 && (p.stride * sizeof(T)) % 16 == 0 &&
+                  (reinterpret_cast<uintptr_t>(p.logits) & 15u) == 0;
+  if (bs == 1) return launch_fast<T, 1>(p, bs, lpg, vec, num_sms, s);
+  if (bs == 2) return launch_fast<T, 2>(p, bs, lpg, vec, num_sms, s);
+  if (bs <= 4) return launch_fast<T, 4>(p, bs, lpg, vec, num_sms, s);
+  if (bs <= 8) return launch_fast<T, 8>(p, bs, lpg, vec, num_sms, s);
+  if (bs <= 16) return launch_fast<T, 16>(p, bs, lpg, vec, num_sms, s);
+  // groups so uneven to the lanes that a lane would hold more than 16 experts
+  const size_t smem = sizeof(double) * kWarps * row64_scratch(p.E);
+  route_experts64_kernel<T><<<blocks_for(p.num_tokens, num_sms), kWarps * 32, smem, s>>>(p);
+}
+
+}  // namespace
+
 int launch_route_experts(int dtype, const RouteExpertsParams& p, int num_sms, cudaStream_t s) {
   if (p.num_tokens <= 0) return 0;
-  const int grid = blocks_for(p.num_tokens, num_sms);
-  const size_t smem = sizeof(double) * kWarps * (2 * p.E + kRouteMaxGroups);
-  if (dtype == kF32) route_experts_kernel<float><<<grid, kWarps * 32, smem, s>>>(p);
-  else if (dtype == kBF16) route_experts_kernel<__nv_bfloat16><<<grid, kWarps * 32, smem, s>>>(p);
-  else route_experts_kernel<__half><<<grid, kWarps * 32, smem, s>>>(p);
+  if (dtype == kF32) launch_route<float>(p, num_sms, s);
+  else if (dtype == kBF16) launch_route<__nv_bfloat16>(p, num_sms, s);
+  else launch_route<__half>(p, num_sms, s);
   return 0;
 }
+
+namespace {
+template <typename T>
+void launch_backward(const RouteExpertsBackwardParams& p, int num_sms, cudaStream_t s) {
+  const int64_t blocks = (p.num_tokens + kFastWarps - 1) / kFastWarps;
+  const int64_t cap = static_cast<int64_t>(num_sms) * 8;
+  const unsigned grid = static_cast<unsigned>(blocks < cap ? blocks : cap);
+  const size_t smem = sizeof(float) * kFastWarps * ((p.E + 7) & ~7);
+  const int vec = (p.E * sizeof(T)) % 16 == 0 &&
+                  (reinterpret_cast<uintptr_t>(p.grad_logits) & 15u) == 0;
+  if (p.scoring == 0 && !p.renormalize)
+    route_experts_backward_kernel<T, true><<<grid, kFastWarps * 32, smem, s>>>(p, vec);
+  else
+    route_experts_backward_kernel<T, false><<<grid, kFastWarps * 32, smem, s>>>(p, vec);
+}
+}  // namespace
 
 int launch_route_experts_backward(int dtype, const RouteExpertsBackwardParams& p, int num_sms,
                                   cudaStream_t s) {
   if (p.num_tokens <= 0) return 0;
-  const int grid = blocks_for(p.num_tokens, num_sms);
-  const size_t smem = sizeof(float) * kWarps * p.E;
-  if (dtype == kF32) route_experts_backward_kernel<float><<<grid, kWarps * 32, smem, s>>>(p);
-  else if (dtype == kBF16)
-    route_experts_backward_kernel<__nv_bfloat16><<<grid, kWarps * 32, smem, s>>>(p);
-  else route_experts_backward_kernel<__half><<<grid, kWarps * 32, smem, s>>>(p);
+  if (dtype == kF32) launch_backward<float>(p, num_sms, s);
+  else if (dtype == kBF16) launch_backward<__nv_bfloat16>(p, num_sms, s);
+  else launch_backward<__half>(p, num_sms, s);
   return 0;
 }
 
