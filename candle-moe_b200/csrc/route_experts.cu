@@ -48,19 +48,6 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// Largest key of the warp's lanes and its id, ties to the lower id.
-__device__ __forceinline__ void warp_best(double& v, int& id) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const double ov = __shfl_xor_sync(0xffffffffu, v, o);
-    const int oi = __shfl_xor_sync(0xffffffffu, id, o);
-    if (ov > v || (ov == v && oi < id)) {
-      v = ov;
-      id = oi;
-    }
-  }
-}
-
 // NaN logits count as -inf.
 template <typename T> __device__ __forceinline__ float logit_of(const T* l, int e) {
   const float x = Elem<T>::to_f(l[e]);
@@ -68,103 +55,128 @@ template <typename T> __device__ __forceinline__ float logit_of(const T* l, int 
 }
 
 // Doubles of scratch per warp of route_row64.
-__host__ __device__ __forceinline__ int row64_scratch(int E) { return E + kRouteMaxGroups; }
+__host__ __device__ __forceinline__ int row64_scratch(int E) { return E; }
 
-// One row by one warp with 64-bit keys, any shape: key and value (the groups') in scratch.
-// Leaves the pick of slot `lane` (id E: none) and its score.
+// Order-preserving map of doubles (no NaN) to unsigned 64-bit keys above 0.
+__device__ __forceinline__ uint64_t order_key64(double v) {
+  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v + 0.0));  // -0 as +0
+  return (b >> 63) ? ~b : (b | (1ull << 63));
+}
+
+// One row by one warp with 64-bit keys, any shape; key: E doubles of scratch.  Leaves the pick of
+// slot `lane` (id E: none) and its score.  A launch waits for its slowest row, so this is
+// written for a short dependent chain (independent iterations unrolled, warp reductions on
+// integer keys) rather than for few instructions.
 template <typename T>
 __device__ __noinline__ void route_row64(const RouteExpertsParams& p, int64_t row, double* key,
                                          float& mine, int& mine_id) {
   const int lane = threadIdx.x & 31;
-  double* value = key + p.E;
-  const int per = p.E / p.num_groups;
   const T* l = static_cast<const T*>(p.logits) + row * p.stride;
   float m = -CUDART_INF_F;
-  for (int e = lane; e < p.E; e += 32) m = fmaxf(m, logit_of(l, e));
-  m = warp_max(m);
-  double total = 0.0;
+  double total = 1.0;
   if (p.scoring == 0) {
+#pragma unroll 4
+    for (int e = lane; e < p.E; e += 32) m = fmaxf(m, logit_of(l, e));
+    m = warp_max(m);
+    total = 0.0;
+#pragma unroll 4
     for (int e = lane; e < p.E; e += 32) {
       const float x = logit_of(l, e);
-      if (x > -CUDART_INF_F) total += exp(static_cast<double>(x) - static_cast<double>(m));
+      total += x > -CUDART_INF_F ? exp(static_cast<double>(x) - static_cast<double>(m)) : 0.0;
     }
     total = warp_sum(total);
   }
   auto score = [&](float x) -> double {
-    if (!(x > -CUDART_INF_F)) return 0.0;
     if (p.scoring == 0) return exp(static_cast<double>(x) - static_cast<double>(m)) / total;
     return 1.0 / (1.0 + exp(-static_cast<double>(x)));
   };
-  // keys; sums: of score + bias (for the groups' sums of two)
-  auto fill = [&](bool sums) {
+  const bool sums = p.num_groups > 1 && p.group_score != 0;
+  if (p.bias || sums) {
+#pragma unroll 4
     for (int e = lane; e < p.E; e += 32) {
       const float x = logit_of(l, e);
-      double k = -CUDART_INF;
-      if (x > -CUDART_INF_F) {
-        k = (p.bias || sums) ? score(x) + (p.bias ? static_cast<double>(p.bias[e]) : 0.0)
-                             : static_cast<double>(x);
-        if (!(k > -CUDART_INF)) k = -CUDART_INF;  // a bias of -inf or NaN shuts the expert off
-      }
-      key[e] = k;
+      const double k = score(x) + (p.bias ? static_cast<double>(p.bias[e]) : 0.0);
+      // a bias of -inf or NaN shuts the expert off
+      key[e] = (x > -CUDART_INF_F && k > -CUDART_INF) ? k : -CUDART_INF;
     }
-    __syncwarp();
-  };
+  } else {
+#pragma unroll 4
+    for (int e = lane; e < p.E; e += 32) key[e] = static_cast<double>(logit_of(l, e));
+  }
+  __syncwarp();
   unsigned open = 0xffffffffu;
+  const int per = p.E / p.num_groups;
   if (p.num_groups > 1) {
-    const bool top2 = p.group_score != 0;
-    fill(top2);
-    for (int g = lane; g < p.num_groups; g += 32) {
-      double a = -CUDART_INF, b = -CUDART_INF;
-      for (int i = 0; i < per; ++i) {
+    const int lpg = 32 / p.num_groups, g = lane / lpg, at = lane % lpg;
+    double a = -CUDART_INF, b = -CUDART_INF;
+    if (g < p.num_groups) {
+#pragma unroll 4
+      for (int i = at; i < per; i += lpg) {
         const double v = key[g * per + i];
-        if (v > a) {
-          b = a;
-          a = v;
-        } else if (v > b) {
-          b = v;
-        }
+        b = fmax(b, fmin(a, v));
+        a = fmax(a, v);
       }
-      value[g] = (!top2 || !(b > -CUDART_INF)) ? a : a + b;
     }
-    __syncwarp();
+    double ga = a, gb = b;
+    for (int o = 1; o < lpg; ++o) {
+      const int from = (g * lpg + (at + o) % lpg) & 31;
+      const double oa = __shfl_sync(0xffffffffu, a, from);
+      const double ob = __shfl_sync(0xffffffffu, b, from);
+      gb = fmax(fmax(gb, ob), fmin(ga, oa));
+      ga = fmax(ga, oa);
+    }
+    double value = sums && gb > -CUDART_INF ? ga + gb : ga;
+    if (g >= p.num_groups) value = -CUDART_INF;
+    int place = 0;
+#pragma unroll 4
+    for (int o = 0; o < p.num_groups; ++o) {
+      const double ov = __shfl_sync(0xffffffffu, value, o * lpg);
+      place += ov > value || (ov == value && o < g);
+    }
+    const unsigned lanes =
+        __ballot_sync(0xffffffffu, value > -CUDART_INF && place < p.topk_groups);
     open = 0;
-    for (int i = 0; i < p.topk_groups; ++i) {
-      double v = -CUDART_INF;
-      int id = 0x7fffffff;
-      if (lane < p.num_groups && !((open >> lane) & 1u)) {
-        v = value[lane];
-        id = lane;
+    for (int o = 0; o < p.num_groups; ++o) open |= ((lanes >> (o * lpg)) & 1u) << o;
+  }
+  // this lane's best key, and the next one whenever it is picked
+  const bool logits = !p.bias;
+  auto key_of = [&](int e) -> uint64_t {
+    if (p.num_groups > 1 && !((open >> (e / per)) & 1u)) return 0;
+    const double k = key[e];
+    if (!(k > -CUDART_INF)) return 0;
+    return order_key64(logits && sums ? static_cast<double>(logit_of(l, e)) : k);
+  };
+  uint64_t best = 0;
+  int id = 0;
+  auto find = [&]() {
+    best = 0;
+#pragma unroll 4
+    for (int e = lane; e < p.E; e += 32) {
+      const uint64_t k = key_of(e);
+      if (k > best) {
+        best = k;
+        id = e;
       }
-      warp_best(v, id);
-      if (!(v > -CUDART_INF)) break;
-      open |= 1u << id;
     }
-  }
-  fill(false);
-  if (p.num_groups > 1) {
-    for (int e = lane; e < p.E; e += 32)
-      if (!((open >> (e / per)) & 1u)) key[e] = -CUDART_INF;
-    __syncwarp();
-  }
+  };
+  find();
   mine = 0.f;
   mine_id = p.E;
   for (int j = 0; j < p.k; ++j) {
-    double v = -CUDART_INF;
-    int id = 0x7fffffff;
-    for (int e = lane; e < p.E; e += 32)
-      if (key[e] > v) {
-        v = key[e];
-        id = e;
-      }
-    warp_best(v, id);
-    if (!(v > -CUDART_INF)) break;
-    if (lane == j) {
-      mine = static_cast<float>(score(logit_of(l, id)));
-      mine_id = id;
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(best >> 32));
+    if (hi == 0) break;
+    const bool top = static_cast<uint32_t>(best >> 32) == hi;
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, top ? static_cast<uint32_t>(best) : 0u);
+    const unsigned pick = __reduce_min_sync(
+        0xffffffffu, top && static_cast<uint32_t>(best) == lo ? static_cast<unsigned>(id)
+                                                              : 0xffffffffu);
+    if (lane == j) mine_id = static_cast<int>(pick);
+    if (static_cast<int>(pick) % 32 == lane) {
+      key[pick] = -CUDART_INF;
+      find();
     }
-    if (id % 32 == lane) key[id] = -CUDART_INF;
-    __syncwarp();
   }
+  if (mine_id < p.E) mine = static_cast<float>(score(logit_of(l, mine_id)));
 }
 
 // Writes the row's k slots from the pick that each lane holds (slot `lane`).
@@ -449,6 +461,302 @@ __global__ void __launch_bounds__(kFastWarps * 32)
   }
 }
 
+// ---- several rows per warp, k <= 8 -------------------------------------------------------------
+
+__device__ __forceinline__ void order2(float& a, float& b) {  // a >= b
+  const float hi = fmaxf(a, b);
+  b = fminf(a, b);
+  a = hi;
+}
+
+// Descending sort of 8 (19 comparators) and of a bitonic sequence of 8.
+__device__ __forceinline__ void sort8(float (&x)[8]) {
+  order2(x[0], x[1]); order2(x[2], x[3]); order2(x[4], x[5]); order2(x[6], x[7]);
+  order2(x[0], x[2]); order2(x[1], x[3]); order2(x[4], x[6]); order2(x[5], x[7]);
+  order2(x[1], x[2]); order2(x[5], x[6]);
+  order2(x[0], x[4]); order2(x[1], x[5]); order2(x[2], x[6]); order2(x[3], x[7]);
+  order2(x[2], x[4]); order2(x[3], x[5]);
+  order2(x[1], x[2]); order2(x[3], x[4]); order2(x[5], x[6]);
+}
+__device__ __forceinline__ void sort_bitonic8(float (&x)[8]) {
+#pragma unroll
+  for (int d = 4; d > 0; d >>= 1)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if ((i & d) == 0) order2(x[i], x[i + d]);
+}
+
+constexpr int kRowCand = 16;  // candidates of a row
+constexpr int kRowWarps = 4;
+
+// LPR lanes per row, each with up to VPL experts in registers; k <= 8.
+//
+// As in the kernel above the picks come from a lower bound t of the k-th largest key and a
+// ranking of the keys at or above it, with less work per row: t is the k-th largest of the
+// maxima of small blocks (VPL / 8 experts of a lane), sorted by a network in each lane and merged
+// over the row's lanes.  With 32 blocks and k = 8 about ten keys reach t.  The work is
+// instructions, not bytes: a whole warp per row spent 560 warp instructions on a row of 128
+// experts.
+//
+// Expert i of a lane is base + (i / 4) * cs + i % 4: without groups the row's lanes take pieces of
+// four in turn (64 contiguous bytes of f32), with groups a lane holds one stretch of one group.
+// NaN needs no care where it is compared: it is never >= t nor > -inf.
+template <typename T, int LPR, int VPL, bool kBias>
+__global__ void __launch_bounds__(kRowWarps * 32)
+    route_experts_rows_kernel(RouteExpertsParams p, int bs, int lpg, int vec) {
+  extern __shared__ double smem_d[];
+  constexpr int RPW = 32 / LPR;
+  // (order-preserving key, ~id) of the candidates; then key and id by place
+  __shared__ alignas(16) uint64_t s_cand[kRowWarps][RPW][kRowCand];
+  __shared__ uint64_t s_rank[kRowWarps][RPW][kRowCand];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sub = lane / LPR, q = lane % LPR;
+  const float kNone = -CUDART_INF_F;
+  uint64_t* cand = s_cand[warp][sub];
+  uint64_t* ranked = s_rank[warp][sub];
+  const bool groups = p.num_groups > 1;
+  const int per = p.E / p.num_groups;
+  const int g = groups ? q / lpg : 0;
+  const int cs = groups ? 4 : 4 * LPR;
+  const int base = groups ? g * per + (q % lpg) * bs : 4 * q;
+  const int lim = groups ? min(bs, per - (q % lpg) * bs) : p.E - base;
+  const bool sums = groups && p.group_score != 0;
+  const bool need_total = p.scoring == 0 && (kBias || sums || !p.renormalize);
+  auto row_max = [&](float x) {
+#pragma unroll
+    for (int d = LPR / 2; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+    return x;
+  };
+  auto row_sum = [&](float x) {
+#pragma unroll
+    for (int d = LPR / 2; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    return x;
+  };
+  for (int64_t row0 = (static_cast<int64_t>(blockIdx.x) * kRowWarps + warp) * RPW;
+       row0 < p.num_tokens; row0 += static_cast<int64_t>(gridDim.x) * kRowWarps * RPW) {
+    const int64_t row = row0 + sub;
+    const bool live = row < p.num_tokens;
+    const T* l = static_cast<const T*>(p.logits) + (live ? row : row0) * p.stride;
+    float v[VPL];
+#pragma unroll
+    for (int c = 0; c < VPL / 4; ++c) {
+      if (vec) {  // every piece of four is whole and aligned
+        struct alignas(4 * sizeof(T)) Four { T x[4]; };
+        Four f;
+        const bool in = c * cs < lim;
+        if (in) f = *reinterpret_cast<const Four*>(l + base + c * cs);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[4 * c + i] = in ? Elem<T>::to_f(f.x[i]) : kNone;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v[4 * c + i] = c * cs + i < lim ? Elem<T>::to_f(l[base + c * cs + i]) : kNone;
+      }
+    }
+    float m = 0.f, inv = 1.f, delta = 0.f;
+    if (need_total) {
+      m = kNone;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) m = fmaxf(m, v[i]);
+      m = row_max(m);
+      float total = 0.f;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (v[i] > kNone) total += expf(v[i] - m);
+      inv = 1.f / row_sum(total);
+    }
+    bool unsure = false;
+    float a = kNone, a2 = kNone;  // the lane's two largest score + bias
+    if (kBias || sums) {
+      // fast exponentials and quotients: their errors are inside delta (a sigmoid's exponential is
+      // off by (2 + 1.16 |x|) ulp, times s (1 - s): under one ulp of 1)
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        const int off = (i / 4) * cs + i % 4;
+        float x = p.scoring == 0 ? __expf(v[i] - m) * inv : __fdividef(1.f, 1.f + __expf(-v[i]));
+        if (kBias && off < lim) x += __ldg(p.bias + base + off);
+        x = v[i] > kNone ? x : kNone;
+        if (kBias) v[i] = x;
+        if (sums) {
+          a2 = fmaxf(a2, fminf(a, x == x ? x : kNone));
+          a = fmaxf(a, x);
+        }
+      }
+      // score(m) = inv is the largest softmax score
+      delta = p.scoring == 0 ? 6e-6f * inv : 4e-7f;
+    }
+    // maxima of blocks
+    float top[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      constexpr int kBlock = VPL >= 8 ? VPL / 8 : 1;
+      top[j] = kNone;
+#pragma unroll
+      for (int i = 0; i < kBlock; ++i)
+        if (j * kBlock + i < VPL) top[j] = fmaxf(top[j], v[(j * kBlock + i) % VPL]);
+    }
+    sort8(top);
+    if (groups) {
+      float value, magnitude;
+      if (sums) {
+        for (int d = 1; d < lpg; d <<= 1) {
+          const float oa = __shfl_xor_sync(0xffffffffu, a, d);
+          const float o2 = __shfl_xor_sync(0xffffffffu, a2, d);
+          a2 = fmaxf(fmaxf(a2, o2), fminf(a, oa));
+          a = fmaxf(a, oa);
+        }
+        value = a2 > kNone ? a + a2 : a;
+        magnitude = fmaxf(fabsf(a), a2 > kNone ? fabsf(a2) : 0.f);
+      } else {
+        value = top[0];
+        for (int d = 1; d < lpg; d <<= 1)
+          value = fmaxf(value, __shfl_xor_sync(0xffffffffu, value, d));
+        magnitude = fabsf(value);
+      }
+      // a group's place among the groups, and whether the 32-bit values may mislead about it
+      const float slack = !kBias && !sums ? -1.f : 4.f * delta + 5e-7f * magnitude;
+      int place = 0;
+      for (int o = 0; o < p.num_groups; ++o) {
+        const float ov = __shfl_sync(0xffffffffu, value, o * lpg, LPR);
+        place += ov > value || (ov == value && o < g);
+        unsure |= o != g && fabsf(ov - value) <= slack;
+      }
+      unsure = unsure && value > kNone;
+      if (!(place < p.topk_groups)) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) v[i] = kNone;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top[j] = kNone;
+      }
+    }
+    // lower bound of the k-th largest key
+#pragma unroll
+    for (int d = 1; d < LPR; d <<= 1) {
+      float other[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) other[j] = __shfl_xor_sync(0xffffffffu, top[j], d);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top[j] = fmaxf(top[j], other[7 - j]);
+      sort_bitonic8(top);
+    }
+    float t = top[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) t = j < p.k ? top[j] : t;
+    if (kBias) {
+      delta += 1.2e-7f * fmaxf(fabsf(top[0]), t > kNone ? fabsf(t) : 0.f);
+      t -= 4.f * delta;
+    }
+    t = fmaxf(t, -3.402823466e38f);  // an unavailable expert is no candidate
+    // renormalised softmax weights need no common factor
+    if (p.scoring == 0 && !need_total) m = top[0];
+    // candidates, into the row's list
+    uint32_t mask = 0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (v[i] >= t) mask |= 1u << i;
+    const int mine = __popc(mask);
+    int before = mine;
+#pragma unroll
+    for (int d = 1; d < LPR; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, before, d, LPR);
+      if (q >= d) before += up;
+    }
+    const int count = __shfl_sync(0xffffffffu, before, LPR - 1, LPR);
+    before -= mine;
+#pragma unroll
+    for (int i = q; i < kRowCand; i += LPR) cand[i] = 0;
+    __syncwarp();
+    const bool fits = count <= kRowCand;
+    if (!fits) mask = 0;
+    unsure |= !fits;
+    while (mask) {
+      const int i = __ffs(mask) - 1;
+      mask &= mask - 1;
+      const int id = base + (i >> 2) * cs + (i & 3);
+      float x = Elem<T>::to_f(l[id]);
+      if (kBias) {
+        x = p.scoring == 0 ? __expf(x - m) * inv : __fdividef(1.f, 1.f + __expf(-x));
+        x += __ldg(p.bias + id);
+      }
+      const uint32_t b = __float_as_uint(x + 0.f);  // -0 as +0
+      const uint32_t key = (b >> 31) ? ~b : (b | 0x80000000u);
+      cand[before] = (static_cast<uint64_t>(key) << 32) | static_cast<uint32_t>(~id);
+      ++before;
+    }
+    __syncwarp();
+    // each lane ranks every LPR-th candidate: larger key first, then the lower id
+    const int most = min(__reduce_max_sync(0xffffffffu, count), kRowCand);
+#pragma unroll
+    for (int h = 0; h < kRowCand / LPR; ++h) {
+      if (h * LPR < most) {
+        const uint64_t x = cand[q + h * LPR];
+        int at = 0;
+        for (int j = 0; j < most; j += 2) {
+          const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(cand + j);
+          at += o.x > x;
+          at += o.y > x;
+        }
+        if (x) ranked[at] = x;
+      }
+    }
+    __syncwarp();
+    // each lane takes every LPR-th slot
+    constexpr int kSlots = (8 + LPR - 1) / LPR;
+    const int picks = fits ? min(count, p.k) : 0;
+    float r[kSlots], sum = 0.f;
+    int id[kSlots];
+#pragma unroll
+    for (int h = 0; h < kSlots; ++h) {
+      const int j = q + h * LPR;
+      r[h] = 0.f;
+      id[h] = p.E;
+      if (j < picks) {
+        const uint64_t c = ranked[j];
+        id[h] = static_cast<int>(~static_cast<uint32_t>(c));
+        const float x = Elem<T>::to_f(l[id[h]]);
+        r[h] = p.scoring == 0 ? expf(x - m) * inv : 1.f / (1.f + expf(-x));
+        sum += r[h];
+        if (kBias && j + 1 < count) {  // is the next one certainly behind?
+          const uint64_t n = ranked[j + 1];
+          const uint32_t k0 = static_cast<uint32_t>(c >> 32), k1 = static_cast<uint32_t>(n >> 32);
+          const float f0 = __uint_as_float((k0 >> 31) ? k0 & 0x7fffffffu : ~k0);
+          const float f1 = __uint_as_float((k1 >> 31) ? k1 & 0x7fffffffu : ~k1);
+          if (f0 - f1 <= 2.f * delta) {
+            const int o = static_cast<int>(~static_cast<uint32_t>(n));
+            // the same numbers tie for certain, but what follows the last slot may hide another
+            unsure |= j + 1 == p.k || x != Elem<T>::to_f(l[o]) || p.bias[id[h]] != p.bias[o];
+          }
+        }
+      }
+    }
+    float scale = p.scaling;
+    if (p.renormalize) {
+      sum = row_sum(sum);
+      scale = sum > 0.f ? p.scaling / sum : scale;
+    }
+    if (live) {
+#pragma unroll
+      for (int h = 0; h < kSlots; ++h)
+        if (q + h * LPR < p.k) {
+          p.weights[row * p.k + q + h * LPR] = r[h] * scale;
+          p.indices[row * p.k + q + h * LPR] = id[h];
+        }
+    }
+    // rows that 32 bits do not decide, or with many equal keys, one after the other
+    unsigned left = __ballot_sync(0xffffffffu, unsure && live);
+    while (left) {
+      const int s = (__ffs(left) - 1) / LPR;
+      left &= ~(((1u << LPR) - 1u) << (s * LPR));
+      float r1;
+      int id1;
+      route_row64<T>(p, row0 + s, smem_d + warp * row64_scratch(p.E), r1, id1);
+      store_row(p, row0 + s, r1, id1);
+      __syncwarp();
+    }
+    __syncwarp();
+  }
+}
+
 // One row per warp; the row is put together in shared memory (zero except at the picks) and leaves
 // in 16-byte stores.  kDense (softmax weights that are not renormalised): every expert has a
 // gradient, so the logits are read whole; else at most the picks' logits are, since
@@ -575,8 +883,42 @@ void launch_fast(const RouteExpertsParams& p, int bs, int lpg, int vec, int num_
   }
 }
 
+template <typename T, int LPR, int VPL>
+void launch_rows(const RouteExpertsParams& p, int bs, int lpg, int num_sms, cudaStream_t s) {
+  constexpr int rows = kRowWarps * (32 / LPR);
+  const int64_t blocks = (p.num_tokens + rows - 1) / rows, cap = static_cast<int64_t>(num_sms) * 16;
+  const unsigned grid = static_cast<unsigned>(blocks < cap ? blocks : cap);
+  const size_t smem = sizeof(double) * kRowWarps * row64_scratch(p.E);
+  const int per = p.E / p.num_groups;
+  const int vec = (p.num_groups > 1 ? bs % 4 == 0 && per % bs == 0 : p.E % 4 == 0) &&
+                  p.stride % 4 == 0 &&
+                  (reinterpret_cast<uintptr_t>(p.logits) & (4 * sizeof(T) - 1)) == 0;
+  if (p.bias)
+    route_experts_rows_kernel<T, LPR, VPL, true><<<grid, kRowWarps * 32, smem, s>>>(p, bs, lpg, vec);
+  else
+    route_experts_rows_kernel<T, LPR, VPL, false><<<grid, kRowWarps * 32, smem, s>>>(p, bs, lpg,
+                                                                                       vec);
+}
+
+// Whether the kernel of LPR lanes per row and 32 experts per lane can take p.
+template <typename T, int LPR>
+bool try_rows(const RouteExpertsParams& p, int num_sms, cudaStream_t s) {
+  if (LPR % p.num_groups != 0) return false;
+  const int lpg = LPR / p.num_groups, bs = (p.E / p.num_groups + lpg - 1) / lpg;
+  if (p.num_groups == 1 ? p.E > 32 * LPR : bs > 32) return false;
+  launch_rows<T, LPR, 32>(p, bs, lpg, num_sms, s);
+  return true;
+}
+
 template <typename T>
 void launch_route(const RouteExpertsParams& p, int num_sms, cudaStream_t s) {
+  if (p.k <= 8) {
+    if (p.num_groups == 1 && p.E <= 16) return launch_rows<T, 4, 4>(p, 4, 4, num_sms, s);
+    if (p.num_groups == 1 && p.E <= 64) return launch_rows<T, 4, 16>(p, 16, 4, num_sms, s);
+    if (try_rows<T, 4>(p, num_sms, s) || try_rows<T, 8>(p, num_sms, s) ||
+        try_rows<T, 16>(p, num_sms, s))
+      return;
+  }
   const int lpg = 32 / p.num_groups;
   const int per = p.E / p.num_groups;
   const int bs = (per + lpg - 1) / lpg;
