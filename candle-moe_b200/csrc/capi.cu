@@ -99,7 +99,8 @@ int init_device(int dev, DeviceState** out) {
     if (cudaMemset(d.err_word, 0, sizeof(uint32_t)) != cudaSuccess) return MOE_ERR_CUDA;
     const bool attrs_ok = route_prep_set_attributes() && sm100_set_attributes() &&
                           sm100_pair_set_attributes() && decode_set_attributes() &&
-                          router_project_set_attributes() && tf32x3_set_attributes();
+                          router_project_set_attributes() && tf32x3_set_attributes() &&
+                          int4_set_attributes();
     cudaGetLastError();  // attribute failures are reported here, not by a later call
     if (!attrs_ok) return MOE_ERR_CUDA;
     d.max_pairs = sm100_pair_max_clusters();
@@ -977,14 +978,6 @@ int int4_shape_status(int64_t E, int64_t K, int64_t N, int32_t G, uint32_t dtype
   return MOE_OK;
 }
 
-Int4Layout int4_layout(int64_t E, int64_t K, int64_t N, int32_t G, bool zeros) {
-  Int4Layout L;
-  L.scales = align256(static_cast<size_t>(E * K * N / 2));
-  L.zeros = L.scales + align256(static_cast<size_t>(E * (K / G) * N) * 2);
-  L.total = L.zeros + (zeros ? align256(static_cast<size_t>(E * (K / G) * N)) : 0);
-  return L;
-}
-
 struct Int4WsLayout {
   size_t offsets, chunk_prefix, sorted_token, sorted_flat, sorted_w, prep_scratch, inter, slots,
       total;
@@ -1019,7 +1012,8 @@ bool int4_expands(int64_t T, int H, int I, int E, int k) {
 CMOE_API size_t moe_int4_packed_size(int32_t num_experts, int32_t k_dim, int32_t n_dim,
                                      int32_t group_size, uint32_t dtype, int32_t has_zeros) {
   if (int4_shape_status(num_experts, k_dim, n_dim, group_size, dtype) != MOE_OK) return 0;
-  return int4_layout(num_experts, k_dim, n_dim, group_size, has_zeros != 0).total;
+  return static_cast<size_t>(num_experts) * (n_dim / 16) * (k_dim / 64) *
+         int4_record_bytes(group_size, has_zeros != 0);
 }
 
 CMOE_API int moe_int4_quantize(const void* weights, int32_t num_experts, int32_t k_dim,
@@ -1048,10 +1042,9 @@ CMOE_API int moe_int4_pack(const uint8_t* q, const void* scales, const uint8_t* 
   DeviceState* ds = nullptr;
   int st = current_device_state(&ds);
   if (st != MOE_OK) return st;
-  g_launches += launch_int4_pack(
-      static_cast<int>(dtype), q, scales, zeros, num_experts, k_dim, n_dim, group_size,
-      int4_layout(num_experts, k_dim, n_dim, group_size, zeros != nullptr), packed, ds->num_sms,
-      static_cast<cudaStream_t>(stream));
+  g_launches += launch_int4_pack(static_cast<int>(dtype), q, scales, zeros, num_experts, k_dim,
+                                 n_dim, group_size, packed, ds->num_sms,
+                                 static_cast<cudaStream_t>(stream));
   return finish(MOE_OK);
 }
 
@@ -1112,28 +1105,20 @@ CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const vo
   const int64_t rows = num_tokens * topk;
   const int chunk = int4_chunk_rows(rows, E);
   Int4Params g1 = {}, g2 = {};
-  const Int4Layout l1 = int4_layout(E, H, I, group_size, has_zeros != 0);
-  const Int4Layout l2 = int4_layout(E, I, H, group_size, has_zeros != 0);
-  auto matrix = [&](Int4Params& p, int m, const void* packed, const Int4Layout& l) {
-    const char* b = static_cast<const char*>(packed);
-    p.w[m] = b;
-    p.scale[m] = b + l.scales;
-    p.zero[m] = has_zeros ? reinterpret_cast<const uint8_t*>(b + l.zeros) : nullptr;
-  };
-  matrix(g1, 0, gate_packed, l1);
-  if (up_packed) matrix(g1, 1, up_packed, l1);
-  matrix(g2, 0, down_packed, l2);
+  g1.w[0] = gate_packed;
+  g1.w[1] = up_packed;
+  g2.w[0] = down_packed;
+  g1.zeros = g2.zeros = has_zeros != 0;
+  g1.rec = g2.rec = int4_record_bytes(group_size, has_zeros != 0);
   if (int4_expands(num_tokens, H, I, E, topk) && aligned16(output)) {
     // two-matrix experts: the grouped GEMMs read the second matrix as [E, H, I]
     const size_t size = align256(2 * static_cast<size_t>(E) * H * I);
     const int dt = static_cast<int>(dtype);
-    launch_int4_expand(dt, g1.w[0], g1.scale[0], g1.zero[0], E, H, I, group_size, false, ws, s);
+    launch_int4_expand(dt, gate_packed, E, H, I, group_size, g1.zeros, false, ws, s);
     if (up_packed)
-      launch_int4_expand(dt, g1.w[1], g1.scale[1], g1.zero[1], E, H, I, group_size, false,
-                         ws + size, s);
+      launch_int4_expand(dt, up_packed, E, H, I, group_size, g1.zeros, false, ws + size, s);
     char* down = ws + (up_packed ? 2 : 1) * size;
-    launch_int4_expand(dt, g2.w[0], g2.scale[0], g2.zero[0], E, I, H, group_size, !up_packed, down,
-                       s);
+    launch_int4_expand(dt, down_packed, E, I, H, group_size, g1.zeros, !up_packed, down, s);
     g_launches += up_packed ? 3 : 2;
     st = fused_impl(input, ws, up_packed ? ws + size : down, up_packed ? down : nullptr,
                     routing_weights, expert_indices, output, num_tokens, H, I, E, topk,
@@ -1174,10 +1159,10 @@ CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const vo
                         s) != 0)
     st = MOE_ERR_CUDA;
   if (st == MOE_OK) {
-    int64_t n = route_prep_scratch_bytes(rows, E) ? 3 : 1;
-    n += launch_int4_ffn(static_cast<int>(dtype), chunk, g1, g2, expert_indices, num_tokens, topk,
-                         output, ds->num_sms, s);
-    g_launches += n;
+    const int n = launch_int4_ffn(static_cast<int>(dtype), chunk, g1, g2, expert_indices,
+                                  num_tokens, topk, output, ds->num_sms, s);
+    if (n == 0) st = MOE_ERR_CUDA;
+    g_launches += n + (route_prep_scratch_bytes(rows, E) ? 3 : 1);
   }
   if (owned) cudaFreeAsync(ws, s);
   return finish(st);

@@ -164,14 +164,8 @@ int launch_decode_ffn(int dtype, int mode, int n, const CUtensorMap& a0, const C
                       const DecodeParams& p, int grid, cudaStream_t s);
 
 // ---- moe_int4.cu (Q: the expert FFN on 4-bit weights) -----------------------------------------
-// Byte offsets inside one packed matrix (the weights start at 0).
-struct Int4Layout {
-  size_t scales, zeros, total;
-};
 struct Int4Params {
   const void* w[2];             // packed weights: gate (and up, else null), or down
-  const void* scale[2];
-  const uint8_t* zero[2];       // null: zero point 8
   const void* x;                // first product: x [T, K]; second: intermediate [rows, K]
   void* out;                    // first: intermediate [rows, N]; second: f32 slots [T*k, N]
   const int32_t* offsets;       // [E+2]
@@ -180,17 +174,22 @@ struct Int4Params {
   const int32_t* sorted_flat;   // [rows]
   const float* sorted_w;        // [rows]
   int N, K, G, E, act;
+  int rec;                      // int4_record_bytes()
+  int wk;                       // set by the launch: pieces that the warps split K into
+  bool zeros;                   // else every zero point is 8
 };
+// Bytes of a packed record (16 columns x 64 k).
+int int4_record_bytes(int G, bool zeros);
+bool int4_set_attributes();
 int int4_chunk_rows(int64_t rows, int E);
 int launch_int4_quantize(int dtype, const void* w, int E, int K, int N, int G, int symmetric,
                          uint8_t* q, void* scales, uint8_t* zeros, int num_sms, cudaStream_t s);
-// Both return the number of kernels launched.
+// Both return the number of kernels launched (0: a launch failed).
 int launch_int4_pack(int dtype, const uint8_t* q, const void* scales, const uint8_t* zeros, int E,
-                     int K, int N, int G, const Int4Layout& L, void* packed, int num_sms,
-                     cudaStream_t s);
+                     int K, int N, int G, void* packed, int num_sms, cudaStream_t s);
 // out [E,K,N], or [E,N,K] with trans, in 16 bits; N a multiple of 128.
-void launch_int4_expand(int dtype, const void* w, const void* scale, const uint8_t* zero, int E,
-                        int K, int N, int G, bool trans, void* out, cudaStream_t s);
+void launch_int4_expand(int dtype, const void* w, int E, int K, int N, int G, bool zeros,
+                        bool trans, void* out, cudaStream_t s);
 int launch_int4_ffn(int dtype, int chunk_rows, const Int4Params& g1, const Int4Params& g2,
                     const uint32_t* idx, int64_t num_tokens, int k, void* out, int num_sms,
                     cudaStream_t s);

@@ -9,9 +9,10 @@ import candle_moe as cm
 
 def test_sizes():
     lib = cm.lib()
-    assert lib.moe_int4_packed_size(2, 128, 64, 64, 1, 0) == 2 * 128 * 64 // 2 + 2 * 2 * 64 * 2
-    assert lib.moe_int4_packed_size(2, 128, 64, 64, 1, 1) == \
-        2 * 128 * 64 // 2 + 2 * 2 * 64 * 2 + 256
+    # nibbles, scales and zero points of each 16 columns x 64 k
+    for G, per in ((32, 2), (64, 1), (128, 1)):
+        assert lib.moe_int4_packed_size(2, 128, 64, G, 1, 0) == 2 * 4 * 2 * (512 + 32 * per)
+        assert lib.moe_int4_packed_size(2, 128, 64, G, 1, 1) == 2 * 4 * 2 * (512 + 48 * per)
     for bad in [(0, 128, 64, 64, 1, 0), (2, 96, 64, 32, 1, 0), (2, 128, 72, 64, 1, 0),
                 (2, 128, 64, 48, 1, 0), (2, 64, 64, 128, 1, 0), (2, 128, 64, 64, 2, 0),
                 (2, 128, 64, 64, 5, 0)]:
