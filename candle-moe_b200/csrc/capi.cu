@@ -1108,6 +1108,7 @@ CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const vo
   g1.w[0] = gate_packed;
   g1.w[1] = up_packed;
   g2.w[0] = down_packed;
+  g1.err = g2.err = ds->err_word;
   g1.zeros = g2.zeros = has_zeros != 0;
   g1.rec = g2.rec = int4_record_bytes(group_size, has_zeros != 0);
   if (int4_expands(num_tokens, H, I, E, topk) && aligned16(output)) {

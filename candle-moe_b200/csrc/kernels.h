@@ -176,6 +176,7 @@ struct Int4Params {
   int N, K, G, E, act;
   int rec;                      // int4_record_bytes()
   int wk;                       // set by the launch: pieces that the warps split K into
+  uint32_t* err;                // device error word
   bool zeros;                   // else every zero point is 8
 };
 // Bytes of a packed record (16 columns x 64 k).

@@ -232,15 +232,21 @@ __global__ void __launch_bounds__(256)
 constexpr int kWarps = 8;
 constexpr int kMaxRecord = 608;  // int4_record_bytes(32, true)
 constexpr int kStageBlocks = 2;  // k64 blocks of a ring stage
+constexpr int kRing = 4;         // stages of a ring
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ void cp_async_commit() {
   asm volatile("cp.async.commit_group;" ::: "memory");
 }
 template <int N> __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
 }
 
 // Expert of chunk c: the number of experts whose chunks all come before it.
@@ -253,228 +259,408 @@ __device__ __forceinline__ int find_expert(const int32_t* __restrict__ prefix, i
   return e;
 }
 
-// A unit is (chunk of at most 8 NT rows of one expert, WN strips of 16 output columns); the warps
-// of a CTA are WN strips x WK pieces of K, and the CTA takes every gridDim-th unit.  A warp
-// streams the records of its piece through a ring of its own in shared memory (16-byte cp.async,
-// kStages - 1 stages ahead, across units), so no warp waits for another except to add up the
-// WK partial sums of a unit.  MATS = 2: gate and up.  kDown: rows are sorted rows of the
-// intermediate, the result is weighted and goes to the (token, slot) row of the f32 slot
-// buffer; else rows are tokens and the activation is applied.
-template <typename T, int MATS, bool kDown, int NT, bool kG32>
-__global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 2 : 1) int4_gemm_kernel(Int4Params p) {
+// A warp's stream of weight records: for every unit of the CTA the records [b0, b1) of one column
+// strip (of MATS matrices), through a ring of kRing stages of kStageBlocks records in shared
+// memory.  One lane issues bulk copies that signal a barrier per stage; the ring runs ahead
+// across units, so memory stays busy while a unit is finished.
+template <int MATS>
+struct WeightRing {
+  const Int4Params& p;
+  char* ring;
+  uint32_t bars;
+  volatile int* abort_flag;
+  int lane, b0, b1, nstages, nunits, stride, wn;  // wn: this warp's strip of a unit
+  int64_t units, unit, strip;
+  int stage_in = 0, slot_in = 0, slot = 0;
+  uint32_t phase = 0;
+
+  __device__ __forceinline__ int stage_bytes() const { return MATS * kStageBlocks * p.rec; }
+
+  __device__ __forceinline__ void locate() {
+    if (unit >= units) return;
+    const int ntiles = p.N / 16;
+    const int c = static_cast<int>(unit / nunits);
+    // a strip past the last one repeats it, and its results are dropped
+    const int nt = min(static_cast<int>(unit % nunits) * stride + wn, ntiles - 1);
+    strip = (static_cast<int64_t>(find_expert(p.chunk_prefix, p.E, c)) * ntiles + nt) * (p.K / 64);
+  }
+  __device__ __forceinline__ void issue() {
+    if (unit >= units) return;
+    const int b = b0 + stage_in * kStageBlocks;
+    const uint32_t bytes = max(min(kStageBlocks, b1 - b), 0) * p.rec;
+    if (lane == 0) {
+      const uint32_t bar = bars + 8 * slot_in;
+      mbar_arrive_expect_tx(bar, MATS * bytes);
+      if (bytes) {
+        const uint32_t dst = smem_addr(ring) + slot_in * stage_bytes();
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+          bulk_load(dst + m * kStageBlocks * p.rec,
+                    static_cast<const char*>(p.w[m]) + (strip + b) * p.rec, bytes, bar);
+      }
+    }
+    if (++stage_in == nstages) {
+      stage_in = 0;
+      unit += gridDim.x;
+      locate();
+    }
+    slot_in = (slot_in + 1) & (kRing - 1);
+  }
+  // The stage's records, or whatever is there once a wait has run out (the error word is set).
+  __device__ __forceinline__ const char* wait() {
+    mbar_wait_bounded(bars + 8 * slot, phase, abort_flag, p.err, kErrWaitFull);
+    return ring + slot * stage_bytes();
+  }
+  // After a wait that ran out: no copy may land once the CTA is gone (each wait again bounded).
+  __device__ __forceinline__ void drain() {
+    if (!*abort_flag) return;
+    const unsigned long long t0 = globaltimer_ns();
+    for (int i = 0; i < kRing; ++i)
+      while (!mbar_try_wait(bars + 8 * i, i < slot ? phase : phase ^ 1u))
+        if (globaltimer_ns() - t0 > kWaitLimitNs) break;
+  }
+  __device__ __forceinline__ void release() {
+    __syncwarp();
+    slot = (slot + 1) & (kRing - 1);
+    phase ^= slot == 0;
+  }
+};
+
+// q + 16 of the two columns' zero points (24 without).
+__device__ __forceinline__ void zero_points(const char* record, int per, int h, int gid, bool zeros,
+                                            float& z0, float& z1) {
+  z0 = z1 = 24.f;
+  if (zeros) {
+    const uint32_t z = *reinterpret_cast<const uint16_t*>(record + 512 + 32 * per + 16 * h + 2 * gid);
+    z0 = 16.f + static_cast<float>(z & 0xffu);
+    z1 = 16.f + static_cast<float>(z >> 8);
+  }
+}
+
+// Chunks of at most 8 rows.  A unit is (chunk, WN strips of 16 output columns); the CTA's warps are
+// WN strips x WK pieces of K, so that one token's experts spread over the GPU, and nothing but
+// the sum of a unit's WK partial results makes a warp wait for another.  The activations come
+// straight from L1 / L2: a step's two vectors per lane, loaded before the wait for the weights.
+// Rows past the chunk's repeat its last one (columns of the product do not mix).  MATS = 2: gate
+// and up.  kDown: rows are sorted rows of the intermediate, the result is weighted and goes to
+// the (token, slot) row of the f32 slot buffer; else rows are tokens and the activation is
+// applied.
+template <typename T, int MATS, bool kDown, bool kG32>
+__global__ void __launch_bounds__(kWarps * 32, 2) int4_few_kernel(Int4Params p) {
   using T2 = typename Pair<T>::type;
-  constexpr int kStages = MATS == 2 ? 4 : 6;
-  constexpr int kRows = 8 * NT, kPitch = 20;  // partial sums [row][16 + 4]
+  constexpr int kPitch = 20;  // partial sums [row][16 + 4]
   constexpr int kPer = kG32 ? 2 : 1;
-  constexpr bool kOnes = NT == 1;
-  extern __shared__ __align__(16) char smem[];
+  extern __shared__ __align__(128) char smem[];
+  __shared__ alignas(8) uint64_t s_bar[kWarps][kRing];
+  __shared__ int s_abort;
   float* red = reinterpret_cast<float*>(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, tig = lane & 3;
-  const int rec = p.rec;
-  const int stage_bytes = MATS * kStageBlocks * rec;
-  char* ring = smem + kWarps * MATS * kRows * kPitch * 4 + warp * kStages * stage_bytes;
-  const uint32_t ring_addr = smem_addr(ring);
-  const int wk = warp % p.wk, wn = warp / p.wk, wn_count = kWarps / p.wk;
-  const int ntiles = p.N / 16, kb = p.K / 64;
-  const int nunits = (ntiles + wn_count - 1) / wn_count;
-  const int per = (kb + p.wk - 1) / p.wk;
-  const int b0 = min(wk * per, kb), b1 = min(b0 + per, kb);
-  const int nstages = (per + kStageBlocks - 1) / kStageBlocks;
+  const int wk = warp % p.wk, wn_count = kWarps / p.wk;
+  const int kb = p.K / 64, ntiles = p.N / 16, per = (kb + p.wk - 1) / p.wk;
+  if (lane == 0)
+    for (int i = 0; i < kRing; ++i) mbar_init(smem_addr(&s_bar[warp][i]), 1);
+  if (threadIdx.x == 0) s_abort = 0;
+  fence_barrier_init();
+  __syncthreads();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int nunits = (ntiles + wn_count - 1) / wn_count;
   const int64_t units = static_cast<int64_t>(__ldg(p.chunk_prefix + p.E)) * nunits;
-
-  // the ring's producer side: unit pu, stage ps
-  int64_t pu = blockIdx.x;
-  int ps = 0, slot_in = 0;
-  int64_t strip = 0;  // first record of the strip
-  auto locate = [&]() {
-    if (pu < units) {
-      const int c = static_cast<int>(pu / nunits);
-      const int nt = static_cast<int>(pu % nunits) * wn_count + wn;
-      strip = nt < ntiles
-                  ? (static_cast<int64_t>(find_expert(p.chunk_prefix, p.E, c)) * ntiles + nt) * kb
-                  : -1;
-    }
-  };
-  auto issue = [&]() {
-    if (pu < units) {
-      const int b = b0 + ps * kStageBlocks;
-      if (strip >= 0 && b < b1) {
-        const int n16 = min(kStageBlocks, b1 - b) * rec / 16;
+  WeightRing<MATS> w{p, smem + kWarps * MATS * 8 * kPitch * 4 + warp * kRing * MATS * kStageBlocks * p.rec,
+                     smem_addr(&s_bar[warp][0]), &s_abort, lane, min(wk * per, kb),
+                     min(wk * per + per, kb), (per + kStageBlocks - 1) / kStageBlocks, nunits,
+                     wn_count, warp / p.wk, units, blockIdx.x, 0};
+  w.locate();
 #pragma unroll
-        for (int m = 0; m < MATS; ++m) {
-          const char* src = static_cast<const char*>(p.w[m]) + (strip + b) * rec;
-          const uint32_t dst = ring_addr + slot_in * stage_bytes + m * kStageBlocks * rec;
-          for (int i = lane; i < n16; i += 32) cp_async16(dst + i * 16, src + i * 16);
-        }
-      }
-      if (++ps == nstages) {
-        ps = 0;
-        pu += gridDim.x;
-        locate();
-      }
-    }
-    cp_async_commit();
-    slot_in = slot_in + 1 == kStages ? 0 : slot_in + 1;
-  };
-  locate();
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) issue();
+  for (int i = 0; i < kRing - 1; ++i) w.issue();
 
-  int slot = 0;
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const int c = static_cast<int>(u / nunits);
-    const int nt = static_cast<int>(u % nunits) * wn_count + wn;
     const int e = find_expert(p.chunk_prefix, p.E, c);
-    const int row0 = __ldg(p.offsets + e) + (c - __ldg(p.chunk_prefix + e)) * kRows;
-    const int rows = min(kRows, __ldg(p.offsets + e + 1) - row0);
-    const T* xr[NT];
+    const int row0 = __ldg(p.offsets + e) + (c - __ldg(p.chunk_prefix + e)) * 8;
+    const int rows = min(8, __ldg(p.offsets + e + 1) - row0);
+    const int r = row0 + min(gid, rows - 1);
+    const T* xr = static_cast<const T*>(p.x) +
+                  static_cast<int64_t>(kDown ? r : __ldg(p.sorted_token + r)) * p.K + 8 * tig;
+    float fin[MATS][4] = {};
+    for (int st = 0; st < w.nstages; ++st) {
+      const int b = w.b0 + st * kStageBlocks;
+      uint4 xv[kStageBlocks][2];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int r = 8 * j + gid;
-      xr[j] = nullptr;
-      if (r < rows)
-        xr[j] = static_cast<const T*>(p.x) +
-                static_cast<int64_t>(kDown ? row0 + r : __ldg(p.sorted_token + row0 + r)) * p.K +
-                8 * tig;
-    }
-    const int tiles = (rows + 7) / 8;
-    float fin[MATS][NT][4] = {};
-    for (int st = 0; st < nstages; ++st) {
-      const int b = b0 + st * kStageBlocks;
-      const int blocks = nt < ntiles ? min(kStageBlocks, b1 - b) : 0;
-      uint4 xv[kStageBlocks][NT][2];
-      if (NT == 1) {  // few enough registers to have them under way before the wait
-#pragma unroll
-        for (int i = 0; i < kStageBlocks; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            xv[i][0][h] = make_uint4(0, 0, 0, 0);
-            if (i < blocks && xr[0])
-              xv[i][0][h] = *reinterpret_cast<const uint4*>(xr[0] + 64 * (b + i) + 32 * h);
-          }
-      }
-      cp_async_wait<kStages - 2>();
-      __syncwarp();
-      const char* stage = ring + slot * stage_bytes;
+      for (int i = 0; i < kStageBlocks; ++i)
+        if (b + i < w.b1) {
+          xv[i][0] = *reinterpret_cast<const uint4*>(xr + 64 * (b + i));
+          xv[i][1] = *reinterpret_cast<const uint4*>(xr + 64 * (b + i) + 32);
+        }
+      const char* stage = w.wait();
 #pragma unroll
       for (int i = 0; i < kStageBlocks; ++i) {
-        if (i >= blocks) break;
-        if (NT > 1) {
+        if (b + i >= w.b1) break;
+        float xs[kPer][4] = {};  // sums of the activations over the group
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              xv[i][j][h] = make_uint4(0, 0, 0, 0);
-              if (j < tiles && xr[j])
-                xv[i][j][h] = *reinterpret_cast<const uint4*>(xr[j] + 64 * (b + i) + 32 * h);
-            }
-        }
-        float xs[kPer][4] = {};
-        if (kOnes) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint4 v = xv[i][0][h];
-            mma16816<T>(xs[h & (kPer - 1)], Nib<T>::kOne, Nib<T>::kOne, Nib<T>::kOne, Nib<T>::kOne,
-                        v.x, v.y);
-            mma16816<T>(xs[h & (kPer - 1)], Nib<T>::kOne, Nib<T>::kOne, Nib<T>::kOne, Nib<T>::kOne,
-                        v.z, v.w);
-          }
+        for (int h = 0; h < 2; ++h) {
+          constexpr uint32_t one = Nib<T>::kOne;
+          mma16816<T>(xs[h & (kPer - 1)], one, one, one, one, xv[i][h].x, xv[i][h].y);
+          mma16816<T>(xs[h & (kPer - 1)], one, one, one, one, xv[i][h].z, xv[i][h].w);
         }
 #pragma unroll
         for (int m = 0; m < MATS; ++m) {
-          const char* record = stage + (m * kStageBlocks + i) * rec;
+          const char* record = stage + (m * kStageBlocks + i) * p.rec;
           const uint4 wq = *(reinterpret_cast<const uint4*>(record) + lane);
           const uint32_t word[4] = {wq.x, wq.y, wq.z, wq.w};
-          float acc[NT][4];
+          float acc[kPer][4] = {};
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
-            const int hg = (s >> 1) & (kPer - 1);
-            float z0 = 24.f, z1 = 24.f;
-            if (p.zeros) {
-              const uint8_t* zp =
-                  reinterpret_cast<const uint8_t*>(record + 512 + 32 * kPer + 16 * hg) + 2 * gid;
-              z0 = 16.f + static_cast<float>(zp[0]);
-              z1 = 16.f + static_cast<float>(zp[1]);
-            }
-            uint32_t a[4];
+            const uint4 v = xv[i][s >> 1];
+            mma16816<T>(acc[(s >> 1) & (kPer - 1)], nib_pair<T>(word[s], 0), nib_pair<T>(word[s], 1),
+                        nib_pair<T>(word[s], 2), nib_pair<T>(word[s], 3), (s & 1) ? v.z : v.x,
+                        (s & 1) ? v.w : v.y);
+          }
 #pragma unroll
-            for (int f = 0; f < 4; ++f) {
-              a[f] = nib_pair<T>(word[s], f);
-              if (!kOnes) {  // q - z, exact
-                T2 off;
-                off.x = off.y = Elem<T>::from_f((f & 1) ? z1 : z0);
-                const T2 v = __hsub2(*reinterpret_cast<const T2*>(&a[f]), off);
-                a[f] = *reinterpret_cast<const uint32_t*>(&v);
-              }
-            }
-            const bool first = s == 0 || (kG32 && s == 2), last = s == 3 || (kG32 && s == 1);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              if (NT > 1 && j >= tiles) break;
-              if (first) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-              const uint4 v = xv[i][j][s >> 1];
-              mma16816<T>(acc[j], a[0], a[1], a[2], a[3], (s & 1) ? v.z : v.x, (s & 1) ? v.w : v.y);
-            }
-            if (last) {
-              const T2 sc = *(reinterpret_cast<const T2*>(record + 512 + 32 * hg) + gid);
-              const float s0 = Elem<T>::to_f(sc.x), s1 = Elem<T>::to_f(sc.y);
-#pragma unroll
-              for (int j = 0; j < NT; ++j) {
-                if (NT > 1 && j >= tiles) break;
-                if (kOnes) {
-                  acc[j][0] -= z0 * xs[hg][0];
-                  acc[j][1] -= z0 * xs[hg][1];
-                  acc[j][2] -= z1 * xs[hg][0];
-                  acc[j][3] -= z1 * xs[hg][1];
-                }
-                fin[m][j][0] += s0 * acc[j][0];
-                fin[m][j][1] += s0 * acc[j][1];
-                fin[m][j][2] += s1 * acc[j][2];
-                fin[m][j][3] += s1 * acc[j][3];
-              }
-            }
+          for (int h = 0; h < kPer; ++h) {
+            float z0, z1;
+            zero_points(record, kPer, h, gid, p.zeros, z0, z1);
+            const T2 sc = *(reinterpret_cast<const T2*>(record + 512 + 32 * h) + gid);
+            const float s0 = Elem<T>::to_f(sc.x), s1 = Elem<T>::to_f(sc.y);
+            fin[m][0] += s0 * (acc[h][0] - z0 * xs[h][0]);
+            fin[m][1] += s0 * (acc[h][1] - z0 * xs[h][1]);
+            fin[m][2] += s1 * (acc[h][2] - z1 * xs[h][0]);
+            fin[m][3] += s1 * (acc[h][3] - z1 * xs[h][1]);
           }
         }
       }
-      __syncwarp();
-      issue();
-      slot = slot + 1 == kStages ? 0 : slot + 1;
+      w.release();
+      w.issue();
     }
 #pragma unroll
     for (int m = 0; m < MATS; ++m)
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          red[((warp * MATS + m) * kRows + 8 * j + 2 * tig + (i & 1)) * kPitch + gid +
-              8 * (i >> 1)] = fin[m][j][i];
+      for (int i = 0; i < 4; ++i)
+        red[((warp * MATS + m) * 8 + 2 * tig + (i & 1)) * kPitch + gid + 8 * (i >> 1)] = fin[m][i];
     __syncthreads();
     for (int i = threadIdx.x; i < wn_count * rows * 16; i += kWarps * 32) {
-      const int n = i & 15, r = (i >> 4) % rows, w = (i >> 4) / rows;
-      const int col = (static_cast<int>(u % nunits) * wn_count + w) * 16 + n;
+      const int n = i & 15, at = (i >> 4) % rows, strip = (i >> 4) / rows;
+      const int col = (static_cast<int>(u % nunits) * wn_count + strip) * 16 + n;
       if (col >= p.N) continue;
       float v = 0.f, v1 = 0.f;
       for (int q = 0; q < p.wk; ++q) {  // in the order of k
-        const float* from = red + ((w * p.wk + q) * MATS * kRows + r) * kPitch + n;
+        const float* from = red + ((strip * p.wk + q) * MATS * 8 + at) * kPitch + n;
         v += from[0];
-        if (MATS == 2) v1 += from[kRows * kPitch];
+        if (MATS == 2) v1 += from[8 * kPitch];
       }
       if (kDown) {
-        static_cast<float*>(p.out)[static_cast<int64_t>(__ldg(p.sorted_flat + row0 + r)) * p.N +
-                                   col] = v * __ldg(p.sorted_w + row0 + r);
+        static_cast<float*>(p.out)[static_cast<int64_t>(__ldg(p.sorted_flat + row0 + at)) * p.N +
+                                   col] = v * __ldg(p.sorted_w + row0 + at);
       } else {
         v = act_apply(v, p.act);
         if (MATS == 2) v *= v1;
         // the intermediate is rounded to the 16-bit type that the second product reads
-        static_cast<T*>(p.out)[static_cast<int64_t>(row0 + r) * p.N + col] = Elem<T>::from_f(v);
+        static_cast<T*>(p.out)[static_cast<int64_t>(row0 + at) * p.N + col] = Elem<T>::from_f(v);
       }
     }
     __syncthreads();
   }
+  w.drain();
+}
+
+// Chunks of 8 NT rows.  A unit is (chunk, 8 strips of 16 output columns), a strip per warp over all
+// of K; the activations are staged in shared memory, 128 k at a time, for all eight warps
+// (cp.async, kXRing - 1 stages ahead across units), whose rows are 320 bytes apart so that a
+// fragment load meets no bank twice.  q - z is made in registers (exact) and the scale acts on
+// the f32 sums of 32 k.  Bound by the tensor cores' mma.sync rate (2 cycles an SM for 16 x 8 x
+// 16, a quarter of the tcgen05 rate): a record costs 8 cycles per 8 rows, and 24 cycles of
+// memory time.
+constexpr int kXRing = 3;
+constexpr int kXPitch = 320;
+
+template <typename T, int MATS, bool kDown, int NT>
+__global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) int4_some_kernel(Int4Params p) {
+  using T2 = typename Pair<T>::type;
+  constexpr int kRows = 8 * NT;
+  constexpr int kXBytes = kRows * kXPitch;
+  constexpr int kLoads = kRows * 16 / (kWarps * 32);  // 16-byte pieces per thread and stage
+  constexpr int kPitch = 20;
+  extern __shared__ __align__(128) char smem[];
+  __shared__ alignas(8) uint64_t s_bar[kWarps][kRing];
+  __shared__ alignas(16) float s_out[kWarps][MATS][8][kPitch];
+  __shared__ int s_abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int gid = lane >> 2, tig = lane & 3;
+  const int kb = p.K / 64, ntiles = p.N / 16, rec_per = p.G == 32 ? 2 : 1;
+  if (lane == 0)
+    for (int i = 0; i < kRing; ++i) mbar_init(smem_addr(&s_bar[warp][i]), 1);
+  if (threadIdx.x == 0) s_abort = 0;
+  fence_barrier_init();
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int nunits = (ntiles + kWarps - 1) / kWarps;
+  const int64_t units = static_cast<int64_t>(__ldg(p.chunk_prefix + p.E)) * nunits;
+  WeightRing<MATS> w{p, smem + kXRing * kXBytes + warp * kRing * MATS * kStageBlocks * p.rec,
+                     smem_addr(&s_bar[warp][0]), &s_abort, lane, 0, kb,
+                     (kb + kStageBlocks - 1) / kStageBlocks, nunits, kWarps, warp, units,
+                     blockIdx.x, 0};
+  auto chunk_rows = [&](int64_t u, int& row0, int& rows) {
+    const int c = static_cast<int>(u / nunits);
+    const int e = find_expert(p.chunk_prefix, p.E, c);
+    row0 = __ldg(p.offsets + e) + (c - __ldg(p.chunk_prefix + e)) * kRows;
+    rows = min(kRows, __ldg(p.offsets + e + 1) - row0);
+  };
+  // the activations' producer side; a thread copies piece threadIdx.x % 16 of every 16th row
+  int64_t xu = blockIdx.x;
+  int xs_stage = 0, xs_slot = 0;
+  const T* xp[kLoads];
+  auto x_locate = [&]() {
+    if (xu >= units) return;
+    int row0, rows;
+    chunk_rows(xu, row0, rows);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int at = threadIdx.x / 16 + 16 * i;
+      const int r = row0 + min(at, rows - 1);
+      xp[i] = at < (rows + 7) / 8 * 8
+                  ? static_cast<const T*>(p.x) +
+                        static_cast<int64_t>(kDown ? r : __ldg(p.sorted_token + r)) * p.K
+                  : nullptr;
+    }
+  };
+  auto x_issue = [&]() {
+    if (xu < units) {
+      const int k = xs_stage * 128 + (threadIdx.x % 16) * 8;
+      if (k < p.K) {
+        const uint32_t dst = smem_addr(smem) + xs_slot * kXBytes + (threadIdx.x / 16) * kXPitch +
+                             (threadIdx.x % 16) * 16;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+          if (xp[i]) cp_async16(dst + 16 * i * kXPitch, xp[i] + k);
+      }
+      if (++xs_stage == w.nstages) {
+        xs_stage = 0;
+        xu += gridDim.x;
+        x_locate();
+      }
+    }
+    cp_async_commit();
+    xs_slot = xs_slot + 1 == kXRing ? 0 : xs_slot + 1;
+  };
+  w.locate();
+  x_locate();
+#pragma unroll
+  for (int i = 0; i < kRing - 1; ++i) w.issue();
+#pragma unroll
+  for (int i = 0; i < kXRing - 1; ++i) x_issue();
+  int x_slot = 0;
+
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    int row0, rows;
+    chunk_rows(u, row0, rows);
+    const int tiles = (rows + 7) / 8;
+    float fin[MATS][NT][4] = {};
+    for (int st = 0; st < w.nstages; ++st) {
+      cp_async_wait<kXRing - 2>();
+      __syncthreads();  // the stage is there for all, and all are done with the one before
+      x_issue();
+      const char* stage = w.wait();
+      const char* xst = smem + x_slot * kXBytes + gid * kXPitch + 16 * tig;
+#pragma unroll
+      for (int i = 0; i < kStageBlocks; ++i) {
+        if (st * kStageBlocks + i >= kb) break;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint4 xv[NT];
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+            if (j < tiles)
+              xv[j] = *reinterpret_cast<const uint4*>(xst + 8 * j * kXPitch + 128 * i + 64 * h);
+#pragma unroll
+          for (int m = 0; m < MATS; ++m) {
+            const char* record = stage + (m * kStageBlocks + i) * p.rec;
+            const uint2 wq = *reinterpret_cast<const uint2*>(record + 16 * lane + 8 * h);
+            const int hg = h & (rec_per - 1);
+            float z0, z1;
+            zero_points(record, rec_per, hg, gid, p.zeros, z0, z1);
+            T2 off[2];
+            off[0].x = off[0].y = Elem<T>::from_f(z0);
+            off[1].x = off[1].y = Elem<T>::from_f(z1);
+            uint32_t a[2][4];
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+              for (int f = 0; f < 4; ++f) {
+                const uint32_t v = nib_pair<T>(s ? wq.y : wq.x, f);
+                const T2 d = __hsub2(*reinterpret_cast<const T2*>(&v), off[f & 1]);
+                a[s][f] = *reinterpret_cast<const uint32_t*>(&d);
+              }
+            const T2 sc = *(reinterpret_cast<const T2*>(record + 512 + 32 * hg) + gid);
+            const float s0 = Elem<T>::to_f(sc.x), s1 = Elem<T>::to_f(sc.y);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              if (j < tiles) {
+                float acc[4] = {};
+                mma16816<T>(acc, a[0][0], a[0][1], a[0][2], a[0][3], xv[j].x, xv[j].y);
+                mma16816<T>(acc, a[1][0], a[1][1], a[1][2], a[1][3], xv[j].z, xv[j].w);
+                fin[m][j][0] += s0 * acc[0];
+                fin[m][j][1] += s0 * acc[1];
+                fin[m][j][2] += s1 * acc[2];
+                fin[m][j][3] += s1 * acc[3];
+              }
+            }
+          }
+        }
+      }
+      w.release();
+      w.issue();
+      x_slot = x_slot + 1 == kXRing ? 0 : x_slot + 1;
+    }
+    // out, 8 rows at a time: a lane takes 4 columns of one row
+    const int nt = static_cast<int>(u % nunits) * kWarps + warp;
+    const int at = lane >> 2, n4 = (lane & 3) * 4;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      if (j < tiles) {
+        __syncwarp();
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            s_out[warp][m][2 * tig + (i & 1)][gid + 8 * (i >> 1)] = fin[m][j][i];
+        __syncwarp();
+        const int r = 8 * j + at;
+        if (r < rows && nt < ntiles) {
+          float4 v = *reinterpret_cast<const float4*>(&s_out[warp][0][at][n4]);
+          if (kDown) {
+            const float wt = __ldg(p.sorted_w + row0 + r);
+            v.x *= wt;
+            v.y *= wt;
+            v.z *= wt;
+            v.w *= wt;
+            *reinterpret_cast<float4*>(static_cast<float*>(p.out) +
+                                       static_cast<int64_t>(__ldg(p.sorted_flat + row0 + r)) * p.N +
+                                       nt * 16 + n4) = v;
+          } else {
+            v.x = act_apply(v.x, p.act);
+            v.y = act_apply(v.y, p.act);
+            v.z = act_apply(v.z, p.act);
+            v.w = act_apply(v.w, p.act);
+            if (MATS == 2) {
+              const float4 g = *reinterpret_cast<const float4*>(&s_out[warp][MATS - 1][at][n4]);
+              v.x *= g.x;
+              v.y *= g.y;
+              v.z *= g.z;
+              v.w *= g.w;
+            }
+            // the intermediate is rounded to the 16-bit type that the second product reads
+            *reinterpret_cast<uint2*>(static_cast<T*>(p.out) +
+                                      static_cast<int64_t>(row0 + r) * p.N + nt * 16 + n4) =
+                make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+          }
+        }
+      }
+    }
+  }
   cp_async_wait<0>();
+  w.drain();
 }
 
 // out[t] = sum over the token's slots in slot order, one rounding.
@@ -523,55 +709,66 @@ int pieces_of(int K) {
   return wk;
 }
 
-template <typename T, int MATS, bool kDown, int NT, bool kG32>
-struct Gemm {
-  static constexpr auto kernel = int4_gemm_kernel<T, MATS, kDown, NT, kG32>;
+template <typename T, int MATS, bool kDown, bool kG32>
+struct Few {
+  static constexpr auto kernel = int4_few_kernel<T, MATS, kDown, kG32>;
   static size_t smem(int rec) {
-    return static_cast<size_t>(kWarps) *
-           (MATS * 8 * NT * 20 * 4 + (MATS == 2 ? 4 : 6) * MATS * kStageBlocks * rec);
-  }
-  static bool attributes() {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                static_cast<int>(smem(kMaxRecord))) == cudaSuccess;
+    return static_cast<size_t>(kWarps) * MATS * (8 * 20 * 4 + kRing * kStageBlocks * rec);
   }
   static bool launch(Int4Params p, int num_sms, cudaStream_t s) {
     p.wk = pieces_of(p.K);
-    // resident CTAs: two on an SM where registers and shared memory allow (227 KB, 1 KB a CTA)
-    const size_t bytes = smem(p.rec);
-    const int per_sm = NT <= 2 && 2 * (bytes + 1024) <= 227 * 1024 ? 2 : 1;
-    return launch_dependent(kernel, num_sms * per_sm, kWarps * 32, bytes, s, p);
+    // two CTAs on an SM: 2 x (10 + 76 KB) at most
+    return launch_dependent(kernel, num_sms * 2, kWarps * 32, smem(p.rec), s, p);
   }
 };
 
-template <typename T, int NT, bool kG32>
-bool launch_gemms(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
-  const bool ok = g1.w[1] ? Gemm<T, 2, false, NT, kG32>::launch(g1, num_sms, s)
-                          : Gemm<T, 1, false, NT, kG32>::launch(g1, num_sms, s);
-  return ok && Gemm<T, 1, true, NT, kG32>::launch(g2, num_sms, s);
+template <typename T, int MATS, bool kDown, int NT>
+struct Some {
+  static constexpr auto kernel = int4_some_kernel<T, MATS, kDown, NT>;
+  static size_t smem(int rec) {
+    return static_cast<size_t>(kXRing) * 8 * NT * kXPitch +
+           static_cast<size_t>(kWarps) * MATS * kRing * kStageBlocks * rec;
+  }
+  static bool launch(Int4Params p, int num_sms, cudaStream_t s) {
+    // two CTAs on an SM where the registers allow: 2 x (30 + 76 KB + 10 KB static) at most
+    return launch_dependent(kernel, num_sms * (NT <= 4 ? 2 : 1), kWarps * 32, smem(p.rec), s, p);
+  }
+};
+
+template <typename K> bool allow_smem() {
+  return cudaFuncSetAttribute(K::kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              static_cast<int>(K::smem(kMaxRecord))) == cudaSuccess;
 }
 
-template <typename T, int NT, bool kG32> bool gemm_attributes() {
-  return Gemm<T, 2, false, NT, kG32>::attributes() && Gemm<T, 1, false, NT, kG32>::attributes() &&
-         Gemm<T, 1, true, NT, kG32>::attributes();
-}
 template <typename T> bool gemm_attributes() {
-  return gemm_attributes<T, 1, false>() && gemm_attributes<T, 2, false>() &&
-         gemm_attributes<T, 4, false>() && gemm_attributes<T, 1, true>() &&
-         gemm_attributes<T, 2, true>() && gemm_attributes<T, 4, true>();
+  return allow_smem<Few<T, 2, false, false>>() && allow_smem<Few<T, 2, false, true>>() &&
+         allow_smem<Few<T, 1, false, false>>() && allow_smem<Few<T, 1, false, true>>() &&
+         allow_smem<Few<T, 1, true, false>>() && allow_smem<Few<T, 1, true, true>>() &&
+         allow_smem<Some<T, 2, false, 4>>() && allow_smem<Some<T, 2, false, 8>>() &&
+         allow_smem<Some<T, 1, false, 4>>() && allow_smem<Some<T, 1, false, 8>>() &&
+         allow_smem<Some<T, 1, true, 4>>() && allow_smem<Some<T, 1, true, 8>>();
+}
+
+template <typename T, bool kG32>
+bool launch_few(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
+  return (g1.w[1] ? Few<T, 2, false, kG32>::launch(g1, num_sms, s)
+                  : Few<T, 1, false, kG32>::launch(g1, num_sms, s)) &&
+         Few<T, 1, true, kG32>::launch(g2, num_sms, s);
+}
+template <typename T, int NT>
+bool launch_some(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
+  return (g1.w[1] ? Some<T, 2, false, NT>::launch(g1, num_sms, s)
+                  : Some<T, 1, false, NT>::launch(g1, num_sms, s)) &&
+         Some<T, 1, true, NT>::launch(g2, num_sms, s);
 }
 
 template <typename T>
-bool launch_ffn(int nt, const Int4Params& g1, const Int4Params& g2, const uint32_t* idx,
+bool launch_ffn(int chunk, const Int4Params& g1, const Int4Params& g2, const uint32_t* idx,
                 int64_t T_, int k, void* out, int num_sms, cudaStream_t s) {
-  bool ok;
-  if (g1.G == 32)
-    ok = nt == 1   ? launch_gemms<T, 1, true>(g1, g2, num_sms, s)
-         : nt == 2 ? launch_gemms<T, 2, true>(g1, g2, num_sms, s)
-                   : launch_gemms<T, 4, true>(g1, g2, num_sms, s);
-  else
-    ok = nt == 1   ? launch_gemms<T, 1, false>(g1, g2, num_sms, s)
-         : nt == 2 ? launch_gemms<T, 2, false>(g1, g2, num_sms, s)
-                   : launch_gemms<T, 4, false>(g1, g2, num_sms, s);
+  const bool ok = chunk == 8    ? (g1.G == 32 ? launch_few<T, true>(g1, g2, num_sms, s)
+                                              : launch_few<T, false>(g1, g2, num_sms, s))
+                  : chunk == 32 ? launch_some<T, 4>(g1, g2, num_sms, s)
+                                : launch_some<T, 8>(g1, g2, num_sms, s);
   return ok && launch_dependent(int4_combine_kernel<T>, grid_for(T_ * g2.N, num_sms), 256, 0, s,
                                 static_cast<const float*>(g2.out), idx, T_, k, g2.N, g2.E,
                                 static_cast<T*>(out));
@@ -604,7 +801,7 @@ void launch_int4_expand(int dtype, const void* w, int E, int K, int N, int G, bo
 
 int int4_chunk_rows(int64_t rows, int E) {
   const int64_t per = rows / E;
-  return per <= 6 ? 8 : per <= 12 ? 16 : 32;
+  return per <= 4 ? 8 : per <= 24 ? 32 : 64;
 }
 
 int launch_int4_quantize(int dtype, const void* w, int E, int K, int N, int G, int symmetric,
@@ -638,8 +835,8 @@ int launch_int4_ffn(int dtype, int chunk_rows, const Int4Params& g1, const Int4P
                     cudaStream_t s) {
   const bool ok =
       dtype == kBF16
-          ? launch_ffn<__nv_bfloat16>(chunk_rows / 8, g1, g2, idx, num_tokens, k, out, num_sms, s)
-          : launch_ffn<__half>(chunk_rows / 8, g1, g2, idx, num_tokens, k, out, num_sms, s);
+          ? launch_ffn<__nv_bfloat16>(chunk_rows, g1, g2, idx, num_tokens, k, out, num_sms, s)
+          : launch_ffn<__half>(chunk_rows, g1, g2, idx, num_tokens, k, out, num_sms, s);
   return ok ? 3 : 0;
 }
 
