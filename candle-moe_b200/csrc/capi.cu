@@ -975,6 +975,7 @@ int int4_shape_status(int64_t E, int64_t K, int64_t N, int32_t G, uint32_t dtype
   if (G != 32 && G != 64 && G != 128) return MOE_ERR_INVALID_ARG;
   if (K % G != 0) return MOE_ERR_INVALID_ARG;
   if (dtype == kF32 || K % 64 != 0 || N % 64 != 0) return MOE_ERR_UNSUPPORTED;
+  if (K > 1 << 20 || N > 1 << 20) return MOE_ERR_UNSUPPORTED;  // units are counted in 32 bits
   return MOE_OK;
 }
 
@@ -1151,6 +1152,18 @@ CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const vo
   g2.G = group_size;
   g2.E = E;
   g2.act = activation_type;
+  if (rows <= int4_table_rows()) {
+    g1.idx = g2.idx = expert_indices;
+    g1.rows = g2.rows = static_cast<int>(rows);
+    g1.k = g2.k = topk;
+    g2.sorted_w = routing_weights;
+    g2.out = output;
+    const int n = launch_int4_table_ffn(static_cast<int>(dtype), g1, g2, ds->num_sms, s);
+    if (n == 0) st = MOE_ERR_CUDA;
+    g_launches += n;
+    if (owned) cudaFreeAsync(ws, s);
+    return finish(st);
+  }
   if (launch_route_prep(expert_indices, routing_weights, num_tokens, topk, E, chunk,
                         reinterpret_cast<int32_t*>(ws + L.offsets),
                         reinterpret_cast<int32_t*>(ws + L.chunk_prefix),

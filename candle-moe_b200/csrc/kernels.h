@@ -178,7 +178,15 @@ struct Int4Params {
   int wk;                       // set by the launch: pieces that the warps split K into
   uint32_t* err;                // device error word
   bool zeros;                   // else every zero point is 8
+  // calls of at most int4_table_rows() rows (no route preparation; sorted_w: the [T, k] weights,
+  // out of the second product: the output [T, N])
+  const uint32_t* idx;          // [T, k]
+  int rows, k;                  // T*k, k
 };
+int int4_table_rows();
+// Both products of such a call; returns the number of kernels launched (0: a launch failed).
+int launch_int4_table_ffn(int dtype, const Int4Params& g1, const Int4Params& g2, int num_sms,
+                          cudaStream_t s);
 // Bytes of a packed record (16 columns x 64 k).
 int int4_record_bytes(int G, bool zeros);
 bool int4_set_attributes();

@@ -74,6 +74,31 @@ __device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The same with a zero accumulator.
+template <typename T>
+__device__ __forceinline__ void mma16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816_zero<__nv_bfloat16>(float (&d)[4], uint32_t a0,
+                                                             uint32_t a1, uint32_t a2, uint32_t a3,
+                                                             uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+template <>
+__device__ __forceinline__ void mma16816_zero<__half>(float (&d)[4], uint32_t a0, uint32_t a1,
+                                                      uint32_t a2, uint32_t a3, uint32_t b0,
+                                                      uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 // ---- quantisation and packing (once per set of weights) --------------------------------------
 
 // One thread per (expert, group, column): min / max over the group's k, then the nibbles.
@@ -259,57 +284,36 @@ __device__ __forceinline__ int find_expert(const int32_t* __restrict__ prefix, i
   return e;
 }
 
-// A warp's stream of weight records: for every unit of the CTA the records [b0, b1) of one column
-// strip (of MATS matrices), through a ring of kRing stages of kStageBlocks records in shared
-// memory.  One lane issues bulk copies that signal a barrier per stage; the ring runs ahead
-// across units, so memory stays busy while a unit is finished.
+// A warp's ring of kRing stages in shared memory, a stage holding `blocks` records of each of MATS
+// matrices.  One lane issues bulk copies that signal a barrier per stage, so a warp waits for no
+// other one, and the ring runs ahead across units of work: memory stays busy while a unit is
+// finished.
 template <int MATS>
 struct WeightRing {
-  const Int4Params& p;
   char* ring;
-  uint32_t bars;
+  uint32_t bars;  // kRing barriers
   volatile int* abort_flag;
-  int lane, b0, b1, nstages, nunits, stride, wn;  // wn: this warp's strip of a unit
-  int64_t units, unit, strip;
-  int stage_in = 0, slot_in = 0, slot = 0;
+  uint32_t* err;
+  int lane, matrix_bytes;  // of a stage, per matrix
+  int slot_in = 0, slot = 0;
   uint32_t phase = 0;
 
-  __device__ __forceinline__ int stage_bytes() const { return MATS * kStageBlocks * p.rec; }
-
-  __device__ __forceinline__ void locate() {
-    if (unit >= units) return;
-    const int ntiles = p.N / 16;
-    const int c = static_cast<int>(unit / nunits);
-    // a strip past the last one repeats it, and its results are dropped
-    const int nt = min(static_cast<int>(unit % nunits) * stride + wn, ntiles - 1);
-    strip = (static_cast<int64_t>(find_expert(p.chunk_prefix, p.E, c)) * ntiles + nt) * (p.K / 64);
-  }
-  __device__ __forceinline__ void issue() {
-    if (unit >= units) return;
-    const int b = b0 + stage_in * kStageBlocks;
-    const uint32_t bytes = max(min(kStageBlocks, b1 - b), 0) * p.rec;
+  __device__ __forceinline__ void issue(const char* src0, const char* src1, uint32_t bytes) {
     if (lane == 0) {
       const uint32_t bar = bars + 8 * slot_in;
       mbar_arrive_expect_tx(bar, MATS * bytes);
       if (bytes) {
-        const uint32_t dst = smem_addr(ring) + slot_in * stage_bytes();
-#pragma unroll
-        for (int m = 0; m < MATS; ++m)
-          bulk_load(dst + m * kStageBlocks * p.rec,
-                    static_cast<const char*>(p.w[m]) + (strip + b) * p.rec, bytes, bar);
+        const uint32_t dst = smem_addr(ring) + slot_in * MATS * matrix_bytes;
+        bulk_load(dst, src0, bytes, bar);
+        if (MATS == 2) bulk_load(dst + matrix_bytes, src1, bytes, bar);
       }
-    }
-    if (++stage_in == nstages) {
-      stage_in = 0;
-      unit += gridDim.x;
-      locate();
     }
     slot_in = (slot_in + 1) & (kRing - 1);
   }
   // The stage's records, or whatever is there once a wait has run out (the error word is set).
   __device__ __forceinline__ const char* wait() {
-    mbar_wait_bounded(bars + 8 * slot, phase, abort_flag, p.err, kErrWaitFull);
-    return ring + slot * stage_bytes();
+    mbar_wait_bounded(bars + 8 * slot, phase, abort_flag, err, kErrWaitFull);
+    return ring + slot * MATS * matrix_bytes;
   }
   // After a wait that ran out: no copy may land once the CTA is gone (each wait again bounded).
   __device__ __forceinline__ void drain() {
@@ -337,117 +341,234 @@ __device__ __forceinline__ void zero_points(const char* record, int per, int h, 
   }
 }
 
+// One k64 block of at most 8 rows: fin += the products of MATS records with the activations xv
+// (two vectors of 32 k).  With the weights as 16 + q the sum of the activations is needed as
+// well; the tensor cores, which have the time, make it.
+template <typename T, int MATS, bool kG32>
+__device__ __forceinline__ void few_block(const char* stage, int matrix_bytes, bool zeros, int lane,
+                                          const uint4 (&xv)[2], float (&fin)[MATS][4]) {
+  using T2 = typename Pair<T>::type;
+  constexpr int kPer = kG32 ? 2 : 1;
+  constexpr uint32_t one = Nib<T>::kOne;
+  const int gid = lane >> 2;
+  float xs[kPer][4];
+  mma16816_zero<T>(xs[0], one, one, one, one, xv[0].x, xv[0].y);
+  mma16816<T>(xs[0], one, one, one, one, xv[0].z, xv[0].w);
+  if (kG32) mma16816_zero<T>(xs[kPer - 1], one, one, one, one, xv[1].x, xv[1].y);
+  else mma16816<T>(xs[0], one, one, one, one, xv[1].x, xv[1].y);
+  mma16816<T>(xs[kPer - 1], one, one, one, one, xv[1].z, xv[1].w);
+#pragma unroll
+  for (int m = 0; m < MATS; ++m) {
+    const char* record = stage + m * matrix_bytes;
+    const uint4 wq = *(reinterpret_cast<const uint4*>(record) + lane);
+    const uint32_t word[4] = {wq.x, wq.y, wq.z, wq.w};
+    float acc[kPer][4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const uint4 v = xv[s >> 1];
+      const uint32_t b0 = (s & 1) ? v.z : v.x, b1 = (s & 1) ? v.w : v.y;
+      const uint32_t a0 = nib_pair<T>(word[s], 0), a1 = nib_pair<T>(word[s], 1),
+                     a2 = nib_pair<T>(word[s], 2), a3 = nib_pair<T>(word[s], 3);
+      if (s == 0 || (kG32 && s == 2))
+        mma16816_zero<T>(acc[(s >> 1) & (kPer - 1)], a0, a1, a2, a3, b0, b1);
+      else
+        mma16816<T>(acc[(s >> 1) & (kPer - 1)], a0, a1, a2, a3, b0, b1);
+    }
+#pragma unroll
+    for (int h = 0; h < kPer; ++h) {
+      float z0, z1;
+      zero_points(record, kPer, h, gid, zeros, z0, z1);
+      const T2 sc = *(reinterpret_cast<const T2*>(record + 512 + 32 * h) + gid);
+      const float s0 = Elem<T>::to_f(sc.x), s1 = Elem<T>::to_f(sc.y);
+      fin[m][0] += s0 * (acc[h][0] - z0 * xs[h][0]);
+      fin[m][1] += s0 * (acc[h][1] - z0 * xs[h][1]);
+      fin[m][2] += s1 * (acc[h][2] - z1 * xs[h][0]);
+      fin[m][3] += s1 * (acc[h][3] - z1 * xs[h][1]);
+    }
+  }
+}
+
+constexpr int kFewPitch = 20;  // floats of a row of 16 partial sums
+
+__device__ __forceinline__ void store_partial(float* to, int lane, const float (&fin)[4]) {
+  const int gid = lane >> 2, tig = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    to[(2 * tig + (i & 1)) * kFewPitch + gid + 8 * (i >> 1)] = fin[i];
+}
+
+__device__ __forceinline__ void init_rings(uint64_t (&bar)[kWarps][kRing], int* abort_flag) {
+  if ((threadIdx.x & 31) == 0)
+    for (int i = 0; i < kRing; ++i) mbar_init(smem_addr(&bar[threadIdx.x >> 5][i]), 1);
+  if (threadIdx.x == 0) *abort_flag = 0;
+  fence_barrier_init();
+  __syncthreads();
+}
+
+// Calls of at most kTableRows rows need no route preparation: every CTA sorts the rows by expert
+// itself (stable, as the route preparation does).
+constexpr int kTableRows = 64;
+struct RowTable {
+  int row[kTableRows];               // flat row t*k + j of each sorted position
+  int place[kTableRows];             // sorted position of each flat row, -1: id >= E
+  int chunk_of[kTableRows];          // chunk of each sorted position
+  int first[kTableRows + 1];         // first position of each chunk of at most 8 rows
+  int expert[kTableRows];            // expert of each chunk
+  int chunks;
+  uint32_t id[kTableRows];           // scratch
+  unsigned starts[kTableRows / 32];  // scratch
+
+  __device__ __forceinline__ void build(const uint32_t* __restrict__ idx, int n, int E) {
+    const int i = threadIdx.x;
+    uint32_t e = 0xffffffffu;
+    if (i < kTableRows) {
+      if (i < n) e = __ldg(idx + i);
+      if (e >= static_cast<uint32_t>(E)) e = 0xffffffffu;
+      id[i] = e;
+    }
+    __syncthreads();
+    int before = 0, same = 0, valid = 0;
+    if (i < kTableRows) {
+      for (int j = 0; j < n; ++j) {
+        const uint32_t o = id[j];
+        before += o < e || (o == e && j < i);
+        same += o == e && j < i;
+        valid += o != 0xffffffffu;
+      }
+      place[i] = e != 0xffffffffu ? before : -1;
+      if (e != 0xffffffffu) {
+        row[before] = i;
+        chunk_of[before] = same % 8 == 0;  // a chunk starts here
+      } else if (before < kTableRows) {
+        // positions past the valid rows (invalid ids sort last, in order)
+        if (i < n) chunk_of[before] = 0;
+      }
+      if (i >= n) chunk_of[i] = 0;
+    }
+    __syncthreads();
+    bool start = false;
+    if (i < kTableRows) {
+      start = chunk_of[i] != 0 && i < valid;
+      const unsigned b = __ballot_sync(0xffffffffu, start);
+      if ((i & 31) == 0) starts[i >> 5] = b;
+    }
+    __syncthreads();
+    if (i < kTableRows) {
+      const unsigned upto = starts[i >> 5] & (0xffffffffu >> (31 - (i & 31)));
+      const int c = __popc(upto) + (i >= 32 ? __popc(starts[0]) : 0) - 1;
+      chunk_of[i] = c;
+      if (start) {
+        first[c] = i;
+        expert[c] = static_cast<int>(id[row[i]]);
+      }
+      if (i == 0) {
+        chunks = __popc(starts[0]) + __popc(starts[1]);
+        first[chunks] = valid;
+      }
+    }
+    __syncthreads();
+  }
+};
+
 // Chunks of at most 8 rows.  A unit is (chunk, WN strips of 16 output columns); the CTA's warps are
 // WN strips x WK pieces of K, so that one token's experts spread over the GPU, and nothing but
 // the sum of a unit's WK partial results makes a warp wait for another.  The activations come
-// straight from L1 / L2: a step's two vectors per lane, loaded before the wait for the weights.
-// Rows past the chunk's repeat its last one (columns of the product do not mix).  MATS = 2: gate
-// and up.  kDown: rows are sorted rows of the intermediate, the result is weighted and goes to
-// the (token, slot) row of the f32 slot buffer; else rows are tokens and the activation is
-// applied.
-template <typename T, int MATS, bool kDown, bool kG32>
-__global__ void __launch_bounds__(kWarps * 32, 2) int4_few_kernel(Int4Params p) {
-  using T2 = typename Pair<T>::type;
-  constexpr int kPitch = 20;  // partial sums [row][16 + 4]
-  constexpr int kPer = kG32 ? 2 : 1;
+// straight from L1 / L2, a block ahead.  Rows past the chunk's repeat its last one (columns of
+// the product do not mix).  MATS = 2: gate and up.  kDown: rows are sorted rows of the
+// intermediate, the result is weighted and goes to the (token, slot) row of the f32 slot
+// buffer; else rows are tokens and the activation is applied.  kTable: the rows are sorted here.
+template <typename T, int MATS, bool kDown, bool kG32, bool kTable>
+__global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) {
   extern __shared__ __align__(128) char smem[];
   __shared__ alignas(8) uint64_t s_bar[kWarps][kRing];
   __shared__ int s_abort;
+  __shared__ RowTable s_table[1];
+  RowTable& table = s_table[0];
   float* red = reinterpret_cast<float*>(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, tig = lane & 3;
-  const int wk = warp % p.wk, wn_count = kWarps / p.wk;
+  const int wk = warp % p.wk, wn = warp / p.wk, wn_count = kWarps / p.wk;
   const int kb = p.K / 64, ntiles = p.N / 16, per = (kb + p.wk - 1) / p.wk;
-  if (lane == 0)
-    for (int i = 0; i < kRing; ++i) mbar_init(smem_addr(&s_bar[warp][i]), 1);
-  if (threadIdx.x == 0) s_abort = 0;
-  fence_barrier_init();
-  __syncthreads();
+  const int b0 = min(wk * per, kb), b1 = min(wk * per + per, kb);
+  init_rings(s_bar, &s_abort);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (kTable) table.build(p.idx, p.rows, p.E);
   const int nunits = (ntiles + wn_count - 1) / wn_count;
-  const int64_t units = static_cast<int64_t>(__ldg(p.chunk_prefix + p.E)) * nunits;
-  WeightRing<MATS> w{p, smem + kWarps * MATS * 8 * kPitch * 4 + warp * kRing * MATS * kStageBlocks * p.rec,
-                     smem_addr(&s_bar[warp][0]), &s_abort, lane, min(wk * per, kb),
-                     min(wk * per + per, kb), (per + kStageBlocks - 1) / kStageBlocks, nunits,
-                     wn_count, warp / p.wk, units, blockIdx.x, 0};
-  w.locate();
+  const int units = (kTable ? table.chunks : __ldg(p.chunk_prefix + p.E)) * nunits;
+  auto expert_of = [&](int c) { return kTable ? table.expert[c] : find_expert(p.chunk_prefix, p.E, c); };
+  WeightRing<MATS> w{smem + kWarps * MATS * 8 * kFewPitch * 4 + warp * kRing * MATS * p.rec,
+                     smem_addr(&s_bar[warp][0]), &s_abort, p.err, lane, p.rec};
+  int pu = blockIdx.x, pb = 0;  // the next record to ask for: unit, block within [0, per)
+  int64_t offset = 0;           // of its strip's record b0
+  auto locate = [&]() {
+    if (pu < units) {
+      // a strip past the last one repeats it, and its results are dropped
+      const int nt = min(pu % nunits * wn_count + wn, ntiles - 1);
+      offset = ((static_cast<int64_t>(expert_of(pu / nunits)) * ntiles + nt) * kb + b0) * p.rec;
+    }
+  };
+  auto issue = [&]() {
+    if (pu >= units) return;
+    w.issue(static_cast<const char*>(p.w[0]) + offset, static_cast<const char*>(p.w[1]) + offset,
+            b0 + pb < b1 ? p.rec : 0);
+    offset += p.rec;
+    if (++pb == per) {
+      pb = 0;
+      pu += gridDim.x;
+      locate();
+    }
+  };
+  locate();
 #pragma unroll
-  for (int i = 0; i < kRing - 1; ++i) w.issue();
+  for (int i = 0; i < kRing - 1; ++i) issue();
 
-  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-    const int c = static_cast<int>(u / nunits);
-    const int e = find_expert(p.chunk_prefix, p.E, c);
-    const int row0 = __ldg(p.offsets + e) + (c - __ldg(p.chunk_prefix + e)) * 8;
-    const int rows = min(8, __ldg(p.offsets + e + 1) - row0);
+  for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    const int c = u / nunits;
+    int row0, rows;
+    if (kTable) {
+      row0 = table.first[c];
+      rows = table.first[c + 1] - row0;
+    } else {
+      const int e = expert_of(c);
+      row0 = __ldg(p.offsets + e) + (c - __ldg(p.chunk_prefix + e)) * 8;
+      rows = min(8, __ldg(p.offsets + e + 1) - row0);
+    }
     const int r = row0 + min(gid, rows - 1);
-    const T* xr = static_cast<const T*>(p.x) +
-                  static_cast<int64_t>(kDown ? r : __ldg(p.sorted_token + r)) * p.K + 8 * tig;
+    const T* xr = static_cast<const T*>(p.x) + 8 * tig + 64 * b0 +
+                  static_cast<int64_t>(kDown    ? r
+                                       : kTable ? table.row[r] / p.k
+                                                : __ldg(p.sorted_token + r)) * p.K;
     float fin[MATS][4] = {};
-    for (int st = 0; st < w.nstages; ++st) {
-      const int b = w.b0 + st * kStageBlocks;
-      uint4 xv[kStageBlocks][2];
-#pragma unroll
-      for (int i = 0; i < kStageBlocks; ++i)
-        if (b + i < w.b1) {
-          xv[i][0] = *reinterpret_cast<const uint4*>(xr + 64 * (b + i));
-          xv[i][1] = *reinterpret_cast<const uint4*>(xr + 64 * (b + i) + 32);
-        }
-      const char* stage = w.wait();
-#pragma unroll
-      for (int i = 0; i < kStageBlocks; ++i) {
-        if (b + i >= w.b1) break;
-        float xs[kPer][4] = {};  // sums of the activations over the group
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          constexpr uint32_t one = Nib<T>::kOne;
-          mma16816<T>(xs[h & (kPer - 1)], one, one, one, one, xv[i][h].x, xv[i][h].y);
-          mma16816<T>(xs[h & (kPer - 1)], one, one, one, one, xv[i][h].z, xv[i][h].w);
-        }
-#pragma unroll
-        for (int m = 0; m < MATS; ++m) {
-          const char* record = stage + (m * kStageBlocks + i) * p.rec;
-          const uint4 wq = *(reinterpret_cast<const uint4*>(record) + lane);
-          const uint32_t word[4] = {wq.x, wq.y, wq.z, wq.w};
-          float acc[kPer][4] = {};
-#pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            const uint4 v = xv[i][s >> 1];
-            mma16816<T>(acc[(s >> 1) & (kPer - 1)], nib_pair<T>(word[s], 0), nib_pair<T>(word[s], 1),
-                        nib_pair<T>(word[s], 2), nib_pair<T>(word[s], 3), (s & 1) ? v.z : v.x,
-                        (s & 1) ? v.w : v.y);
-          }
-#pragma unroll
-          for (int h = 0; h < kPer; ++h) {
-            float z0, z1;
-            zero_points(record, kPer, h, gid, p.zeros, z0, z1);
-            const T2 sc = *(reinterpret_cast<const T2*>(record + 512 + 32 * h) + gid);
-            const float s0 = Elem<T>::to_f(sc.x), s1 = Elem<T>::to_f(sc.y);
-            fin[m][0] += s0 * (acc[h][0] - z0 * xs[h][0]);
-            fin[m][1] += s0 * (acc[h][1] - z0 * xs[h][1]);
-            fin[m][2] += s1 * (acc[h][2] - z1 * xs[h][0]);
-            fin[m][3] += s1 * (acc[h][3] - z1 * xs[h][1]);
-          }
-        }
+    uint4 xn[2];
+    auto load_x = [&](int i) {
+      if (b0 + i < b1) {
+        xn[0] = *reinterpret_cast<const uint4*>(xr + 64 * i);
+        xn[1] = *reinterpret_cast<const uint4*>(xr + 64 * i + 32);
       }
+    };
+    load_x(0);
+    for (int i = 0; i < per; ++i) {
+      const uint4 xv[2] = {xn[0], xn[1]};
+      load_x(i + 1);
+      const char* stage = w.wait();
+      if (b0 + i < b1) few_block<T, MATS, kG32>(stage, p.rec, p.zeros, lane, xv, fin);
       w.release();
-      w.issue();
+      issue();
     }
 #pragma unroll
     for (int m = 0; m < MATS; ++m)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        red[((warp * MATS + m) * 8 + 2 * tig + (i & 1)) * kPitch + gid + 8 * (i >> 1)] = fin[m][i];
+      store_partial(red + (warp * MATS + m) * 8 * kFewPitch, lane, fin[m]);
     __syncthreads();
     for (int i = threadIdx.x; i < wn_count * rows * 16; i += kWarps * 32) {
       const int n = i & 15, at = (i >> 4) % rows, strip = (i >> 4) / rows;
-      const int col = (static_cast<int>(u % nunits) * wn_count + strip) * 16 + n;
+      const int col = (u % nunits * wn_count + strip) * 16 + n;
       if (col >= p.N) continue;
       float v = 0.f, v1 = 0.f;
       for (int q = 0; q < p.wk; ++q) {  // in the order of k
-        const float* from = red + ((strip * p.wk + q) * MATS * 8 + at) * kPitch + n;
+        const float* from = red + ((strip * p.wk + q) * MATS * 8 + at) * kFewPitch + n;
         v += from[0];
-        if (MATS == 2) v1 += from[8 * kPitch];
+        if (MATS == 2) v1 += from[8 * kFewPitch];
       }
       if (kDown) {
         static_cast<float*>(p.out)[static_cast<int64_t>(__ldg(p.sorted_flat + row0 + at)) * p.N +
@@ -458,6 +579,103 @@ __global__ void __launch_bounds__(kWarps * 32, 2) int4_few_kernel(Int4Params p) 
         // the intermediate is rounded to the 16-bit type that the second product reads
         static_cast<T*>(p.out)[static_cast<int64_t>(row0 + at) * p.N + col] = Elem<T>::from_f(v);
       }
+    }
+    __syncthreads();
+  }
+  w.drain();
+}
+
+// The second product of a call of at most kTableRows rows, with the combine: a CTA takes a strip of
+// 16 output columns of every token.  A warp's task is (chunk, piece of K); the partial results
+// of all tasks meet in shared memory, where the strip's outputs are summed in slot order.
+template <typename T, bool kG32>
+__global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Params p) {
+  extern __shared__ __align__(128) char smem[];
+  __shared__ alignas(8) uint64_t s_bar[kWarps][kRing];
+  __shared__ int s_abort;
+  __shared__ RowTable table;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int gid = lane >> 2, tig = lane & 3;
+  const int kb = p.K / 64, ntiles = p.N / 16;
+  init_rings(s_bar, &s_abort);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  table.build(p.idx, p.rows, p.E);
+  const int chunks = table.chunks;
+  // pieces of K: enough tasks for the warps, of three blocks or more
+  int pieces = 1;
+  while (pieces * 2 * chunks <= kWarps && kb >= 6 * pieces) pieces *= 2;
+  const int tasks = chunks * pieces, per = (kb + pieces - 1) / pieces;
+  float* part = reinterpret_cast<float*>(smem + kWarps * kRing * p.rec);
+  WeightRing<1> w{smem + warp * kRing * p.rec, smem_addr(&s_bar[warp][0]), &s_abort, p.err, lane,
+                  p.rec};
+  int pn = blockIdx.x, pt = warp, pb = 0;  // the next record to ask for: strip, task, block
+  int64_t offset = 0;
+  int left = 0;
+  auto locate = [&]() {
+    if (pt >= tasks) {
+      pt = warp;
+      pn += gridDim.x;
+    }
+    if (pn < ntiles && pt < tasks) {
+      const int b0 = pt % pieces * per;
+      left = min(per, kb - b0);
+      offset = ((static_cast<int64_t>(table.expert[pt / pieces]) * ntiles + pn) * kb + b0) * p.rec;
+    }
+  };
+  auto issue = [&]() {
+    if (pn >= ntiles || warp >= tasks) return;
+    w.issue(static_cast<const char*>(p.w[0]) + offset, nullptr, pb < left ? p.rec : 0);
+    offset += p.rec;
+    if (++pb == per) {
+      pb = 0;
+      pt += kWarps;
+      locate();
+    }
+  };
+  locate();
+#pragma unroll
+  for (int i = 0; i < kRing - 1; ++i) issue();
+
+  for (int nt = blockIdx.x; nt < ntiles; nt += gridDim.x) {
+    for (int t = warp; t < tasks; t += kWarps) {
+      const int c = t / pieces, b0 = t % pieces * per, blocks = min(per, kb - b0);
+      const int row0 = table.first[c], rows = table.first[c + 1] - row0;
+      const T* xr = static_cast<const T*>(p.x) + 8 * tig + 64 * b0 +
+                    static_cast<int64_t>(row0 + min(gid, rows - 1)) * p.K;
+      float fin[1][4] = {};
+      uint4 xn[2];
+      auto load_x = [&](int i) {
+        if (i < blocks) {
+          xn[0] = *reinterpret_cast<const uint4*>(xr + 64 * i);
+          xn[1] = *reinterpret_cast<const uint4*>(xr + 64 * i + 32);
+        }
+      };
+      load_x(0);
+      for (int i = 0; i < per; ++i) {
+        const uint4 xv[2] = {xn[0], xn[1]};
+        load_x(i + 1);
+        const char* stage = w.wait();
+        if (i < blocks) few_block<T, 1, kG32>(stage, p.rec, p.zeros, lane, xv, fin);
+        w.release();
+        issue();
+      }
+      store_partial(part + t * 8 * kFewPitch, lane, fin[0]);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.rows / p.k * 16; i += kWarps * 32) {
+      const int n = i & 15, t = i >> 4;
+      float v = 0.f;
+      for (int j = 0; j < p.k; ++j) {
+        const int at = table.place[t * p.k + j];
+        if (at < 0) continue;
+        const int c = table.chunk_of[at];
+        const float* from = part + (c * pieces * 8 + at - table.first[c]) * kFewPitch + n;
+        float y = 0.f;
+        for (int q = 0; q < pieces; ++q) y += from[q * 8 * kFewPitch];
+        v += y * __ldg(p.sorted_w + t * p.k + j);  // the caller's [T, k] weights
+      }
+      static_cast<T*>(p.out)[static_cast<int64_t>(t) * p.N + nt * 16 + n] = Elem<T>::from_f(v);
     }
     __syncthreads();
   }
@@ -488,19 +706,35 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) int4_some_kernel
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, tig = lane & 3;
   const int kb = p.K / 64, ntiles = p.N / 16, rec_per = p.G == 32 ? 2 : 1;
-  if (lane == 0)
-    for (int i = 0; i < kRing; ++i) mbar_init(smem_addr(&s_bar[warp][i]), 1);
-  if (threadIdx.x == 0) s_abort = 0;
-  fence_barrier_init();
-  __syncthreads();
+  init_rings(s_bar, &s_abort);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int nunits = (ntiles + kWarps - 1) / kWarps;
   const int64_t units = static_cast<int64_t>(__ldg(p.chunk_prefix + p.E)) * nunits;
-  WeightRing<MATS> w{p, smem + kXRing * kXBytes + warp * kRing * MATS * kStageBlocks * p.rec,
-                     smem_addr(&s_bar[warp][0]), &s_abort, lane, 0, kb,
-                     (kb + kStageBlocks - 1) / kStageBlocks, nunits, kWarps, warp, units,
-                     blockIdx.x, 0};
+  WeightRing<MATS> w{smem + kXRing * kXBytes + warp * kRing * MATS * kStageBlocks * p.rec,
+                     smem_addr(&s_bar[warp][0]), &s_abort, p.err, lane, kStageBlocks * p.rec};
+  const int nstages = (kb + kStageBlocks - 1) / kStageBlocks;
+  int64_t pu = blockIdx.x, strip = 0;  // the next stage to ask for: unit (its strip), stage
+  int ps = 0;
+  auto locate = [&]() {
+    if (pu < units) {
+      // a strip past the last one repeats it, and its results are dropped
+      const int nt = min(static_cast<int>(pu % nunits) * kWarps + warp, ntiles - 1);
+      const int e = find_expert(p.chunk_prefix, p.E, static_cast<int>(pu / nunits));
+      strip = (static_cast<int64_t>(e) * ntiles + nt) * kb;
+    }
+  };
+  auto issue = [&]() {
+    if (pu >= units) return;
+    const int64_t from = (strip + ps * kStageBlocks) * p.rec;
+    w.issue(static_cast<const char*>(p.w[0]) + from, static_cast<const char*>(p.w[1]) + from,
+            min(kStageBlocks, kb - ps * kStageBlocks) * p.rec);
+    if (++ps == nstages) {
+      ps = 0;
+      pu += gridDim.x;
+      locate();
+    }
+  };
   auto chunk_rows = [&](int64_t u, int& row0, int& rows) {
     const int c = static_cast<int>(u / nunits);
     const int e = find_expert(p.chunk_prefix, p.E, c);
@@ -535,7 +769,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) int4_some_kernel
         for (int i = 0; i < kLoads; ++i)
           if (xp[i]) cp_async16(dst + 16 * i * kXPitch, xp[i] + k);
       }
-      if (++xs_stage == w.nstages) {
+      if (++xs_stage == nstages) {
         xs_stage = 0;
         xu += gridDim.x;
         x_locate();
@@ -544,10 +778,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) int4_some_kernel
     cp_async_commit();
     xs_slot = xs_slot + 1 == kXRing ? 0 : xs_slot + 1;
   };
-  w.locate();
+  locate();
   x_locate();
 #pragma unroll
-  for (int i = 0; i < kRing - 1; ++i) w.issue();
+  for (int i = 0; i < kRing - 1; ++i) issue();
 #pragma unroll
   for (int i = 0; i < kXRing - 1; ++i) x_issue();
   int x_slot = 0;
@@ -557,7 +791,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) int4_some_kernel
     chunk_rows(u, row0, rows);
     const int tiles = (rows + 7) / 8;
     float fin[MATS][NT][4] = {};
-    for (int st = 0; st < w.nstages; ++st) {
+    for (int st = 0; st < nstages; ++st) {
       cp_async_wait<kXRing - 2>();
       __syncthreads();  // the stage is there for all, and all are done with the one before
       x_issue();
@@ -597,8 +831,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) int4_some_kernel
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
               if (j < tiles) {
-                float acc[4] = {};
-                mma16816<T>(acc, a[0][0], a[0][1], a[0][2], a[0][3], xv[j].x, xv[j].y);
+                float acc[4];
+                mma16816_zero<T>(acc, a[0][0], a[0][1], a[0][2], a[0][3], xv[j].x, xv[j].y);
                 mma16816<T>(acc, a[1][0], a[1][1], a[1][2], a[1][3], xv[j].z, xv[j].w);
                 fin[m][j][0] += s0 * acc[0];
                 fin[m][j][1] += s0 * acc[1];
@@ -610,7 +844,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) int4_some_kernel
         }
       }
       w.release();
-      w.issue();
+      issue();
       x_slot = x_slot + 1 == kXRing ? 0 : x_slot + 1;
     }
     // out, 8 rows at a time: a lane takes 4 columns of one row
@@ -702,23 +936,34 @@ bool launch_dependent(void (*kernel)(Args...), int grid, int threads, size_t sme
   return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess;
 }
 
-// Pieces of K: as many as leave a warp three k64 blocks or more.
-int pieces_of(int K) {
-  int wk = kWarps;
-  while (wk > 1 && K / 64 < 3 * wk) wk /= 2;
-  return wk;
-}
-
-template <typename T, int MATS, bool kDown, bool kG32>
+template <typename T, int MATS, bool kDown, bool kG32, bool kTable>
 struct Few {
-  static constexpr auto kernel = int4_few_kernel<T, MATS, kDown, kG32>;
+  static constexpr auto kernel = int4_few_kernel<T, MATS, kDown, kG32, kTable>;
   static size_t smem(int rec) {
-    return static_cast<size_t>(kWarps) * MATS * (8 * 20 * 4 + kRing * kStageBlocks * rec);
+    return static_cast<size_t>(kWarps) * MATS * (8 * kFewPitch * 4 + kRing * rec);
   }
   static bool launch(Int4Params p, int num_sms, cudaStream_t s) {
-    p.wk = pieces_of(p.K);
-    // two CTAs on an SM: 2 x (10 + 76 KB) at most
-    return launch_dependent(kernel, num_sms * 2, kWarps * 32, smem(p.rec), s, p);
+    // pieces of K: a call that the table serves has few units, so as many as leave a warp three
+    // blocks; else eight blocks, for fewer sums across warps
+    p.wk = kWarps;
+    while (p.wk > 1 && p.K / 64 < (kTable ? 3 : 8) * p.wk) p.wk /= 2;
+    // three CTAs on an SM: 3 x (10 + 38 + 2 KB) at most
+    return launch_dependent(kernel, num_sms * 3, kWarps * 32, smem(p.rec), s, p);
+  }
+};
+
+template <typename T, bool kG32>
+struct FewDown {
+  static constexpr auto kernel = int4_few_down_kernel<T, kG32>;
+  static size_t smem(int rec) { return smem(rec, kTableRows); }
+  // partial results: one task per chunk, or fewer than 2 kWarps with K in pieces
+  static size_t smem(int rec, int rows) {
+    const int tasks = rows > kWarps ? rows : kWarps;
+    return static_cast<size_t>(kWarps) * kRing * rec + static_cast<size_t>(tasks) * 8 * kFewPitch * 4;
+  }
+  static bool launch(const Int4Params& p, int num_sms, cudaStream_t s) {
+    const int grid = p.N / 16 < num_sms * 3 ? p.N / 16 : num_sms * 3;
+    return launch_dependent(kernel, grid, kWarps * 32, smem(p.rec, p.rows), s, p);
   }
 };
 
@@ -740,20 +985,27 @@ template <typename K> bool allow_smem() {
                               static_cast<int>(K::smem(kMaxRecord))) == cudaSuccess;
 }
 
+template <typename T, bool kG32> bool allow_few() {
+  return allow_smem<Few<T, 2, false, kG32, false>>() && allow_smem<Few<T, 1, false, kG32, false>>() &&
+         allow_smem<Few<T, 1, true, kG32, false>>() && allow_smem<Few<T, 2, false, kG32, true>>() &&
+         allow_smem<Few<T, 1, false, kG32, true>>() && allow_smem<FewDown<T, kG32>>();
+}
 template <typename T> bool gemm_attributes() {
-  return allow_smem<Few<T, 2, false, false>>() && allow_smem<Few<T, 2, false, true>>() &&
-         allow_smem<Few<T, 1, false, false>>() && allow_smem<Few<T, 1, false, true>>() &&
-         allow_smem<Few<T, 1, true, false>>() && allow_smem<Few<T, 1, true, true>>() &&
-         allow_smem<Some<T, 2, false, 4>>() && allow_smem<Some<T, 2, false, 8>>() &&
-         allow_smem<Some<T, 1, false, 4>>() && allow_smem<Some<T, 1, false, 8>>() &&
-         allow_smem<Some<T, 1, true, 4>>() && allow_smem<Some<T, 1, true, 8>>();
+  return allow_few<T, false>() && allow_few<T, true>() && allow_smem<Some<T, 2, false, 4>>() &&
+         allow_smem<Some<T, 2, false, 8>>() && allow_smem<Some<T, 1, false, 4>>() &&
+         allow_smem<Some<T, 1, false, 8>>() && allow_smem<Some<T, 1, true, 4>>() &&
+         allow_smem<Some<T, 1, true, 8>>();
 }
 
+template <typename T, bool kG32, bool kTable>
+bool launch_few_first(const Int4Params& g1, int num_sms, cudaStream_t s) {
+  return g1.w[1] ? Few<T, 2, false, kG32, kTable>::launch(g1, num_sms, s)
+                 : Few<T, 1, false, kG32, kTable>::launch(g1, num_sms, s);
+}
 template <typename T, bool kG32>
 bool launch_few(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
-  return (g1.w[1] ? Few<T, 2, false, kG32>::launch(g1, num_sms, s)
-                  : Few<T, 1, false, kG32>::launch(g1, num_sms, s)) &&
-         Few<T, 1, true, kG32>::launch(g2, num_sms, s);
+  return launch_few_first<T, kG32, false>(g1, num_sms, s) &&
+         Few<T, 1, true, kG32, false>::launch(g2, num_sms, s);
 }
 template <typename T, int NT>
 bool launch_some(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
@@ -828,6 +1080,26 @@ int launch_int4_pack(int dtype, const uint8_t* q, const void* scales, const uint
   int4_pack_groups_kernel<<<grid_for(static_cast<int64_t>(E) * (K / 32) * N, num_sms), 256, 0, s>>>(
       static_cast<const uint16_t*>(scales), zeros, E, K, N, G, rec, base);
   return 2;
+}
+
+int int4_table_rows() { return kTableRows; }
+
+namespace {
+template <typename T, bool kG32>
+bool launch_table(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
+  return launch_few_first<T, kG32, true>(g1, num_sms, s) &&
+         FewDown<T, kG32>::launch(g2, num_sms, s);
+}
+}  // namespace
+
+int launch_int4_table_ffn(int dtype, const Int4Params& g1, const Int4Params& g2, int num_sms,
+                          cudaStream_t s) {
+  const bool ok = dtype == kBF16
+                      ? (g1.G == 32 ? launch_table<__nv_bfloat16, true>(g1, g2, num_sms, s)
+                                    : launch_table<__nv_bfloat16, false>(g1, g2, num_sms, s))
+                      : (g1.G == 32 ? launch_table<__half, true>(g1, g2, num_sms, s)
+                                    : launch_table<__half, false>(g1, g2, num_sms, s));
+  return ok ? 2 : 0;
 }
 
 int launch_int4_ffn(int dtype, int chunk_rows, const Int4Params& g1, const Int4Params& g2,

@@ -15,7 +15,7 @@ def test_sizes():
         assert lib.moe_int4_packed_size(2, 128, 64, G, 1, 1) == 2 * 4 * 2 * (512 + 48 * per)
     for bad in [(0, 128, 64, 64, 1, 0), (2, 96, 64, 32, 1, 0), (2, 128, 72, 64, 1, 0),
                 (2, 128, 64, 48, 1, 0), (2, 64, 64, 128, 1, 0), (2, 128, 64, 64, 2, 0),
-                (2, 128, 64, 64, 5, 0)]:
+                (2, 128, 64, 64, 5, 0), (2, 1 << 21, 64, 64, 1, 0), (2, 64, 1 << 21, 64, 1, 0)]:
         assert lib.moe_int4_packed_size(*bad) == 0, bad
     n = cm.int4_workspace_size(64, 256, 128, 8, 2)
     assert n >= 128 * (128 * 2 + 256 * 2) and n % 256 == 0
