@@ -100,7 +100,7 @@ int init_device(int dev, DeviceState** out) {
     const bool attrs_ok = route_prep_set_attributes() && sm100_set_attributes() &&
                           sm100_pair_set_attributes() && decode_set_attributes() &&
                           router_project_set_attributes() && tf32x3_set_attributes() &&
-                          int4_set_attributes();
+                          int4_set_attributes() && route_experts_set_attributes();
     cudaGetLastError();  // attribute failures are reported here, not by a later call
     if (!attrs_ok) return MOE_ERR_CUDA;
     d.max_pairs = sm100_pair_max_clusters();

@@ -53,6 +53,7 @@ struct RouteExpertsBackwardParams {
   int E, k, scoring, renormalize;
   float scaling;
 };
+bool route_experts_set_attributes();
 int launch_route_experts(int dtype, const RouteExpertsParams& p, int num_sms, cudaStream_t s);
 int launch_route_experts_backward(int dtype, const RouteExpertsBackwardParams& p, int num_sms,
                                   cudaStream_t s);

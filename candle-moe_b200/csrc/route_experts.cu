@@ -757,97 +757,160 @@ __global__ void __launch_bounds__(kRowWarps * 32)
   }
 }
 
-// One row per warp; the row is put together in shared memory (zero except at the picks) and leaves
-// in 16-byte stores.  kDense (softmax weights that are not renormalised): every expert has a
-// gradient, so the logits are read whole; else at most the picks' logits are, since
+// ---- gradient ----------------------------------------------------------------------------------
+
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
+               "r"(smem_addr(src)), "r"(bytes)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+template <int N> __device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+
+// Gradients that are zero except at the picks:
 //     softmax, renormalised:  dl_j = w_j (g_j - G),            G = sum_i g_i w_i / c
 //     sigmoid:                dl_j = w_j (g_j - G) (1 - s_j),  G = 0 unless renormalised
-// The kernel is bound by the T*E gradients it writes.
-template <typename T, bool kDense>
-__global__ void __launch_bounds__(kFastWarps * 32)
-    route_experts_backward_kernel(RouteExpertsBackwardParams p, int vec) {
-  extern __shared__ float smem_f[];
+// so at most the picks' logits are read.  LPR lanes per row, a lane per slot (k <= LPR): a warp
+// reads the slots of 32 / LPR rows at once, drops their gradients into a tile of zeros in shared
+// memory and sends the tile out in one bulk copy; two tiles in turn, and the places written
+// are cleared once the copy has read them.  Bound by the T*E gradients written (a warp per row,
+// with its own stores, took 162 instructions a row and 3 times as long).
+template <typename T, int LPR>
+__global__ void __launch_bounds__(kRowWarps * 32)
+    route_experts_backward_kernel(RouteExpertsBackwardParams p, int bulk) {
+  extern __shared__ __align__(128) char smem_c[];
+  constexpr int RW = 32 / LPR;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kPer = 16 / sizeof(T);
-  const int pitch = (p.E + 7) & ~7;
-  float* ds = smem_f + warp * pitch;
-  for (int e = lane; e < pitch; e += 32) ds[e] = 0.f;
+  const int sub = lane / LPR, q = lane % LPR;
+  const int tile = RW * p.E;                              // elements
+  const int pitch = (tile * static_cast<int>(sizeof(T)) + 15) & ~15;  // bytes
+  char* base = smem_c + warp * 2 * pitch;
+  for (int i = lane * 4; i < 2 * pitch; i += 128) *reinterpret_cast<uint32_t*>(base + i) = 0u;
   __syncwarp();
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * kFastWarps;
-  int64_t row = static_cast<int64_t>(blockIdx.x) * kFastWarps + warp;
-  // the next row's picks are loaded while this row is written
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kRowWarps * RW;
+  int64_t row0 = (static_cast<int64_t>(blockIdx.x) * kRowWarps + warp) * RW;
+  // the next rows' picks are loaded while these rows are written
   float gn = 0.f, wn = 0.f;
   int idn = -1;
-  auto load = [&](int64_t r) {
-    if (r < p.num_tokens && lane < p.k) {
-      gn = __ldcs(p.grad_weights + r * p.k + lane);
-      wn = __ldcs(p.weights + r * p.k + lane);
-      idn = __ldcs(p.indices + r * p.k + lane);
+  auto load = [&](int64_t r0) {
+    const int64_t r = r0 + sub;
+    idn = -1;
+    if (q < p.k && r < p.num_tokens) {
+      gn = __ldcs(p.grad_weights + r * p.k + q);
+      wn = __ldcs(p.weights + r * p.k + q);
+      idn = __ldcs(p.indices + r * p.k + q);
     }
   };
-  load(row);
-  for (; row < p.num_tokens; row += stride) {
-    const T* l = static_cast<const T*>(p.logits) + row * p.stride;
-    T* out = static_cast<T*>(p.grad_logits) + row * p.E;
-    const bool ok = lane < p.k && idn >= 0 && idn < p.E;
+  load(row0);
+  int held[2] = {-1, -1};  // place this lane wrote in each tile
+  int side = 0;
+  for (; row0 < p.num_tokens; row0 += stride) {
+    const bool ok = idn >= 0 && idn < p.E;
     const int id = ok ? idn : 0;
     const float g = ok ? gn : 0.f, w = ok ? wn : 0.f;
-    load(row + stride);
-    const float gw = g * w;
-    float d = gw, D = 0.f;
-    if (kDense) {
-      D = warp_sum(gw);
-      d = g * p.scaling;
+    float x = 0.f;
+    if (p.scoring != 0 && ok)
+      x = logit_of(static_cast<const T*>(p.logits) + (row0 + sub) * p.stride, id);
+    load(row0 + stride);
+    float d = g * w;
+    if (p.renormalize) {
+      float G = d;
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) G += __shfl_xor_sync(0xffffffffu, G, o);
+      d = w * (g - G / p.scaling);
+    }
+    if (p.scoring != 0) d *= 1.f / (1.f + expf(x));
+    T* buf = reinterpret_cast<T*>(base + side * pitch);
+    bulk_wait_read<1>();  // the copy before the last, out of this tile, has read it
+    __syncwarp();
+    if (held[side] >= 0) buf[held[side]] = Elem<T>::from_f(0.f);
+    __syncwarp();
+    const int at = ok ? sub * p.E + id : -1;
+    // one id twice in a row: the first lane of it adds the others' in slot order
+    const unsigned peers = __match_any_sync(0xffffffffu, ok ? at : -1 - lane);
+    const bool first = (peers & ((1u << lane) - 1u)) == 0;
+    if (__any_sync(0xffffffffu, ok && !first)) {
+      float sum = 0.f;
+      for (int j = 0; j < 32; ++j) {
+        const float o = __shfl_sync(0xffffffffu, d, j);
+        if ((peers >> j) & 1u) sum += o;
+      }
+      d = sum;
+    }
+    if (ok && first) buf[at] = Elem<T>::from_f(d);
+    held[side] = ok && first ? at : -1;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(RW), p.num_tokens - row0));
+    T* out = static_cast<T*>(p.grad_logits) + row0 * p.E;
+    const uint32_t bytes = rows * p.E * sizeof(T);
+    if (bulk && bytes % 16 == 0) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bulk_store(out, buf, bytes);
     } else {
-      if (p.renormalize) d = w * (g - warp_sum(gw) / p.scaling);
-      if (p.scoring != 0 && ok) {
-        const float x = logit_of(l, id);
-        d *= 1.f / (1.f + expf(x));
+      __syncwarp();
+      for (int i = lane; i < rows * p.E; i += 32) out[i] = buf[i];
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+    __syncwarp();
+    side ^= 1;
+  }
+  bulk_wait_read<0>();
+}
+
+// Softmax weights that are not renormalised: every expert has a gradient,
+//     dl_e = s_e (c g_e - sum_i g_i w_i)
+// One row per warp, the picks' share through a row of zeros in shared memory.
+template <typename T>
+__global__ void __launch_bounds__(kFastWarps * 32)
+    route_experts_backward_dense_kernel(RouteExpertsBackwardParams p) {
+  extern __shared__ float smem_f[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* ds = smem_f + warp * p.E;
+  for (int e = lane; e < p.E; e += 32) ds[e] = 0.f;
+  __syncwarp();
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kFastWarps + warp; row < p.num_tokens;
+       row += static_cast<int64_t>(gridDim.x) * kFastWarps) {
+    const T* l = static_cast<const T*>(p.logits) + row * p.stride;
+    T* out = static_cast<T*>(p.grad_logits) + row * p.E;
+    float g = 0.f, w = 0.f;
+    int id = -1;
+    if (lane < p.k) {
+      id = p.indices[row * p.k + lane];
+      if (id >= 0 && id < p.E) {
+        g = p.grad_weights[row * p.k + lane];
+        w = p.weights[row * p.k + lane];
+      } else {
+        id = -1;
       }
     }
+    float m = -CUDART_INF_F, total = 0.f;
+    for (int e = lane; e < p.E; e += 32) m = fmaxf(m, logit_of(l, e));
+    m = warp_max(m);
+    for (int e = lane; e < p.E; e += 32) {
+      const float x = logit_of(l, e);
+      if (x > -CUDART_INF_F) total += expf(x - m);
+    }
+    const float inv = 1.f / warp_sum(total);
+    const float D = warp_sum(g * w);
     // one id twice in a row adds up in slot order
-    const unsigned peers = __match_any_sync(0xffffffffu, ok ? id : -1 - lane);
-    const bool twice = ok && (peers & (peers - 1)) != 0;
-    if (!__any_sync(0xffffffffu, twice)) {
-      if (ok) ds[id] = d;
+    const unsigned peers = __match_any_sync(0xffffffffu, id >= 0 ? id : -1 - lane);
+    if (!__any_sync(0xffffffffu, id >= 0 && (peers & (peers - 1)) != 0)) {
+      if (id >= 0) ds[id] = g * p.scaling;
     } else {
       for (int j = 0; j < p.k; ++j) {
-        if (lane == j && ok) ds[id] += d;
+        if (lane == j && id >= 0) ds[id] += g * p.scaling;
         __syncwarp();
       }
     }
     __syncwarp();
-    if (kDense) {
-      float m = -CUDART_INF_F, total = 0.f;
-      for (int e = lane; e < p.E; e += 32) m = fmaxf(m, logit_of(l, e));
-      m = warp_max(m);
-      for (int e = lane; e < p.E; e += 32) {
-        const float x = logit_of(l, e);
-        if (x > -CUDART_INF_F) total += expf(x - m);
-      }
-      const float inv = 1.f / warp_sum(total);
-      for (int e = lane; e < p.E; e += 32) {
-        const float x = logit_of(l, e);
-        out[e] = Elem<T>::from_f(x > -CUDART_INF_F ? expf(x - m) * inv * (ds[e] - D) : 0.f);
-      }
-    } else if (vec) {
-      for (int e = lane * kPer; e < p.E; e += 32 * kPer) {
-        alignas(16) T q[kPer];
-#pragma unroll
-        for (int i = 0; i < kPer; i += 4) {
-          const float4 f = *reinterpret_cast<const float4*>(ds + e + i);
-          q[i] = Elem<T>::from_f(f.x);
-          q[i + 1] = Elem<T>::from_f(f.y);
-          q[i + 2] = Elem<T>::from_f(f.z);
-          q[i + 3] = Elem<T>::from_f(f.w);
-        }
-        __stcs(reinterpret_cast<uint4*>(out + e), *reinterpret_cast<const uint4*>(q));
-      }
-    } else {
-      for (int e = lane; e < p.E; e += 32) out[e] = Elem<T>::from_f(ds[e]);
+    for (int e = lane; e < p.E; e += 32) {
+      const float x = logit_of(l, e);
+      out[e] = Elem<T>::from_f(x > -CUDART_INF_F ? expf(x - m) * inv * (ds[e] - D) : 0.f);
     }
     __syncwarp();
-    if (ok) ds[id] = 0.f;
+    if (id >= 0) ds[id] = 0.f;
     __syncwarp();
   }
 }
@@ -945,20 +1008,41 @@ int launch_route_experts(int dtype, const RouteExpertsParams& p, int num_sms, cu
 }
 
 namespace {
+template <typename T, int LPR>
+void launch_backward_picks(const RouteExpertsBackwardParams& p, int num_sms, cudaStream_t s) {
+  constexpr int rows = kRowWarps * (32 / LPR);
+  const int64_t blocks = (p.num_tokens + rows - 1) / rows, cap = static_cast<int64_t>(num_sms) * 16;
+  const unsigned grid = static_cast<unsigned>(blocks < cap ? blocks : cap);
+  const int tile = (32 / LPR) * p.E * static_cast<int>(sizeof(T));
+  const size_t smem = static_cast<size_t>(kRowWarps) * 2 * ((tile + 15) & ~15);
+  // a warp's rows start on 16 bytes
+  const int bulk = tile % 16 == 0 && (reinterpret_cast<uintptr_t>(p.grad_logits) & 15u) == 0;
+  route_experts_backward_kernel<T, LPR><<<grid, kRowWarps * 32, smem, s>>>(p, bulk);
+}
+
 template <typename T>
 void launch_backward(const RouteExpertsBackwardParams& p, int num_sms, cudaStream_t s) {
-  const int64_t blocks = (p.num_tokens + kFastWarps - 1) / kFastWarps;
-  const int64_t cap = static_cast<int64_t>(num_sms) * 8;
-  const unsigned grid = static_cast<unsigned>(blocks < cap ? blocks : cap);
-  const size_t smem = sizeof(float) * kFastWarps * ((p.E + 7) & ~7);
-  const int vec = (p.E * sizeof(T)) % 16 == 0 &&
-                  (reinterpret_cast<uintptr_t>(p.grad_logits) & 15u) == 0;
-  if (p.scoring == 0 && !p.renormalize)
-    route_experts_backward_kernel<T, true><<<grid, kFastWarps * 32, smem, s>>>(p, vec);
-  else
-    route_experts_backward_kernel<T, false><<<grid, kFastWarps * 32, smem, s>>>(p, vec);
+  if (p.scoring == 0 && !p.renormalize) {
+    const int64_t blocks = (p.num_tokens + kFastWarps - 1) / kFastWarps;
+    const int64_t cap = static_cast<int64_t>(num_sms) * 8;
+    const unsigned grid = static_cast<unsigned>(blocks < cap ? blocks : cap);
+    route_experts_backward_dense_kernel<T>
+        <<<grid, kFastWarps * 32, sizeof(float) * kFastWarps * p.E, s>>>(p);
+  } else if (p.k <= 8) {
+    launch_backward_picks<T, 8>(p, num_sms, s);
+  } else if (p.k <= 16) {
+    launch_backward_picks<T, 16>(p, num_sms, s);
+  } else {
+    launch_backward_picks<T, 32>(p, num_sms, s);
+  }
 }
 }  // namespace
+
+bool route_experts_set_attributes() {
+  const int most = kRowWarps * 2 * 4 * kRouteMaxExperts * 4;  // 64 KB: f32, eight lanes per row
+  return cudaFuncSetAttribute(route_experts_backward_kernel<float, 8>,
+                              cudaFuncAttributeMaxDynamicSharedMemorySize, most) == cudaSuccess;
+}
 
 int launch_route_experts_backward(int dtype, const RouteExpertsBackwardParams& p, int num_sms,
                                   cudaStream_t s) {
