@@ -502,7 +502,7 @@ constexpr int kRowWarps = 4;
 // four in turn (64 contiguous bytes of f32), with groups a lane holds one stretch of one group.
 // NaN needs no care where it is compared: it is never >= t nor > -inf.
 template <typename T, int LPR, int VPL, bool kBias>
-__global__ void __launch_bounds__(kRowWarps * 32)
+__global__ void __launch_bounds__(kRowWarps * 32, 6)
     route_experts_rows_kernel(RouteExpertsParams p, int bs, int lpg, int vec) {
   extern __shared__ double smem_d[];
   constexpr int RPW = 32 / LPR;
@@ -787,8 +787,6 @@ __global__ void __launch_bounds__(kRowWarps * 32)
   const int tile = RW * p.E;                              // elements
   const int pitch = (tile * static_cast<int>(sizeof(T)) + 15) & ~15;  // bytes
   char* base = smem_c + warp * 2 * pitch;
-  for (int i = lane * 4; i < 2 * pitch; i += 128) *reinterpret_cast<uint32_t*>(base + i) = 0u;
-  __syncwarp();
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kRowWarps * RW;
   int64_t row0 = (static_cast<int64_t>(blockIdx.x) * kRowWarps + warp) * RW;
   // the next rows' picks are loaded while these rows are written
@@ -803,16 +801,23 @@ __global__ void __launch_bounds__(kRowWarps * 32)
       idn = __ldcs(p.indices + r * p.k + q);
     }
   };
+  float xn = 0.f;
+  auto load_logit = [&](int64_t r0) {
+    if (p.scoring != 0 && idn >= 0 && idn < p.E)
+      xn = logit_of(static_cast<const T*>(p.logits) + (r0 + sub) * p.stride, idn);
+  };
   load(row0);
+  const int tiles = row0 + stride < p.num_tokens ? 2 : 1;
+  for (int i = lane * 16; i < tiles * pitch; i += 512)
+    *reinterpret_cast<uint4*>(base + i) = make_uint4(0, 0, 0, 0);
+  load_logit(row0);
   int held[2] = {-1, -1};  // place this lane wrote in each tile
   int side = 0;
   for (; row0 < p.num_tokens; row0 += stride) {
     const bool ok = idn >= 0 && idn < p.E;
     const int id = ok ? idn : 0;
     const float g = ok ? gn : 0.f, w = ok ? wn : 0.f;
-    float x = 0.f;
-    if (p.scoring != 0 && ok)
-      x = logit_of(static_cast<const T*>(p.logits) + (row0 + sub) * p.stride, id);
+    const float x = xn;
     load(row0 + stride);
     float d = g * w;
     if (p.renormalize) {
@@ -855,6 +860,7 @@ __global__ void __launch_bounds__(kRowWarps * 32)
     }
     __syncwarp();
     side ^= 1;
+    load_logit(row0 + stride);
   }
   bulk_wait_read<0>();
 }
