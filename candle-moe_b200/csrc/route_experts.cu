@@ -63,10 +63,16 @@ __device__ __forceinline__ uint64_t order_key64(double v) {
   return (b >> 63) ? ~b : (b | (1ull << 63));
 }
 
+// A score in 64 bits.  One copy of the code (and loops that are not unrolled) in what follows:
+// these paths run for a row in thousands, and what they cost then is fetching instructions.
+__device__ __noinline__ double score64(float x, float m, double total, int scoring) {
+  const double e = exp(scoring == 0 ? static_cast<double>(x) - static_cast<double>(m)
+                                    : -static_cast<double>(x));
+  return scoring == 0 ? e / total : 1.0 / (1.0 + e);
+}
+
 // One row by one warp with 64-bit keys, any shape; key: E doubles of scratch.  Leaves the pick of
-// slot `lane` (id E: none) and its score.  A launch waits for its slowest row, so this is
-// written for a short dependent chain (independent iterations unrolled, warp reductions on
-// integer keys) rather than for few instructions.
+// slot `lane` (id E: none) and its score.
 template <typename T>
 __device__ __noinline__ void route_row64(const RouteExpertsParams& p, int64_t row, double* key,
                                          float& mine, int& mine_id) {
@@ -75,33 +81,28 @@ __device__ __noinline__ void route_row64(const RouteExpertsParams& p, int64_t ro
   float m = -CUDART_INF_F;
   double total = 1.0;
   if (p.scoring == 0) {
-#pragma unroll 4
+#pragma unroll 1
     for (int e = lane; e < p.E; e += 32) m = fmaxf(m, logit_of(l, e));
     m = warp_max(m);
-    total = 0.0;
-#pragma unroll 4
+    double sum = 0.0;
+#pragma unroll 1
     for (int e = lane; e < p.E; e += 32) {
       const float x = logit_of(l, e);
-      total += x > -CUDART_INF_F ? exp(static_cast<double>(x) - static_cast<double>(m)) : 0.0;
+      sum += x > -CUDART_INF_F ? score64(x, m, 1.0, 0) : 0.0;
     }
-    total = warp_sum(total);
+    total = warp_sum(sum);
   }
-  auto score = [&](float x) -> double {
-    if (p.scoring == 0) return exp(static_cast<double>(x) - static_cast<double>(m)) / total;
-    return 1.0 / (1.0 + exp(-static_cast<double>(x)));
-  };
   const bool sums = p.num_groups > 1 && p.group_score != 0;
-  if (p.bias || sums) {
-#pragma unroll 4
-    for (int e = lane; e < p.E; e += 32) {
-      const float x = logit_of(l, e);
-      const double k = score(x) + (p.bias ? static_cast<double>(p.bias[e]) : 0.0);
+#pragma unroll 1
+  for (int e = lane; e < p.E; e += 32) {
+    const float x = logit_of(l, e);
+    double k = static_cast<double>(x);
+    if (p.bias || sums) {
+      k = score64(x, m, total, p.scoring) + (p.bias ? static_cast<double>(p.bias[e]) : 0.0);
       // a bias of -inf or NaN shuts the expert off
-      key[e] = (x > -CUDART_INF_F && k > -CUDART_INF) ? k : -CUDART_INF;
+      if (!(x > -CUDART_INF_F && k > -CUDART_INF)) k = -CUDART_INF;
     }
-  } else {
-#pragma unroll 4
-    for (int e = lane; e < p.E; e += 32) key[e] = static_cast<double>(logit_of(l, e));
+    key[e] = k;
   }
   __syncwarp();
   unsigned open = 0xffffffffu;
@@ -110,7 +111,7 @@ __device__ __noinline__ void route_row64(const RouteExpertsParams& p, int64_t ro
     const int lpg = 32 / p.num_groups, g = lane / lpg, at = lane % lpg;
     double a = -CUDART_INF, b = -CUDART_INF;
     if (g < p.num_groups) {
-#pragma unroll 4
+#pragma unroll 1
       for (int i = at; i < per; i += lpg) {
         const double v = key[g * per + i];
         b = fmax(b, fmin(a, v));
@@ -118,6 +119,7 @@ __device__ __noinline__ void route_row64(const RouteExpertsParams& p, int64_t ro
       }
     }
     double ga = a, gb = b;
+#pragma unroll 1
     for (int o = 1; o < lpg; ++o) {
       const int from = (g * lpg + (at + o) % lpg) & 31;
       const double oa = __shfl_sync(0xffffffffu, a, from);
@@ -128,7 +130,7 @@ __device__ __noinline__ void route_row64(const RouteExpertsParams& p, int64_t ro
     double value = sums && gb > -CUDART_INF ? ga + gb : ga;
     if (g >= p.num_groups) value = -CUDART_INF;
     int place = 0;
-#pragma unroll 4
+#pragma unroll 1
     for (int o = 0; o < p.num_groups; ++o) {
       const double ov = __shfl_sync(0xffffffffu, value, o * lpg);
       place += ov > value || (ov == value && o < g);
@@ -136,33 +138,36 @@ __device__ __noinline__ void route_row64(const RouteExpertsParams& p, int64_t ro
     const unsigned lanes =
         __ballot_sync(0xffffffffu, value > -CUDART_INF && place < p.topk_groups);
     open = 0;
+#pragma unroll 1
     for (int o = 0; o < p.num_groups; ++o) open |= ((lanes >> (o * lpg)) & 1u) << o;
   }
-  // this lane's best key, and the next one whenever it is picked
-  const bool logits = !p.bias;
-  auto key_of = [&](int e) -> uint64_t {
-    if (p.num_groups > 1 && !((open >> (e / per)) & 1u)) return 0;
-    const double k = key[e];
-    if (!(k > -CUDART_INF)) return 0;
-    return order_key64(logits && sums ? static_cast<double>(logit_of(l, e)) : k);
-  };
-  uint64_t best = 0;
-  int id = 0;
-  auto find = [&]() {
-    best = 0;
-#pragma unroll 4
-    for (int e = lane; e < p.E; e += 32) {
-      const uint64_t k = key_of(e);
-      if (k > best) {
-        best = k;
-        id = e;
-      }
-    }
-  };
-  find();
+  // keys as ordered integers, 0: not to be picked
+  uint64_t* order = reinterpret_cast<uint64_t*>(key);
+#pragma unroll 1
+  for (int e = lane; e < p.E; e += 32) {
+    double k = key[e];
+    const bool out = !(k > -CUDART_INF) || !((open >> (p.num_groups > 1 ? e / per : 0)) & 1u);
+    if (!p.bias && sums) k = static_cast<double>(logit_of(l, e));
+    order[e] = out ? 0 : order_key64(k);
+  }
+  __syncwarp();
   mine = 0.f;
   mine_id = p.E;
+  uint64_t best = 0;
+  int id = 0;
+  bool stale = true;  // this lane's best key was picked (or none is known yet)
+#pragma unroll 1
   for (int j = 0; j < p.k; ++j) {
+    if (stale) {
+      best = 0;
+#pragma unroll 1
+      for (int e = lane; e < p.E; e += 32)
+        if (order[e] > best) {
+          best = order[e];
+          id = e;
+        }
+    }
+    __syncwarp();
     const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(best >> 32));
     if (hi == 0) break;
     const bool top = static_cast<uint32_t>(best >> 32) == hi;
@@ -171,12 +176,11 @@ __device__ __noinline__ void route_row64(const RouteExpertsParams& p, int64_t ro
         0xffffffffu, top && static_cast<uint32_t>(best) == lo ? static_cast<unsigned>(id)
                                                               : 0xffffffffu);
     if (lane == j) mine_id = static_cast<int>(pick);
-    if (static_cast<int>(pick) % 32 == lane) {
-      key[pick] = -CUDART_INF;
-      find();
-    }
+    stale = static_cast<int>(pick) % 32 == lane;
+    if (stale) order[pick] = 0;
   }
-  if (mine_id < p.E) mine = static_cast<float>(score(logit_of(l, mine_id)));
+  if (mine_id < p.E)
+    mine = static_cast<float>(score64(logit_of(l, mine_id), m, total, p.scoring));
 }
 
 // Writes the row's k slots from the pick that each lane holds (slot `lane`).
@@ -487,6 +491,50 @@ __device__ __forceinline__ void sort_bitonic8(float (&x)[8]) {
 }
 
 constexpr int kRowCand = 16;  // candidates of a row
+
+// The float of a candidate's order-preserving key.
+__device__ __forceinline__ float from_key(uint64_t c) {
+  const uint32_t k = static_cast<uint32_t>(c >> 32);
+  return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
+}
+
+// Ranks the `count` candidates (key << 32 | ~id) of each of a warp's rows by sigmoid + bias in 64
+// bits, ties to the lower id; cand is overwritten.
+template <typename T, int LPR>
+__device__ __noinline__ void rank64(const T* l, const float* __restrict__ bias, uint64_t* cand,
+                                    uint64_t* ranked, int count) {
+  const int q = (threadIdx.x & 31) % LPR;
+#pragma unroll 1
+  for (int i = q; i < count; i += LPR) {
+    const uint64_t c = cand[i];
+    const int id = static_cast<int>(~static_cast<uint32_t>(c));
+    ranked[i] = c;  // by position; its key in 64 bits in cand
+    cand[i] = order_key64(score64(Elem<T>::to_f(l[id]), 0.f, 1.0, 1) +
+                          static_cast<double>(bias[id]));
+  }
+  __syncwarp();
+  uint64_t mine[kRowCand / LPR];
+  int at[kRowCand / LPR];
+#pragma unroll
+  for (int h = 0; h < kRowCand / LPR; ++h) {
+    const int i = q + h * LPR;
+    at[h] = 0;
+    mine[h] = 0;
+    if (i < count) {
+      mine[h] = ranked[i];
+      const uint64_t key = cand[i];
+#pragma unroll 1
+      for (int j = 0; j < count; ++j)  // ~id: larger for the lower id
+        at[h] += cand[j] > key || (cand[j] == key && static_cast<uint32_t>(ranked[j]) >
+                                                         static_cast<uint32_t>(mine[h]));
+    }
+  }
+  __syncwarp();
+#pragma unroll
+  for (int h = 0; h < kRowCand / LPR; ++h)
+    if (mine[h]) ranked[at[h]] = mine[h];
+  __syncwarp();
+}
 constexpr int kRowWarps = 4;
 
 // LPR lanes per row, each with up to VPL experts in registers; k <= 8.
@@ -619,10 +667,13 @@ __global__ void __launch_bounds__(kRowWarps * 32, 6)
       for (int o = 0; o < p.num_groups; ++o) {
         const float ov = __shfl_sync(0xffffffffu, value, o * lpg, LPR);
         place += ov > value || (ov == value && o < g);
-        unsure |= o != g && fabsf(ov - value) <= slack;
       }
-      unsure = unsure && value > kNone;
-      if (!(place < p.topk_groups)) {
+      const bool chosen = place < p.topk_groups;
+      // the best group left out, and whether a chosen one is nearer to it than the errors
+      const float out = row_max(chosen ? kNone : value);
+      const float reach = row_max(chosen ? kNone : slack);
+      unsure = chosen && value > kNone && out > kNone && value - out <= fmaxf(slack, reach);
+      if (!chosen) {
 #pragma unroll
         for (int i = 0; i < VPL; ++i) v[i] = kNone;
 #pragma unroll
@@ -700,6 +751,19 @@ __global__ void __launch_bounds__(kRowWarps * 32, 6)
       }
     }
     __syncwarp();
+    if (kBias) {
+      // is every pick certainly ahead of the next candidate?
+      bool close = false;
+      for (int j = q; j < min(p.k, count - 1) && fits; j += LPR)
+        close |= from_key(ranked[j]) - from_key(ranked[j + 1]) <= 2.f * delta;
+      if (__any_sync(0xffffffffu, close)) {
+        if (p.scoring == 0) {
+          unsure |= close;
+        } else {  // rank again in 64 bits; every candidate that matters is in the list
+          rank64<T, LPR>(l, p.bias, cand, ranked, fits ? count : 0);
+        }
+      }
+    }
     // each lane takes every LPR-th slot
     constexpr int kSlots = (8 + LPR - 1) / LPR;
     const int picks = fits ? min(count, p.k) : 0;
@@ -716,17 +780,6 @@ __global__ void __launch_bounds__(kRowWarps * 32, 6)
         const float x = Elem<T>::to_f(l[id[h]]);
         r[h] = p.scoring == 0 ? expf(x - m) * inv : 1.f / (1.f + expf(-x));
         sum += r[h];
-        if (kBias && j + 1 < count) {  // is the next one certainly behind?
-          const uint64_t n = ranked[j + 1];
-          const uint32_t k0 = static_cast<uint32_t>(c >> 32), k1 = static_cast<uint32_t>(n >> 32);
-          const float f0 = __uint_as_float((k0 >> 31) ? k0 & 0x7fffffffu : ~k0);
-          const float f1 = __uint_as_float((k1 >> 31) ? k1 & 0x7fffffffu : ~k1);
-          if (f0 - f1 <= 2.f * delta) {
-            const int o = static_cast<int>(~static_cast<uint32_t>(n));
-            // the same numbers tie for certain, but what follows the last slot may hide another
-            unsure |= j + 1 == p.k || x != Elem<T>::to_f(l[o]) || p.bias[id[h]] != p.bias[o];
-          }
-        }
       }
     }
     float scale = p.scaling;
