@@ -257,7 +257,8 @@ __global__ void __launch_bounds__(256)
 constexpr int kWarps = 8;
 constexpr int kMaxRecord = 608;  // int4_record_bytes(32, true)
 constexpr int kStageBlocks = 2;  // k64 blocks of a ring stage
-constexpr int kRing = 4;         // stages of a ring
+constexpr int kRing = 4;         // stages of a ring of int4_some_kernel
+constexpr int kFewRing = 3;      // and of the kernels for few rows
 
 __device__ __forceinline__ void cp_async_commit() {
   asm volatile("cp.async.commit_group;" ::: "memory");
@@ -284,14 +285,14 @@ __device__ __forceinline__ int find_expert(const int32_t* __restrict__ prefix, i
   return e;
 }
 
-// A warp's ring of kRing stages in shared memory, a stage holding `blocks` records of each of MATS
+// A warp's ring of kSlots stages in shared memory, a stage holding `blocks` records of each of MATS
 // matrices.  One lane issues bulk copies that signal a barrier per stage, so a warp waits for no
 // other one, and the ring runs ahead across units of work: memory stays busy while a unit is
 // finished.
-template <int MATS>
+template <int MATS, int kSlots>
 struct WeightRing {
   char* ring;
-  uint32_t bars;  // kRing barriers
+  uint32_t bars;  // kSlots barriers
   volatile int* abort_flag;
   uint32_t* err;
   int lane, matrix_bytes;  // of a stage, per matrix
@@ -308,7 +309,7 @@ struct WeightRing {
         if (MATS == 2) bulk_load(dst + matrix_bytes, src1, bytes, bar);
       }
     }
-    slot_in = (slot_in + 1) & (kRing - 1);
+    slot_in = slot_in + 1 == kSlots ? 0 : slot_in + 1;
   }
   // The stage's records, or whatever is there once a wait has run out (the error word is set).
   __device__ __forceinline__ const char* wait() {
@@ -319,26 +320,25 @@ struct WeightRing {
   __device__ __forceinline__ void drain() {
     if (!*abort_flag) return;
     const unsigned long long t0 = globaltimer_ns();
-    for (int i = 0; i < kRing; ++i)
+    for (int i = 0; i < kSlots; ++i)
       while (!mbar_try_wait(bars + 8 * i, i < slot ? phase : phase ^ 1u))
         if (globaltimer_ns() - t0 > kWaitLimitNs) break;
   }
   __device__ __forceinline__ void release() {
     __syncwarp();
-    slot = (slot + 1) & (kRing - 1);
+    slot = slot + 1 == kSlots ? 0 : slot + 1;
     phase ^= slot == 0;
   }
 };
 
-// q + 16 of the two columns' zero points (24 without).
+// 16 + the zero points of the two columns (24 without): as the nibbles, a zero point at the top of
+// the mantissa of a number in [16, 32).
 __device__ __forceinline__ void zero_points(const char* record, int per, int h, int gid, bool zeros,
                                             float& z0, float& z1) {
-  z0 = z1 = 24.f;
-  if (zeros) {
-    const uint32_t z = *reinterpret_cast<const uint16_t*>(record + 512 + 32 * per + 16 * h + 2 * gid);
-    z0 = 16.f + static_cast<float>(z & 0xffu);
-    z1 = 16.f + static_cast<float>(z >> 8);
-  }
+  uint32_t z = 0x0808u;
+  if (zeros) z = *reinterpret_cast<const uint16_t*>(record + 512 + 32 * per + 16 * h + 2 * gid);
+  z0 = __uint_as_float(0x41800000u | ((z & 15u) << 19));
+  z1 = __uint_as_float(0x41800000u | ((z & 0x0f00u) << 11));
 }
 
 // One k64 block of at most 8 rows: fin += the products of MATS records with the activations xv
@@ -388,6 +388,40 @@ __device__ __forceinline__ void few_block(const char* stage, int matrix_bytes, b
   }
 }
 
+// The `blocks` blocks of a warp's slice (of `per` that the ring holds places for): the activations
+// of a stage are under way while the one before is worked on.
+template <typename T, int MATS, bool kG32, typename Issue>
+__device__ __forceinline__ void few_slice(WeightRing<MATS, kFewRing>& w, const T* xr, int per,
+                                          int blocks, int rec, bool zeros, int lane,
+                                          float (&fin)[MATS][4], Issue& issue) {
+  uint4 xn[kStageBlocks][2];
+  auto load_x = [&](int b) {
+#pragma unroll
+    for (int i = 0; i < kStageBlocks; ++i)
+      if (b + i < blocks) {
+        xn[i][0] = *reinterpret_cast<const uint4*>(xr + 64 * (b + i));
+        xn[i][1] = *reinterpret_cast<const uint4*>(xr + 64 * (b + i) + 32);
+      }
+  };
+  load_x(0);
+  for (int b = 0; b < per; b += kStageBlocks) {
+    uint4 xv[kStageBlocks][2];
+#pragma unroll
+    for (int i = 0; i < kStageBlocks; ++i) {
+      xv[i][0] = xn[i][0];
+      xv[i][1] = xn[i][1];
+    }
+    load_x(b + kStageBlocks);
+    const char* stage = w.wait();
+#pragma unroll
+    for (int i = 0; i < kStageBlocks; ++i)
+      if (b + i < blocks)
+        few_block<T, MATS, kG32>(stage + i * rec, w.matrix_bytes, zeros, lane, xv[i], fin);
+    w.release();
+    issue();
+  }
+}
+
 constexpr int kFewPitch = 20;  // floats of a row of 16 partial sums
 
 __device__ __forceinline__ void store_partial(float* to, int lane, const float (&fin)[4]) {
@@ -397,9 +431,10 @@ __device__ __forceinline__ void store_partial(float* to, int lane, const float (
     to[(2 * tig + (i & 1)) * kFewPitch + gid + 8 * (i >> 1)] = fin[i];
 }
 
-__device__ __forceinline__ void init_rings(uint64_t (&bar)[kWarps][kRing], int* abort_flag) {
+template <int kSlots>
+__device__ __forceinline__ void init_rings(uint64_t (&bar)[kWarps][kSlots], int* abort_flag) {
   if ((threadIdx.x & 31) == 0)
-    for (int i = 0; i < kRing; ++i) mbar_init(smem_addr(&bar[threadIdx.x >> 5][i]), 1);
+    for (int i = 0; i < kSlots; ++i) mbar_init(smem_addr(&bar[threadIdx.x >> 5][i]), 1);
   if (threadIdx.x == 0) *abort_flag = 0;
   fence_barrier_init();
   __syncthreads();
@@ -480,7 +515,7 @@ struct RowTable {
 template <typename T, int MATS, bool kDown, bool kG32, bool kTable>
 __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) {
   extern __shared__ __align__(128) char smem[];
-  __shared__ alignas(8) uint64_t s_bar[kWarps][kRing];
+  __shared__ alignas(8) uint64_t s_bar[kWarps][kFewRing];
   __shared__ int s_abort;
   __shared__ RowTable s_table[1];
   RowTable& table = s_table[0];
@@ -497,10 +532,12 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) 
   const int nunits = (ntiles + wn_count - 1) / wn_count;
   const int units = (kTable ? table.chunks : __ldg(p.chunk_prefix + p.E)) * nunits;
   auto expert_of = [&](int c) { return kTable ? table.expert[c] : find_expert(p.chunk_prefix, p.E, c); };
-  WeightRing<MATS> w{smem + kWarps * MATS * 8 * kFewPitch * 4 + warp * kRing * MATS * p.rec,
-                     smem_addr(&s_bar[warp][0]), &s_abort, p.err, lane, p.rec};
-  int pu = blockIdx.x, pb = 0;  // the next record to ask for: unit, block within [0, per)
-  int64_t offset = 0;           // of its strip's record b0
+  const int matrix_bytes = kStageBlocks * p.rec;
+  WeightRing<MATS, kFewRing> w{
+      smem + kWarps * MATS * 8 * kFewPitch * 4 + warp * kFewRing * MATS * matrix_bytes,
+      smem_addr(&s_bar[warp][0]), &s_abort, p.err, lane, matrix_bytes};
+  int pu = blockIdx.x, pb = 0;  // the next stage to ask for: unit, first block within [0, per)
+  int64_t offset = 0;           // of its first record
   auto locate = [&]() {
     if (pu < units) {
       // a strip past the last one repeats it, and its results are dropped
@@ -511,9 +548,10 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) 
   auto issue = [&]() {
     if (pu >= units) return;
     w.issue(static_cast<const char*>(p.w[0]) + offset, static_cast<const char*>(p.w[1]) + offset,
-            b0 + pb < b1 ? p.rec : 0);
-    offset += p.rec;
-    if (++pb == per) {
+            max(min(kStageBlocks, b1 - b0 - pb), 0) * p.rec);
+    offset += matrix_bytes;
+    pb += kStageBlocks;
+    if (pb >= per) {
       pb = 0;
       pu += gridDim.x;
       locate();
@@ -521,7 +559,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) 
   };
   locate();
 #pragma unroll
-  for (int i = 0; i < kRing - 1; ++i) issue();
+  for (int i = 0; i < kFewRing - 1; ++i) issue();
 
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
     const int c = u / nunits;
@@ -540,22 +578,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) 
                                        : kTable ? table.row[r] / p.k
                                                 : __ldg(p.sorted_token + r)) * p.K;
     float fin[MATS][4] = {};
-    uint4 xn[2];
-    auto load_x = [&](int i) {
-      if (b0 + i < b1) {
-        xn[0] = *reinterpret_cast<const uint4*>(xr + 64 * i);
-        xn[1] = *reinterpret_cast<const uint4*>(xr + 64 * i + 32);
-      }
-    };
-    load_x(0);
-    for (int i = 0; i < per; ++i) {
-      const uint4 xv[2] = {xn[0], xn[1]};
-      load_x(i + 1);
-      const char* stage = w.wait();
-      if (b0 + i < b1) few_block<T, MATS, kG32>(stage, p.rec, p.zeros, lane, xv, fin);
-      w.release();
-      issue();
-    }
+    few_slice<T, MATS, kG32>(w, xr, per, b1 - b0, p.rec, p.zeros, lane, fin, issue);
 #pragma unroll
     for (int m = 0; m < MATS; ++m)
       store_partial(red + (warp * MATS + m) * 8 * kFewPitch, lane, fin[m]);
@@ -591,7 +614,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) 
 template <typename T, bool kG32>
 __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Params p) {
   extern __shared__ __align__(128) char smem[];
-  __shared__ alignas(8) uint64_t s_bar[kWarps][kRing];
+  __shared__ alignas(8) uint64_t s_bar[kWarps][kFewRing];
   __shared__ int s_abort;
   __shared__ RowTable table;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -606,10 +629,11 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Param
   int pieces = 1;
   while (pieces * 2 * chunks <= kWarps && kb >= 6 * pieces) pieces *= 2;
   const int tasks = chunks * pieces, per = (kb + pieces - 1) / pieces;
-  float* part = reinterpret_cast<float*>(smem + kWarps * kRing * p.rec);
-  WeightRing<1> w{smem + warp * kRing * p.rec, smem_addr(&s_bar[warp][0]), &s_abort, p.err, lane,
-                  p.rec};
-  int pn = blockIdx.x, pt = warp, pb = 0;  // the next record to ask for: strip, task, block
+  const int matrix_bytes = kStageBlocks * p.rec;
+  float* part = reinterpret_cast<float*>(smem + kWarps * kFewRing * matrix_bytes);
+  WeightRing<1, kFewRing> w{smem + warp * kFewRing * matrix_bytes, smem_addr(&s_bar[warp][0]),
+                            &s_abort, p.err, lane, matrix_bytes};
+  int pn = blockIdx.x, pt = warp, pb = 0;  // the next stage to ask for: strip, task, block
   int64_t offset = 0;
   int left = 0;
   auto locate = [&]() {
@@ -625,9 +649,11 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Param
   };
   auto issue = [&]() {
     if (pn >= ntiles || warp >= tasks) return;
-    w.issue(static_cast<const char*>(p.w[0]) + offset, nullptr, pb < left ? p.rec : 0);
-    offset += p.rec;
-    if (++pb == per) {
+    w.issue(static_cast<const char*>(p.w[0]) + offset, nullptr,
+            max(min(kStageBlocks, left - pb), 0) * p.rec);
+    offset += matrix_bytes;
+    pb += kStageBlocks;
+    if (pb >= per) {
       pb = 0;
       pt += kWarps;
       locate();
@@ -635,7 +661,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Param
   };
   locate();
 #pragma unroll
-  for (int i = 0; i < kRing - 1; ++i) issue();
+  for (int i = 0; i < kFewRing - 1; ++i) issue();
 
   for (int nt = blockIdx.x; nt < ntiles; nt += gridDim.x) {
     for (int t = warp; t < tasks; t += kWarps) {
@@ -644,22 +670,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Param
       const T* xr = static_cast<const T*>(p.x) + 8 * tig + 64 * b0 +
                     static_cast<int64_t>(row0 + min(gid, rows - 1)) * p.K;
       float fin[1][4] = {};
-      uint4 xn[2];
-      auto load_x = [&](int i) {
-        if (i < blocks) {
-          xn[0] = *reinterpret_cast<const uint4*>(xr + 64 * i);
-          xn[1] = *reinterpret_cast<const uint4*>(xr + 64 * i + 32);
-        }
-      };
-      load_x(0);
-      for (int i = 0; i < per; ++i) {
-        const uint4 xv[2] = {xn[0], xn[1]};
-        load_x(i + 1);
-        const char* stage = w.wait();
-        if (i < blocks) few_block<T, 1, kG32>(stage, p.rec, p.zeros, lane, xv, fin);
-        w.release();
-        issue();
-      }
+      few_slice<T, 1, kG32>(w, xr, per, blocks, p.rec, p.zeros, lane, fin, issue);
       store_partial(part + t * 8 * kFewPitch, lane, fin[0]);
     }
     __syncthreads();
@@ -711,7 +722,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) int4_some_kernel
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int nunits = (ntiles + kWarps - 1) / kWarps;
   const int64_t units = static_cast<int64_t>(__ldg(p.chunk_prefix + p.E)) * nunits;
-  WeightRing<MATS> w{smem + kXRing * kXBytes + warp * kRing * MATS * kStageBlocks * p.rec,
+  WeightRing<MATS, kRing> w{smem + kXRing * kXBytes + warp * kRing * MATS * kStageBlocks * p.rec,
                      smem_addr(&s_bar[warp][0]), &s_abort, p.err, lane, kStageBlocks * p.rec};
   const int nstages = (kb + kStageBlocks - 1) / kStageBlocks;
   int64_t pu = blockIdx.x, strip = 0;  // the next stage to ask for: unit (its strip), stage
@@ -940,14 +951,15 @@ template <typename T, int MATS, bool kDown, bool kG32, bool kTable>
 struct Few {
   static constexpr auto kernel = int4_few_kernel<T, MATS, kDown, kG32, kTable>;
   static size_t smem(int rec) {
-    return static_cast<size_t>(kWarps) * MATS * (8 * kFewPitch * 4 + kRing * rec);
+    return static_cast<size_t>(kWarps) * MATS *
+           (8 * kFewPitch * 4 + kFewRing * kStageBlocks * rec);
   }
   static bool launch(Int4Params p, int num_sms, cudaStream_t s) {
     // pieces of K: a call that the table serves has few units, so as many as leave a warp three
     // blocks; else eight blocks, for fewer sums across warps
     p.wk = kWarps;
     while (p.wk > 1 && p.K / 64 < (kTable ? 3 : 8) * p.wk) p.wk /= 2;
-    // three CTAs on an SM: 3 x (10 + 38 + 2 KB) at most
+    // three CTAs on an SM: 3 x (10 + 57 + 2 KB) at most
     return launch_dependent(kernel, num_sms * 3, kWarps * 32, smem(p.rec), s, p);
   }
 };
@@ -959,7 +971,8 @@ struct FewDown {
   // partial results: one task per chunk, or fewer than 2 kWarps with K in pieces
   static size_t smem(int rec, int rows) {
     const int tasks = rows > kWarps ? rows : kWarps;
-    return static_cast<size_t>(kWarps) * kRing * rec + static_cast<size_t>(tasks) * 8 * kFewPitch * 4;
+    return static_cast<size_t>(kWarps) * kFewRing * kStageBlocks * rec +
+           static_cast<size_t>(tasks) * 8 * kFewPitch * 4;
   }
   static bool launch(const Int4Params& p, int num_sms, cudaStream_t s) {
     const int grid = p.N / 16 < num_sms * 3 ? p.N / 16 : num_sms * 3;
@@ -1053,7 +1066,7 @@ void launch_int4_expand(int dtype, const void* w, int E, int K, int N, int G, bo
 
 int int4_chunk_rows(int64_t rows, int E) {
   const int64_t per = rows / E;
-  return per <= 4 ? 8 : per <= 24 ? 32 : 64;
+  return per <= 4 ? 8 : 32;
 }
 
 int launch_int4_quantize(int dtype, const void* w, int E, int K, int N, int G, int symmetric,
