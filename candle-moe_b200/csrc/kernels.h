@@ -184,6 +184,12 @@ struct Int4Params {
   const uint32_t* idx;          // [T, k]
   int rows, k;                  // T*k, k
 };
+// moe_int4_mma.cu: both products of calls with many rows per expert (route preparation in chunks of
+// int4_many_rows()); N and K of both multiples of 128.  False: a launch failed.
+int int4_many_rows();
+bool int4_many_set_attributes();
+bool launch_int4_many(int dtype, const Int4Params& g1, const Int4Params& g2, int num_sms,
+                      cudaStream_t s);
 int int4_table_rows();
 // Both products of such a call; returns the number of kernels launched (0: a launch failed).
 int launch_int4_table_ffn(int dtype, const Int4Params& g1, const Int4Params& g2, int num_sms,
@@ -191,7 +197,8 @@ int launch_int4_table_ffn(int dtype, const Int4Params& g1, const Int4Params& g2,
 // Bytes of a packed record (16 columns x 64 k).
 int int4_record_bytes(int G, bool zeros);
 bool int4_set_attributes();
-int int4_chunk_rows(int64_t rows, int E);
+// Rows per chunk of the kernel that serves a call of this many rows.
+int int4_chunk_rows(int64_t rows, int E, int H, int I);
 int launch_int4_quantize(int dtype, const void* w, int E, int K, int N, int G, int symmetric,
                          uint8_t* q, void* scales, uint8_t* zeros, int num_sms, cudaStream_t s);
 // Both return the number of kernels launched (0: a launch failed).

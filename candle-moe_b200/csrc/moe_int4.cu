@@ -26,29 +26,15 @@
 // of the mantissa.
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "common.cuh"
+#include "int4.cuh"
 #include "kernels.h"
 
 namespace cmoe {
 
 namespace {
-
-template <typename T> struct Nib;
-template <> struct Nib<__nv_bfloat16> {
-  static constexpr int kShift = 3;  // 7 mantissa bits
-  static constexpr uint32_t kMask = 0x00780078u, kMagic = 0x41804180u, kOne = 0x3f803f80u;
-};
-template <> struct Nib<__half> {
-  static constexpr int kShift = 6;  // 10 mantissa bits
-  static constexpr uint32_t kMask = 0x03c003c0u, kMagic = 0x4c004c00u, kOne = 0x3c003c00u;
-};
-
-__device__ __forceinline__ uint32_t rotr(uint32_t v, int n) { return __funnelshift_r(v, v, n); }
-
-// Fragment register i of a packed word: the pair (16 + q_lo, 16 + q_hi).
-template <typename T> __device__ __forceinline__ uint32_t nib_pair(uint32_t w, int i) {
-  return (rotr(w, 4 * i) & Nib<T>::kMask) | Nib<T>::kMagic;
-}
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -188,10 +174,6 @@ __global__ void int4_pack_groups_kernel(const uint16_t* __restrict__ scales,
 
 // ---- weights back in 16 bits (for calls of many rows) --------------------------------------------
 
-template <typename T> struct Pair;
-template <> struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
-template <> struct Pair<__half> { using type = __half2; };
-
 // One CTA per (expert, 64 k, 128 n): a warp takes 16 n (one packed tile), the rows leave through
 // shared memory in 256-byte (out [E,K,N]) or 128-byte (kTrans: out [E,N,K]) pieces.  q - z is
 // exact, the product with the scale is rounded once.
@@ -255,7 +237,6 @@ __global__ void __launch_bounds__(256)
 // ---- the products ------------------------------------------------------------------------------
 
 constexpr int kWarps = 8;
-constexpr int kMaxRecord = 608;  // int4_record_bytes(32, true)
 constexpr int kStageBlocks = 2;  // k64 blocks of a ring stage
 constexpr int kRing = 4;         // stages of a ring of int4_some_kernel
 constexpr int kFewRing = 3;      // and of the kernels for few rows
@@ -266,15 +247,6 @@ __device__ __forceinline__ void cp_async_commit() {
 template <int N> __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
-                                          uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          dst),
-      "l"(src), "r"(bytes), "r"(bar)
-      : "memory");
-}
-
 // Expert of chunk c: the number of experts whose chunks all come before it.
 __device__ __forceinline__ int find_expert(const int32_t* __restrict__ prefix, int E, int c) {
   int e = 0;
@@ -284,52 +256,6 @@ __device__ __forceinline__ int find_expert(const int32_t* __restrict__ prefix, i
   }
   return e;
 }
-
-// A warp's ring of kSlots stages in shared memory, a stage holding `blocks` records of each of MATS
-// matrices.  One lane issues bulk copies that signal a barrier per stage, so a warp waits for no
-// other one, and the ring runs ahead across units of work: memory stays busy while a unit is
-// finished.
-template <int MATS, int kSlots>
-struct WeightRing {
-  char* ring;
-  uint32_t bars;  // kSlots barriers
-  volatile int* abort_flag;
-  uint32_t* err;
-  int lane, matrix_bytes;  // of a stage, per matrix
-  int slot_in = 0, slot = 0;
-  uint32_t phase = 0;
-
-  __device__ __forceinline__ void issue(const char* src0, const char* src1, uint32_t bytes) {
-    if (lane == 0) {
-      const uint32_t bar = bars + 8 * slot_in;
-      mbar_arrive_expect_tx(bar, MATS * bytes);
-      if (bytes) {
-        const uint32_t dst = smem_addr(ring) + slot_in * MATS * matrix_bytes;
-        bulk_load(dst, src0, bytes, bar);
-        if (MATS == 2) bulk_load(dst + matrix_bytes, src1, bytes, bar);
-      }
-    }
-    slot_in = slot_in + 1 == kSlots ? 0 : slot_in + 1;
-  }
-  // The stage's records, or whatever is there once a wait has run out (the error word is set).
-  __device__ __forceinline__ const char* wait() {
-    mbar_wait_bounded(bars + 8 * slot, phase, abort_flag, err, kErrWaitFull);
-    return ring + slot * MATS * matrix_bytes;
-  }
-  // After a wait that ran out: no copy may land once the CTA is gone (each wait again bounded).
-  __device__ __forceinline__ void drain() {
-    if (!*abort_flag) return;
-    const unsigned long long t0 = globaltimer_ns();
-    for (int i = 0; i < kSlots; ++i)
-      while (!mbar_try_wait(bars + 8 * i, i < slot ? phase : phase ^ 1u))
-        if (globaltimer_ns() - t0 > kWaitLimitNs) break;
-  }
-  __device__ __forceinline__ void release() {
-    __syncwarp();
-    slot = slot + 1 == kSlots ? 0 : slot + 1;
-    phase ^= slot == 0;
-  }
-};
 
 // 16 + the zero points of the two columns (24 without): as the nibbles, a zero point at the top of
 // the mantissa of a number in [16, 32).
@@ -930,23 +856,6 @@ int grid_for(int64_t n, int num_sms) {
   return static_cast<int>(b < cap ? b : cap);
 }
 
-// Launched as a programmatic dependent: waits for the kernel before it with griddepcontrol.wait.
-template <typename... Args>
-bool launch_dependent(void (*kernel)(Args...), int grid, int threads, size_t smem, cudaStream_t s,
-                      Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(static_cast<unsigned>(threads));
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess;
-}
-
 template <typename T, int MATS, bool kDown, bool kG32, bool kTable>
 struct Few {
   static constexpr auto kernel = int4_few_kernel<T, MATS, kDown, kG32, kTable>;
@@ -1005,9 +914,7 @@ template <typename T, bool kG32> bool allow_few() {
 }
 template <typename T> bool gemm_attributes() {
   return allow_few<T, false>() && allow_few<T, true>() && allow_smem<Some<T, 2, false, 4>>() &&
-         allow_smem<Some<T, 2, false, 8>>() && allow_smem<Some<T, 1, false, 4>>() &&
-         allow_smem<Some<T, 1, false, 8>>() && allow_smem<Some<T, 1, true, 4>>() &&
-         allow_smem<Some<T, 1, true, 8>>();
+         allow_smem<Some<T, 1, false, 4>>() && allow_smem<Some<T, 1, true, 4>>();
 }
 
 template <typename T, bool kG32, bool kTable>
@@ -1033,7 +940,8 @@ bool launch_ffn(int chunk, const Int4Params& g1, const Int4Params& g2, const uin
   const bool ok = chunk == 8    ? (g1.G == 32 ? launch_few<T, true>(g1, g2, num_sms, s)
                                               : launch_few<T, false>(g1, g2, num_sms, s))
                   : chunk == 32 ? launch_some<T, 4>(g1, g2, num_sms, s)
-                                : launch_some<T, 8>(g1, g2, num_sms, s);
+                                : launch_int4_many(std::is_same<T, __nv_bfloat16>::value ? kBF16 : kF16, g1,
+                                                   g2, num_sms, s);
   return ok && launch_dependent(int4_combine_kernel<T>, grid_for(T_ * g2.N, num_sms), 256, 0, s,
                                 static_cast<const float*>(g2.out), idx, T_, k, g2.N, g2.E,
                                 static_cast<T*>(out));
@@ -1056,7 +964,9 @@ void expand(const void* w, int E, int K, int N, int G, bool zeros, bool trans, v
 
 int int4_record_bytes(int G, bool zeros) { return 512 + (G == 32 ? 2 : 1) * (zeros ? 48 : 32); }
 
-bool int4_set_attributes() { return gemm_attributes<__nv_bfloat16>() && gemm_attributes<__half>(); }
+bool int4_set_attributes() {
+  return gemm_attributes<__nv_bfloat16>() && gemm_attributes<__half>() && int4_many_set_attributes();
+}
 
 void launch_int4_expand(int dtype, const void* w, int E, int K, int N, int G, bool zeros,
                         bool trans, void* out, cudaStream_t s) {
@@ -1064,9 +974,9 @@ void launch_int4_expand(int dtype, const void* w, int E, int K, int N, int G, bo
   else expand<__half>(w, E, K, N, G, zeros, trans, out, s);
 }
 
-int int4_chunk_rows(int64_t rows, int E) {
-  const int64_t per = rows / E;
-  return per <= 4 ? 8 : 32;
+int int4_chunk_rows(int64_t rows, int E, int H, int I) {
+  if (rows <= 4 * static_cast<int64_t>(E)) return 8;
+  return H % 128 == 0 && I % 128 == 0 ? int4_many_rows() : 32;
 }
 
 int launch_int4_quantize(int dtype, const void* w, int E, int K, int N, int G, int symmetric,

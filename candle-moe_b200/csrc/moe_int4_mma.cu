@@ -1,0 +1,444 @@
+// Q, many rows per expert: the products on the fifth-generation tensor cores.
+//
+// A tile is 128 weight columns (of gate and of up, or of down) times at most 64 rows of one expert.
+// The weights are the MMA's 128-row operand and come from tensor memory: eight warps stream
+// their records through rings in shared memory, unpack them in registers -- (q - z) exactly,
+// times the scale, one rounding to the 16-bit type -- and store them as they lie: the packed
+// fragment order is the 16x128b shape of tcgen05.st, so nothing is shuffled and shared memory
+// carries only the packed nibbles.  The rows are the other operand, from shared memory in the
+// 128-byte swizzle.  The order of k inside a fragment (see moe_int4.cu) makes column 4 c + t of
+// a half the k pair 4 t + c of it, so the warps that gather the rows put their 4-byte pairs
+// there.  The sums stay in tensor memory for all of K (two sets, so that the epilogue of a tile
+// runs under the next one) and leave it one weight column per thread.
+//
+// What bounds it: unpacking, 75 to 85 warp instructions for a record of 1024 weights, 20 to 25
+// cycles of an SM's issue slots against 24 cycles of its share of the memory rate; the MMAs of
+// 64 rows take 16 cycles.
+#include <stdint.h>
+
+#include "common.cuh"
+#include "int4.cuh"
+#include "kernels.h"
+
+namespace cmoe {
+
+namespace {
+
+constexpr int kTileRows = 64;
+constexpr int kUnpackWarps = 8, kOutWarps = 4, kGatherWarps = 4;
+constexpr int kThreads = (kUnpackWarps + kOutWarps + kGatherWarps + 1) * 32;
+constexpr int kAStages = 4;  // k64 blocks of unpacked weights
+constexpr int kXStages = 6;  // k64 blocks of rows
+constexpr int kXBytes = kTileRows * 128;
+constexpr int kRingSlots = 4, kRingRecords = 4;
+
+// D[tmem] (+)= A[tmem] * B[smem], kind::f16.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 16 lanes x 32 columns: register 2 j + r of lane (gid, tig) goes to lane gid + 8 r, column 4 j + tig.
+__device__ __forceinline__ void tmem_st_16x128b_x8(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+template <typename T> struct Fmt;
+template <> struct Fmt<__half> { static constexpr uint32_t v = 0; };
+template <> struct Fmt<__nv_bfloat16> { static constexpr uint32_t v = 1; };
+
+// The 16-bit pattern of 16 + z, twice.
+template <typename T> __device__ __forceinline__ uint32_t zero_pair(uint32_t z) {
+  return Nib<T>::kMagic | ((z << Nib<T>::kShift) * 0x10001u);
+}
+
+// The record's weights in the order of tmem_st_16x128b_x8.
+template <typename T>
+__device__ __forceinline__ void unpack_record(const char* record, int per, bool zeros, int lane,
+                                              uint32_t (&out)[16]) {
+  using T2 = typename Pair<T>::type;
+  const int gid = lane >> 2;
+  const uint4 wq = *(reinterpret_cast<const uint4*>(record) + lane);
+  const uint32_t word[4] = {wq.x, wq.y, wq.z, wq.w};
+  T2 sc[2], off[2];
+  auto group = [&](int h) {
+    const T2 s = *(reinterpret_cast<const T2*>(record + 512 + 32 * h) + gid);
+    sc[0].x = sc[0].y = s.x;
+    sc[1].x = sc[1].y = s.y;
+    uint32_t z = 0x0808u;
+    if (zeros) z = *reinterpret_cast<const uint16_t*>(record + 512 + 32 * per + 16 * h + 2 * gid);
+    const uint32_t z0 = zero_pair<T>(z & 15u), z1 = zero_pair<T>((z >> 8) & 15u);
+    off[0] = *reinterpret_cast<const T2*>(&z0);
+    off[1] = *reinterpret_cast<const T2*>(&z1);
+  };
+  group(0);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (h == 1 && per == 2) group(1);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t u = nib_pair<T>(word[2 * h + (c >> 1)], 2 * (c & 1) + r);
+        const T2 v = __hmul2(__hsub2(*reinterpret_cast<const T2*>(&u), off[r]), sc[r]);
+        out[2 * (4 * h + c) + r] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+  }
+}
+
+template <typename T, int MATS, bool kDown>
+__global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
+  constexpr int kStrips = MATS;                            // of an unpacking warp
+  constexpr int kStageBlocks = kRingRecords / kStrips;     // k64 blocks of a ring stage
+  constexpr int kAccCols = MATS * kTileRows;               // of one set of sums
+  constexpr int kACols = MATS * 32;                        // of one block of weights
+  constexpr int kTmemCols = MATS == 2 ? 512 : 256;
+  static_assert(2 * kAccCols + kAStages * kACols <= kTmemCols, "tensor memory");
+  extern __shared__ __align__(128) char smem_raw[];
+  __shared__ alignas(8) uint64_t s_ring[kUnpackWarps][kRingSlots];
+  __shared__ alignas(8) uint64_t a_full[kAStages], a_empty[kAStages];
+  __shared__ alignas(8) uint64_t x_full[kXStages], x_empty[kXStages];
+  __shared__ alignas(8) uint64_t acc_full[2], acc_empty[2], s_done;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort, s_never;
+  const uint32_t raw = smem_addr(smem_raw);
+  const uint32_t x_base = (raw + 1023u) & ~1023u;
+  char* x_smem = smem_raw + (x_base - raw);
+  char* rings = x_smem + kXStages * kXBytes;
+  int32_t* s_cp = reinterpret_cast<int32_t*>(rings + kUnpackWarps * kRingSlots * kRingRecords * p.rec);
+  int32_t* s_off = s_cp + p.E + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int E = p.E, kb = p.K / 64, MT = p.N / 128;
+
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < kUnpackWarps; ++w)
+      for (int i = 0; i < kRingSlots; ++i) mbar_init(smem_addr(&s_ring[w][i]), 1);
+    for (int i = 0; i < kAStages; ++i) {
+      mbar_init(smem_addr(&a_full[i]), kUnpackWarps);
+      mbar_init(smem_addr(&a_empty[i]), 1);
+    }
+    for (int i = 0; i < kXStages; ++i) {
+      mbar_init(smem_addr(&x_full[i]), kGatherWarps);
+      mbar_init(smem_addr(&x_empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_addr(&acc_full[i]), 1);
+      mbar_init(smem_addr(&acc_empty[i]), kOutWarps);
+    }
+    mbar_init(smem_addr(&s_done), 1);
+    s_abort = s_never = 0;
+    fence_barrier_init();
+  }
+  if (warp == kThreads / 32 - 1) {
+    tmem_alloc(smem_addr(&s_tmem), kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem, tmem_a = tmem + 2 * kAccCols;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  for (int i = threadIdx.x; i <= E; i += kThreads) {
+    s_cp[i] = __ldg(p.chunk_prefix + i);
+    s_off[i] = __ldg(p.offsets + i);
+  }
+  __syncthreads();
+  const int64_t units = static_cast<int64_t>(s_cp[E]) * MT;
+  struct Unit {
+    int e, mt, row0, rows;
+  };
+  auto unit_of = [&](int64_t u) {
+    Unit d;
+    const int c = static_cast<int>(u / MT);
+    d.mt = static_cast<int>(u % MT);
+    d.e = expert_of_tile_smem(s_cp, E, c);
+    d.row0 = s_off[d.e] + (c - s_cp[d.e]) * kTileRows;
+    d.rows = min(kTileRows, s_off[d.e + 1] - d.row0);
+    return d;
+  };
+
+  if (warp < kUnpackWarps) {
+    // ------------------------------------------------------------------ weights into TMEM
+    const int q = warp & 3, half = warp >> 2;
+    const int m = MATS == 2 ? half : 0;                     // matrix
+    const int strip0 = 2 * q + (MATS == 2 ? 0 : half);      // first strip of the tile's eight
+    const uint32_t lanes = static_cast<uint32_t>(16 * strip0) << 16;
+    const int per = p.G == 32 ? 2 : 1;
+    const int matrix_bytes = kStageBlocks * p.rec;
+    WeightRing<kStrips, kRingSlots> w{rings + warp * kRingSlots * kRingRecords * p.rec,
+                                      smem_addr(&s_ring[warp][0]), &s_abort, p.err, lane,
+                                      matrix_bytes};
+    int64_t pu = blockIdx.x;  // the next stage to ask for: unit, first block
+    int pb = 0;
+    const char* src = nullptr;
+    const int64_t strip_bytes = static_cast<int64_t>(kb) * p.rec;
+    auto locate = [&]() {
+      if (pu < units) {
+        const Unit d = unit_of(pu);
+        src = static_cast<const char*>(p.w[m]) +
+              (static_cast<int64_t>(d.e) * (p.N / 16) + d.mt * 8 + strip0) * strip_bytes;
+      }
+    };
+    auto issue = [&]() {
+      if (pu >= units) return;
+      w.issue(src, src + strip_bytes, min(kStageBlocks, kb - pb) * p.rec);
+      src += matrix_bytes;
+      pb += kStageBlocks;
+      if (pb >= kb) {
+        pb = 0;
+        pu += gridDim.x;
+        locate();
+      }
+    };
+    locate();
+#pragma unroll
+    for (int i = 0; i < kRingSlots - 1; ++i) issue();
+    int as = 0;
+    uint32_t phase = 0;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+      for (int b = 0; b < kb; b += kStageBlocks) {
+        const char* stage = w.wait();
+#pragma unroll
+        for (int i = 0; i < kStageBlocks; ++i) {
+          if (b + i >= kb) break;
+          uint32_t regs[kStrips][16];
+#pragma unroll
+          for (int s = 0; s < kStrips; ++s)
+            unpack_record<T>(stage + s * matrix_bytes + i * p.rec, per, p.zeros, lane, regs[s]);
+          // after a wait that ran out this goes on with what is there, to the end of the units
+          mbar_wait_bounded(smem_addr(&a_empty[as]), phase ^ 1u, &s_abort, p.err, kErrWaitEmpty);
+          __syncwarp();
+          tc_fence_after();
+#pragma unroll
+          for (int s = 0; s < kStrips; ++s)
+            tmem_st_16x128b_x8(tmem_a + as * kACols + m * 32 + lanes + ((16u * s) << 16), regs[s]);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_addr(&a_full[as]));
+          if (++as == kAStages) {
+            as = 0;
+            phase ^= 1u;
+          }
+        }
+        w.release();
+        issue();
+      }
+    }
+    w.drain();
+  } else if (warp < kUnpackWarps + kOutWarps) {
+    // ------------------------------------------------------------------ sums out of TMEM
+    const int q = warp & 3;
+    int buf = 0;
+    uint32_t phase = 0;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+      const Unit d = unit_of(u);
+      const int col = d.mt * 128 + 32 * q + lane;
+      const bool ok = mbar_wait_bounded(smem_addr(&acc_full[buf]), phase, &s_abort, p.err,
+                                        kErrWaitAccFull);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      const uint32_t t = tmem + buf * kAccCols + (static_cast<uint32_t>(32 * q) << 16);
+      for (int r0 = 0; r0 < d.rows; r0 += 16) {
+        uint32_t v[16], g[16];
+        tmem_ld_32x32b_x16(t + r0, v);
+        if (MATS == 2) tmem_ld_32x32b_x16(t + kTileRows + r0, g);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (r0 + i >= d.rows) break;
+          const int row = d.row0 + r0 + i;
+          float y = __uint_as_float(v[i]);
+          if (kDown) {
+            static_cast<float*>(p.out)[static_cast<int64_t>(__ldg(p.sorted_flat + row)) * p.N + col] =
+                y * __ldg(p.sorted_w + row);
+          } else {
+            y = act_apply(y, p.act);
+            if (MATS == 2) y *= __uint_as_float(g[i]);
+            // the intermediate is rounded to the 16-bit type that the second product reads
+            static_cast<T*>(p.out)[static_cast<int64_t>(row) * p.N + col] = Elem<T>::from_f(y);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_addr(&acc_empty[buf]));
+      buf ^= 1;
+      phase ^= buf == 0;
+    }
+  } else if (warp < kUnpackWarps + kOutWarps + kGatherWarps) {
+    // ------------------------------------------------------------------ rows into shared memory
+    // Thread g takes 16 bytes (half h, t: k pairs 4 t .. 4 t + 3 of the half) of rows q + 16 i,
+    // and stores pair 4 t + c at 4 c + t.  Rows past the tile's repeat its last one; their sums
+    // are not read.
+    const int g = threadIdx.x - (kUnpackWarps + kOutWarps) * 32;
+    const int c8 = g & 7, q = g >> 3, h = c8 >> 2, t = c8 & 3;
+    const T* src[4];
+    int64_t lu = blockIdx.x;  // the load side runs three blocks ahead of the store side
+    int lb = 0, lrows = 0;
+    auto locate = [&]() {
+      if (lu >= units) return;
+      const Unit d = unit_of(lu);
+      lrows = d.rows;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = d.row0 + min(q + 16 * i, d.rows - 1);
+        src[i] = static_cast<const T*>(p.x) +
+                 static_cast<int64_t>(kDown ? r : __ldg(p.sorted_token + r)) * p.K + c8 * 8;
+      }
+    };
+    auto load = [&](uint4 (&v)[4]) {
+      if (lu >= units) return;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (16 * i < lrows) v[i] = *reinterpret_cast<const uint4*>(src[i] + lb * 64);
+      if (++lb == kb) {
+        lb = 0;
+        lu += gridDim.x;
+        locate();
+      }
+    };
+    uint4 v[3][4];
+    locate();
+#pragma unroll
+    for (int i = 0; i < 3; ++i) load(v[i]);
+    int64_t su = blockIdx.x;
+    int sb = 0, srows = su < units ? unit_of(su).rows : 0, xs = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    while (ok && su < units) {
+#pragma unroll
+      for (int s = 0; s < 3; ++s) {
+        if (su >= units) break;
+        ok = mbar_wait_bounded(smem_addr(&x_empty[xs]), phase ^ 1u, &s_abort, p.err, kErrWaitEmpty);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        char* to = x_smem + xs * kXBytes + q * 128 + 4 * t;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (16 * i < srows) {
+            const uint32_t w[4] = {v[s][i].x, v[s][i].y, v[s][i].z, v[s][i].w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              *reinterpret_cast<uint32_t*>(to + i * 2048 + (((4 * h + c) ^ (q & 7)) << 4)) = w[c];
+          }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&x_full[xs]));
+        load(v[s]);
+        if (++xs == kXStages) {
+          xs = 0;
+          phase ^= 1u;
+        }
+        if (++sb == kb) {
+          sb = 0;
+          su += gridDim.x;
+          if (su < units) srows = unit_of(su).rows;
+        }
+      }
+    }
+  } else if (lane == 0) {
+    // ------------------------------------------------------------------ MMA issuer
+    int as = 0, xs = 0, buf = 0;
+    uint32_t a_phase = 0, x_phase = 0, acc_phase = 0;
+    bool ok = true;
+    for (int64_t u = blockIdx.x; ok && u < units; u += gridDim.x) {
+      const Unit d = unit_of(u);
+      const uint32_t idesc = umma_idesc(Fmt<T>::v, 0, 128, (d.rows + 15) & ~15);
+      ok = mbar_wait_bounded(smem_addr(&acc_empty[buf]), acc_phase ^ 1u, &s_abort, p.err,
+                             kErrWaitAccEmpty);
+      if (!ok) break;
+      tc_fence_after();
+      for (int b = 0; b < kb; ++b) {
+        ok = mbar_wait_bounded(smem_addr(&x_full[xs]), x_phase, &s_abort, p.err, kErrWaitFull) &&
+             mbar_wait_bounded(smem_addr(&a_full[as]), a_phase, &s_abort, p.err, kErrWaitFull);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          const uint64_t bdesc = umma_sdesc(x_base + xs * kXBytes + ks * 32, 16, 1024);
+#pragma unroll
+          for (int m = 0; m < MATS; ++m)
+            umma_f16_ts(tmem + buf * kAccCols + m * kTileRows,
+                        tmem_a + as * kACols + m * 32 + ks * 8, bdesc, idesc, b > 0 || ks > 0);
+        }
+        umma_commit(smem_addr(&a_empty[as]));
+        umma_commit(smem_addr(&x_empty[xs]));
+        if (++as == kAStages) {
+          as = 0;
+          a_phase ^= 1u;
+        }
+        if (++xs == kXStages) {
+          xs = 0;
+          x_phase ^= 1u;
+        }
+      }
+      if (!ok) break;
+      umma_commit(smem_addr(&acc_full[buf]));
+      buf ^= 1;
+      acc_phase ^= buf == 0;
+    }
+    // every MMA is done before the tensor memory and the operands go
+    umma_commit(smem_addr(&s_done));
+    mbar_wait_bounded(smem_addr(&s_done), 0, &s_never, p.err, kErrWaitDrain);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kThreads / 32 - 1) tmem_dealloc(tmem, kTmemCols);
+}
+
+size_t smem_bytes(int rec, int E) {
+  return 1024 + static_cast<size_t>(kXStages) * kXBytes +
+         static_cast<size_t>(kUnpackWarps) * kRingSlots * kRingRecords * rec +
+         static_cast<size_t>(2 * E + 2) * sizeof(int32_t);
+}
+
+template <typename T, int MATS, bool kDown>
+bool attribute() {
+  return cudaFuncSetAttribute(int4_many_kernel<T, MATS, kDown>,
+                              cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              static_cast<int>(smem_bytes(kMaxRecord, route_prep_max_experts()))) ==
+         cudaSuccess;
+}
+
+template <typename T>
+bool launch(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
+  const size_t smem = smem_bytes(g1.rec, g1.E);
+  return (g1.w[1] ? launch_dependent(int4_many_kernel<T, 2, false>, num_sms, kThreads, smem, s, g1)
+                  : launch_dependent(int4_many_kernel<T, 1, false>, num_sms, kThreads, smem, s,
+                                     g1)) &&
+         launch_dependent(int4_many_kernel<T, 1, true>, num_sms, kThreads, smem, s, g2);
+}
+
+}  // namespace
+
+int int4_many_rows() { return kTileRows; }
+
+bool int4_many_set_attributes() {
+  return attribute<__nv_bfloat16, 2, false>() && attribute<__nv_bfloat16, 1, false>() &&
+         attribute<__nv_bfloat16, 1, true>() && attribute<__half, 2, false>() &&
+         attribute<__half, 1, false>() && attribute<__half, 1, true>();
+}
+
+bool launch_int4_many(int dtype, const Int4Params& g1, const Int4Params& g2, int num_sms,
+                      cudaStream_t s) {
+  return dtype == kBF16 ? launch<__nv_bfloat16>(g1, g2, num_sms, s)
+                        : launch<__half>(g1, g2, num_sms, s);
+}
+
+}  // namespace cmoe

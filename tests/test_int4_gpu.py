@@ -37,7 +37,8 @@ def run(x, mats, w, idx, act, rounded=False):
 def test_ffn(T, E, k, H, I, G, dtype, zeros):
     for nomic in (False, True):
         x, mats, w, idx = make(T + E + H, T, E, k, H, I, G, dtype, zeros, nomic)
-        run(x, mats, w, idx, cm.Activation.Gelu if nomic else cm.Activation.Silu)
+        run(x, mats, w, idx, cm.Activation.Gelu if nomic else cm.Activation.Silu,
+            rounded=T * k > 4 * E)
 
 
 @pytest.mark.parametrize("act", [0, 1, 2])
@@ -54,7 +55,7 @@ def test_skipped_slots(T):
     idx[T - 1, 0] = -1
     if T > 3:
         idx[2] = 4
-    got = run(x, mats, w, idx, 0)
+    got = run(x, mats, w, idx, 0, rounded=True)
     if T > 1:
         assert (got[0] == 0).all()
     idx.fill_(6)
@@ -64,7 +65,7 @@ def test_skipped_slots(T):
 def test_all_rows_on_one_expert():
     x, mats, w, idx = make(78, 150, 5, 1, 128, 192, 32, "bf16", True, False)
     idx.fill_(3)
-    run(x, mats, w, idx, 0)
+    run(x, mats, w, idx, 0, rounded=True)
 
 
 def test_zero_tokens():
@@ -123,7 +124,7 @@ def test_quantised_layer_is_near_the_layer():
         step = np.repeat(m.scales.double().cpu().numpy(), 64, axis=1)
         assert (np.abs(v - w.double().cpu().numpy()) <= step * (1.0 + 16 * 2.0 ** -8)).all()
     w, idx = routing(np.random.default_rng(0), T, E, k)
-    got = run(x, mats, w, idx, 0)
+    got = run(x, mats, w, idx, 0, rounded=True)
     again = cm.FusedMoE(E, k).forward_int4(
         x, cm.Int4Experts.quantize(g, u, d, group_size=64, symmetric=False), w, idx)
     assert torch.equal(got, again)
@@ -208,4 +209,17 @@ def test_many_rows(T, E, k, H, I, G, dtype, zeros):
     """Calls whose weights are expanded to 16 bits (the bound counts those roundings)."""
     for nomic in (False, True):
         x, mats, w, idx = make(T + E, T, E, k, H, I, G, dtype, zeros, nomic, skip=0.1)
+        run(x, mats, w, idx, cm.Activation.Gelu if nomic else cm.Activation.Silu, rounded=True)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("T,E,k,H,I,G", [(40, 3, 2, 128, 128, 32), (33, 2, 1, 256, 128, 128),
+                                         (64, 4, 1, 128, 384, 64), (150, 9, 3, 512, 256, 64),
+                                         (70, 1, 1, 256, 256, 128), (100, 16, 4, 384, 640, 32)])
+def test_some_rows_per_expert(T, E, k, H, I, G, dtype, zeros):
+    """A few to a few tens of rows per expert, ragged, with experts of none and of many."""
+    for nomic in (False, True):
+        x, mats, w, idx = make(T + E + G, T, E, k, H, I, G, dtype, zeros, nomic, skip=0.1)
+        idx[: T // 2, 0] = 0
         run(x, mats, w, idx, cm.Activation.Gelu if nomic else cm.Activation.Silu, rounded=True)
