@@ -1,8 +1,9 @@
 // Q, many rows per expert: the products on the fifth-generation tensor cores.
 //
-// A tile is 128 weight columns (of gate and of up, or of down) times at most 64 rows of one expert.
-// The weights are the MMA's 128-row operand and come from tensor memory: eight warps stream
-// their records through rings in shared memory, unpack them in registers -- (q - z) exactly,
+// A tile is two panels of 128 weight columns (the same columns of gate and up, or 256 columns of one
+// matrix) times at most 64 rows of one expert.  The weights are the MMA's 128-row operand and
+// come from tensor memory: sixteen warps, a strip of 16 columns each, stream their records
+// through rings in shared memory, unpack them in registers -- (q - z) exactly,
 // times the scale, one rounding to the 16-bit type -- and store them as they lie: the packed
 // fragment order is the 16x128b shape of tcgen05.st, so nothing is shuffled and shared memory
 // carries only the packed nibbles.  The rows are the other operand, from shared memory in the
@@ -13,7 +14,8 @@
 //
 // What bounds it: unpacking, 75 to 85 warp instructions for a record of 1024 weights, 20 to 25
 // cycles of an SM's issue slots against 24 cycles of its share of the memory rate; the MMAs of
-// 64 rows take 16 cycles.
+// 64 rows take 16 cycles.  With eight unpacking warps the chain from a record to tensor memory
+// (600 cycles) set the pace, hence sixteen.
 #include <stdint.h>
 
 #include "common.cuh"
@@ -25,12 +27,16 @@ namespace cmoe {
 namespace {
 
 constexpr int kTileRows = 64;
-constexpr int kUnpackWarps = 8, kOutWarps = 4, kGatherWarps = 4;
+constexpr int kUnpackWarps = 16, kOutWarps = 4, kGatherWarps = 4;
 constexpr int kThreads = (kUnpackWarps + kOutWarps + kGatherWarps + 1) * 32;
 constexpr int kAStages = 4;  // k64 blocks of unpacked weights
 constexpr int kXStages = 6;  // k64 blocks of rows
 constexpr int kXBytes = kTileRows * 128;
-constexpr int kRingSlots = 4, kRingRecords = 4;
+constexpr int kRingSlots = 4, kRingRecords = 2;
+constexpr int kAccCols = 2 * kTileRows;  // of one set of sums, two panels
+constexpr int kACols = 2 * 32;           // of one block of weights
+constexpr int kTmemCols = 512;
+static_assert(2 * kAccCols + kAStages * kACols <= kTmemCols, "tensor memory");
 
 // D[tmem] (+)= A[tmem] * B[smem], kind::f16.
 __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
@@ -99,14 +105,10 @@ __device__ __forceinline__ void unpack_record(const char* record, int per, bool 
   }
 }
 
-template <typename T, int MATS, bool kDown>
+// kDual: the panels are gate and up, else the two halves of 256 columns.
+template <typename T, bool kDual, bool kDown>
 __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
-  constexpr int kStrips = MATS;                            // of an unpacking warp
-  constexpr int kStageBlocks = kRingRecords / kStrips;     // k64 blocks of a ring stage
-  constexpr int kAccCols = MATS * kTileRows;               // of one set of sums
-  constexpr int kACols = MATS * 32;                        // of one block of weights
-  constexpr int kTmemCols = MATS == 2 ? 512 : 256;
-  static_assert(2 * kAccCols + kAStages * kACols <= kTmemCols, "tensor memory");
+  constexpr int kCols = kDual ? 128 : 256;  // output columns of a unit
   extern __shared__ __align__(128) char smem_raw[];
   __shared__ alignas(8) uint64_t s_ring[kUnpackWarps][kRingSlots];
   __shared__ alignas(8) uint64_t a_full[kAStages], a_empty[kAStages];
@@ -121,7 +123,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
   int32_t* s_cp = reinterpret_cast<int32_t*>(rings + kUnpackWarps * kRingSlots * kRingRecords * p.rec);
   int32_t* s_off = s_cp + p.E + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int E = p.E, kb = p.K / 64, MT = p.N / 128;
+  const int E = p.E, kb = p.K / 64, MT = (p.N + kCols - 1) / kCols;
 
   if (threadIdx.x == 0) {
     for (int w = 0; w < kUnpackWarps; ++w)
@@ -173,31 +175,32 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
 
   if (warp < kUnpackWarps) {
     // ------------------------------------------------------------------ weights into TMEM
-    const int q = warp & 3, half = warp >> 2;
-    const int m = MATS == 2 ? half : 0;                     // matrix
-    const int strip0 = 2 * q + (MATS == 2 ? 0 : half);      // first strip of the tile's eight
-    const uint32_t lanes = static_cast<uint32_t>(16 * strip0) << 16;
+    const int panel = warp >> 3;
+    const int strip = 2 * (warp & 3) + ((warp >> 2) & 1);  // in this warp's quarter of the lanes
+    const uint32_t lanes = static_cast<uint32_t>(16 * strip) << 16;
     const int per = p.G == 32 ? 2 : 1;
-    const int matrix_bytes = kStageBlocks * p.rec;
-    WeightRing<kStrips, kRingSlots> w{rings + warp * kRingSlots * kRingRecords * p.rec,
+    const int matrix_bytes = kRingRecords * p.rec;
+    WeightRing<1, kRingSlots> w{rings + warp * kRingSlots * kRingRecords * p.rec,
                                       smem_addr(&s_ring[warp][0]), &s_abort, p.err, lane,
                                       matrix_bytes};
     int64_t pu = blockIdx.x;  // the next stage to ask for: unit, first block
     int pb = 0;
     const char* src = nullptr;
-    const int64_t strip_bytes = static_cast<int64_t>(kb) * p.rec;
     auto locate = [&]() {
       if (pu < units) {
         const Unit d = unit_of(pu);
-        src = static_cast<const char*>(p.w[m]) +
-              (static_cast<int64_t>(d.e) * (p.N / 16) + d.mt * 8 + strip0) * strip_bytes;
+        // a panel past the last column repeats the first strips; its sums are not read
+        int at = d.mt * (kCols / 16) + (kDual ? 0 : panel * 8) + strip;
+        if (at >= p.N / 16) at = strip;
+        src = static_cast<const char*>(p.w[kDual ? panel : 0]) +
+              (static_cast<int64_t>(d.e) * (p.N / 16) + at) * kb * p.rec;
       }
     };
     auto issue = [&]() {
       if (pu >= units) return;
-      w.issue(src, src + strip_bytes, min(kStageBlocks, kb - pb) * p.rec);
+      w.issue(src, nullptr, min(kRingRecords, kb - pb) * p.rec);
       src += matrix_bytes;
-      pb += kStageBlocks;
+      pb += kRingRecords;
       if (pb >= kb) {
         pb = 0;
         pu += gridDim.x;
@@ -210,22 +213,18 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
     int as = 0;
     uint32_t phase = 0;
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-      for (int b = 0; b < kb; b += kStageBlocks) {
+      for (int b = 0; b < kb; b += kRingRecords) {
         const char* stage = w.wait();
 #pragma unroll
-        for (int i = 0; i < kStageBlocks; ++i) {
+        for (int i = 0; i < kRingRecords; ++i) {
           if (b + i >= kb) break;
-          uint32_t regs[kStrips][16];
-#pragma unroll
-          for (int s = 0; s < kStrips; ++s)
-            unpack_record<T>(stage + s * matrix_bytes + i * p.rec, per, p.zeros, lane, regs[s]);
+          uint32_t regs[16];
+          unpack_record<T>(stage + i * p.rec, per, p.zeros, lane, regs);
           // after a wait that ran out this goes on with what is there, to the end of the units
           mbar_wait_bounded(smem_addr(&a_empty[as]), phase ^ 1u, &s_abort, p.err, kErrWaitEmpty);
           __syncwarp();
           tc_fence_after();
-#pragma unroll
-          for (int s = 0; s < kStrips; ++s)
-            tmem_st_16x128b_x8(tmem_a + as * kACols + m * 32 + lanes + ((16u * s) << 16), regs[s]);
+          tmem_st_16x128b_x8(tmem_a + as * kACols + panel * 32 + lanes, regs);
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
@@ -247,7 +246,8 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
     uint32_t phase = 0;
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
       const Unit d = unit_of(u);
-      const int col = d.mt * 128 + 32 * q + lane;
+      const int col = d.mt * kCols + 32 * q + lane;
+      const bool second = kDual || d.mt * kCols + 128 < p.N;
       const bool ok = mbar_wait_bounded(smem_addr(&acc_full[buf]), phase, &s_abort, p.err,
                                         kErrWaitAccFull);
       if (!__all_sync(0xffffffffu, ok)) break;
@@ -256,21 +256,33 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
       for (int r0 = 0; r0 < d.rows; r0 += 16) {
         uint32_t v[16], g[16];
         tmem_ld_32x32b_x16(t + r0, v);
-        if (MATS == 2) tmem_ld_32x32b_x16(t + kTileRows + r0, g);
+        tmem_ld_32x32b_x16(t + kTileRows + r0, g);
+        int flat = 0;
+        float wt = 0.f;
+        if (kDown) {  // a lane's row, handed around below
+          const int row = d.row0 + min(r0 + (lane & 15), d.rows - 1);
+          flat = __ldg(p.sorted_flat + row);
+          wt = __ldg(p.sorted_w + row);
+        }
         tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          if (r0 + i >= d.rows) break;
-          const int row = d.row0 + r0 + i;
-          float y = __uint_as_float(v[i]);
-          if (kDown) {
-            static_cast<float*>(p.out)[static_cast<int64_t>(__ldg(p.sorted_flat + row)) * p.N + col] =
-                y * __ldg(p.sorted_w + row);
-          } else {
-            y = act_apply(y, p.act);
-            if (MATS == 2) y *= __uint_as_float(g[i]);
-            // the intermediate is rounded to the 16-bit type that the second product reads
-            static_cast<T*>(p.out)[static_cast<int64_t>(row) * p.N + col] = Elem<T>::from_f(y);
+          const int64_t row = kDown ? __shfl_sync(0xffffffffu, flat, i) : d.row0 + r0 + i;
+          const float w = kDown ? __shfl_sync(0xffffffffu, wt, i) : 1.f;
+          if (r0 + i < d.rows) {
+            float y = __uint_as_float(v[i]), y2 = __uint_as_float(g[i]);
+            if (kDown) {
+              float* out = static_cast<float*>(p.out) + row * p.N + col;
+              out[0] = y * w;
+              if (second) out[128] = y2 * w;
+            } else {
+              // the intermediate is rounded to the 16-bit type that the second product reads
+              T* out = static_cast<T*>(p.out) + row * p.N + col;
+              y = act_apply(y, p.act);
+              if (kDual) y *= y2;
+              out[0] = Elem<T>::from_f(y);
+              if (!kDual && second) out[128] = Elem<T>::from_f(act_apply(y2, p.act));
+            }
           }
         }
       }
@@ -288,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
     const int g = threadIdx.x - (kUnpackWarps + kOutWarps) * 32;
     const int c8 = g & 7, q = g >> 3, h = c8 >> 2, t = c8 & 3;
     const T* src[4];
-    int64_t lu = blockIdx.x;  // the load side runs three blocks ahead of the store side
+    int64_t lu = blockIdx.x;  // the load side runs kAhead blocks ahead of the store side
     int lb = 0, lrows = 0;
     auto locate = [&]() {
       if (lu >= units) return;
@@ -312,17 +324,18 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
         locate();
       }
     };
-    uint4 v[3][4];
+    constexpr int kAhead = 2;
+    uint4 v[kAhead][4];
     locate();
 #pragma unroll
-    for (int i = 0; i < 3; ++i) load(v[i]);
+    for (int i = 0; i < kAhead; ++i) load(v[i]);
     int64_t su = blockIdx.x;
     int sb = 0, srows = su < units ? unit_of(su).rows : 0, xs = 0;
     uint32_t phase = 0;
     bool ok = true;
     while (ok && su < units) {
 #pragma unroll
-      for (int s = 0; s < 3; ++s) {
+      for (int s = 0; s < kAhead; ++s) {
         if (su >= units) break;
         ok = mbar_wait_bounded(smem_addr(&x_empty[xs]), phase ^ 1u, &s_abort, p.err, kErrWaitEmpty);
         ok = __all_sync(0xffffffffu, ok);
@@ -372,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
         for (int ks = 0; ks < 4; ++ks) {
           const uint64_t bdesc = umma_sdesc(x_base + xs * kXBytes + ks * 32, 16, 1024);
 #pragma unroll
-          for (int m = 0; m < MATS; ++m)
+          for (int m = 0; m < 2; ++m)
             umma_f16_ts(tmem + buf * kAccCols + m * kTileRows,
                         tmem_a + as * kACols + m * 32 + ks * 8, bdesc, idesc, b > 0 || ks > 0);
         }
@@ -408,9 +421,9 @@ size_t smem_bytes(int rec, int E) {
          static_cast<size_t>(2 * E + 2) * sizeof(int32_t);
 }
 
-template <typename T, int MATS, bool kDown>
+template <typename T, bool kDual, bool kDown>
 bool attribute() {
-  return cudaFuncSetAttribute(int4_many_kernel<T, MATS, kDown>,
+  return cudaFuncSetAttribute(int4_many_kernel<T, kDual, kDown>,
                               cudaFuncAttributeMaxDynamicSharedMemorySize,
                               static_cast<int>(smem_bytes(kMaxRecord, route_prep_max_experts()))) ==
          cudaSuccess;
@@ -419,10 +432,10 @@ bool attribute() {
 template <typename T>
 bool launch(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
   const size_t smem = smem_bytes(g1.rec, g1.E);
-  return (g1.w[1] ? launch_dependent(int4_many_kernel<T, 2, false>, num_sms, kThreads, smem, s, g1)
-                  : launch_dependent(int4_many_kernel<T, 1, false>, num_sms, kThreads, smem, s,
+  return (g1.w[1] ? launch_dependent(int4_many_kernel<T, true, false>, num_sms, kThreads, smem, s, g1)
+                  : launch_dependent(int4_many_kernel<T, false, false>, num_sms, kThreads, smem, s,
                                      g1)) &&
-         launch_dependent(int4_many_kernel<T, 1, true>, num_sms, kThreads, smem, s, g2);
+         launch_dependent(int4_many_kernel<T, false, true>, num_sms, kThreads, smem, s, g2);
 }
 
 }  // namespace
@@ -430,9 +443,9 @@ bool launch(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_
 int int4_many_rows() { return kTileRows; }
 
 bool int4_many_set_attributes() {
-  return attribute<__nv_bfloat16, 2, false>() && attribute<__nv_bfloat16, 1, false>() &&
-         attribute<__nv_bfloat16, 1, true>() && attribute<__half, 2, false>() &&
-         attribute<__half, 1, false>() && attribute<__half, 1, true>();
+  return attribute<__nv_bfloat16, true, false>() && attribute<__nv_bfloat16, false, false>() &&
+         attribute<__nv_bfloat16, false, true>() && attribute<__half, true, false>() &&
+         attribute<__half, false, false>() && attribute<__half, false, true>();
 }
 
 bool launch_int4_many(int dtype, const Int4Params& g1, const Int4Params& g2, int num_sms,
