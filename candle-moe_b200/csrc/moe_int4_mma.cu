@@ -349,7 +349,8 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
             for (int c = 0; c < 4; ++c)
               *reinterpret_cast<uint32_t*>(to + i * 2048 + (((4 * h + c) ^ (q & 7)) << 4)) = w[c];
           }
-        fence_proxy_async_smem();
+        // the MMA issuer orders these writes before its reads: a proxy fence here would wait for
+        // the loads under way as well
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_addr(&x_full[xs]));
         load(v[s]);
@@ -380,6 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
         ok = mbar_wait_bounded(smem_addr(&x_full[xs]), x_phase, &s_abort, p.err, kErrWaitFull) &&
              mbar_wait_bounded(smem_addr(&a_full[as]), a_phase, &s_abort, p.err, kErrWaitFull);
         if (!ok) break;
+        fence_proxy_async_smem();  // the rows were written through the generic proxy
         tc_fence_after();
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
