@@ -10,6 +10,33 @@
 namespace cmoe {
 namespace {
 
+// mbar_wait_bounded that parks the warp in each try (up to 10 us) instead of polling: with 25 warps
+// on an SM, most of them waiting, the polls take the issue slots of those that work.
+__device__ __forceinline__ bool mbar_wait_parked(uint32_t bar, uint32_t parity,
+                                                 volatile int* abort_flag, uint32_t* err,
+                                                 uint32_t code) {
+  unsigned long long t0 = 0;
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(10000u)
+        : "memory");
+    if (ok) return true;
+    if (*abort_flag) return false;
+    const unsigned long long now = globaltimer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > kWaitLimitNs) {
+      *abort_flag = 1;
+      if (err) atomicOr(err, code);
+      return false;
+    }
+  }
+}
+
 constexpr int kMaxRecord = 608;  // int4_record_bytes(32, true)
 
 template <typename T> struct Nib;
@@ -70,7 +97,7 @@ struct WeightRing {
   }
   // The stage's records, or whatever is there once a wait has run out (the error word is set).
   __device__ __forceinline__ const char* wait() {
-    mbar_wait_bounded(bars + 8 * slot, phase, abort_flag, err, kErrWaitFull);
+    mbar_wait_parked(bars + 8 * slot, phase, abort_flag, err, kErrWaitFull);
     return ring + slot * MATS * matrix_bytes;
   }
   // After a wait that ran out: no copy may land once the CTA is gone (each wait again bounded).

@@ -29,14 +29,14 @@ namespace {
 constexpr int kTileRows = 64;
 constexpr int kUnpackWarps = 16, kOutWarps = 4, kGatherWarps = 4;
 constexpr int kThreads = (kUnpackWarps + kOutWarps + kGatherWarps + 1) * 32;
-constexpr int kAStages = 4;  // k64 blocks of unpacked weights
-constexpr int kXStages = 6;  // k64 blocks of rows
-constexpr int kXBytes = kTileRows * 128;
-constexpr int kRingSlots = 4, kRingRecords = 2;
-constexpr int kAccCols = 2 * kTileRows;  // of one set of sums, two panels
-constexpr int kACols = 2 * 32;           // of one block of weights
+constexpr int kStages = 2;       // of two k64 blocks: weights in tensor memory, rows in shared memory
+constexpr int kStageBlocks = 2;
+constexpr int kXBytes = kTileRows * 128;  // a block's rows
+constexpr int kRingSlots = 4;             // of kStageBlocks records
+constexpr int kAccCols = 2 * kTileRows;   // of one set of sums, two panels
+constexpr int kACols = 2 * 32;            // of one block of weights
 constexpr int kTmemCols = 512;
-static_assert(2 * kAccCols + kAStages * kACols <= kTmemCols, "tensor memory");
+static_assert(2 * kAccCols + kStages * kStageBlocks * kACols <= kTmemCols, "tensor memory");
 
 // D[tmem] (+)= A[tmem] * B[smem], kind::f16.
 __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
@@ -111,30 +111,27 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
   constexpr int kCols = kDual ? 128 : 256;  // output columns of a unit
   extern __shared__ __align__(128) char smem_raw[];
   __shared__ alignas(8) uint64_t s_ring[kUnpackWarps][kRingSlots];
-  __shared__ alignas(8) uint64_t a_full[kAStages], a_empty[kAStages];
-  __shared__ alignas(8) uint64_t x_full[kXStages], x_empty[kXStages];
+  __shared__ alignas(8) uint64_t s_full[kStages], s_empty[kStages];
   __shared__ alignas(8) uint64_t acc_full[2], acc_empty[2], s_done;
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_never;
   const uint32_t raw = smem_addr(smem_raw);
   const uint32_t x_base = (raw + 1023u) & ~1023u;
   char* x_smem = smem_raw + (x_base - raw);
-  char* rings = x_smem + kXStages * kXBytes;
-  int32_t* s_cp = reinterpret_cast<int32_t*>(rings + kUnpackWarps * kRingSlots * kRingRecords * p.rec);
+  char* rings = x_smem + kStages * kStageBlocks * kXBytes;
+  int32_t* s_cp = reinterpret_cast<int32_t*>(rings + kUnpackWarps * kRingSlots * kStageBlocks * p.rec);
   int32_t* s_off = s_cp + p.E + 1;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // from a shuffle, so that the compiler knows it to be the same in the warp
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
   const int E = p.E, kb = p.K / 64, MT = (p.N + kCols - 1) / kCols;
 
   if (threadIdx.x == 0) {
     for (int w = 0; w < kUnpackWarps; ++w)
       for (int i = 0; i < kRingSlots; ++i) mbar_init(smem_addr(&s_ring[w][i]), 1);
-    for (int i = 0; i < kAStages; ++i) {
-      mbar_init(smem_addr(&a_full[i]), kUnpackWarps);
-      mbar_init(smem_addr(&a_empty[i]), 1);
-    }
-    for (int i = 0; i < kXStages; ++i) {
-      mbar_init(smem_addr(&x_full[i]), kGatherWarps);
-      mbar_init(smem_addr(&x_empty[i]), 1);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(smem_addr(&s_full[i]), kUnpackWarps + kGatherWarps);
+      mbar_init(smem_addr(&s_empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_addr(&acc_full[i]), 1);
@@ -179,8 +176,8 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
     const int strip = 2 * (warp & 3) + ((warp >> 2) & 1);  // in this warp's quarter of the lanes
     const uint32_t lanes = static_cast<uint32_t>(16 * strip) << 16;
     const int per = p.G == 32 ? 2 : 1;
-    const int matrix_bytes = kRingRecords * p.rec;
-    WeightRing<1, kRingSlots> w{rings + warp * kRingSlots * kRingRecords * p.rec,
+    const int matrix_bytes = kStageBlocks * p.rec;
+    WeightRing<1, kRingSlots> w{rings + warp * kRingSlots * matrix_bytes,
                                       smem_addr(&s_ring[warp][0]), &s_abort, p.err, lane,
                                       matrix_bytes};
     int64_t pu = blockIdx.x;  // the next stage to ask for: unit, first block
@@ -198,9 +195,9 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
     };
     auto issue = [&]() {
       if (pu >= units) return;
-      w.issue(src, nullptr, min(kRingRecords, kb - pb) * p.rec);
+      w.issue(src, nullptr, min(kStageBlocks, kb - pb) * p.rec);
       src += matrix_bytes;
-      pb += kRingRecords;
+      pb += kStageBlocks;
       if (pb >= kb) {
         pb = 0;
         pu += gridDim.x;
@@ -210,32 +207,31 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
     locate();
 #pragma unroll
     for (int i = 0; i < kRingSlots - 1; ++i) issue();
-    int as = 0;
+    int at = 0;
     uint32_t phase = 0;
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-      for (int b = 0; b < kb; b += kRingRecords) {
+      for (int b = 0; b < kb; b += kStageBlocks) {
         const char* stage = w.wait();
+        uint32_t regs[kStageBlocks][16];
 #pragma unroll
-        for (int i = 0; i < kRingRecords; ++i) {
-          if (b + i >= kb) break;
-          uint32_t regs[16];
-          unpack_record<T>(stage + i * p.rec, per, p.zeros, lane, regs);
-          // after a wait that ran out this goes on with what is there, to the end of the units
-          mbar_wait_bounded(smem_addr(&a_empty[as]), phase ^ 1u, &s_abort, p.err, kErrWaitEmpty);
-          __syncwarp();
-          tc_fence_after();
-          tmem_st_16x128b_x8(tmem_a + as * kACols + panel * 32 + lanes, regs);
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_addr(&a_full[as]));
-          if (++as == kAStages) {
-            as = 0;
-            phase ^= 1u;
-          }
-        }
+        for (int i = 0; i < kStageBlocks; ++i)
+          if (b + i < kb) unpack_record<T>(stage + i * p.rec, per, p.zeros, lane, regs[i]);
         w.release();
         issue();
+        // after a wait that ran out this goes on with what is there, to the end of the units
+        mbar_wait_parked(smem_addr(&s_empty[at]), phase ^ 1u, &s_abort, p.err, kErrWaitEmpty);
+        __syncwarp();
+        tc_fence_after();
+        const uint32_t to = tmem_a + at * kStageBlocks * kACols + panel * 32 + lanes;
+#pragma unroll
+        for (int i = 0; i < kStageBlocks; ++i)
+          if (b + i < kb) tmem_st_16x128b_x8(to + i * kACols, regs[i]);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&s_full[at]));
+        at ^= 1;
+        phase ^= at == 0;
       }
     }
     w.drain();
@@ -248,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
       const Unit d = unit_of(u);
       const int col = d.mt * kCols + 32 * q + lane;
       const bool second = kDual || d.mt * kCols + 128 < p.N;
-      const bool ok = mbar_wait_bounded(smem_addr(&acc_full[buf]), phase, &s_abort, p.err,
+      const bool ok = mbar_wait_parked(smem_addr(&acc_full[buf]), phase, &s_abort, p.err,
                                         kErrWaitAccFull);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
@@ -300,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
     const int g = threadIdx.x - (kUnpackWarps + kOutWarps) * 32;
     const int c8 = g & 7, q = g >> 3, h = c8 >> 2, t = c8 & 3;
     const T* src[4];
-    int64_t lu = blockIdx.x;  // the load side runs kAhead blocks ahead of the store side
+    int64_t lu = blockIdx.x;  // the load side runs a stage ahead of the store side
     int lb = 0, lrows = 0;
     auto locate = [&]() {
       if (lu >= units) return;
@@ -313,103 +309,108 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
                  static_cast<int64_t>(kDown ? r : __ldg(p.sorted_token + r)) * p.K + c8 * 8;
       }
     };
-    auto load = [&](uint4 (&v)[4]) {
+    uint4 v[kStageBlocks][4];
+    auto load = [&]() {
       if (lu >= units) return;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (16 * i < lrows) v[i] = *reinterpret_cast<const uint4*>(src[i] + lb * 64);
-      if (++lb == kb) {
+      for (int j = 0; j < kStageBlocks; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (16 * i < lrows && lb + j < kb)
+            v[j][i] = *reinterpret_cast<const uint4*>(src[i] + (lb + j) * 64);
+      lb += kStageBlocks;
+      if (lb >= kb) {
         lb = 0;
         lu += gridDim.x;
         locate();
       }
     };
-    constexpr int kAhead = 2;
-    uint4 v[kAhead][4];
     locate();
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) load(v[i]);
-    int64_t su = blockIdx.x;
-    int sb = 0, srows = su < units ? unit_of(su).rows : 0, xs = 0;
+    load();
+    int at = 0;
     uint32_t phase = 0;
     bool ok = true;
-    while (ok && su < units) {
-#pragma unroll
-      for (int s = 0; s < kAhead; ++s) {
-        if (su >= units) break;
-        ok = mbar_wait_bounded(smem_addr(&x_empty[xs]), phase ^ 1u, &s_abort, p.err, kErrWaitEmpty);
+    for (int64_t u = blockIdx.x; ok && u < units; u += gridDim.x) {
+      const int rows = unit_of(u).rows;
+      for (int b = 0; b < kb; b += kStageBlocks) {
+        ok = mbar_wait_parked(smem_addr(&s_empty[at]), phase ^ 1u, &s_abort, p.err, kErrWaitEmpty);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        char* to = x_smem + xs * kXBytes + q * 128 + 4 * t;
+        char* to = x_smem + at * kStageBlocks * kXBytes + q * 128 + 4 * t;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (16 * i < srows) {
-            const uint32_t w[4] = {v[s][i].x, v[s][i].y, v[s][i].z, v[s][i].w};
+        for (int j = 0; j < kStageBlocks; ++j)
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-              *reinterpret_cast<uint32_t*>(to + i * 2048 + (((4 * h + c) ^ (q & 7)) << 4)) = w[c];
-          }
+          for (int i = 0; i < 4; ++i)
+            if (16 * i < rows) {
+              const uint32_t w[4] = {v[j][i].x, v[j][i].y, v[j][i].z, v[j][i].w};
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                *reinterpret_cast<uint32_t*>(to + j * kXBytes + i * 2048 +
+                                             (((4 * h + c) ^ (q & 7)) << 4)) = w[c];
+            }
         // the MMA issuer orders these writes before its reads: a proxy fence here would wait for
         // the loads under way as well
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_addr(&x_full[xs]));
-        load(v[s]);
-        if (++xs == kXStages) {
-          xs = 0;
-          phase ^= 1u;
-        }
-        if (++sb == kb) {
-          sb = 0;
-          su += gridDim.x;
-          if (su < units) srows = unit_of(su).rows;
-        }
+        if (lane == 0) mbar_arrive(smem_addr(&s_full[at]));
+        load();
+        at ^= 1;
+        phase ^= at == 0;
       }
     }
-  } else if (lane == 0) {
+  } else {
     // ------------------------------------------------------------------ MMA issuer
-    int as = 0, xs = 0, buf = 0;
-    uint32_t a_phase = 0, x_phase = 0, acc_phase = 0;
+    // The whole warp walks the units, so that descriptors and addresses are uniform values; one
+    // elected lane issues.  With one lane alone in this branch, two waits and eight MMAs took
+    // the issuer 1500 cycles a block among 24 busy warps, and set the pace.
+    uint32_t elected;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b32 r;\n\t"
+        "elect.sync r|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(elected));
+    int at = 0, buf = 0;
+    uint32_t phase = 0, acc_phase = 0;
     bool ok = true;
+    const uint64_t desc0 = umma_sdesc(x_base, 16, 1024);
     for (int64_t u = blockIdx.x; ok && u < units; u += gridDim.x) {
-      const Unit d = unit_of(u);
-      const uint32_t idesc = umma_idesc(Fmt<T>::v, 0, 128, (d.rows + 15) & ~15);
-      ok = mbar_wait_bounded(smem_addr(&acc_empty[buf]), acc_phase ^ 1u, &s_abort, p.err,
-                             kErrWaitAccEmpty);
-      if (!ok) break;
-      tc_fence_after();
-      for (int b = 0; b < kb; ++b) {
-        ok = mbar_wait_bounded(smem_addr(&x_full[xs]), x_phase, &s_abort, p.err, kErrWaitFull) &&
-             mbar_wait_bounded(smem_addr(&a_full[as]), a_phase, &s_abort, p.err, kErrWaitFull);
+      const int rows = unit_of(u).rows;
+      const uint32_t idesc = umma_idesc(Fmt<T>::v, 0, 128, (rows + 15) & ~15);
+      const uint32_t acc = tmem + buf * kAccCols;
+      ok = mbar_wait_parked(smem_addr(&acc_empty[buf]), acc_phase ^ 1u, &s_abort, p.err,
+                            kErrWaitAccEmpty);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      for (int b = 0; b < kb; b += kStageBlocks) {
+        ok = mbar_wait_parked(smem_addr(&s_full[at]), phase, &s_abort, p.err, kErrWaitFull);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        fence_proxy_async_smem();  // the rows were written through the generic proxy
-        tc_fence_after();
+        if (elected) {
+          fence_proxy_async_smem();  // the rows were written through the generic proxy
+          tc_fence_after();
+          const uint64_t desc = desc0 + at * (kStageBlocks * kXBytes >> 4);
+          const uint32_t a = tmem_a + at * kStageBlocks * kACols;
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          const uint64_t bdesc = umma_sdesc(x_base + xs * kXBytes + ks * 32, 16, 1024);
+          for (int i = 0; i < kStageBlocks; ++i)
+            if (b + i < kb) {
 #pragma unroll
-          for (int m = 0; m < 2; ++m)
-            umma_f16_ts(tmem + buf * kAccCols + m * kTileRows,
-                        tmem_a + as * kACols + m * 32 + ks * 8, bdesc, idesc, b > 0 || ks > 0);
+              for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+                  umma_f16_ts(acc + m * kTileRows, a + i * kACols + m * 32 + ks * 8,
+                              desc + i * (kXBytes >> 4) + ks * 2, idesc, b + i + ks > 0);
+            }
+          umma_commit(smem_addr(&s_empty[at]));
+          if (b + kStageBlocks >= kb) umma_commit(smem_addr(&acc_full[buf]));
         }
-        umma_commit(smem_addr(&a_empty[as]));
-        umma_commit(smem_addr(&x_empty[xs]));
-        if (++as == kAStages) {
-          as = 0;
-          a_phase ^= 1u;
-        }
-        if (++xs == kXStages) {
-          xs = 0;
-          x_phase ^= 1u;
-        }
+        __syncwarp();
+        at ^= 1;
+        phase ^= at == 0;
       }
-      if (!ok) break;
-      umma_commit(smem_addr(&acc_full[buf]));
       buf ^= 1;
       acc_phase ^= buf == 0;
     }
     // every MMA is done before the tensor memory and the operands go
-    umma_commit(smem_addr(&s_done));
-    mbar_wait_bounded(smem_addr(&s_done), 0, &s_never, p.err, kErrWaitDrain);
+    if (elected) umma_commit(smem_addr(&s_done));
+    __syncwarp();
+    mbar_wait_parked(smem_addr(&s_done), 0, &s_never, p.err, kErrWaitDrain);
   }
   tc_fence_before();
   __syncthreads();
@@ -418,8 +419,8 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
 }
 
 size_t smem_bytes(int rec, int E) {
-  return 1024 + static_cast<size_t>(kXStages) * kXBytes +
-         static_cast<size_t>(kUnpackWarps) * kRingSlots * kRingRecords * rec +
+  return 1024 + static_cast<size_t>(kStages) * kStageBlocks * kXBytes +
+         static_cast<size_t>(kUnpackWarps) * kRingSlots * kStageBlocks * rec +
          static_cast<size_t>(2 * E + 2) * sizeof(int32_t);
 }
 
