@@ -53,7 +53,12 @@ __device__ __forceinline__ uint32_t rotr(uint32_t v, int n) { return __funnelshi
 
 // Fragment register i of a packed word: the pair (16 + q_lo, 16 + q_hi).
 template <typename T> __device__ __forceinline__ uint32_t nib_pair(uint32_t w, int i) {
-  return (rotr(w, 4 * i) & Nib<T>::kMask) | Nib<T>::kMagic;
+  // (w & mask) | magic in one instruction, both from registers
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;"
+      : "=r"(r)
+      : "r"(rotr(w, 4 * i)), "r"(Nib<T>::kMask), "r"(Nib<T>::kMagic));
+  return r;
 }
 
 template <typename T> struct Pair;
