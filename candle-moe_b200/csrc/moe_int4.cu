@@ -19,11 +19,9 @@
 // group (two with G = 32, else one) 8 x 2 scales (n = gid, gid + 8) and, with zero points, 8 x 2
 // bytes of them.  A column strip is one contiguous stream that holds all that its products
 // need.  The nibbles are one 16-byte vector per lane (gid = lane / 4, tig = lane % 4), one
-// 32-bit word per k16 step s, nibble i of its halves (h = 0, 1):
-//     n = 16 tile + gid + 8 (i & 1),  k = 64 block + 32 (s >> 1) + 8 tig + 4 (s & 1) + 2 (i >> 1) + h
-// This k order makes the activations of two steps 16 consecutive bytes per lane, and a pair of
-// steps never leaves a group of 32.  The word is rotated left so that nibble 0 sits at the top
-// of the mantissa.
+// 32-bit word per k16 step s, nibble i of its halves (h = 0, 1) as the fragment has it:
+//     n = 16 tile + gid + 8 (i & 1),  k = 64 block + 16 s + 8 (i >> 1) + 2 tig + h
+// The word is rotated left so that nibble 0 sits at the top of the mantissa.
 #include <stdint.h>
 
 #include <type_traits>
@@ -142,7 +140,7 @@ __global__ void int4_pack_kernel(const uint8_t* __restrict__ q, int E, int K, in
     uint32_t w = 0;
     for (int f = 0; f < 4; ++f) {
       const int n = n0 + gid + 8 * (f & 1);
-      const int k = 64 * b + 32 * (s >> 1) + 8 * tig + 4 * (s & 1) + 2 * (f >> 1);
+      const int k = 64 * b + 16 * s + 8 * (f >> 1) + 2 * tig;
       const uint32_t two = q[(e * (K / 2) + k / 2) * N + n];  // k even: low nibble k, high k + 1
       w |= (two & 15u) << (4 * f);
       w |= (two >> 4) << (16 + 4 * f);
@@ -213,7 +211,7 @@ __global__ void __launch_bounds__(256)
         const uint32_t u = nib_pair<T>(word[2 * h + s], f);
         const T2 v = __hmul2(__hsub2(*reinterpret_cast<const T2*>(&u), off[f & 1]), sc[f & 1]);
         const int n = 16 * warp + gid + 8 * (f & 1);
-        const int k = 32 * h + 8 * tig + 4 * s + 2 * (f >> 1);
+        const int k = 32 * h + 16 * s + 8 * (f >> 1) + 2 * tig;
         if (kTrans) {
           *reinterpret_cast<T2*>(buf + n * kPitch + k) = v;
         } else {
@@ -268,21 +266,23 @@ __device__ __forceinline__ void zero_points(const char* record, int per, int h, 
 }
 
 // One k64 block of at most 8 rows: fin += the products of MATS records with the activations xv
-// (two vectors of 32 k).  With the weights as 16 + q the sum of the activations is needed as
+// (two registers per k16 step).  With the weights as 16 + q the sum of the activations is needed as
 // well; the tensor cores, which have the time, make it.
 template <typename T, int MATS, bool kG32>
 __device__ __forceinline__ void few_block(const char* stage, int matrix_bytes, bool zeros, int lane,
-                                          const uint4 (&xv)[2], float (&fin)[MATS][4]) {
+                                          const uint32_t (&xv)[4][2], float (&fin)[MATS][4]) {
   using T2 = typename Pair<T>::type;
   constexpr int kPer = kG32 ? 2 : 1;
   constexpr uint32_t one = Nib<T>::kOne;
   const int gid = lane >> 2;
   float xs[kPer][4];
-  mma16816_zero<T>(xs[0], one, one, one, one, xv[0].x, xv[0].y);
-  mma16816<T>(xs[0], one, one, one, one, xv[0].z, xv[0].w);
-  if (kG32) mma16816_zero<T>(xs[kPer - 1], one, one, one, one, xv[1].x, xv[1].y);
-  else mma16816<T>(xs[0], one, one, one, one, xv[1].x, xv[1].y);
-  mma16816<T>(xs[kPer - 1], one, one, one, one, xv[1].z, xv[1].w);
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    if (s == 0 || (kG32 && s == 2))
+      mma16816_zero<T>(xs[(s >> 1) & (kPer - 1)], one, one, one, one, xv[s][0], xv[s][1]);
+    else
+      mma16816<T>(xs[(s >> 1) & (kPer - 1)], one, one, one, one, xv[s][0], xv[s][1]);
+  }
 #pragma unroll
   for (int m = 0; m < MATS; ++m) {
     const char* record = stage + m * matrix_bytes;
@@ -291,14 +291,12 @@ __device__ __forceinline__ void few_block(const char* stage, int matrix_bytes, b
     float acc[kPer][4];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      const uint4 v = xv[s >> 1];
-      const uint32_t b0 = (s & 1) ? v.z : v.x, b1 = (s & 1) ? v.w : v.y;
       const uint32_t a0 = nib_pair<T>(word[s], 0), a1 = nib_pair<T>(word[s], 1),
                      a2 = nib_pair<T>(word[s], 2), a3 = nib_pair<T>(word[s], 3);
       if (s == 0 || (kG32 && s == 2))
-        mma16816_zero<T>(acc[(s >> 1) & (kPer - 1)], a0, a1, a2, a3, b0, b1);
+        mma16816_zero<T>(acc[(s >> 1) & (kPer - 1)], a0, a1, a2, a3, xv[s][0], xv[s][1]);
       else
-        mma16816<T>(acc[(s >> 1) & (kPer - 1)], a0, a1, a2, a3, b0, b1);
+        mma16816<T>(acc[(s >> 1) & (kPer - 1)], a0, a1, a2, a3, xv[s][0], xv[s][1]);
     }
 #pragma unroll
     for (int h = 0; h < kPer; ++h) {
@@ -320,23 +318,23 @@ template <typename T, int MATS, bool kG32, typename Issue>
 __device__ __forceinline__ void few_slice(WeightRing<MATS, kFewRing>& w, const T* xr, int per,
                                           int blocks, int rec, bool zeros, int lane,
                                           float (&fin)[MATS][4], Issue& issue) {
-  uint4 xn[kStageBlocks][2];
+  uint32_t xn[kStageBlocks][4][2];
   auto load_x = [&](int b) {
 #pragma unroll
     for (int i = 0; i < kStageBlocks; ++i)
       if (b + i < blocks) {
-        xn[i][0] = *reinterpret_cast<const uint4*>(xr + 64 * (b + i));
-        xn[i][1] = *reinterpret_cast<const uint4*>(xr + 64 * (b + i) + 32);
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          xn[i][s >> 1][s & 1] = *reinterpret_cast<const uint32_t*>(xr + 64 * (b + i) + 8 * s);
       }
   };
   load_x(0);
   for (int b = 0; b < per; b += kStageBlocks) {
-    uint4 xv[kStageBlocks][2];
+    uint32_t xv[kStageBlocks][4][2];
 #pragma unroll
-    for (int i = 0; i < kStageBlocks; ++i) {
-      xv[i][0] = xn[i][0];
-      xv[i][1] = xn[i][1];
-    }
+    for (int i = 0; i < kStageBlocks; ++i)
+#pragma unroll
+      for (int s = 0; s < 8; ++s) xv[i][s >> 1][s & 1] = xn[i][s >> 1][s & 1];
     load_x(b + kStageBlocks);
     const char* stage = w.wait();
 #pragma unroll
@@ -499,7 +497,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) 
       rows = min(8, __ldg(p.offsets + e + 1) - row0);
     }
     const int r = row0 + min(gid, rows - 1);
-    const T* xr = static_cast<const T*>(p.x) + 8 * tig + 64 * b0 +
+    const T* xr = static_cast<const T*>(p.x) + 2 * tig + 64 * b0 +
                   static_cast<int64_t>(kDown    ? r
                                        : kTable ? table.row[r] / p.k
                                                 : __ldg(p.sorted_token + r)) * p.K;
@@ -593,7 +591,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Param
     for (int t = warp; t < tasks; t += kWarps) {
       const int c = t / pieces, b0 = t % pieces * per, blocks = min(per, kb - b0);
       const int row0 = table.first[c], rows = table.first[c + 1] - row0;
-      const T* xr = static_cast<const T*>(p.x) + 8 * tig + 64 * b0 +
+      const T* xr = static_cast<const T*>(p.x) + 2 * tig + 64 * b0 +
                     static_cast<int64_t>(row0 + min(gid, rows - 1)) * p.K;
       float fin[1][4] = {};
       few_slice<T, 1, kG32>(w, xr, per, blocks, p.rec, p.zeros, lane, fin, issue);
@@ -621,13 +619,13 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Param
 
 // Chunks of 8 NT rows.  A unit is (chunk, 8 strips of 16 output columns), a strip per warp over all
 // of K; the activations are staged in shared memory, 128 k at a time, for all eight warps
-// (cp.async, kXRing - 1 stages ahead across units), whose rows are 320 bytes apart so that a
+// (cp.async, kXRing - 1 stages ahead across units), whose rows are 272 bytes apart so that a
 // fragment load meets no bank twice.  q - z is made in registers (exact) and the scale acts on
 // the f32 sums of 32 k.  Bound by the tensor cores' mma.sync rate (2 cycles an SM for 16 x 8 x
 // 16, a quarter of the tcgen05 rate): a record costs 8 cycles per 8 rows, and 24 cycles of
 // memory time.
 constexpr int kXRing = 3;
-constexpr int kXPitch = 320;
+constexpr int kXPitch = 272;
 
 template <typename T, int MATS, bool kDown, int NT>
 __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) int4_some_kernel(Int4Params p) {
@@ -733,7 +731,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) int4_some_kernel
       __syncthreads();  // the stage is there for all, and all are done with the one before
       x_issue();
       const char* stage = w.wait();
-      const char* xst = smem + x_slot * kXBytes + gid * kXPitch + 16 * tig;
+      const char* xst = smem + x_slot * kXBytes + gid * kXPitch + 4 * tig;
 #pragma unroll
       for (int i = 0; i < kStageBlocks; ++i) {
         if (st * kStageBlocks + i >= kb) break;
@@ -742,8 +740,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) int4_some_kernel
           uint4 xv[NT];
 #pragma unroll
           for (int j = 0; j < NT; ++j)
-            if (j < tiles)
-              xv[j] = *reinterpret_cast<const uint4*>(xst + 8 * j * kXPitch + 128 * i + 64 * h);
+            if (j < tiles) {
+              const char* f = xst + 8 * j * kXPitch + 128 * i + 64 * h;
+              xv[j] = make_uint4(*reinterpret_cast<const uint32_t*>(f),
+                                 *reinterpret_cast<const uint32_t*>(f + 16),
+                                 *reinterpret_cast<const uint32_t*>(f + 32),
+                                 *reinterpret_cast<const uint32_t*>(f + 48));
+            }
 #pragma unroll
           for (int m = 0; m < MATS; ++m) {
             const char* record = stage + (m * kStageBlocks + i) * p.rec;

@@ -6,10 +6,8 @@
 // through rings in shared memory, unpack them in registers -- (q - z) exactly,
 // times the scale, one rounding to the 16-bit type -- and store them as they lie: the packed
 // fragment order is the 16x128b shape of tcgen05.st, so nothing is shuffled and shared memory
-// carries only the packed nibbles.  The rows are the other operand, from shared memory in the
-// 128-byte swizzle.  The order of k inside a fragment (see moe_int4.cu) makes column 4 c + t of
-// a half the k pair 4 t + c of it, so the warps that gather the rows put their 4-byte pairs
-// there.  The sums stay in tensor memory for all of K (two sets, so that the epilogue of a tile
+// carries only the packed nibbles.  The rows are the other operand, gathered by cp.async into
+// the 128-byte swizzle.  The sums stay in tensor memory for all of K (two sets, so that the epilogue of a tile
 // runs under the next one) and leave it one weight column per thread.
 //
 // What bounds it: unpacking, 75 to 85 warp instructions for a record of 1024 weights, 20 to 25
@@ -29,10 +27,11 @@ namespace {
 constexpr int kTileRows = 64;
 constexpr int kUnpackWarps = 16, kOutWarps = 4, kGatherWarps = 4;
 constexpr int kThreads = (kUnpackWarps + kOutWarps + kGatherWarps + 1) * 32;
-constexpr int kStages = 2;       // of two k64 blocks: weights in tensor memory, rows in shared memory
-constexpr int kStageBlocks = 2;
+constexpr int kStageBlocks = 2;           // k64 blocks that are handed over at once
+constexpr int kStages = 2;                // of weights in tensor memory
+constexpr int kXSlots = 4;                // stages of rows in shared memory
 constexpr int kXBytes = kTileRows * 128;  // a block's rows
-constexpr int kRingSlots = 4;             // of kStageBlocks records
+constexpr int kRingSlots = 3, kRingBlocks = 4;
 constexpr int kAccCols = 2 * kTileRows;   // of one set of sums, two panels
 constexpr int kACols = 2 * 32;            // of one block of weights
 constexpr int kTmemCols = 512;
@@ -72,8 +71,8 @@ template <typename T> __device__ __forceinline__ uint32_t zero_pair(uint32_t z) 
 }
 
 // The record's weights in the order of tmem_st_16x128b_x8.
-template <typename T>
-__device__ __forceinline__ void unpack_record(const char* record, int per, bool zeros, int lane,
+template <typename T, bool kZeros>
+__device__ __forceinline__ void unpack_record(const char* record, int per, int lane,
                                               uint32_t (&out)[16]) {
   using T2 = typename Pair<T>::type;
   const int gid = lane >> 2;
@@ -85,7 +84,7 @@ __device__ __forceinline__ void unpack_record(const char* record, int per, bool 
     sc[0].x = sc[0].y = s.x;
     sc[1].x = sc[1].y = s.y;
     uint32_t z = 0x0808u;
-    if (zeros) z = *reinterpret_cast<const uint16_t*>(record + 512 + 32 * per + 16 * h + 2 * gid);
+    if (kZeros) z = *reinterpret_cast<const uint16_t*>(record + 512 + 32 * per + 16 * h + 2 * gid);
     const uint32_t z0 = zero_pair<T>(z & 15u), z1 = zero_pair<T>((z >> 8) & 15u);
     off[0] = *reinterpret_cast<const T2*>(&z0);
     off[1] = *reinterpret_cast<const T2*>(&z1);
@@ -106,7 +105,7 @@ __device__ __forceinline__ void unpack_record(const char* record, int per, bool 
 }
 
 // kDual: the panels are gate and up, else the two halves of 256 columns.
-template <typename T, bool kDual, bool kDown>
+template <typename T, bool kDual, bool kDown, bool kZeros>
 __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
   constexpr int kCols = kDual ? 128 : 256;  // output columns of a unit
   extern __shared__ __align__(128) char smem_raw[];
@@ -118,8 +117,8 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
   const uint32_t raw = smem_addr(smem_raw);
   const uint32_t x_base = (raw + 1023u) & ~1023u;
   char* x_smem = smem_raw + (x_base - raw);
-  char* rings = x_smem + kStages * kStageBlocks * kXBytes;
-  int32_t* s_cp = reinterpret_cast<int32_t*>(rings + kUnpackWarps * kRingSlots * kStageBlocks * p.rec);
+  char* rings = x_smem + kXSlots * kStageBlocks * kXBytes;
+  int32_t* s_cp = reinterpret_cast<int32_t*>(rings + kUnpackWarps * kRingSlots * kRingBlocks * p.rec);
   int32_t* s_off = s_cp + p.E + 1;
   // from a shuffle, so that the compiler knows it to be the same in the warp
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
@@ -176,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
     const int strip = 2 * (warp & 3) + ((warp >> 2) & 1);  // in this warp's quarter of the lanes
     const uint32_t lanes = static_cast<uint32_t>(16 * strip) << 16;
     const int per = p.G == 32 ? 2 : 1;
-    const int matrix_bytes = kStageBlocks * p.rec;
+    const int matrix_bytes = kRingBlocks * p.rec;
     WeightRing<1, kRingSlots> w{rings + warp * kRingSlots * matrix_bytes,
                                       smem_addr(&s_ring[warp][0]), &s_abort, p.err, lane,
                                       matrix_bytes};
@@ -195,9 +194,9 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
     };
     auto issue = [&]() {
       if (pu >= units) return;
-      w.issue(src, nullptr, min(kStageBlocks, kb - pb) * p.rec);
+      w.issue(src, nullptr, min(kRingBlocks, kb - pb) * p.rec);
       src += matrix_bytes;
-      pb += kStageBlocks;
+      pb += kRingBlocks;
       if (pb >= kb) {
         pb = 0;
         pu += gridDim.x;
@@ -210,28 +209,33 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
     int at = 0;
     uint32_t phase = 0;
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-      for (int b = 0; b < kb; b += kStageBlocks) {
+      for (int r = 0; r < kb; r += kRingBlocks) {
         const char* stage = w.wait();
-        uint32_t regs[kStageBlocks][16];
 #pragma unroll
-        for (int i = 0; i < kStageBlocks; ++i)
-          if (b + i < kb) unpack_record<T>(stage + i * p.rec, per, p.zeros, lane, regs[i]);
+        for (int b = 0; b < kRingBlocks; b += kStageBlocks) {
+          if (r + b >= kb) break;
+          uint32_t regs[kStageBlocks][16];
+#pragma unroll
+          for (int i = 0; i < kStageBlocks; ++i)
+            if (r + b + i < kb)
+              unpack_record<T, kZeros>(stage + (b + i) * p.rec, per, lane, regs[i]);
+          // after a wait that ran out this goes on with what is there, to the end of the units
+          mbar_wait_parked(smem_addr(&s_empty[at]), phase ^ 1u, &s_abort, p.err, kErrWaitEmpty);
+          __syncwarp();
+          tc_fence_after();
+          const uint32_t to = tmem_a + at * kStageBlocks * kACols + panel * 32 + lanes;
+#pragma unroll
+          for (int i = 0; i < kStageBlocks; ++i)
+            if (r + b + i < kb) tmem_st_16x128b_x8(to + i * kACols, regs[i]);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_addr(&s_full[at]));
+          at ^= 1;
+          phase ^= at == 0;
+        }
         w.release();
         issue();
-        // after a wait that ran out this goes on with what is there, to the end of the units
-        mbar_wait_parked(smem_addr(&s_empty[at]), phase ^ 1u, &s_abort, p.err, kErrWaitEmpty);
-        __syncwarp();
-        tc_fence_after();
-        const uint32_t to = tmem_a + at * kStageBlocks * kACols + panel * 32 + lanes;
-#pragma unroll
-        for (int i = 0; i < kStageBlocks; ++i)
-          if (b + i < kb) tmem_st_16x128b_x8(to + i * kACols, regs[i]);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_addr(&s_full[at]));
-        at ^= 1;
-        phase ^= at == 0;
       }
     }
     w.drain();
@@ -290,14 +294,16 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
     }
   } else if (warp < kUnpackWarps + kOutWarps + kGatherWarps) {
     // ------------------------------------------------------------------ rows into shared memory
-    // Thread g takes 16 bytes (half h, t: k pairs 4 t .. 4 t + 3 of the half) of rows q + 16 i,
-    // and stores pair 4 t + c at 4 c + t.  Rows past the tile's repeat its last one; their sums
-    // are not read.
+    // Thread g copies 16-byte piece g % 8 of each block's rows q + 16 i (q = g / 8) to its place in
+    // the 128-byte swizzle (piece c of row r at c ^ (r % 8)).  Rows past the tile's repeat its
+    // last one; their sums are not read.  The copies run two stages ahead: those of stage
+    // n + 2 take the slot of stage n - 2, whose MMAs are done when stage n may be filled.
     const int g = threadIdx.x - (kUnpackWarps + kOutWarps) * 32;
-    const int c8 = g & 7, q = g >> 3, h = c8 >> 2, t = c8 & 3;
+    const int c8 = g & 7, q = g >> 3;
+    const uint32_t to = x_base + q * 128 + ((c8 ^ (q & 7)) << 4);
     const T* src[4];
-    int64_t lu = blockIdx.x;  // the load side runs a stage ahead of the store side
-    int lb = 0, lrows = 0;
+    int64_t lu = blockIdx.x;
+    int lb = 0, lrows = 0, slot = 0;
     auto locate = [&]() {
       if (lu >= units) return;
       const Unit d = unit_of(lu);
@@ -309,54 +315,45 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
                  static_cast<int64_t>(kDown ? r : __ldg(p.sorted_token + r)) * p.K + c8 * 8;
       }
     };
-    uint4 v[kStageBlocks][4];
     auto load = [&]() {
-      if (lu >= units) return;
+      if (lu < units) {
+        const uint32_t dst = to + slot * kStageBlocks * kXBytes;
 #pragma unroll
-      for (int j = 0; j < kStageBlocks; ++j)
+        for (int j = 0; j < kStageBlocks; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (16 * i < lrows && lb + j < kb)
-            v[j][i] = *reinterpret_cast<const uint4*>(src[i] + (lb + j) * 64);
-      lb += kStageBlocks;
-      if (lb >= kb) {
-        lb = 0;
-        lu += gridDim.x;
-        locate();
+          for (int i = 0; i < 4; ++i)
+            if (16 * i < lrows && lb + j < kb)
+              cp_async16(dst + j * kXBytes + i * 2048, src[i] + (lb + j) * 64);
+        lb += kStageBlocks;
+        if (lb >= kb) {
+          lb = 0;
+          lu += gridDim.x;
+          locate();
+        }
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      slot = (slot + 1) & (kXSlots - 1);
     };
     locate();
+    load();
     load();
     int at = 0;
     uint32_t phase = 0;
     bool ok = true;
     for (int64_t u = blockIdx.x; ok && u < units; u += gridDim.x) {
-      const int rows = unit_of(u).rows;
       for (int b = 0; b < kb; b += kStageBlocks) {
         ok = mbar_wait_parked(smem_addr(&s_empty[at]), phase ^ 1u, &s_abort, p.err, kErrWaitEmpty);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        char* to = x_smem + at * kStageBlocks * kXBytes + q * 128 + 4 * t;
-#pragma unroll
-        for (int j = 0; j < kStageBlocks; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (16 * i < rows) {
-              const uint32_t w[4] = {v[j][i].x, v[j][i].y, v[j][i].z, v[j][i].w};
-#pragma unroll
-              for (int c = 0; c < 4; ++c)
-                *reinterpret_cast<uint32_t*>(to + j * kXBytes + i * 2048 +
-                                             (((4 * h + c) ^ (q & 7)) << 4)) = w[c];
-            }
-        // the MMA issuer orders these writes before its reads: a proxy fence here would wait for
-        // the loads under way as well
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_addr(&s_full[at]));
         load();
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+        __syncwarp();  // the MMA issuer orders these writes before its reads
+        if (lane == 0) mbar_arrive(smem_addr(&s_full[at]));
         at ^= 1;
         phase ^= at == 0;
       }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else {
     // ------------------------------------------------------------------ MMA issuer
     // The whole warp walks the units, so that descriptors and addresses are uniform values; one
@@ -367,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
         "{\n\t.reg .pred p;\n\t.reg .b32 r;\n\t"
         "elect.sync r|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(elected));
-    int at = 0, buf = 0;
+    int at = 0, slot = 0, buf = 0;
     uint32_t phase = 0, acc_phase = 0;
     bool ok = true;
     const uint64_t desc0 = umma_sdesc(x_base, 16, 1024);
@@ -385,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
         if (elected) {
           fence_proxy_async_smem();  // the rows were written through the generic proxy
           tc_fence_after();
-          const uint64_t desc = desc0 + at * (kStageBlocks * kXBytes >> 4);
+          const uint64_t desc = desc0 + slot * (kStageBlocks * kXBytes >> 4);
           const uint32_t a = tmem_a + at * kStageBlocks * kACols;
 #pragma unroll
           for (int i = 0; i < kStageBlocks; ++i)
@@ -403,6 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
         __syncwarp();
         at ^= 1;
         phase ^= at == 0;
+        slot = (slot + 1) & (kXSlots - 1);
       }
       buf ^= 1;
       acc_phase ^= buf == 0;
@@ -419,26 +417,34 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
 }
 
 size_t smem_bytes(int rec, int E) {
-  return 1024 + static_cast<size_t>(kStages) * kStageBlocks * kXBytes +
-         static_cast<size_t>(kUnpackWarps) * kRingSlots * kStageBlocks * rec +
+  return 1024 + static_cast<size_t>(kXSlots) * kStageBlocks * kXBytes +
+         static_cast<size_t>(kUnpackWarps) * kRingSlots * kRingBlocks * rec +
          static_cast<size_t>(2 * E + 2) * sizeof(int32_t);
 }
 
-template <typename T, bool kDual, bool kDown>
+template <typename T, bool kDual, bool kDown, bool kZeros>
 bool attribute() {
-  return cudaFuncSetAttribute(int4_many_kernel<T, kDual, kDown>,
+  return cudaFuncSetAttribute(int4_many_kernel<T, kDual, kDown, kZeros>,
                               cudaFuncAttributeMaxDynamicSharedMemorySize,
                               static_cast<int>(smem_bytes(kMaxRecord, route_prep_max_experts()))) ==
          cudaSuccess;
 }
 
-template <typename T>
+template <typename T, bool kZeros>
 bool launch(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
   const size_t smem = smem_bytes(g1.rec, g1.E);
-  return (g1.w[1] ? launch_dependent(int4_many_kernel<T, true, false>, num_sms, kThreads, smem, s, g1)
-                  : launch_dependent(int4_many_kernel<T, false, false>, num_sms, kThreads, smem, s,
-                                     g1)) &&
-         launch_dependent(int4_many_kernel<T, false, true>, num_sms, kThreads, smem, s, g2);
+  const bool ok =
+      g1.w[1] ? launch_dependent(int4_many_kernel<T, true, false, kZeros>, num_sms, kThreads, smem, s,
+                                 g1)
+              : launch_dependent(int4_many_kernel<T, false, false, kZeros>, num_sms, kThreads, smem,
+                                 s, g1);
+  return ok && launch_dependent(int4_many_kernel<T, false, true, kZeros>, num_sms, kThreads, smem, s,
+                                g2);
+}
+
+template <typename T, bool kZeros> bool attributes() {
+  return attribute<T, true, false, kZeros>() && attribute<T, false, false, kZeros>() &&
+         attribute<T, false, true, kZeros>();
 }
 
 }  // namespace
@@ -446,15 +452,17 @@ bool launch(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_
 int int4_many_rows() { return kTileRows; }
 
 bool int4_many_set_attributes() {
-  return attribute<__nv_bfloat16, true, false>() && attribute<__nv_bfloat16, false, false>() &&
-         attribute<__nv_bfloat16, false, true>() && attribute<__half, true, false>() &&
-         attribute<__half, false, false>() && attribute<__half, false, true>();
+  return attributes<__nv_bfloat16, false>() && attributes<__nv_bfloat16, true>() &&
+         attributes<__half, false>() && attributes<__half, true>();
 }
 
 bool launch_int4_many(int dtype, const Int4Params& g1, const Int4Params& g2, int num_sms,
                       cudaStream_t s) {
-  return dtype == kBF16 ? launch<__nv_bfloat16>(g1, g2, num_sms, s)
-                        : launch<__half>(g1, g2, num_sms, s);
+  if (dtype == kBF16)
+    return g1.zeros ? launch<__nv_bfloat16, true>(g1, g2, num_sms, s)
+                    : launch<__nv_bfloat16, false>(g1, g2, num_sms, s);
+  return g1.zeros ? launch<__half, true>(g1, g2, num_sms, s)
+                  : launch<__half, false>(g1, g2, num_sms, s);
 }
 
 }  // namespace cmoe
