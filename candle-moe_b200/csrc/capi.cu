@@ -1104,7 +1104,7 @@ CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const vo
     return MOE_ERR_WORKSPACE;
   }
   const int64_t rows = num_tokens * topk;
-  const int chunk = int4_chunk_rows(rows, E, H, I);
+  const int chunk = int4_chunk_rows(rows, E);
   Int4Params g1 = {}, g2 = {};
   g1.w[0] = gate_packed;
   g1.w[1] = up_packed;

@@ -185,7 +185,7 @@ struct Int4Params {
   int rows, k;                  // T*k, k
 };
 // moe_int4_mma.cu: both products of calls with many rows per expert (route preparation in chunks of
-// int4_many_rows()); N and K of both multiples of 128.  False: a launch failed.
+// int4_many_rows()).  False: a launch failed.
 int int4_many_rows();
 bool int4_many_set_attributes();
 bool launch_int4_many(int dtype, const Int4Params& g1, const Int4Params& g2, int num_sms,
@@ -198,7 +198,7 @@ int launch_int4_table_ffn(int dtype, const Int4Params& g1, const Int4Params& g2,
 int int4_record_bytes(int G, bool zeros);
 bool int4_set_attributes();
 // Rows per chunk of the kernel that serves a call of this many rows.
-int int4_chunk_rows(int64_t rows, int E, int H, int I);
+int int4_chunk_rows(int64_t rows, int E);
 int launch_int4_quantize(int dtype, const void* w, int E, int K, int N, int G, int symmetric,
                          uint8_t* q, void* scales, uint8_t* zeros, int num_sms, cudaStream_t s);
 // Both return the number of kernels launched (0: a launch failed).

@@ -236,15 +236,8 @@ __global__ void __launch_bounds__(256)
 
 constexpr int kWarps = 8;
 constexpr int kStageBlocks = 2;  // k64 blocks of a ring stage
-constexpr int kRing = 4;         // stages of a ring of int4_some_kernel
-constexpr int kFewRing = 3;      // and of the kernels for few rows
+constexpr int kFewRing = 3;      // stages of a ring
 
-__device__ __forceinline__ void cp_async_commit() {
-  asm volatile("cp.async.commit_group;" ::: "memory");
-}
-template <int N> __device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 // Expert of chunk c: the number of experts whose chunks all come before it.
 __device__ __forceinline__ int find_expert(const int32_t* __restrict__ prefix, int E, int c) {
   int e = 0;
@@ -617,226 +610,6 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Param
   w.drain();
 }
 
-// Chunks of 8 NT rows.  A unit is (chunk, 8 strips of 16 output columns), a strip per warp over all
-// of K; the activations are staged in shared memory, 128 k at a time, for all eight warps
-// (cp.async, kXRing - 1 stages ahead across units), whose rows are 272 bytes apart so that a
-// fragment load meets no bank twice.  q - z is made in registers (exact) and the scale acts on
-// the f32 sums of 32 k.  Bound by the tensor cores' mma.sync rate (2 cycles an SM for 16 x 8 x
-// 16, a quarter of the tcgen05 rate): a record costs 8 cycles per 8 rows, and 24 cycles of
-// memory time.
-constexpr int kXRing = 3;
-constexpr int kXPitch = 272;
-
-template <typename T, int MATS, bool kDown, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) int4_some_kernel(Int4Params p) {
-  using T2 = typename Pair<T>::type;
-  constexpr int kRows = 8 * NT;
-  constexpr int kXBytes = kRows * kXPitch;
-  constexpr int kLoads = kRows * 16 / (kWarps * 32);  // 16-byte pieces per thread and stage
-  constexpr int kPitch = 20;
-  extern __shared__ __align__(128) char smem[];
-  __shared__ alignas(8) uint64_t s_bar[kWarps][kRing];
-  __shared__ alignas(16) float s_out[kWarps][MATS][8][kPitch];
-  __shared__ int s_abort;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int gid = lane >> 2, tig = lane & 3;
-  const int kb = p.K / 64, ntiles = p.N / 16, rec_per = p.G == 32 ? 2 : 1;
-  init_rings(s_bar, &s_abort);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int nunits = (ntiles + kWarps - 1) / kWarps;
-  const int64_t units = static_cast<int64_t>(__ldg(p.chunk_prefix + p.E)) * nunits;
-  WeightRing<MATS, kRing> w{smem + kXRing * kXBytes + warp * kRing * MATS * kStageBlocks * p.rec,
-                     smem_addr(&s_bar[warp][0]), &s_abort, p.err, lane, kStageBlocks * p.rec};
-  const int nstages = (kb + kStageBlocks - 1) / kStageBlocks;
-  int64_t pu = blockIdx.x, strip = 0;  // the next stage to ask for: unit (its strip), stage
-  int ps = 0;
-  auto locate = [&]() {
-    if (pu < units) {
-      // a strip past the last one repeats it, and its results are dropped
-      const int nt = min(static_cast<int>(pu % nunits) * kWarps + warp, ntiles - 1);
-      const int e = find_expert(p.chunk_prefix, p.E, static_cast<int>(pu / nunits));
-      strip = (static_cast<int64_t>(e) * ntiles + nt) * kb;
-    }
-  };
-  auto issue = [&]() {
-    if (pu >= units) return;
-    const int64_t from = (strip + ps * kStageBlocks) * p.rec;
-    w.issue(static_cast<const char*>(p.w[0]) + from, static_cast<const char*>(p.w[1]) + from,
-            min(kStageBlocks, kb - ps * kStageBlocks) * p.rec);
-    if (++ps == nstages) {
-      ps = 0;
-      pu += gridDim.x;
-      locate();
-    }
-  };
-  auto chunk_rows = [&](int64_t u, int& row0, int& rows) {
-    const int c = static_cast<int>(u / nunits);
-    const int e = find_expert(p.chunk_prefix, p.E, c);
-    row0 = __ldg(p.offsets + e) + (c - __ldg(p.chunk_prefix + e)) * kRows;
-    rows = min(kRows, __ldg(p.offsets + e + 1) - row0);
-  };
-  // the activations' producer side; a thread copies piece threadIdx.x % 16 of every 16th row
-  int64_t xu = blockIdx.x;
-  int xs_stage = 0, xs_slot = 0;
-  const T* xp[kLoads];
-  auto x_locate = [&]() {
-    if (xu >= units) return;
-    int row0, rows;
-    chunk_rows(xu, row0, rows);
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int at = threadIdx.x / 16 + 16 * i;
-      const int r = row0 + min(at, rows - 1);
-      xp[i] = at < (rows + 7) / 8 * 8
-                  ? static_cast<const T*>(p.x) +
-                        static_cast<int64_t>(kDown ? r : __ldg(p.sorted_token + r)) * p.K
-                  : nullptr;
-    }
-  };
-  auto x_issue = [&]() {
-    if (xu < units) {
-      const int k = xs_stage * 128 + (threadIdx.x % 16) * 8;
-      if (k < p.K) {
-        const uint32_t dst = smem_addr(smem) + xs_slot * kXBytes + (threadIdx.x / 16) * kXPitch +
-                             (threadIdx.x % 16) * 16;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i)
-          if (xp[i]) cp_async16(dst + 16 * i * kXPitch, xp[i] + k);
-      }
-      if (++xs_stage == nstages) {
-        xs_stage = 0;
-        xu += gridDim.x;
-        x_locate();
-      }
-    }
-    cp_async_commit();
-    xs_slot = xs_slot + 1 == kXRing ? 0 : xs_slot + 1;
-  };
-  locate();
-  x_locate();
-#pragma unroll
-  for (int i = 0; i < kRing - 1; ++i) issue();
-#pragma unroll
-  for (int i = 0; i < kXRing - 1; ++i) x_issue();
-  int x_slot = 0;
-
-  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-    int row0, rows;
-    chunk_rows(u, row0, rows);
-    const int tiles = (rows + 7) / 8;
-    float fin[MATS][NT][4] = {};
-    for (int st = 0; st < nstages; ++st) {
-      cp_async_wait<kXRing - 2>();
-      __syncthreads();  // the stage is there for all, and all are done with the one before
-      x_issue();
-      const char* stage = w.wait();
-      const char* xst = smem + x_slot * kXBytes + gid * kXPitch + 4 * tig;
-#pragma unroll
-      for (int i = 0; i < kStageBlocks; ++i) {
-        if (st * kStageBlocks + i >= kb) break;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint4 xv[NT];
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-            if (j < tiles) {
-              const char* f = xst + 8 * j * kXPitch + 128 * i + 64 * h;
-              xv[j] = make_uint4(*reinterpret_cast<const uint32_t*>(f),
-                                 *reinterpret_cast<const uint32_t*>(f + 16),
-                                 *reinterpret_cast<const uint32_t*>(f + 32),
-                                 *reinterpret_cast<const uint32_t*>(f + 48));
-            }
-#pragma unroll
-          for (int m = 0; m < MATS; ++m) {
-            const char* record = stage + (m * kStageBlocks + i) * p.rec;
-            const uint2 wq = *reinterpret_cast<const uint2*>(record + 16 * lane + 8 * h);
-            const int hg = h & (rec_per - 1);
-            float z0, z1;
-            zero_points(record, rec_per, hg, gid, p.zeros, z0, z1);
-            T2 off[2];
-            off[0].x = off[0].y = Elem<T>::from_f(z0);
-            off[1].x = off[1].y = Elem<T>::from_f(z1);
-            uint32_t a[2][4];
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-              for (int f = 0; f < 4; ++f) {
-                const uint32_t v = nib_pair<T>(s ? wq.y : wq.x, f);
-                const T2 d = __hsub2(*reinterpret_cast<const T2*>(&v), off[f & 1]);
-                a[s][f] = *reinterpret_cast<const uint32_t*>(&d);
-              }
-            const T2 sc = *(reinterpret_cast<const T2*>(record + 512 + 32 * hg) + gid);
-            const float s0 = Elem<T>::to_f(sc.x), s1 = Elem<T>::to_f(sc.y);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              if (j < tiles) {
-                float acc[4];
-                mma16816_zero<T>(acc, a[0][0], a[0][1], a[0][2], a[0][3], xv[j].x, xv[j].y);
-                mma16816<T>(acc, a[1][0], a[1][1], a[1][2], a[1][3], xv[j].z, xv[j].w);
-                fin[m][j][0] += s0 * acc[0];
-                fin[m][j][1] += s0 * acc[1];
-                fin[m][j][2] += s1 * acc[2];
-                fin[m][j][3] += s1 * acc[3];
-              }
-            }
-          }
-        }
-      }
-      w.release();
-      issue();
-      x_slot = x_slot + 1 == kXRing ? 0 : x_slot + 1;
-    }
-    // out, 8 rows at a time: a lane takes 4 columns of one row
-    const int nt = static_cast<int>(u % nunits) * kWarps + warp;
-    const int at = lane >> 2, n4 = (lane & 3) * 4;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      if (j < tiles) {
-        __syncwarp();
-#pragma unroll
-        for (int m = 0; m < MATS; ++m)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            s_out[warp][m][2 * tig + (i & 1)][gid + 8 * (i >> 1)] = fin[m][j][i];
-        __syncwarp();
-        const int r = 8 * j + at;
-        if (r < rows && nt < ntiles) {
-          float4 v = *reinterpret_cast<const float4*>(&s_out[warp][0][at][n4]);
-          if (kDown) {
-            const float wt = __ldg(p.sorted_w + row0 + r);
-            v.x *= wt;
-            v.y *= wt;
-            v.z *= wt;
-            v.w *= wt;
-            *reinterpret_cast<float4*>(static_cast<float*>(p.out) +
-                                       static_cast<int64_t>(__ldg(p.sorted_flat + row0 + r)) * p.N +
-                                       nt * 16 + n4) = v;
-          } else {
-            v.x = act_apply(v.x, p.act);
-            v.y = act_apply(v.y, p.act);
-            v.z = act_apply(v.z, p.act);
-            v.w = act_apply(v.w, p.act);
-            if (MATS == 2) {
-              const float4 g = *reinterpret_cast<const float4*>(&s_out[warp][MATS - 1][at][n4]);
-              v.x *= g.x;
-              v.y *= g.y;
-              v.z *= g.z;
-              v.w *= g.w;
-            }
-            // the intermediate is rounded to the 16-bit type that the second product reads
-            *reinterpret_cast<uint2*>(static_cast<T*>(p.out) +
-                                      static_cast<int64_t>(row0 + r) * p.N + nt * 16 + n4) =
-                make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
-          }
-        }
-      }
-    }
-  }
-  cp_async_wait<0>();
-  w.drain();
-}
-
 // out[t] = sum over the token's slots in slot order, one rounding.
 template <typename T>
 __global__ void int4_combine_kernel(const float* __restrict__ slots, const uint32_t* __restrict__ idx,
@@ -892,19 +665,6 @@ struct FewDown {
   }
 };
 
-template <typename T, int MATS, bool kDown, int NT>
-struct Some {
-  static constexpr auto kernel = int4_some_kernel<T, MATS, kDown, NT>;
-  static size_t smem(int rec) {
-    return static_cast<size_t>(kXRing) * 8 * NT * kXPitch +
-           static_cast<size_t>(kWarps) * MATS * kRing * kStageBlocks * rec;
-  }
-  static bool launch(Int4Params p, int num_sms, cudaStream_t s) {
-    // two CTAs on an SM where the registers allow: 2 x (30 + 76 KB + 10 KB static) at most
-    return launch_dependent(kernel, num_sms * (NT <= 4 ? 2 : 1), kWarps * 32, smem(p.rec), s, p);
-  }
-};
-
 template <typename K> bool allow_smem() {
   return cudaFuncSetAttribute(K::kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                               static_cast<int>(K::smem(kMaxRecord))) == cudaSuccess;
@@ -916,8 +676,7 @@ template <typename T, bool kG32> bool allow_few() {
          allow_smem<Few<T, 1, false, kG32, true>>() && allow_smem<FewDown<T, kG32>>();
 }
 template <typename T> bool gemm_attributes() {
-  return allow_few<T, false>() && allow_few<T, true>() && allow_smem<Some<T, 2, false, 4>>() &&
-         allow_smem<Some<T, 1, false, 4>>() && allow_smem<Some<T, 1, true, 4>>();
+  return allow_few<T, false>() && allow_few<T, true>();
 }
 
 template <typename T, bool kG32, bool kTable>
@@ -930,21 +689,14 @@ bool launch_few(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStr
   return launch_few_first<T, kG32, false>(g1, num_sms, s) &&
          Few<T, 1, true, kG32, false>::launch(g2, num_sms, s);
 }
-template <typename T, int NT>
-bool launch_some(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
-  return (g1.w[1] ? Some<T, 2, false, NT>::launch(g1, num_sms, s)
-                  : Some<T, 1, false, NT>::launch(g1, num_sms, s)) &&
-         Some<T, 1, true, NT>::launch(g2, num_sms, s);
-}
-
 template <typename T>
 bool launch_ffn(int chunk, const Int4Params& g1, const Int4Params& g2, const uint32_t* idx,
                 int64_t T_, int k, void* out, int num_sms, cudaStream_t s) {
-  const bool ok = chunk == 8    ? (g1.G == 32 ? launch_few<T, true>(g1, g2, num_sms, s)
-                                              : launch_few<T, false>(g1, g2, num_sms, s))
-                  : chunk == 32 ? launch_some<T, 4>(g1, g2, num_sms, s)
-                                : launch_int4_many(std::is_same<T, __nv_bfloat16>::value ? kBF16 : kF16, g1,
-                                                   g2, num_sms, s);
+  const bool ok =
+      chunk != 8      ? launch_int4_many(std::is_same<T, __nv_bfloat16>::value ? kBF16 : kF16, g1, g2,
+                                         num_sms, s)
+      : g1.G == 32 ? launch_few<T, true>(g1, g2, num_sms, s)
+                   : launch_few<T, false>(g1, g2, num_sms, s);
   return ok && launch_dependent(int4_combine_kernel<T>, grid_for(T_ * g2.N, num_sms), 256, 0, s,
                                 static_cast<const float*>(g2.out), idx, T_, k, g2.N, g2.E,
                                 static_cast<T*>(out));
@@ -977,9 +729,8 @@ void launch_int4_expand(int dtype, const void* w, int E, int K, int N, int G, bo
   else expand<__half>(w, E, K, N, G, zeros, trans, out, s);
 }
 
-int int4_chunk_rows(int64_t rows, int E, int H, int I) {
-  if (rows <= 4 * static_cast<int64_t>(E)) return 8;
-  return H % 128 == 0 && I % 128 == 0 ? int4_many_rows() : 32;
+int int4_chunk_rows(int64_t rows, int E) {
+  return rows <= 4 * static_cast<int64_t>(E) ? 8 : int4_many_rows();
 }
 
 int launch_int4_quantize(int dtype, const void* w, int E, int K, int N, int G, int symmetric,

@@ -185,9 +185,8 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
     auto locate = [&]() {
       if (pu < units) {
         const Unit d = unit_of(pu);
-        // a panel past the last column repeats the first strips; its sums are not read
-        int at = d.mt * (kCols / 16) + (kDual ? 0 : panel * 8) + strip;
-        if (at >= p.N / 16) at = strip;
+        // a strip past the last column repeats the last one; its sums are not read
+        const int at = min(d.mt * (kCols / 16) + (kDual ? 0 : panel * 8) + strip, p.N / 16 - 1);
         src = static_cast<const char*>(p.w[kDual ? panel : 0]) +
               (static_cast<int64_t>(d.e) * (p.N / 16) + at) * kb * p.rec;
       }
@@ -247,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
       const Unit d = unit_of(u);
       const int col = d.mt * kCols + 32 * q + lane;
-      const bool second = kDual || d.mt * kCols + 128 < p.N;
+      const bool first = col < p.N, second = col + 128 < p.N;
       const bool ok = mbar_wait_parked(smem_addr(&acc_full[buf]), phase, &s_abort, p.err,
                                         kErrWaitAccFull);
       if (!__all_sync(0xffffffffu, ok)) break;
@@ -273,14 +272,14 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
             float y = __uint_as_float(v[i]), y2 = __uint_as_float(g[i]);
             if (kDown) {
               float* out = static_cast<float*>(p.out) + row * p.N + col;
-              out[0] = y * w;
+              if (first) out[0] = y * w;
               if (second) out[128] = y2 * w;
             } else {
               // the intermediate is rounded to the 16-bit type that the second product reads
               T* out = static_cast<T*>(p.out) + row * p.N + col;
               y = act_apply(y, p.act);
               if (kDual) y *= y2;
-              out[0] = Elem<T>::from_f(y);
+              if (first) out[0] = Elem<T>::from_f(y);
               if (!kDual && second) out[128] = Elem<T>::from_f(act_apply(y2, p.act));
             }
           }
