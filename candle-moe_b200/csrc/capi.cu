@@ -1004,7 +1004,7 @@ Int4WsLayout int4_ws_layout(int64_t T, int H, int I, int E, int k) {
 // expansion moves 2.5 bytes a weight and is paid once, where the packed kernels unpack a weight
 // again for every chunk of rows.
 bool int4_expands(int64_t T, int H, int I, int E, int k) {
-  return H % 128 == 0 && I % 128 == 0 && E <= sm100_max_experts() && T * k >= 64 * E;
+  return H % 128 == 0 && I % 128 == 0 && E <= sm100_max_experts() && T * k >= 256 * E;
 }
 
 }  // namespace

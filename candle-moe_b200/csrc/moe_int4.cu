@@ -730,7 +730,9 @@ void launch_int4_expand(int dtype, const void* w, int E, int K, int N, int G, bo
 }
 
 int int4_chunk_rows(int64_t rows, int E) {
-  return rows <= 4 * static_cast<int64_t>(E) ? 8 : int4_many_rows();
+  (void)E;
+  (void)rows;
+  return int4_many_rows();
 }
 
 int launch_int4_quantize(int dtype, const void* w, int E, int K, int N, int G, int symmetric,

@@ -26,7 +26,7 @@ namespace {
 
 constexpr int kTileRows = 64;
 constexpr int kUnpackWarps = 16, kOutWarps = 4, kGatherWarps = 4;
-constexpr int kThreads = (kUnpackWarps + kOutWarps + kGatherWarps + 1) * 32;
+constexpr int kThreads = (kUnpackWarps + kOutWarps + kGatherWarps + 2) * 32;
 constexpr int kStageBlocks = 2;           // k64 blocks that are handed over at once
 constexpr int kStages = 2;                // of weights in tensor memory
 constexpr int kXSlots = 4;                // stages of rows in shared memory
@@ -109,7 +109,7 @@ template <typename T, bool kDual, bool kDown, bool kZeros>
 __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
   constexpr int kCols = kDual ? 128 : 256;  // output columns of a unit
   extern __shared__ __align__(128) char smem_raw[];
-  __shared__ alignas(8) uint64_t s_ring[kUnpackWarps][kRingSlots];
+  __shared__ alignas(8) uint64_t s_ring[kUnpackWarps][kRingSlots], s_free[kUnpackWarps][kRingSlots];
   __shared__ alignas(8) uint64_t s_full[kStages], s_empty[kStages];
   __shared__ alignas(8) uint64_t acc_full[2], acc_empty[2], s_done;
   __shared__ uint32_t s_tmem;
@@ -127,7 +127,10 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
 
   if (threadIdx.x == 0) {
     for (int w = 0; w < kUnpackWarps; ++w)
-      for (int i = 0; i < kRingSlots; ++i) mbar_init(smem_addr(&s_ring[w][i]), 1);
+      for (int i = 0; i < kRingSlots; ++i) {
+        mbar_init(smem_addr(&s_ring[w][i]), 1);
+        mbar_init(smem_addr(&s_free[w][i]), 1);
+      }
     for (int i = 0; i < kStages; ++i) {
       mbar_init(smem_addr(&s_full[i]), kUnpackWarps + kGatherWarps);
       mbar_init(smem_addr(&s_empty[i]), 1);
@@ -179,32 +182,6 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
     WeightRing<1, kRingSlots> w{rings + warp * kRingSlots * matrix_bytes,
                                       smem_addr(&s_ring[warp][0]), &s_abort, p.err, lane,
                                       matrix_bytes};
-    int64_t pu = blockIdx.x;  // the next stage to ask for: unit, first block
-    int pb = 0;
-    const char* src = nullptr;
-    auto locate = [&]() {
-      if (pu < units) {
-        const Unit d = unit_of(pu);
-        // a strip past the last column repeats the last one; its sums are not read
-        const int at = min(d.mt * (kCols / 16) + (kDual ? 0 : panel * 8) + strip, p.N / 16 - 1);
-        src = static_cast<const char*>(p.w[kDual ? panel : 0]) +
-              (static_cast<int64_t>(d.e) * (p.N / 16) + at) * kb * p.rec;
-      }
-    };
-    auto issue = [&]() {
-      if (pu >= units) return;
-      w.issue(src, nullptr, min(kRingBlocks, kb - pb) * p.rec);
-      src += matrix_bytes;
-      pb += kRingBlocks;
-      if (pb >= kb) {
-        pb = 0;
-        pu += gridDim.x;
-        locate();
-      }
-    };
-    locate();
-#pragma unroll
-    for (int i = 0; i < kRingSlots - 1; ++i) issue();
     int at = 0;
     uint32_t phase = 0;
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
@@ -233,8 +210,9 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
           at ^= 1;
           phase ^= at == 0;
         }
+        const int slot = w.slot;
         w.release();
-        issue();
+        if (lane == 0) mbar_arrive(smem_addr(&s_free[warp][slot]));
       }
     }
     w.drain();
@@ -353,6 +331,38 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
       }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+  } else if (warp == kUnpackWarps + kOutWarps + kGatherWarps) {
+    // ------------------------------------------------------------------ weight copies
+    // Lane w feeds the ring of unpacking warp w, kRingBlocks records at a time.
+    if (lane < kUnpackWarps) {
+      const int panel = lane >> 3;
+      const int strip = 2 * (lane & 3) + ((lane >> 2) & 1);
+      const uint32_t full = smem_addr(&s_ring[lane][0]), empty = smem_addr(&s_free[lane][0]);
+      const uint32_t stage_bytes = kRingBlocks * p.rec;
+      const uint32_t to = smem_addr(rings) + lane * kRingSlots * stage_bytes;
+      int slot = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int64_t u = blockIdx.x; ok && u < units; u += gridDim.x) {
+        const Unit d = unit_of(u);
+        // a strip past the last column repeats the last one; its sums are not read
+        const int at = min(d.mt * (kCols / 16) + (kDual ? 0 : panel * 8) + strip, p.N / 16 - 1);
+        const char* src = static_cast<const char*>(p.w[kDual ? panel : 0]) +
+                          (static_cast<int64_t>(d.e) * (p.N / 16) + at) * kb * p.rec;
+        for (int b = 0; b < kb; b += kRingBlocks) {
+          ok = mbar_wait_parked(empty + 8 * slot, phase ^ 1u, &s_abort, p.err, kErrWaitEmpty);
+          if (!ok) break;
+          const uint32_t bytes = min(kRingBlocks, kb - b) * p.rec;
+          mbar_arrive_expect_tx(full + 8 * slot, bytes);
+          bulk_load(to + slot * stage_bytes, src, bytes, full + 8 * slot);
+          src += stage_bytes;
+          if (++slot == kRingSlots) {
+            slot = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
   } else {
     // ------------------------------------------------------------------ MMA issuer
     // The whole warp walks the units, so that descriptors and addresses are uniform values; one
