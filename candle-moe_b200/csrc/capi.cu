@@ -1104,7 +1104,6 @@ CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const vo
     return MOE_ERR_WORKSPACE;
   }
   const int64_t rows = num_tokens * topk;
-  const int chunk = int4_chunk_rows(rows, E);
   Int4Params g1 = {}, g2 = {};
   g1.w[0] = gate_packed;
   g1.w[1] = up_packed;
@@ -1156,7 +1155,7 @@ CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const vo
     g1.idx = g2.idx = expert_indices;
     g1.rows = g2.rows = static_cast<int>(rows);
     g1.k = g2.k = topk;
-    g2.sorted_w = routing_weights;
+    g1.sorted_w = g2.sorted_w = routing_weights;
     g2.out = output;
     const int n = launch_int4_table_ffn(static_cast<int>(dtype), g1, g2, ds->num_sms, s);
     if (n == 0) st = MOE_ERR_CUDA;
@@ -1164,7 +1163,7 @@ CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const vo
     if (owned) cudaFreeAsync(ws, s);
     return finish(st);
   }
-  if (launch_route_prep(expert_indices, routing_weights, num_tokens, topk, E, chunk,
+  if (launch_route_prep(expert_indices, routing_weights, num_tokens, topk, E, int4_many_rows(),
                         reinterpret_cast<int32_t*>(ws + L.offsets),
                         reinterpret_cast<int32_t*>(ws + L.chunk_prefix),
                         reinterpret_cast<int32_t*>(ws + L.sorted_token),
@@ -1173,7 +1172,7 @@ CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const vo
                         s) != 0)
     st = MOE_ERR_CUDA;
   if (st == MOE_OK) {
-    const int n = launch_int4_ffn(static_cast<int>(dtype), chunk, g1, g2, expert_indices,
+    const int n = launch_int4_ffn(static_cast<int>(dtype), g1, g2, expert_indices,
                                   num_tokens, topk, output, ds->num_sms, s);
     if (n == 0) st = MOE_ERR_CUDA;
     g_launches += n + (route_prep_scratch_bytes(rows, E) ? 3 : 1);

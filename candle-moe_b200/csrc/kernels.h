@@ -170,7 +170,7 @@ struct Int4Params {
   const void* x;                // first product: x [T, K]; second: intermediate [rows, K]
   void* out;                    // first: intermediate [rows, N]; second: f32 slots [T*k, N]
   const int32_t* offsets;       // [E+2]
-  const int32_t* chunk_prefix;  // [E+1], chunks of int4_chunk_rows() rows
+  const int32_t* chunk_prefix;  // [E+1], chunks of int4_many_rows() rows
   const int32_t* sorted_token;  // [rows]
   const int32_t* sorted_flat;   // [rows]
   const float* sorted_w;        // [rows]
@@ -179,8 +179,8 @@ struct Int4Params {
   int wk;                       // set by the launch: pieces that the warps split K into
   uint32_t* err;                // device error word
   bool zeros;                   // else every zero point is 8
-  // calls of at most int4_table_rows() rows (no route preparation; sorted_w: the [T, k] weights,
-  // out of the second product: the output [T, N])
+  // calls of at most int4_table_rows() rows (no route preparation; sorted_w: the [T, k] weights, in
+  // both products; out of the second one: the output [T, N])
   const uint32_t* idx;          // [T, k]
   int rows, k;                  // T*k, k
 };
@@ -197,8 +197,6 @@ int launch_int4_table_ffn(int dtype, const Int4Params& g1, const Int4Params& g2,
 // Bytes of a packed record (16 columns x 64 k).
 int int4_record_bytes(int G, bool zeros);
 bool int4_set_attributes();
-// Rows per chunk of the kernel that serves a call of this many rows.
-int int4_chunk_rows(int64_t rows, int E);
 int launch_int4_quantize(int dtype, const void* w, int E, int K, int N, int G, int symmetric,
                          uint8_t* q, void* scales, uint8_t* zeros, int num_sms, cudaStream_t s);
 // Both return the number of kernels launched (0: a launch failed).
@@ -207,9 +205,8 @@ int launch_int4_pack(int dtype, const uint8_t* q, const void* scales, const uint
 // out [E,K,N], or [E,N,K] with trans, in 16 bits; N a multiple of 128.
 void launch_int4_expand(int dtype, const void* w, int E, int K, int N, int G, bool zeros,
                         bool trans, void* out, cudaStream_t s);
-int launch_int4_ffn(int dtype, int chunk_rows, const Int4Params& g1, const Int4Params& g2,
-                    const uint32_t* idx, int64_t num_tokens, int k, void* out, int num_sms,
-                    cudaStream_t s);
+int launch_int4_ffn(int dtype, const Int4Params& g1, const Int4Params& g2, const uint32_t* idx,
+                    int64_t num_tokens, int k, void* out, int num_sms, cudaStream_t s);
 
 // ---- ep_kernels.cu -------------------------------------------------------------------------
 constexpr int kMaxEpBins = 12288;  // (chunk, rank) counters of ep_dest_groups (48 KB smem)

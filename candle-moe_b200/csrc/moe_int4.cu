@@ -24,8 +24,6 @@
 // The word is rotated left so that nibble 0 sits at the top of the mantissa.
 #include <stdint.h>
 
-#include <type_traits>
-
 #include "common.cuh"
 #include "int4.cuh"
 #include "kernels.h"
@@ -235,18 +233,9 @@ __global__ void __launch_bounds__(256)
 // ---- the products ------------------------------------------------------------------------------
 
 constexpr int kWarps = 8;
-constexpr int kStageBlocks = 2;  // k64 blocks of a ring stage
-constexpr int kFewRing = 3;      // stages of a ring
-
-// Expert of chunk c: the number of experts whose chunks all come before it.
-__device__ __forceinline__ int find_expert(const int32_t* __restrict__ prefix, int E, int c) {
-  int e = 0;
-  for (int i = 0; i < E; i += 32) {
-    const int at = i + (threadIdx.x & 31) + 1;
-    e += __popc(__ballot_sync(0xffffffffu, at <= E && __ldg(prefix + at) <= c));
-  }
-  return e;
-}
+constexpr int kRingBlocks = 4;  // k64 blocks of a ring stage
+// Stages of a warp's ring: one ahead of two matrices, two of one, 4 KB a warp either way.
+template <int MATS> constexpr int kFewRing = MATS == 2 ? 2 : 3;
 
 // 16 + the zero points of the two columns (24 without): as the nibbles, a zero point at the top of
 // the mantissa of a number in [16, 32).
@@ -306,15 +295,15 @@ __device__ __forceinline__ void few_block(const char* stage, int matrix_bytes, b
 }
 
 // The `blocks` blocks of a warp's slice (of `per` that the ring holds places for): the activations
-// of a stage are under way while the one before is worked on.
+// of two blocks are under way while the two before are worked on.
 template <typename T, int MATS, bool kG32, typename Issue>
-__device__ __forceinline__ void few_slice(WeightRing<MATS, kFewRing>& w, const T* xr, int per,
+__device__ __forceinline__ void few_slice(WeightRing<MATS, kFewRing<MATS>>& w, const T* xr, int per,
                                           int blocks, int rec, bool zeros, int lane,
                                           float (&fin)[MATS][4], Issue& issue) {
-  uint32_t xn[kStageBlocks][4][2];
+  uint32_t xn[2][4][2];
   auto load_x = [&](int b) {
 #pragma unroll
-    for (int i = 0; i < kStageBlocks; ++i)
+    for (int i = 0; i < 2; ++i)
       if (b + i < blocks) {
 #pragma unroll
         for (int s = 0; s < 8; ++s)
@@ -322,18 +311,22 @@ __device__ __forceinline__ void few_slice(WeightRing<MATS, kFewRing>& w, const T
       }
   };
   load_x(0);
-  for (int b = 0; b < per; b += kStageBlocks) {
-    uint32_t xv[kStageBlocks][4][2];
-#pragma unroll
-    for (int i = 0; i < kStageBlocks; ++i)
-#pragma unroll
-      for (int s = 0; s < 8; ++s) xv[i][s >> 1][s & 1] = xn[i][s >> 1][s & 1];
-    load_x(b + kStageBlocks);
+  for (int r = 0; r < per; r += kRingBlocks) {
     const char* stage = w.wait();
 #pragma unroll
-    for (int i = 0; i < kStageBlocks; ++i)
-      if (b + i < blocks)
-        few_block<T, MATS, kG32>(stage + i * rec, w.matrix_bytes, zeros, lane, xv[i], fin);
+    for (int b = 0; b < kRingBlocks; b += 2) {
+      if (r + b >= blocks) break;
+      uint32_t xv[2][4][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int s = 0; s < 8; ++s) xv[i][s >> 1][s & 1] = xn[i][s >> 1][s & 1];
+      load_x(r + b + 2);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (r + b + i < blocks)
+          few_block<T, MATS, kG32>(stage + (b + i) * rec, w.matrix_bytes, zeros, lane, xv[i], fin);
+    }
     w.release();
     issue();
   }
@@ -366,15 +359,20 @@ struct RowTable {
   int chunk_of[kTableRows];          // chunk of each sorted position
   int first[kTableRows + 1];         // first position of each chunk of at most 8 rows
   int expert[kTableRows];            // expert of each chunk
+  float weight[kTableRows];          // of each flat row
   int chunks;
   uint32_t id[kTableRows];           // scratch
   unsigned starts[kTableRows / 32];  // scratch
 
-  __device__ __forceinline__ void build(const uint32_t* __restrict__ idx, int n, int E) {
+  __device__ __forceinline__ void build(const uint32_t* __restrict__ idx,
+                                        const float* __restrict__ weights, int n, int E) {
     const int i = threadIdx.x;
     uint32_t e = 0xffffffffu;
     if (i < kTableRows) {
-      if (i < n) e = __ldg(idx + i);
+      if (i < n) {
+        e = __ldg(idx + i);
+        weight[i] = __ldg(weights + i);
+      }
       if (e >= static_cast<uint32_t>(E)) e = 0xffffffffu;
       id[i] = e;
     }
@@ -422,20 +420,18 @@ struct RowTable {
   }
 };
 
-// Chunks of at most 8 rows.  A unit is (chunk, WN strips of 16 output columns); the CTA's warps are
-// WN strips x WK pieces of K, so that one token's experts spread over the GPU, and nothing but
-// the sum of a unit's WK partial results makes a warp wait for another.  The activations come
-// straight from L1 / L2, a block ahead.  Rows past the chunk's repeat its last one (columns of
-// the product do not mix).  MATS = 2: gate and up.  kDown: rows are sorted rows of the
-// intermediate, the result is weighted and goes to the (token, slot) row of the f32 slot
-// buffer; else rows are tokens and the activation is applied.  kTable: the rows are sorted here.
-template <typename T, int MATS, bool kDown, bool kG32, bool kTable>
+// The first product of such a call, in chunks of at most 8 rows.  A unit is (chunk, WN strips of 16
+// output columns); the CTA's warps are WN strips x WK pieces of K, so that one token's experts
+// spread over the GPU, and nothing but the sum of a unit's WK partial results makes a warp wait
+// for another.  The activations come straight from L1 / L2, two blocks ahead.  Rows past the
+// chunk's repeat its last one (columns of the product do not mix).  MATS = 2: gate and up.
+template <typename T, int MATS, bool kG32>
 __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) {
+  constexpr int kSlots = kFewRing<MATS>;
   extern __shared__ __align__(128) char smem[];
-  __shared__ alignas(8) uint64_t s_bar[kWarps][kFewRing];
+  __shared__ alignas(8) uint64_t s_bar[kWarps][kSlots];
   __shared__ int s_abort;
-  __shared__ RowTable s_table[1];
-  RowTable& table = s_table[0];
+  __shared__ RowTable table;
   float* red = reinterpret_cast<float*>(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, tig = lane & 3;
@@ -445,29 +441,29 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) 
   init_rings(s_bar, &s_abort);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (kTable) table.build(p.idx, p.rows, p.E);
+  table.build(p.idx, p.sorted_w, p.rows, p.E);
   const int nunits = (ntiles + wn_count - 1) / wn_count;
-  const int units = (kTable ? table.chunks : __ldg(p.chunk_prefix + p.E)) * nunits;
-  auto expert_of = [&](int c) { return kTable ? table.expert[c] : find_expert(p.chunk_prefix, p.E, c); };
-  const int matrix_bytes = kStageBlocks * p.rec;
-  WeightRing<MATS, kFewRing> w{
-      smem + kWarps * MATS * 8 * kFewPitch * 4 + warp * kFewRing * MATS * matrix_bytes,
+  const int units = table.chunks * nunits;
+  const int matrix_bytes = kRingBlocks * p.rec;
+  WeightRing<MATS, kSlots> w{
+      smem + kWarps * MATS * 8 * kFewPitch * 4 + warp * kSlots * MATS * matrix_bytes,
       smem_addr(&s_bar[warp][0]), &s_abort, p.err, lane, matrix_bytes};
   int pu = blockIdx.x, pb = 0;  // the next stage to ask for: unit, first block within [0, per)
   int64_t offset = 0;           // of its first record
   auto locate = [&]() {
     if (pu < units) {
+      const int c = pu / nunits;
       // a strip past the last one repeats it, and its results are dropped
-      const int nt = min(pu % nunits * wn_count + wn, ntiles - 1);
-      offset = ((static_cast<int64_t>(expert_of(pu / nunits)) * ntiles + nt) * kb + b0) * p.rec;
+      const int nt = min((pu - c * nunits) * wn_count + wn, ntiles - 1);
+      offset = ((static_cast<int64_t>(table.expert[c]) * ntiles + nt) * kb + b0) * p.rec;
     }
   };
   auto issue = [&]() {
     if (pu >= units) return;
     w.issue(static_cast<const char*>(p.w[0]) + offset, static_cast<const char*>(p.w[1]) + offset,
-            max(min(kStageBlocks, b1 - b0 - pb), 0) * p.rec);
+            max(min(kRingBlocks, b1 - b0 - pb), 0) * p.rec);
     offset += matrix_bytes;
-    pb += kStageBlocks;
+    pb += kRingBlocks;
     if (pb >= per) {
       pb = 0;
       pu += gridDim.x;
@@ -476,24 +472,13 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) 
   };
   locate();
 #pragma unroll
-  for (int i = 0; i < kFewRing - 1; ++i) issue();
+  for (int i = 0; i < kSlots - 1; ++i) issue();
 
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
     const int c = u / nunits;
-    int row0, rows;
-    if (kTable) {
-      row0 = table.first[c];
-      rows = table.first[c + 1] - row0;
-    } else {
-      const int e = expert_of(c);
-      row0 = __ldg(p.offsets + e) + (c - __ldg(p.chunk_prefix + e)) * 8;
-      rows = min(8, __ldg(p.offsets + e + 1) - row0);
-    }
-    const int r = row0 + min(gid, rows - 1);
+    const int row0 = table.first[c], rows = table.first[c + 1] - row0;
     const T* xr = static_cast<const T*>(p.x) + 2 * tig + 64 * b0 +
-                  static_cast<int64_t>(kDown    ? r
-                                       : kTable ? table.row[r] / p.k
-                                                : __ldg(p.sorted_token + r)) * p.K;
+                  static_cast<int64_t>(table.row[row0 + min(gid, rows - 1)] / p.k) * p.K;
     float fin[MATS][4] = {};
     few_slice<T, MATS, kG32>(w, xr, per, b1 - b0, p.rec, p.zeros, lane, fin, issue);
 #pragma unroll
@@ -502,7 +487,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) 
     __syncthreads();
     for (int i = threadIdx.x; i < wn_count * rows * 16; i += kWarps * 32) {
       const int n = i & 15, at = (i >> 4) % rows, strip = (i >> 4) / rows;
-      const int col = (u % nunits * wn_count + strip) * 16 + n;
+      const int col = ((u - c * nunits) * wn_count + strip) * 16 + n;
       if (col >= p.N) continue;
       float v = 0.f, v1 = 0.f;
       for (int q = 0; q < p.wk; ++q) {  // in the order of k
@@ -510,15 +495,10 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) 
         v += from[0];
         if (MATS == 2) v1 += from[8 * kFewPitch];
       }
-      if (kDown) {
-        static_cast<float*>(p.out)[static_cast<int64_t>(__ldg(p.sorted_flat + row0 + at)) * p.N +
-                                   col] = v * __ldg(p.sorted_w + row0 + at);
-      } else {
-        v = act_apply(v, p.act);
-        if (MATS == 2) v *= v1;
-        // the intermediate is rounded to the 16-bit type that the second product reads
-        static_cast<T*>(p.out)[static_cast<int64_t>(row0 + at) * p.N + col] = Elem<T>::from_f(v);
-      }
+      v = act_apply(v, p.act);
+      if (MATS == 2) v *= v1;
+      // the intermediate is rounded to the 16-bit type that the second product reads
+      static_cast<T*>(p.out)[static_cast<int64_t>(row0 + at) * p.N + col] = Elem<T>::from_f(v);
     }
     __syncthreads();
   }
@@ -531,7 +511,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) 
 template <typename T, bool kG32>
 __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Params p) {
   extern __shared__ __align__(128) char smem[];
-  __shared__ alignas(8) uint64_t s_bar[kWarps][kFewRing];
+  __shared__ alignas(8) uint64_t s_bar[kWarps][kFewRing<1>];
   __shared__ int s_abort;
   __shared__ RowTable table;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -540,15 +520,15 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Param
   init_rings(s_bar, &s_abort);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  table.build(p.idx, p.rows, p.E);
+  table.build(p.idx, p.sorted_w, p.rows, p.E);
   const int chunks = table.chunks;
   // pieces of K: enough tasks for the warps, of three blocks or more
   int pieces = 1;
   while (pieces * 2 * chunks <= kWarps && kb >= 6 * pieces) pieces *= 2;
   const int tasks = chunks * pieces, per = (kb + pieces - 1) / pieces;
-  const int matrix_bytes = kStageBlocks * p.rec;
-  float* part = reinterpret_cast<float*>(smem + kWarps * kFewRing * matrix_bytes);
-  WeightRing<1, kFewRing> w{smem + warp * kFewRing * matrix_bytes, smem_addr(&s_bar[warp][0]),
+  const int matrix_bytes = kRingBlocks * p.rec;
+  float* part = reinterpret_cast<float*>(smem + kWarps * kFewRing<1> * matrix_bytes);
+  WeightRing<1, kFewRing<1>> w{smem + warp * kFewRing<1> * matrix_bytes, smem_addr(&s_bar[warp][0]),
                             &s_abort, p.err, lane, matrix_bytes};
   int pn = blockIdx.x, pt = warp, pb = 0;  // the next stage to ask for: strip, task, block
   int64_t offset = 0;
@@ -567,9 +547,9 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Param
   auto issue = [&]() {
     if (pn >= ntiles || warp >= tasks) return;
     w.issue(static_cast<const char*>(p.w[0]) + offset, nullptr,
-            max(min(kStageBlocks, left - pb), 0) * p.rec);
+            max(min(kRingBlocks, left - pb), 0) * p.rec);
     offset += matrix_bytes;
-    pb += kStageBlocks;
+    pb += kRingBlocks;
     if (pb >= per) {
       pb = 0;
       pt += kWarps;
@@ -578,7 +558,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Param
   };
   locate();
 #pragma unroll
-  for (int i = 0; i < kFewRing - 1; ++i) issue();
+  for (int i = 0; i < kFewRing<1> - 1; ++i) issue();
 
   for (int nt = blockIdx.x; nt < ntiles; nt += gridDim.x) {
     for (int t = warp; t < tasks; t += kWarps) {
@@ -601,7 +581,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Param
         const float* from = part + (c * pieces * 8 + at - table.first[c]) * kFewPitch + n;
         float y = 0.f;
         for (int q = 0; q < pieces; ++q) y += from[q * 8 * kFewPitch];
-        v += y * __ldg(p.sorted_w + t * p.k + j);  // the caller's [T, k] weights
+        v += y * table.weight[t * p.k + j];
       }
       static_cast<T*>(p.out)[static_cast<int64_t>(t) * p.N + nt * 16 + n] = Elem<T>::from_f(v);
     }
@@ -632,19 +612,18 @@ int grid_for(int64_t n, int num_sms) {
   return static_cast<int>(b < cap ? b : cap);
 }
 
-template <typename T, int MATS, bool kDown, bool kG32, bool kTable>
+template <typename T, int MATS, bool kG32>
 struct Few {
-  static constexpr auto kernel = int4_few_kernel<T, MATS, kDown, kG32, kTable>;
+  static constexpr auto kernel = int4_few_kernel<T, MATS, kG32>;
   static size_t smem(int rec) {
     return static_cast<size_t>(kWarps) * MATS *
-           (8 * kFewPitch * 4 + kFewRing * kStageBlocks * rec);
+           (8 * kFewPitch * 4 + kFewRing<MATS> * kRingBlocks * rec);
   }
   static bool launch(Int4Params p, int num_sms, cudaStream_t s) {
-    // pieces of K: a call that the table serves has few units, so as many as leave a warp three
-    // blocks; else eight blocks, for fewer sums across warps
+    // pieces of K: there are few units, so as many as leave a warp three blocks
     p.wk = kWarps;
-    while (p.wk > 1 && p.K / 64 < (kTable ? 3 : 8) * p.wk) p.wk /= 2;
-    // three CTAs on an SM: 3 x (10 + 57 + 2 KB) at most
+    while (p.wk > 1 && p.K / 64 < 3 * p.wk) p.wk /= 2;
+    // three CTAs on an SM: 3 x (10 + 62 + 2 KB) with groups of 64 and more
     return launch_dependent(kernel, num_sms * 3, kWarps * 32, smem(p.rec), s, p);
   }
 };
@@ -656,7 +635,7 @@ struct FewDown {
   // partial results: one task per chunk, or fewer than 2 kWarps with K in pieces
   static size_t smem(int rec, int rows) {
     const int tasks = rows > kWarps ? rows : kWarps;
-    return static_cast<size_t>(kWarps) * kFewRing * kStageBlocks * rec +
+    return static_cast<size_t>(kWarps) * kFewRing<1> * kRingBlocks * rec +
            static_cast<size_t>(tasks) * 8 * kFewPitch * 4;
   }
   static bool launch(const Int4Params& p, int num_sms, cudaStream_t s) {
@@ -669,37 +648,24 @@ template <typename K> bool allow_smem() {
   return cudaFuncSetAttribute(K::kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                               static_cast<int>(K::smem(kMaxRecord))) == cudaSuccess;
 }
-
-template <typename T, bool kG32> bool allow_few() {
-  return allow_smem<Few<T, 2, false, kG32, false>>() && allow_smem<Few<T, 1, false, kG32, false>>() &&
-         allow_smem<Few<T, 1, true, kG32, false>>() && allow_smem<Few<T, 2, false, kG32, true>>() &&
-         allow_smem<Few<T, 1, false, kG32, true>>() && allow_smem<FewDown<T, kG32>>();
-}
-template <typename T> bool gemm_attributes() {
-  return allow_few<T, false>() && allow_few<T, true>();
+template <typename T, bool kG32> bool few_attributes() {
+  return allow_smem<Few<T, 2, kG32>>() && allow_smem<Few<T, 1, kG32>>() &&
+         allow_smem<FewDown<T, kG32>>();
 }
 
-template <typename T, bool kG32, bool kTable>
-bool launch_few_first(const Int4Params& g1, int num_sms, cudaStream_t s) {
-  return g1.w[1] ? Few<T, 2, false, kG32, kTable>::launch(g1, num_sms, s)
-                 : Few<T, 1, false, kG32, kTable>::launch(g1, num_sms, s);
-}
 template <typename T, bool kG32>
-bool launch_few(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
-  return launch_few_first<T, kG32, false>(g1, num_sms, s) &&
-         Few<T, 1, true, kG32, false>::launch(g2, num_sms, s);
+bool launch_table(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
+  return (g1.w[1] ? Few<T, 2, kG32>::launch(g1, num_sms, s)
+                  : Few<T, 1, kG32>::launch(g1, num_sms, s)) &&
+         FewDown<T, kG32>::launch(g2, num_sms, s);
 }
+
 template <typename T>
-bool launch_ffn(int chunk, const Int4Params& g1, const Int4Params& g2, const uint32_t* idx,
-                int64_t T_, int k, void* out, int num_sms, cudaStream_t s) {
-  const bool ok =
-      chunk != 8      ? launch_int4_many(std::is_same<T, __nv_bfloat16>::value ? kBF16 : kF16, g1, g2,
-                                         num_sms, s)
-      : g1.G == 32 ? launch_few<T, true>(g1, g2, num_sms, s)
-                   : launch_few<T, false>(g1, g2, num_sms, s);
-  return ok && launch_dependent(int4_combine_kernel<T>, grid_for(T_ * g2.N, num_sms), 256, 0, s,
-                                static_cast<const float*>(g2.out), idx, T_, k, g2.N, g2.E,
-                                static_cast<T*>(out));
+bool launch_combine(const Int4Params& g2, const uint32_t* idx, int64_t T_, int k, void* out,
+                    int num_sms, cudaStream_t s) {
+  return launch_dependent(int4_combine_kernel<T>, grid_for(T_ * g2.N, num_sms), 256, 0, s,
+                          static_cast<const float*>(g2.out), idx, T_, k, g2.N, g2.E,
+                          static_cast<T*>(out));
 }
 
 template <typename T>
@@ -720,19 +686,15 @@ void expand(const void* w, int E, int K, int N, int G, bool zeros, bool trans, v
 int int4_record_bytes(int G, bool zeros) { return 512 + (G == 32 ? 2 : 1) * (zeros ? 48 : 32); }
 
 bool int4_set_attributes() {
-  return gemm_attributes<__nv_bfloat16>() && gemm_attributes<__half>() && int4_many_set_attributes();
+  return few_attributes<__nv_bfloat16, false>() && few_attributes<__nv_bfloat16, true>() &&
+         few_attributes<__half, false>() && few_attributes<__half, true>() &&
+         int4_many_set_attributes();
 }
 
 void launch_int4_expand(int dtype, const void* w, int E, int K, int N, int G, bool zeros,
                         bool trans, void* out, cudaStream_t s) {
   if (dtype == kBF16) expand<__nv_bfloat16>(w, E, K, N, G, zeros, trans, out, s);
   else expand<__half>(w, E, K, N, G, zeros, trans, out, s);
-}
-
-int int4_chunk_rows(int64_t rows, int E) {
-  (void)E;
-  (void)rows;
-  return int4_many_rows();
 }
 
 int launch_int4_quantize(int dtype, const void* w, int E, int K, int N, int G, int symmetric,
@@ -763,14 +725,6 @@ int launch_int4_pack(int dtype, const uint8_t* q, const void* scales, const uint
 
 int int4_table_rows() { return kTableRows; }
 
-namespace {
-template <typename T, bool kG32>
-bool launch_table(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
-  return launch_few_first<T, kG32, true>(g1, num_sms, s) &&
-         FewDown<T, kG32>::launch(g2, num_sms, s);
-}
-}  // namespace
-
 int launch_int4_table_ffn(int dtype, const Int4Params& g1, const Int4Params& g2, int num_sms,
                           cudaStream_t s) {
   const bool ok = dtype == kBF16
@@ -781,13 +735,12 @@ int launch_int4_table_ffn(int dtype, const Int4Params& g1, const Int4Params& g2,
   return ok ? 2 : 0;
 }
 
-int launch_int4_ffn(int dtype, int chunk_rows, const Int4Params& g1, const Int4Params& g2,
-                    const uint32_t* idx, int64_t num_tokens, int k, void* out, int num_sms,
-                    cudaStream_t s) {
-  const bool ok =
-      dtype == kBF16
-          ? launch_ffn<__nv_bfloat16>(chunk_rows, g1, g2, idx, num_tokens, k, out, num_sms, s)
-          : launch_ffn<__half>(chunk_rows, g1, g2, idx, num_tokens, k, out, num_sms, s);
+int launch_int4_ffn(int dtype, const Int4Params& g1, const Int4Params& g2, const uint32_t* idx,
+                    int64_t num_tokens, int k, void* out, int num_sms, cudaStream_t s) {
+  const bool ok = launch_int4_many(dtype, g1, g2, num_sms, s) &&
+                  (dtype == kBF16
+                       ? launch_combine<__nv_bfloat16>(g2, idx, num_tokens, k, out, num_sms, s)
+                       : launch_combine<__half>(g2, idx, num_tokens, k, out, num_sms, s));
   return ok ? 3 : 0;
 }
 
