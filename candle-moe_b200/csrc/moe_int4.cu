@@ -239,51 +239,63 @@ template <int MATS> constexpr int kFewRing = MATS == 2 ? 2 : 3;
 
 // 16 + the zero points of the two columns (24 without): as the nibbles, a zero point at the top of
 // the mantissa of a number in [16, 32).
-__device__ __forceinline__ void zero_points(const char* record, int per, int h, int gid, bool zeros,
-                                            float& z0, float& z1) {
+template <bool kZeros>
+__device__ __forceinline__ void zero_points(const char* record, int per, int h, int gid, float& z0,
+                                            float& z1) {
   uint32_t z = 0x0808u;
-  if (zeros) z = *reinterpret_cast<const uint16_t*>(record + 512 + 32 * per + 16 * h + 2 * gid);
+  if (kZeros) z = *reinterpret_cast<const uint16_t*>(record + 512 + 32 * per + 16 * h + 2 * gid);
   z0 = __uint_as_float(0x41800000u | ((z & 15u) << 19));
   z1 = __uint_as_float(0x41800000u | ((z & 0x0f00u) << 11));
 }
 
-// One k64 block of at most 8 rows: fin += the products of MATS records with the activations xv
-// (two registers per k16 step).  With the weights as 16 + q the sum of the activations is needed as
-// well; the tensor cores, which have the time, make it.
-template <typename T, int MATS, bool kG32>
-__device__ __forceinline__ void few_block(const char* stage, int matrix_bytes, bool zeros, int lane,
-                                          const uint32_t (&xv)[4][2], float (&fin)[MATS][4]) {
+// NB k64 blocks of at most 8 rows, in one group (two with kG = 32): fin += the products of MATS
+// records a block with the activations xv (two registers per k16 step).  With the weights as
+// 16 + q the sum of the activations is needed as well; the tensor cores, which have the time,
+// make it.
+template <typename T, int MATS, int kG, bool kZeros, int NB>
+__device__ __forceinline__ void few_blocks(const char* stage, int matrix_bytes, int rec, int lane,
+                                           const uint32_t (&xv)[2][4][2], int first,
+                                           float (&fin)[MATS][4]) {
   using T2 = typename Pair<T>::type;
-  constexpr int kPer = kG32 ? 2 : 1;
+  constexpr int kPer = kG == 32 ? 2 : 1;
   constexpr uint32_t one = Nib<T>::kOne;
   const int gid = lane >> 2;
   float xs[kPer][4];
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    if (s == 0 || (kG32 && s == 2))
-      mma16816_zero<T>(xs[(s >> 1) & (kPer - 1)], one, one, one, one, xv[s][0], xv[s][1]);
-    else
-      mma16816<T>(xs[(s >> 1) & (kPer - 1)], one, one, one, one, xv[s][0], xv[s][1]);
-  }
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const uint32_t(&x)[2] = xv[first + b][s];
+      float(&to)[4] = xs[(s >> 1) & (kPer - 1)];
+      if (b == 0 && (s == 0 || (kPer == 2 && s == 2)))
+        mma16816_zero<T>(to, one, one, one, one, x[0], x[1]);
+      else
+        mma16816<T>(to, one, one, one, one, x[0], x[1]);
+    }
 #pragma unroll
   for (int m = 0; m < MATS; ++m) {
     const char* record = stage + m * matrix_bytes;
-    const uint4 wq = *(reinterpret_cast<const uint4*>(record) + lane);
-    const uint32_t word[4] = {wq.x, wq.y, wq.z, wq.w};
     float acc[kPer][4];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const uint32_t a0 = nib_pair<T>(word[s], 0), a1 = nib_pair<T>(word[s], 1),
-                     a2 = nib_pair<T>(word[s], 2), a3 = nib_pair<T>(word[s], 3);
-      if (s == 0 || (kG32 && s == 2))
-        mma16816_zero<T>(acc[(s >> 1) & (kPer - 1)], a0, a1, a2, a3, xv[s][0], xv[s][1]);
-      else
-        mma16816<T>(acc[(s >> 1) & (kPer - 1)], a0, a1, a2, a3, xv[s][0], xv[s][1]);
+    for (int b = 0; b < NB; ++b) {
+      const uint4 wq = *(reinterpret_cast<const uint4*>(record + b * rec) + lane);
+      const uint32_t word[4] = {wq.x, wq.y, wq.z, wq.w};
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const uint32_t(&x)[2] = xv[first + b][s];
+        const uint32_t a0 = nib_pair<T>(word[s], 0), a1 = nib_pair<T>(word[s], 1),
+                       a2 = nib_pair<T>(word[s], 2), a3 = nib_pair<T>(word[s], 3);
+        float(&to)[4] = acc[(s >> 1) & (kPer - 1)];
+        if (b == 0 && (s == 0 || (kPer == 2 && s == 2)))
+          mma16816_zero<T>(to, a0, a1, a2, a3, x[0], x[1]);
+        else
+          mma16816<T>(to, a0, a1, a2, a3, x[0], x[1]);
+      }
     }
 #pragma unroll
     for (int h = 0; h < kPer; ++h) {
       float z0, z1;
-      zero_points(record, kPer, h, gid, zeros, z0, z1);
+      zero_points<kZeros>(record, kPer, h, gid, z0, z1);
       const T2 sc = *(reinterpret_cast<const T2*>(record + 512 + 32 * h) + gid);
       const float s0 = Elem<T>::to_f(sc.x), s1 = Elem<T>::to_f(sc.y);
       fin[m][0] += s0 * (acc[h][0] - z0 * xs[h][0]);
@@ -295,11 +307,12 @@ __device__ __forceinline__ void few_block(const char* stage, int matrix_bytes, b
 }
 
 // The `blocks` blocks of a warp's slice (of `per` that the ring holds places for): the activations
-// of two blocks are under way while the two before are worked on.
-template <typename T, int MATS, bool kG32, typename Issue>
+// of two blocks are under way while the two before are worked on.  With groups of 128 a slice
+// starts on one, and two blocks share their scales.
+template <typename T, int MATS, int kG, bool kZeros, typename Issue>
 __device__ __forceinline__ void few_slice(WeightRing<MATS, kFewRing<MATS>>& w, const T* xr, int per,
-                                          int blocks, int rec, bool zeros, int lane,
-                                          float (&fin)[MATS][4], Issue& issue) {
+                                          int blocks, int rec, int lane, float (&fin)[MATS][4],
+                                          Issue& issue) {
   uint32_t xn[2][4][2];
   auto load_x = [&](int b) {
 #pragma unroll
@@ -322,14 +335,24 @@ __device__ __forceinline__ void few_slice(WeightRing<MATS, kFewRing<MATS>>& w, c
 #pragma unroll
         for (int s = 0; s < 8; ++s) xv[i][s >> 1][s & 1] = xn[i][s >> 1][s & 1];
       load_x(r + b + 2);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (r + b + i < blocks)
-          few_block<T, MATS, kG32>(stage + (b + i) * rec, w.matrix_bytes, zeros, lane, xv[i], fin);
+      const char* from = stage + b * rec;
+      if (kG == 128) {
+        few_blocks<T, MATS, kG, kZeros, 2>(from, w.matrix_bytes, rec, lane, xv, 0, fin);
+      } else {
+        few_blocks<T, MATS, kG, kZeros, 1>(from, w.matrix_bytes, rec, lane, xv, 0, fin);
+        if (r + b + 1 < blocks)
+          few_blocks<T, MATS, kG, kZeros, 1>(from + rec, w.matrix_bytes, rec, lane, xv, 1, fin);
+      }
     }
     w.release();
     issue();
   }
+}
+
+// Blocks of each of `pieces` slices of K: an even number with groups of 128.
+template <int kG> __host__ __device__ __forceinline__ int slice_blocks(int kb, int pieces) {
+  const int n = (kb + pieces - 1) / pieces;
+  return kG == 128 ? (n + 1) & ~1 : n;
 }
 
 constexpr int kFewPitch = 20;  // floats of a row of 16 partial sums
@@ -425,7 +448,7 @@ struct RowTable {
 // spread over the GPU, and nothing but the sum of a unit's WK partial results makes a warp wait
 // for another.  The activations come straight from L1 / L2, two blocks ahead.  Rows past the
 // chunk's repeat its last one (columns of the product do not mix).  MATS = 2: gate and up.
-template <typename T, int MATS, bool kG32>
+template <typename T, int MATS, int kG, bool kZeros>
 __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) {
   constexpr int kSlots = kFewRing<MATS>;
   extern __shared__ __align__(128) char smem[];
@@ -436,7 +459,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, tig = lane & 3;
   const int wk = warp % p.wk, wn = warp / p.wk, wn_count = kWarps / p.wk;
-  const int kb = p.K / 64, ntiles = p.N / 16, per = (kb + p.wk - 1) / p.wk;
+  const int kb = p.K / 64, ntiles = p.N / 16, per = slice_blocks<kG>(kb, p.wk);
   const int b0 = min(wk * per, kb), b1 = min(wk * per + per, kb);
   init_rings(s_bar, &s_abort);
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -480,7 +503,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) 
     const T* xr = static_cast<const T*>(p.x) + 2 * tig + 64 * b0 +
                   static_cast<int64_t>(table.row[row0 + min(gid, rows - 1)] / p.k) * p.K;
     float fin[MATS][4] = {};
-    few_slice<T, MATS, kG32>(w, xr, per, b1 - b0, p.rec, p.zeros, lane, fin, issue);
+    few_slice<T, MATS, kG, kZeros>(w, xr, per, b1 - b0, p.rec, lane, fin, issue);
 #pragma unroll
     for (int m = 0; m < MATS; ++m)
       store_partial(red + (warp * MATS + m) * 8 * kFewPitch, lane, fin[m]);
@@ -508,7 +531,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) 
 // The second product of a call of at most kTableRows rows, with the combine: a CTA takes a strip of
 // 16 output columns of every token.  A warp's task is (chunk, piece of K); the partial results
 // of all tasks meet in shared memory, where the strip's outputs are summed in slot order.
-template <typename T, bool kG32>
+template <typename T, int kG, bool kZeros>
 __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Params p) {
   extern __shared__ __align__(128) char smem[];
   __shared__ alignas(8) uint64_t s_bar[kWarps][kFewRing<1>];
@@ -525,7 +548,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Param
   // pieces of K: enough tasks for the warps, of three blocks or more
   int pieces = 1;
   while (pieces * 2 * chunks <= kWarps && kb >= 6 * pieces) pieces *= 2;
-  const int tasks = chunks * pieces, per = (kb + pieces - 1) / pieces;
+  const int tasks = chunks * pieces, per = slice_blocks<kG>(kb, pieces);
   const int matrix_bytes = kRingBlocks * p.rec;
   float* part = reinterpret_cast<float*>(smem + kWarps * kFewRing<1> * matrix_bytes);
   WeightRing<1, kFewRing<1>> w{smem + warp * kFewRing<1> * matrix_bytes, smem_addr(&s_bar[warp][0]),
@@ -567,7 +590,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Param
       const T* xr = static_cast<const T*>(p.x) + 2 * tig + 64 * b0 +
                     static_cast<int64_t>(row0 + min(gid, rows - 1)) * p.K;
       float fin[1][4] = {};
-      few_slice<T, 1, kG32>(w, xr, per, blocks, p.rec, p.zeros, lane, fin, issue);
+      few_slice<T, 1, kG, kZeros>(w, xr, per, blocks, p.rec, lane, fin, issue);
       store_partial(part + t * 8 * kFewPitch, lane, fin[0]);
     }
     __syncthreads();
@@ -612,9 +635,9 @@ int grid_for(int64_t n, int num_sms) {
   return static_cast<int>(b < cap ? b : cap);
 }
 
-template <typename T, int MATS, bool kG32>
+template <typename T, int MATS, int kG, bool kZeros>
 struct Few {
-  static constexpr auto kernel = int4_few_kernel<T, MATS, kG32>;
+  static constexpr auto kernel = int4_few_kernel<T, MATS, kG, kZeros>;
   static size_t smem(int rec) {
     return static_cast<size_t>(kWarps) * MATS *
            (8 * kFewPitch * 4 + kFewRing<MATS> * kRingBlocks * rec);
@@ -628,9 +651,9 @@ struct Few {
   }
 };
 
-template <typename T, bool kG32>
+template <typename T, int kG, bool kZeros>
 struct FewDown {
-  static constexpr auto kernel = int4_few_down_kernel<T, kG32>;
+  static constexpr auto kernel = int4_few_down_kernel<T, kG, kZeros>;
   static size_t smem(int rec) { return smem(rec, kTableRows); }
   // partial results: one task per chunk, or fewer than 2 kWarps with K in pieces
   static size_t smem(int rec, int rows) {
@@ -648,16 +671,32 @@ template <typename K> bool allow_smem() {
   return cudaFuncSetAttribute(K::kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                               static_cast<int>(K::smem(kMaxRecord))) == cudaSuccess;
 }
-template <typename T, bool kG32> bool few_attributes() {
-  return allow_smem<Few<T, 2, kG32>>() && allow_smem<Few<T, 1, kG32>>() &&
-         allow_smem<FewDown<T, kG32>>();
+template <typename T, int kG, bool kZeros> bool few_attributes() {
+  return allow_smem<Few<T, 2, kG, kZeros>>() && allow_smem<Few<T, 1, kG, kZeros>>() &&
+         allow_smem<FewDown<T, kG, kZeros>>();
+}
+template <typename T> bool few_attributes() {
+  return few_attributes<T, 32, false>() && few_attributes<T, 32, true>() &&
+         few_attributes<T, 64, false>() && few_attributes<T, 64, true>() &&
+         few_attributes<T, 128, false>() && few_attributes<T, 128, true>();
 }
 
-template <typename T, bool kG32>
+template <typename T, int kG, bool kZeros>
 bool launch_table(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
-  return (g1.w[1] ? Few<T, 2, kG32>::launch(g1, num_sms, s)
-                  : Few<T, 1, kG32>::launch(g1, num_sms, s)) &&
-         FewDown<T, kG32>::launch(g2, num_sms, s);
+  return (g1.w[1] ? Few<T, 2, kG, kZeros>::launch(g1, num_sms, s)
+                  : Few<T, 1, kG, kZeros>::launch(g1, num_sms, s)) &&
+         FewDown<T, kG, kZeros>::launch(g2, num_sms, s);
+}
+template <typename T, int kG>
+bool launch_table(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
+  return g1.zeros ? launch_table<T, kG, true>(g1, g2, num_sms, s)
+                  : launch_table<T, kG, false>(g1, g2, num_sms, s);
+}
+template <typename T>
+bool launch_table(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
+  return g1.G == 32   ? launch_table<T, 32>(g1, g2, num_sms, s)
+         : g1.G == 64 ? launch_table<T, 64>(g1, g2, num_sms, s)
+                      : launch_table<T, 128>(g1, g2, num_sms, s);
 }
 
 template <typename T>
@@ -686,9 +725,7 @@ void expand(const void* w, int E, int K, int N, int G, bool zeros, bool trans, v
 int int4_record_bytes(int G, bool zeros) { return 512 + (G == 32 ? 2 : 1) * (zeros ? 48 : 32); }
 
 bool int4_set_attributes() {
-  return few_attributes<__nv_bfloat16, false>() && few_attributes<__nv_bfloat16, true>() &&
-         few_attributes<__half, false>() && few_attributes<__half, true>() &&
-         int4_many_set_attributes();
+  return few_attributes<__nv_bfloat16>() && few_attributes<__half>() && int4_many_set_attributes();
 }
 
 void launch_int4_expand(int dtype, const void* w, int E, int K, int N, int G, bool zeros,
@@ -727,11 +764,8 @@ int int4_table_rows() { return kTableRows; }
 
 int launch_int4_table_ffn(int dtype, const Int4Params& g1, const Int4Params& g2, int num_sms,
                           cudaStream_t s) {
-  const bool ok = dtype == kBF16
-                      ? (g1.G == 32 ? launch_table<__nv_bfloat16, true>(g1, g2, num_sms, s)
-                                    : launch_table<__nv_bfloat16, false>(g1, g2, num_sms, s))
-                      : (g1.G == 32 ? launch_table<__half, true>(g1, g2, num_sms, s)
-                                    : launch_table<__half, false>(g1, g2, num_sms, s));
+  const bool ok = dtype == kBF16 ? launch_table<__nv_bfloat16>(g1, g2, num_sms, s)
+                                 : launch_table<__half>(g1, g2, num_sms, s);
   return ok ? 2 : 0;
 }
 
