@@ -335,26 +335,51 @@ def route_experts(logits: torch.Tensor, top_k: int, scoring: Scoring = Scoring.S
     logits [T,E] f32/f16/bf16, E <= 512; rows may be strided.  Returns (weights [T,k] f32, indices
     [T,k] int32); a slot without an available expert (logit -inf or NaN) holds index E and
     weight 0, which the expert calls skip."""
-    _need_cuda(logits, "logits")
-    _need_rows(logits, "logits")
+    # one test for the ordinary call; what fails it is looked at argument by argument
+    if not (logits.is_cuda and logits.dim() == 2 and logits.is_contiguous()):
+        _need_cuda(logits, "logits")
+        _need_rows(logits, "logits")
     T, E = logits.shape
     dev = logits.device
-    if bias is not None:
+    if bias is not None and not (bias.device == dev and bias.dtype == torch.float32 and
+                                 bias.shape == (E,) and bias.is_contiguous()):
         _need_cuda(bias, "bias")
         _need_contig(bias, "bias")
         if bias.dtype != torch.float32 or tuple(bias.shape) != (E,):
             raise ValueError(f"bias must be a float32 tensor of shape ({E},)")
         _need_same_device(dev, (bias, "bias"))
-    w = torch.empty((T, max(top_k, 0)), dtype=torch.float32, device=dev)
-    idx = torch.empty((T, max(top_k, 0)), dtype=torch.int32, device=dev)
+    slots = (T, top_k if top_k > 0 else 0)
+    w = logits.new_empty(slots, dtype=torch.float32)
+    idx = logits.new_empty(slots, dtype=torch.int32)
     with _on(dev):
-        st = lib().moe_route_experts(_addr(logits), fused_moe_internal_dtype(logits.dtype),
-                                     _row_stride(logits), _addr(bias), T, E, top_k, int(scoring),
-                                     num_groups, topk_groups, int(group_score), int(renormalize),
-                                     scaling, _addr(w), _addr(idx), _raw_stream(dev))
+        st = lib().moe_route_experts(logits.data_ptr(), fused_moe_internal_dtype(logits.dtype),
+                                     _row_stride(logits), None if bias is None else bias.data_ptr(),
+                                     T, E, top_k, scoring, num_groups, topk_groups, group_score,
+                                     renormalize, scaling, w.data_ptr(), idx.data_ptr(),
+                                     _raw_stream(dev))
     if st != MOE_OK:
         raise MoeError(st, "moe_route_experts")
     return w, idx
+
+
+def _check_route_backward(grad_weights, logits, weights, indices) -> None:
+    named = ((grad_weights, "grad_weights"), (weights, "weights"), (indices, "indices"))
+    for t, n in named + ((logits, "logits"),):
+        _need_cuda(t, n)
+    _need_rows(logits, "logits")
+    T = logits.shape[0]
+    if indices.dim() != 2 or indices.shape[0] != T:
+        raise ValueError(f"indices must be [{T}, k], got {tuple(indices.shape)}")
+    if indices.dtype not in _INDEX_DTYPES:
+        raise TypeError("indices must be int32 or uint32")
+    for t, n in named[:2]:
+        if t.dtype != torch.float32:
+            raise TypeError(f"{n} must be float32")
+        if t.shape != indices.shape:
+            raise ValueError(f"{n} must be {tuple(indices.shape)}, got {tuple(t.shape)}")
+    for t, n in named:
+        _need_contig(t, n)
+    _need_same_device(logits.device, *named)
 
 
 def route_experts_backward(grad_weights: torch.Tensor, logits: torch.Tensor,
@@ -365,31 +390,24 @@ def route_experts_backward(grad_weights: torch.Tensor, logits: torch.Tensor,
     grad_weights [T,k] f32; logits, scoring, renormalize and scaling as given to route_experts,
     weights and indices as it returned them.  The picks are constants; the bias has no
     gradient."""
-    for t, n in ((grad_weights, "grad_weights"), (logits, "logits"), (weights, "weights"),
-                 (indices, "indices")):
-        _need_cuda(t, n)
-    _need_rows(logits, "logits")
-    T, E = logits.shape
     dev = logits.device
-    if indices.dim() != 2 or indices.shape[0] != T:
-        raise ValueError(f"indices must be [{T}, k], got {tuple(indices.shape)}")
-    if indices.dtype not in _INDEX_DTYPES:
-        raise TypeError("indices must be int32 or uint32")
-    for t, n in ((grad_weights, "grad_weights"), (weights, "weights")):
-        if t.dtype != torch.float32:
-            raise TypeError(f"{n} must be float32")
-        if t.shape != indices.shape:
-            raise ValueError(f"{n} must be {tuple(indices.shape)}, got {tuple(t.shape)}")
-    for t, n in ((grad_weights, "grad_weights"), (weights, "weights"), (indices, "indices")):
-        _need_contig(t, n)
-    _need_same_device(dev, (grad_weights, "grad_weights"), (weights, "weights"),
-                      (indices, "indices"))
-    grad = torch.empty((T, E), dtype=logits.dtype, device=dev)
+    shape = indices.shape
+    # one test for the ordinary call; what fails it is looked at argument by argument
+    if not (logits.is_cuda and logits.dim() == 2 and logits.is_contiguous() and
+            len(shape) == 2 and shape[0] == logits.shape[0] and
+            indices.dtype in _INDEX_DTYPES and indices.is_contiguous() and indices.device == dev and
+            grad_weights.dtype == torch.float32 and grad_weights.shape == shape and
+            grad_weights.is_contiguous() and grad_weights.device == dev and
+            weights.dtype == torch.float32 and weights.shape == shape and
+            weights.is_contiguous() and weights.device == dev):
+        _check_route_backward(grad_weights, logits, weights, indices)
+    T, E = logits.shape
+    grad = logits.new_empty((T, E))
     with _on(dev):
         st = lib().moe_route_experts_backward(
-            _addr(grad_weights), _addr(logits), fused_moe_internal_dtype(logits.dtype),
-            _row_stride(logits), _addr(weights), _addr(indices), T, E, indices.shape[1],
-            int(scoring), int(renormalize), scaling, _addr(grad), _raw_stream(dev))
+            grad_weights.data_ptr(), logits.data_ptr(), fused_moe_internal_dtype(logits.dtype),
+            _row_stride(logits), weights.data_ptr(), indices.data_ptr(), T, E, shape[1], scoring,
+            renormalize, scaling, grad.data_ptr(), _raw_stream(dev))
     if st != MOE_OK:
         raise MoeError(st, "moe_route_experts_backward")
     return grad
@@ -778,22 +796,15 @@ def int4_workspace_size(num_tokens: int, hidden_dim: int, intermediate_dim: int,
                                                    num_experts, top_k))
 
 
-def fused_moe_int4(input: torch.Tensor, experts: Int4Experts, routing_weights: torch.Tensor,
-                   expert_indices: torch.Tensor, activation: int = Activation.Silu,
-                   out: Optional[torch.Tensor] = None,
-                   workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """fused_moe on 4-bit experts: input [T,H] of the experts' type, routing_weights [T,k] f32,
-    expert_indices [T,k] int32/uint32 (ids >= E are skipped).  workspace: uint8, at least
-    int4_workspace_size() bytes, 256-byte aligned, optional."""
+def _check_int4(input, experts, routing_weights, expert_indices, out, workspace) -> None:
     if input.dim() != 2 or routing_weights.dim() != 2 or expert_indices.dim() != 2:
         raise ValueError("input, routing_weights and expert_indices must be rank 2")
     T, H = input.shape
-    k = expert_indices.shape[1]
     if H != experts.hidden_dim:
         raise ValueError(f"Hidden dimension mismatch (expected {experts.hidden_dim}, got {H})")
     if expert_indices.shape[0] != T or routing_weights.shape[0] != T:
         raise ValueError("Number of tokens mismatch")
-    if routing_weights.shape[1] != k:
+    if routing_weights.shape[1] != expert_indices.shape[1]:
         raise ValueError("Number of selected experts mismatch")
     if input.dtype != experts.dtype:
         raise TypeError(f"input must have the experts' dtype {experts.dtype}, got {input.dtype}")
@@ -812,18 +823,39 @@ def fused_moe_int4(input: torch.Tensor, experts: Int4Experts, routing_weights: t
     for t, n in tensors:
         _need_cuda(t, n)
         _need_contig(t, n)
+    _need_same_device(experts.device, *tensors)
+
+
+def fused_moe_int4(input: torch.Tensor, experts: Int4Experts, routing_weights: torch.Tensor,
+                   expert_indices: torch.Tensor, activation: int = Activation.Silu,
+                   out: Optional[torch.Tensor] = None,
+                   workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """fused_moe on 4-bit experts: input [T,H] of the experts' type, routing_weights [T,k] f32,
+    expert_indices [T,k] int32/uint32 (ids >= E are skipped).  workspace: uint8, at least
+    int4_workspace_size() bytes, 256-byte aligned, optional."""
     dev = experts.device
-    _need_same_device(dev, *tensors)
+    shape = expert_indices.shape
+    # one test for the ordinary call; what fails it is looked at argument by argument
+    if not (input.dim() == 2 and len(shape) == 2 and routing_weights.shape == shape and
+            input.shape == (shape[0], experts.hidden_dim) and input.dtype == experts.dtype and
+            routing_weights.dtype == torch.float32 and expert_indices.dtype in _INDEX_DTYPES and
+            input.is_contiguous() and routing_weights.is_contiguous() and
+            expert_indices.is_contiguous() and input.device == dev and
+            routing_weights.device == dev and expert_indices.device == dev and
+            out is None and workspace is None):
+        _check_int4(input, experts, routing_weights, expert_indices, out, workspace)
+    T, H = input.shape
     if out is None:
-        out = torch.empty((T, H), dtype=input.dtype, device=dev)
+        out = input.new_empty((T, H))
     ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
     with _on(dev):
-        st = lib().moe_fused_int4(_addr(input), _addr(experts.gate), _addr(experts.up),
-                                  _addr(experts.down), _addr(routing_weights), _addr(expert_indices),
-                                  _addr(out), T, H, experts.intermediate_dim, experts.num_experts,
-                                  k, int(activation), fused_moe_internal_dtype(input.dtype),
-                                  experts.group_size, int(experts.has_zeros), _addr(workspace),
-                                  ws_bytes, _raw_stream(dev))
+        st = lib().moe_fused_int4(input.data_ptr(), _addr(experts.gate), _addr(experts.up),
+                                  _addr(experts.down), routing_weights.data_ptr(),
+                                  expert_indices.data_ptr(), out.data_ptr(), T, H,
+                                  experts.intermediate_dim, experts.num_experts, shape[1],
+                                  activation, fused_moe_internal_dtype(input.dtype),
+                                  experts.group_size, experts.has_zeros, _addr(workspace), ws_bytes,
+                                  _raw_stream(dev))
     if st != MOE_OK:
         raise MoeError(st, "moe_fused_int4")
     return out
