@@ -39,7 +39,7 @@ template <>
 __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1,
                                                         uint32_t a2, uint32_t a3, uint32_t b0,
                                                         uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -49,7 +49,7 @@ template <>
 __device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uint32_t a1,
                                                  uint32_t a2, uint32_t a3, uint32_t b0,
                                                  uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -64,7 +64,7 @@ template <>
 __device__ __forceinline__ void mma16816_zero<__nv_bfloat16>(float (&d)[4], uint32_t a0,
                                                              uint32_t a1, uint32_t a2, uint32_t a3,
                                                              uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
@@ -74,7 +74,7 @@ template <>
 __device__ __forceinline__ void mma16816_zero<__half>(float (&d)[4], uint32_t a0, uint32_t a1,
                                                       uint32_t a2, uint32_t a3, uint32_t b0,
                                                       uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
@@ -233,9 +233,10 @@ __global__ void __launch_bounds__(256)
 // ---- the products ------------------------------------------------------------------------------
 
 constexpr int kWarps = 8;
-constexpr int kRingBlocks = 4;  // k64 blocks of a ring stage
-// Stages of a warp's ring: one ahead of two matrices, two of one, 4 KB a warp either way.
-template <int MATS> constexpr int kFewRing = MATS == 2 ? 2 : 3;
+constexpr int kDownWarps = 16;  // of the second product, which has a CTA for each 16 columns
+constexpr int kFewRing = 3;     // stages of a warp's ring
+// k64 blocks of a stage: four records
+template <int MATS> constexpr int kRingBlocks = 4 / MATS;
 
 // 16 + the zero points of the two columns (24 without): as the nibbles, a zero point at the top of
 // the mantissa of a number in [16, 32).
@@ -260,48 +261,45 @@ __device__ __forceinline__ void few_blocks(const char* stage, int matrix_bytes, 
   constexpr int kPer = kG == 32 ? 2 : 1;
   constexpr uint32_t one = Nib<T>::kOne;
   const int gid = lane >> 2;
-  float xs[kPer][4];
+  // an accumulator's MMAs wait for one another, those of different ones do not: step by step, the
+  // sums of the activations and the matrices in turn
+  float xs[kPer][4], acc[MATS][kPer][4];
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
+  for (int b = 0; b < NB; ++b) {
+    uint4 wq[MATS];
+#pragma unroll
+    for (int m = 0; m < MATS; ++m)
+      wq[m] = *(reinterpret_cast<const uint4*>(stage + m * matrix_bytes + b * rec) + lane);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const uint32_t(&x)[2] = xv[first + b][s];
-      float(&to)[4] = xs[(s >> 1) & (kPer - 1)];
-      if (b == 0 && (s == 0 || (kPer == 2 && s == 2)))
-        mma16816_zero<T>(to, one, one, one, one, x[0], x[1]);
-      else
-        mma16816<T>(to, one, one, one, one, x[0], x[1]);
+      const int h = (s >> 1) & (kPer - 1);
+      const bool zero = b == 0 && (s == 0 || (kPer == 2 && s == 2));
+      if (zero) mma16816_zero<T>(xs[h], one, one, one, one, x[0], x[1]);
+      else mma16816<T>(xs[h], one, one, one, one, x[0], x[1]);
+#pragma unroll
+      for (int m = 0; m < MATS; ++m) {
+        const uint32_t word = s == 0 ? wq[m].x : s == 1 ? wq[m].y : s == 2 ? wq[m].z : wq[m].w;
+        const uint32_t a0 = nib_pair<T>(word, 0), a1 = nib_pair<T>(word, 1),
+                       a2 = nib_pair<T>(word, 2), a3 = nib_pair<T>(word, 3);
+        if (zero) mma16816_zero<T>(acc[m][h], a0, a1, a2, a3, x[0], x[1]);
+        else mma16816<T>(acc[m][h], a0, a1, a2, a3, x[0], x[1]);
+      }
     }
+  }
 #pragma unroll
   for (int m = 0; m < MATS; ++m) {
     const char* record = stage + m * matrix_bytes;
-    float acc[kPer][4];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const uint4 wq = *(reinterpret_cast<const uint4*>(record + b * rec) + lane);
-      const uint32_t word[4] = {wq.x, wq.y, wq.z, wq.w};
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const uint32_t(&x)[2] = xv[first + b][s];
-        const uint32_t a0 = nib_pair<T>(word[s], 0), a1 = nib_pair<T>(word[s], 1),
-                       a2 = nib_pair<T>(word[s], 2), a3 = nib_pair<T>(word[s], 3);
-        float(&to)[4] = acc[(s >> 1) & (kPer - 1)];
-        if (b == 0 && (s == 0 || (kPer == 2 && s == 2)))
-          mma16816_zero<T>(to, a0, a1, a2, a3, x[0], x[1]);
-        else
-          mma16816<T>(to, a0, a1, a2, a3, x[0], x[1]);
-      }
-    }
 #pragma unroll
     for (int h = 0; h < kPer; ++h) {
       float z0, z1;
       zero_points<kZeros>(record, kPer, h, gid, z0, z1);
       const T2 sc = *(reinterpret_cast<const T2*>(record + 512 + 32 * h) + gid);
       const float s0 = Elem<T>::to_f(sc.x), s1 = Elem<T>::to_f(sc.y);
-      fin[m][0] += s0 * (acc[h][0] - z0 * xs[h][0]);
-      fin[m][1] += s0 * (acc[h][1] - z0 * xs[h][1]);
-      fin[m][2] += s1 * (acc[h][2] - z1 * xs[h][0]);
-      fin[m][3] += s1 * (acc[h][3] - z1 * xs[h][1]);
+      fin[m][0] += s0 * (acc[m][h][0] - z0 * xs[h][0]);
+      fin[m][1] += s0 * (acc[m][h][1] - z0 * xs[h][1]);
+      fin[m][2] += s1 * (acc[m][h][2] - z1 * xs[h][0]);
+      fin[m][3] += s1 * (acc[m][h][3] - z1 * xs[h][1]);
     }
   }
 }
@@ -310,7 +308,7 @@ __device__ __forceinline__ void few_blocks(const char* stage, int matrix_bytes, 
 // of two blocks are under way while the two before are worked on.  With groups of 128 a slice
 // starts on one, and two blocks share their scales.
 template <typename T, int MATS, int kG, bool kZeros, typename Issue>
-__device__ __forceinline__ void few_slice(WeightRing<MATS, kFewRing<MATS>>& w, const T* xr, int per,
+__device__ __forceinline__ void few_slice(WeightRing<MATS, kFewRing>& w, const T* xr, int per,
                                           int blocks, int rec, int lane, float (&fin)[MATS][4],
                                           Issue& issue) {
   uint32_t xn[2][4][2];
@@ -324,10 +322,10 @@ __device__ __forceinline__ void few_slice(WeightRing<MATS, kFewRing<MATS>>& w, c
       }
   };
   load_x(0);
-  for (int r = 0; r < per; r += kRingBlocks) {
+  for (int r = 0; r < per; r += kRingBlocks<MATS>) {
     const char* stage = w.wait();
 #pragma unroll
-    for (int b = 0; b < kRingBlocks; b += 2) {
+    for (int b = 0; b < kRingBlocks<MATS>; b += 2) {
       if (r + b >= blocks) break;
       uint32_t xv[2][4][2];
 #pragma unroll
@@ -364,8 +362,8 @@ __device__ __forceinline__ void store_partial(float* to, int lane, const float (
     to[(2 * tig + (i & 1)) * kFewPitch + gid + 8 * (i >> 1)] = fin[i];
 }
 
-template <int kSlots>
-__device__ __forceinline__ void init_rings(uint64_t (&bar)[kWarps][kSlots], int* abort_flag) {
+template <int kCount, int kSlots>
+__device__ __forceinline__ void init_rings(uint64_t (&bar)[kCount][kSlots], int* abort_flag) {
   if ((threadIdx.x & 31) == 0)
     for (int i = 0; i < kSlots; ++i) mbar_init(smem_addr(&bar[threadIdx.x >> 5][i]), 1);
   if (threadIdx.x == 0) *abort_flag = 0;
@@ -450,7 +448,8 @@ struct RowTable {
 // chunk's repeat its last one (columns of the product do not mix).  MATS = 2: gate and up.
 template <typename T, int MATS, int kG, bool kZeros>
 __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) {
-  constexpr int kSlots = kFewRing<MATS>;
+  constexpr int kSlots = kFewRing;
+  constexpr int kBlocks = kRingBlocks<MATS>;
   extern __shared__ __align__(128) char smem[];
   __shared__ alignas(8) uint64_t s_bar[kWarps][kSlots];
   __shared__ int s_abort;
@@ -467,7 +466,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) 
   table.build(p.idx, p.sorted_w, p.rows, p.E);
   const int nunits = (ntiles + wn_count - 1) / wn_count;
   const int units = table.chunks * nunits;
-  const int matrix_bytes = kRingBlocks * p.rec;
+  const int matrix_bytes = kBlocks * p.rec;
   WeightRing<MATS, kSlots> w{
       smem + kWarps * MATS * 8 * kFewPitch * 4 + warp * kSlots * MATS * matrix_bytes,
       smem_addr(&s_bar[warp][0]), &s_abort, p.err, lane, matrix_bytes};
@@ -484,9 +483,9 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) 
   auto issue = [&]() {
     if (pu >= units) return;
     w.issue(static_cast<const char*>(p.w[0]) + offset, static_cast<const char*>(p.w[1]) + offset,
-            max(min(kRingBlocks, b1 - b0 - pb), 0) * p.rec);
+            max(min(kBlocks, b1 - b0 - pb), 0) * p.rec);
     offset += matrix_bytes;
-    pb += kRingBlocks;
+    pb += kBlocks;
     if (pb >= per) {
       pb = 0;
       pu += gridDim.x;
@@ -532,9 +531,9 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) 
 // 16 output columns of every token.  A warp's task is (chunk, piece of K); the partial results
 // of all tasks meet in shared memory, where the strip's outputs are summed in slot order.
 template <typename T, int kG, bool kZeros>
-__global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Params p) {
+__global__ void __launch_bounds__(kDownWarps * 32, 1) int4_few_down_kernel(Int4Params p) {
   extern __shared__ __align__(128) char smem[];
-  __shared__ alignas(8) uint64_t s_bar[kWarps][kFewRing<1>];
+  __shared__ alignas(8) uint64_t s_bar[kDownWarps][kFewRing];
   __shared__ int s_abort;
   __shared__ RowTable table;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -547,11 +546,11 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Param
   const int chunks = table.chunks;
   // pieces of K: enough tasks for the warps, of three blocks or more
   int pieces = 1;
-  while (pieces * 2 * chunks <= kWarps && kb >= 6 * pieces) pieces *= 2;
+  while (pieces * 2 * chunks <= kDownWarps && kb >= 6 * pieces) pieces *= 2;
   const int tasks = chunks * pieces, per = slice_blocks<kG>(kb, pieces);
-  const int matrix_bytes = kRingBlocks * p.rec;
-  float* part = reinterpret_cast<float*>(smem + kWarps * kFewRing<1> * matrix_bytes);
-  WeightRing<1, kFewRing<1>> w{smem + warp * kFewRing<1> * matrix_bytes, smem_addr(&s_bar[warp][0]),
+  const int matrix_bytes = kRingBlocks<1> * p.rec;
+  float* part = reinterpret_cast<float*>(smem + kDownWarps * kFewRing * matrix_bytes);
+  WeightRing<1, kFewRing> w{smem + warp * kFewRing * matrix_bytes, smem_addr(&s_bar[warp][0]),
                             &s_abort, p.err, lane, matrix_bytes};
   int pn = blockIdx.x, pt = warp, pb = 0;  // the next stage to ask for: strip, task, block
   int64_t offset = 0;
@@ -570,21 +569,21 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Param
   auto issue = [&]() {
     if (pn >= ntiles || warp >= tasks) return;
     w.issue(static_cast<const char*>(p.w[0]) + offset, nullptr,
-            max(min(kRingBlocks, left - pb), 0) * p.rec);
+            max(min(kRingBlocks<1>, left - pb), 0) * p.rec);
     offset += matrix_bytes;
-    pb += kRingBlocks;
+    pb += kRingBlocks<1>;
     if (pb >= per) {
       pb = 0;
-      pt += kWarps;
+      pt += kDownWarps;
       locate();
     }
   };
   locate();
 #pragma unroll
-  for (int i = 0; i < kFewRing<1> - 1; ++i) issue();
+  for (int i = 0; i < kFewRing - 1; ++i) issue();
 
   for (int nt = blockIdx.x; nt < ntiles; nt += gridDim.x) {
-    for (int t = warp; t < tasks; t += kWarps) {
+    for (int t = warp; t < tasks; t += kDownWarps) {
       const int c = t / pieces, b0 = t % pieces * per, blocks = min(per, kb - b0);
       const int row0 = table.first[c], rows = table.first[c + 1] - row0;
       const T* xr = static_cast<const T*>(p.x) + 2 * tig + 64 * b0 +
@@ -594,7 +593,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_down_kernel(Int4Param
       store_partial(part + t * 8 * kFewPitch, lane, fin[0]);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < p.rows / p.k * 16; i += kWarps * 32) {
+    for (int i = threadIdx.x; i < p.rows / p.k * 16; i += kDownWarps * 32) {
       const int n = i & 15, t = i >> 4;
       float v = 0.f;
       for (int j = 0; j < p.k; ++j) {
@@ -640,13 +639,13 @@ struct Few {
   static constexpr auto kernel = int4_few_kernel<T, MATS, kG, kZeros>;
   static size_t smem(int rec) {
     return static_cast<size_t>(kWarps) * MATS *
-           (8 * kFewPitch * 4 + kFewRing<MATS> * kRingBlocks * rec);
+           (8 * kFewPitch * 4 + kFewRing * kRingBlocks<MATS> * rec);
   }
   static bool launch(Int4Params p, int num_sms, cudaStream_t s) {
     // pieces of K: there are few units, so as many as leave a warp three blocks
     p.wk = kWarps;
     while (p.wk > 1 && p.K / 64 < 3 * p.wk) p.wk /= 2;
-    // three CTAs on an SM: 3 x (10 + 62 + 2 KB) with groups of 64 and more
+    // three CTAs on an SM: 3 x (10 + 52 + 3 KB) with groups of 64 and more
     return launch_dependent(kernel, num_sms * 3, kWarps * 32, smem(p.rec), s, p);
   }
 };
@@ -655,15 +654,15 @@ template <typename T, int kG, bool kZeros>
 struct FewDown {
   static constexpr auto kernel = int4_few_down_kernel<T, kG, kZeros>;
   static size_t smem(int rec) { return smem(rec, kTableRows); }
-  // partial results: one task per chunk, or fewer than 2 kWarps with K in pieces
+  // partial results: one task per chunk, or at most kDownWarps with K in pieces
   static size_t smem(int rec, int rows) {
-    const int tasks = rows > kWarps ? rows : kWarps;
-    return static_cast<size_t>(kWarps) * kFewRing<1> * kRingBlocks * rec +
+    const int tasks = rows > kDownWarps ? rows : kDownWarps;
+    return static_cast<size_t>(kDownWarps) * kFewRing * kRingBlocks<1> * rec +
            static_cast<size_t>(tasks) * 8 * kFewPitch * 4;
   }
   static bool launch(const Int4Params& p, int num_sms, cudaStream_t s) {
-    const int grid = p.N / 16 < num_sms * 3 ? p.N / 16 : num_sms * 3;
-    return launch_dependent(kernel, grid, kWarps * 32, smem(p.rec, p.rows), s, p);
+    const int grid = p.N / 16 < num_sms ? p.N / 16 : num_sms;
+    return launch_dependent(kernel, grid, kDownWarps * 32, smem(p.rec, p.rows), s, p);
   }
 };
 
