@@ -233,7 +233,6 @@ __global__ void __launch_bounds__(256)
 // ---- the products ------------------------------------------------------------------------------
 
 constexpr int kWarps = 8;
-constexpr int kDownWarps = 16;  // of the second product, which has a CTA for each 16 columns
 constexpr int kFewRing = 3;     // stages of a warp's ring
 // k64 blocks of a stage: four records
 template <int MATS> constexpr int kRingBlocks = 4 / MATS;
@@ -530,8 +529,8 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) 
 // The second product of a call of at most kTableRows rows, with the combine: a CTA takes a strip of
 // 16 output columns of every token.  A warp's task is (chunk, piece of K); the partial results
 // of all tasks meet in shared memory, where the strip's outputs are summed in slot order.
-template <typename T, int kG, bool kZeros>
-__global__ void __launch_bounds__(kDownWarps * 32, 1) int4_few_down_kernel(Int4Params p) {
+template <typename T, int kG, bool kZeros, int kDownWarps>
+__global__ void __launch_bounds__(kDownWarps * 32, 16 / kDownWarps) int4_few_down_kernel(Int4Params p) {
   extern __shared__ __align__(128) char smem[];
   __shared__ alignas(8) uint64_t s_bar[kDownWarps][kFewRing];
   __shared__ int s_abort;
@@ -650,9 +649,10 @@ struct Few {
   }
 };
 
-template <typename T, int kG, bool kZeros>
+// kDownWarps 16: one CTA on an SM, for at most as many strips as SMs; 8: two.
+template <typename T, int kG, bool kZeros, int kDownWarps>
 struct FewDown {
-  static constexpr auto kernel = int4_few_down_kernel<T, kG, kZeros>;
+  static constexpr auto kernel = int4_few_down_kernel<T, kG, kZeros, kDownWarps>;
   static size_t smem(int rec) { return smem(rec, kTableRows); }
   // partial results: one task per chunk, or at most kDownWarps with K in pieces
   static size_t smem(int rec, int rows) {
@@ -661,7 +661,8 @@ struct FewDown {
            static_cast<size_t>(tasks) * 8 * kFewPitch * 4;
   }
   static bool launch(const Int4Params& p, int num_sms, cudaStream_t s) {
-    const int grid = p.N / 16 < num_sms ? p.N / 16 : num_sms;
+    const int most = num_sms * (16 / kDownWarps);
+    const int grid = p.N / 16 < most ? p.N / 16 : most;
     return launch_dependent(kernel, grid, kDownWarps * 32, smem(p.rec, p.rows), s, p);
   }
 };
@@ -672,7 +673,7 @@ template <typename K> bool allow_smem() {
 }
 template <typename T, int kG, bool kZeros> bool few_attributes() {
   return allow_smem<Few<T, 2, kG, kZeros>>() && allow_smem<Few<T, 1, kG, kZeros>>() &&
-         allow_smem<FewDown<T, kG, kZeros>>();
+         allow_smem<FewDown<T, kG, kZeros, 8>>() && allow_smem<FewDown<T, kG, kZeros, 16>>();
 }
 template <typename T> bool few_attributes() {
   return few_attributes<T, 32, false>() && few_attributes<T, 32, true>() &&
@@ -684,7 +685,8 @@ template <typename T, int kG, bool kZeros>
 bool launch_table(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
   return (g1.w[1] ? Few<T, 2, kG, kZeros>::launch(g1, num_sms, s)
                   : Few<T, 1, kG, kZeros>::launch(g1, num_sms, s)) &&
-         FewDown<T, kG, kZeros>::launch(g2, num_sms, s);
+         (g2.N / 16 <= num_sms ? FewDown<T, kG, kZeros, 16>::launch(g2, num_sms, s)
+                               : FewDown<T, kG, kZeros, 8>::launch(g2, num_sms, s));
 }
 template <typename T, int kG>
 bool launch_table(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
