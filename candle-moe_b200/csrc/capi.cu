@@ -1004,7 +1004,7 @@ Int4WsLayout int4_ws_layout(int64_t T, int H, int I, int E, int k) {
 // expansion moves 2.5 bytes a weight and is paid once, where the packed kernels unpack a weight
 // again for every chunk of rows.
 bool int4_expands(int64_t T, int H, int I, int E, int k) {
-  return H % 128 == 0 && I % 128 == 0 && E <= sm100_max_experts() && T * k >= 256 * E;
+  return H % 128 == 0 && I % 128 == 0 && E <= sm100_max_experts() && T * k >= 384 * E;
 }
 
 }  // namespace
@@ -1163,19 +1163,23 @@ CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const vo
     if (owned) cudaFreeAsync(ws, s);
     return finish(st);
   }
-  if (launch_route_prep(expert_indices, routing_weights, num_tokens, topk, E, int4_many_rows(),
-                        reinterpret_cast<int32_t*>(ws + L.offsets),
-                        reinterpret_cast<int32_t*>(ws + L.chunk_prefix),
-                        reinterpret_cast<int32_t*>(ws + L.sorted_token),
-                        reinterpret_cast<float*>(ws + L.sorted_w),
-                        reinterpret_cast<int32_t*>(ws + L.sorted_flat), ws + L.prep_scratch,
-                        s) != 0)
+  int32_t* offsets = reinterpret_cast<int32_t*>(ws + L.offsets);
+  int32_t* prefix = reinterpret_cast<int32_t*>(ws + L.chunk_prefix);
+  int32_t* s_token = reinterpret_cast<int32_t*>(ws + L.sorted_token);
+  int32_t* s_flat = reinterpret_cast<int32_t*>(ws + L.sorted_flat);
+  float* s_w = reinterpret_cast<float*>(ws + L.sorted_w);
+  const bool small = rows <= int4_sort_rows();
+  if (small ? !launch_int4_sort(expert_indices, routing_weights, rows, topk, E, int4_many_rows(),
+                                offsets, prefix, s_token, s_w, s_flat, s)
+            : launch_route_prep(expert_indices, routing_weights, num_tokens, topk, E,
+                                int4_many_rows(), offsets, prefix, s_token, s_w, s_flat,
+                                ws + L.prep_scratch, s) != 0)
     st = MOE_ERR_CUDA;
   if (st == MOE_OK) {
     const int n = launch_int4_ffn(static_cast<int>(dtype), g1, g2, expert_indices,
                                   num_tokens, topk, output, ds->num_sms, s);
     if (n == 0) st = MOE_ERR_CUDA;
-    g_launches += n + (route_prep_scratch_bytes(rows, E) ? 3 : 1);
+    g_launches += n + (small || !route_prep_scratch_bytes(rows, E) ? 1 : 3);
   }
   if (owned) cudaFreeAsync(ws, s);
   return finish(st);

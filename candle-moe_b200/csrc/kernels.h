@@ -191,6 +191,12 @@ bool int4_many_set_attributes();
 bool launch_int4_many(int dtype, const Int4Params& g1, const Int4Params& g2, int num_sms,
                       cudaStream_t s);
 int int4_table_rows();
+// The route preparation's tables (all but the scratch) for at most int4_sort_rows() rows.  False: the
+// launch failed.
+int64_t int4_sort_rows();
+bool launch_int4_sort(const uint32_t* idx, const float* weights, int64_t rows, int k, int E,
+                      int chunk, int32_t* offsets, int32_t* chunk_prefix, int32_t* sorted_token,
+                      float* sorted_w, int32_t* sorted_flat, cudaStream_t s);
 // Both products of such a call; returns the number of kernels launched (0: a launch failed).
 int launch_int4_table_ffn(int dtype, const Int4Params& g1, const Int4Params& g2, int num_sms,
                           cudaStream_t s);

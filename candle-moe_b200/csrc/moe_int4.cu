@@ -611,21 +611,131 @@ __global__ void __launch_bounds__(kDownWarps * 32, 16 / kDownWarps) int4_few_dow
   w.drain();
 }
 
-// out[t] = sum over the token's slots in slot order, one rounding.
+// out[t] = sum over the token's slots in slot order, one rounding; four columns a thread.  Bound by
+// the slots it reads.
 template <typename T>
-__global__ void int4_combine_kernel(const float* __restrict__ slots, const uint32_t* __restrict__ idx,
-                                    int64_t T_, int k, int H, int E, T* __restrict__ out) {
+__global__ void __launch_bounds__(256)
+    int4_combine_kernel(const float* __restrict__ slots, const uint32_t* __restrict__ idx, int64_t T_,
+                        int k, int H, int E, T* __restrict__ out) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t total = T_ * H;
+  const int h4 = H / 4;
+  const int64_t total = T_ * h4;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t t = i / H;
-    const int h = static_cast<int>(i % H);
-    float v = 0.f;
+    const int64_t t = i / h4;
+    const int h = static_cast<int>(i - t * h4) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
     for (int j = 0; j < k; ++j)
-      if (__ldg(idx + t * k + j) < static_cast<uint32_t>(E)) v += slots[(t * k + j) * H + h];
-    out[i] = Elem<T>::from_f(v);
+      if (__ldg(idx + t * k + j) < static_cast<uint32_t>(E)) {
+        const float4 y = __ldcs(reinterpret_cast<const float4*>(slots + (t * k + j) * H + h));
+        v.x += y.x;
+        v.y += y.y;
+        v.z += y.z;
+        v.w += y.w;
+      }
+    *reinterpret_cast<uint2*>(out + t * H + h) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
   }
+}
+
+// ---- rows by expert ------------------------------------------------------------------------------
+
+// What the route preparation computes (route_prep.cu: a stable counting sort of the rows by expert,
+// offsets and chunk prefix), in one CTA and three barriers: every warp ranks a run of rows of
+// its own against a table of counts per warp and expert, the table is summed over the warps, and
+// the rows go to base + warps before + rank.  The general kernel takes a barrier for every 512
+// rows (4096 rows: 15 us against 5).
+constexpr int kSortThreads = 1024;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortPer = 4;  // rows of a lane
+
+__device__ __forceinline__ int warp_scan(int v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int n = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += n;
+  }
+  return v;
+}
+
+__global__ void __launch_bounds__(kSortThreads, 1)
+    int4_sort_kernel(const uint32_t* __restrict__ idx, const float* __restrict__ weights, int rows,
+                     int k, int E, int chunk, int32_t* __restrict__ offsets,
+                     int32_t* __restrict__ chunk_prefix, int32_t* __restrict__ sorted_token,
+                     float* __restrict__ sorted_w, int32_t* __restrict__ sorted_flat) {
+  extern __shared__ int smem_i[];
+  int* base = smem_i;                                        // [E]
+  uint16_t* counts = reinterpret_cast<uint16_t*>(base + E);  // [kSortWarps][E], then rows before
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < kSortWarps * E / 2; i += kSortThreads)
+    reinterpret_cast<uint32_t*>(counts)[i] = 0u;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  uint32_t e[kSortPer];
+  float w[kSortPer];
+  int rank[kSortPer];
+#pragma unroll
+  for (int i = 0; i < kSortPer; ++i) {
+    const int r = warp * 32 * kSortPer + i * 32 + lane;
+    e[i] = r < rows ? __ldg(idx + r) : 0xffffffffu;
+    w[i] = r < rows ? __ldg(weights + r) : 0.f;
+  }
+  __syncthreads();
+  uint16_t* mine = counts + warp * E;
+#pragma unroll
+  for (int i = 0; i < kSortPer; ++i) {
+    const bool in = e[i] < static_cast<uint32_t>(E);
+    const unsigned peers = __match_any_sync(0xffffffffu, in ? e[i] : 0xffffffffu);
+    const int before = __popc(peers & ((1u << lane) - 1u));
+    if (in) rank[i] = mine[e[i]] + before;
+    __syncwarp();
+    if (in && before == 0) mine[e[i]] = static_cast<uint16_t>(mine[e[i]] + __popc(peers));
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < E; x += kSortThreads) {
+    int run = 0;
+#pragma unroll 8
+    for (int v = 0; v < kSortWarps; ++v) {
+      const int c = counts[v * E + x];
+      counts[v * E + x] = static_cast<uint16_t>(run);
+      run += c;
+    }
+    base[x] = run;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int rows_before = 0, chunks_before = 0, most = 0;
+    for (int x0 = 0; x0 < E; x0 += 32) {
+      const int x = x0 + lane;
+      const int c = x < E ? base[x] : 0, n = (c + chunk - 1) / chunk;
+      const int ic = warp_scan(c), in = warp_scan(n);
+      if (x < E) {
+        base[x] = rows_before + ic - c;
+        offsets[x] = rows_before + ic - c;
+        chunk_prefix[x] = chunks_before + in - n;
+      }
+      most = max(most, static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<unsigned>(c))));
+      rows_before += __shfl_sync(0xffffffffu, ic, 31);
+      chunks_before += __shfl_sync(0xffffffffu, in, 31);
+    }
+    if (lane == 0) {
+      offsets[E] = rows_before;
+      offsets[E + 1] = most;
+      chunk_prefix[E] = chunks_before;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kSortPer; ++i)
+    if (e[i] < static_cast<uint32_t>(E)) {
+      const int r = warp * 32 * kSortPer + i * 32 + lane;
+      const int at = base[e[i]] + mine[e[i]] + rank[i];
+      sorted_token[at] = r / k;
+      sorted_w[at] = w[i];
+      sorted_flat[at] = r;
+    }
 }
 
 int grid_for(int64_t n, int num_sms) {
@@ -703,7 +813,7 @@ bool launch_table(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaS
 template <typename T>
 bool launch_combine(const Int4Params& g2, const uint32_t* idx, int64_t T_, int k, void* out,
                     int num_sms, cudaStream_t s) {
-  return launch_dependent(int4_combine_kernel<T>, grid_for(T_ * g2.N, num_sms), 256, 0, s,
+  return launch_dependent(int4_combine_kernel<T>, grid_for(T_ * (g2.N / 4), num_sms), 256, 0, s,
                           static_cast<const float*>(g2.out), idx, T_, k, g2.N, g2.E,
                           static_cast<T*>(out));
 }
@@ -726,7 +836,10 @@ void expand(const void* w, int E, int K, int N, int G, bool zeros, bool trans, v
 int int4_record_bytes(int G, bool zeros) { return 512 + (G == 32 ? 2 : 1) * (zeros ? 48 : 32); }
 
 bool int4_set_attributes() {
-  return few_attributes<__nv_bfloat16>() && few_attributes<__half>() && int4_many_set_attributes();
+  return few_attributes<__nv_bfloat16>() && few_attributes<__half>() &&
+         int4_many_set_attributes() &&
+         cudaFuncSetAttribute(int4_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              route_prep_max_experts() * (4 + 2 * kSortWarps)) == cudaSuccess;
 }
 
 void launch_int4_expand(int dtype, const void* w, int E, int K, int N, int G, bool zeros,
@@ -761,7 +874,22 @@ int launch_int4_pack(int dtype, const uint8_t* q, const void* scales, const uint
   return 2;
 }
 
-int int4_table_rows() { return kTableRows; }
+// Up to here the kernels with a table win: 48 rows of 128 experts (2048 x 768) take 42 us against 49,
+// 64 rows of 8 experts (4096 x 1536) 58 against 46.
+int int4_table_rows() { return 48; }
+
+static size_t sort_smem(int E) {
+  return sizeof(int) * E + sizeof(uint16_t) * kSortWarps * static_cast<size_t>(E);
+}
+
+bool launch_int4_sort(const uint32_t* idx, const float* weights, int64_t rows, int k, int E,
+                      int chunk, int32_t* offsets, int32_t* chunk_prefix, int32_t* sorted_token,
+                      float* sorted_w, int32_t* sorted_flat, cudaStream_t s) {
+  return launch_dependent(int4_sort_kernel, 1, kSortThreads, sort_smem(E), s, idx, weights,
+                          static_cast<int>(rows), k, E, chunk, offsets, chunk_prefix, sorted_token,
+                          sorted_w, sorted_flat);
+}
+int64_t int4_sort_rows() { return kSortThreads * kSortPer; }
 
 int launch_int4_table_ffn(int dtype, const Int4Params& g1, const Int4Params& g2, int num_sms,
                           cudaStream_t s) {
