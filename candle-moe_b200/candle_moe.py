@@ -916,6 +916,15 @@ class FusedMoE:
         return fused_moe_int4(input, experts, routing_weights, expert_indices, self.activation)
 
 
+def _router_logits(hidden: torch.Tensor, router_weight: torch.Tensor) -> torch.Tensor:
+    """hidden . router_weight^T in f32: the fused projection kernel's logits where it takes the
+    shape (a power of two of at most 256 experts, H a multiple of 64), else a library GEMM."""
+    E, H = router_weight.shape
+    if E & (E - 1) == 0 and E <= 256 and H % 64 == 0:
+        return router_project_topk(hidden, router_weight, 1, return_logits=True)[3]
+    return torch.mm(hidden, router_weight.t(), out_dtype=torch.float32)
+
+
 class SparseMoeBlock:
     """The MoE layer a model calls around this library (the router Linear, the softmax top-k and
     the expert FFN of README.md:61-97, as in Qwen3-MoE's and Qwen2-MoE's sparse blocks).
@@ -928,17 +937,40 @@ class SparseMoeBlock:
 
     router_weight [E,H]; gate/up [E,H,I]; down [E,I,H] (Qwen3, moe_type 0) or None (Nomic,
     moe_type 1); shared_gate/shared_up [1,H,Is] and shared_down [1,Is,H]; shared_expert_gate
-    [1,H].  All in the hidden states' dtype (f16/bf16)."""
+    [1,H].  All in the hidden states' dtype (f16/bf16).
+
+    Routing other than softmax + top-k -- scoring, correction_bias [E] f32 (steers the picks
+    only), num_groups / topk_groups / group_score, routed_scaling, or a number of experts that is
+    not a power of two -- goes through route_experts.  int4_experts (Int4Experts) takes the place
+    of gate, up and down weights (then None)."""
 
     def __init__(self, router_weight, gate_weights, up_weights, down_weights, top_k: int,
                  activation: Activation = Activation.Silu, norm_topk_prob: bool = True,
-                 shared_gate=None, shared_up=None, shared_down=None, shared_expert_gate=None):
+                 shared_gate=None, shared_up=None, shared_down=None, shared_expert_gate=None,
+                 scoring: Scoring = Scoring.Softmax, correction_bias=None, num_groups: int = 1,
+                 topk_groups: int = 1, group_score: GroupScore = GroupScore.Max,
+                 routed_scaling: float = 1.0, int4_experts: Optional[Int4Experts] = None):
         self.router_weight = router_weight
         self.gate_weights, self.up_weights, self.down_weights = gate_weights, up_weights, down_weights
-        self.moe_type = 0 if down_weights is not None else 1
         self.num_experts = router_weight.shape[0]
+        self.int4_experts = int4_experts
+        if int4_experts is not None:
+            if any(w is not None for w in (gate_weights, up_weights, down_weights)):
+                raise ValueError("int4_experts takes the place of gate, up and down weights")
+            if int4_experts.num_experts != self.num_experts:
+                raise ValueError("Number of experts mismatch")
+            self.moe_type = 0 if int4_experts.up is not None else 1
+        else:
+            self.moe_type = 0 if down_weights is not None else 1
         self.top_k = top_k
         self.norm_topk_prob = norm_topk_prob
+        self.scoring, self.correction_bias = Scoring(scoring), correction_bias
+        self.num_groups, self.topk_groups = num_groups, topk_groups
+        self.group_score, self.routed_scaling = GroupScore(group_score), routed_scaling
+        E = self.num_experts
+        self.general_routing = (self.scoring != Scoring.Softmax or correction_bias is not None or
+                                num_groups != 1 or routed_scaling != 1.0 or E & (E - 1) != 0 or
+                                E > 256)
         self.experts = FusedMoE(self.num_experts, top_k, activation)
         self.shared = None
         if shared_gate is not None:
@@ -948,12 +980,26 @@ class SparseMoeBlock:
             self.shared_moe = FusedMoE(1, 1, activation)
         self.shared_expert_gate = shared_expert_gate
 
-    def forward(self, hidden: torch.Tensor, return_router_logits: bool = False):
+    def route(self, hidden: torch.Tensor):
+        """(weights [T,k] f32, indices [T,k] int32, logits [T,E] f32) of the tokens."""
+        if self.general_routing:
+            logits = _router_logits(hidden, self.router_weight)
+            w, idx = route_experts(logits, self.top_k, self.scoring, self.correction_bias,
+                                   self.num_groups, self.topk_groups, self.group_score,
+                                   self.norm_topk_prob, self.routed_scaling)
+            return w, idx, logits
         w, idx, _, logits = router_project_topk(hidden, self.router_weight, self.top_k,
                                                 renormalize=self.norm_topk_prob,
                                                 return_logits=True)
-        out = self.experts.forward(hidden, self.gate_weights, self.up_weights, self.down_weights,
-                                   w, idx, self.moe_type)
+        return w, idx, logits
+
+    def forward(self, hidden: torch.Tensor, return_router_logits: bool = False):
+        w, idx, logits = self.route(hidden)
+        if self.int4_experts is not None:
+            out = self.experts.forward_int4(hidden, self.int4_experts, w, idx)
+        else:
+            out = self.experts.forward(hidden, self.gate_weights, self.up_weights,
+                                       self.down_weights, w, idx, self.moe_type)
         if self.shared is not None:
             T = hidden.shape[0]
             if self.shared_expert_gate is not None:

@@ -125,4 +125,113 @@ unsafe extern "C" {
         workspace_bytes: usize,
         stream: *mut c_void,
     ) -> c_int;
+
+    /// General routing: softmax (0) or sigmoid (1) scores, a balance bias f32 [num_experts] that
+    /// steers the picks only (may be null), groups of experts, top-k, optional renormalisation.
+    pub(crate) fn moe_route_experts(
+        logits: *const c_void,
+        dtype: u32,
+        logits_stride: i64,
+        bias: *const f32,
+        num_tokens: i64,
+        num_experts: i32,
+        topk: i32,
+        scoring: i32,
+        num_groups: i32,
+        topk_groups: i32,
+        group_score: i32,
+        renormalize: i32,
+        scaling: f32,
+        topk_weights: *mut f32,
+        topk_indices: *mut i32,
+        stream: *mut c_void,
+    ) -> c_int;
+
+    /// Gradient of moe_route_experts' weights with respect to the logits.
+    pub(crate) fn moe_route_experts_backward(
+        grad_weights: *const f32,
+        logits: *const c_void,
+        dtype: u32,
+        logits_stride: i64,
+        topk_weights: *const f32,
+        topk_indices: *const i32,
+        num_tokens: i64,
+        num_experts: i32,
+        topk: i32,
+        scoring: i32,
+        renormalize: i32,
+        scaling: f32,
+        grad_logits: *mut c_void,
+        stream: *mut c_void,
+    ) -> c_int;
+
+    /// Bytes of a 4-bit weight matrix in the layout moe_fused_int4 reads (0: not a valid shape).
+    pub(crate) fn moe_int4_packed_size(
+        num_experts: i32,
+        k_dim: i32,
+        n_dim: i32,
+        group_size: i32,
+        dtype: u32,
+        has_zeros: i32,
+    ) -> usize;
+
+    /// Nibbles, scales and (when not null) zero points of f16/bf16 weights.
+    pub(crate) fn moe_int4_quantize(
+        weights: *const c_void,
+        num_experts: i32,
+        k_dim: i32,
+        n_dim: i32,
+        group_size: i32,
+        dtype: u32,
+        q: *mut u8,
+        scales: *mut c_void,
+        zeros: *mut u8,
+        stream: *mut c_void,
+    ) -> c_int;
+
+    /// Copy of nibbles, scales and zero points (may be null) into that layout.
+    pub(crate) fn moe_int4_pack(
+        q: *const u8,
+        scales: *const c_void,
+        zeros: *const u8,
+        num_experts: i32,
+        k_dim: i32,
+        n_dim: i32,
+        group_size: i32,
+        dtype: u32,
+        packed: *mut c_void,
+        stream: *mut c_void,
+    ) -> c_int;
+
+    /// Bytes of workspace moe_fused_int4 needs for a call of these sizes.
+    pub(crate) fn moe_fused_int4_workspace_size(
+        num_tokens: i64,
+        hidden_dim: i32,
+        intermediate_dim: i32,
+        num_experts: i32,
+        topk: i32,
+    ) -> usize;
+
+    /// moe_fused_v2 on packed 4-bit weights (up_packed null: two-matrix experts).
+    pub(crate) fn moe_fused_int4(
+        input: *const c_void,
+        gate_packed: *const c_void,
+        up_packed: *const c_void,
+        down_packed: *const c_void,
+        routing_weights: *const f32,
+        expert_indices: *const u32,
+        output: *mut c_void,
+        num_tokens: i64,
+        hidden_dim: i32,
+        intermediate_dim: i32,
+        num_experts: i32,
+        topk: i32,
+        activation_type: i32,
+        dtype: u32,
+        group_size: i32,
+        has_zeros: i32,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        stream: *mut c_void,
+    ) -> c_int;
 }
