@@ -280,7 +280,12 @@ int moe_fused_v2(const void* input, const void* gate_weights, const void* up_wei
  * moe_fused_int4: moe_fused_v2 on packed weights, f16/bf16.  up_packed NULL: out = sum_j w
  *   act(x.Gate).Down (the Nomic form; its second matrix packed as [E, I, H]).  has_zeros tells
  *   whether all matrices were packed with zeros.  workspace as moe_fused_v2, of
- *   moe_fused_int4_workspace_size() bytes.
+ *   moe_fused_int4_workspace_size() bytes.  input, output and the packed matrices 16-byte
+ *   aligned (else MOE_ERR_UNSUPPORTED); output must not overlap input (MOE_ERR_INVALID_ARG).  The intermediate is rounded to `dtype`.  Calls of at
+ *   most 48 rows (num_tokens * topk) apply scales and zero points to f32 sums; larger ones
+ *   round each weight to `dtype` once, and from 384 rows per expert on each slot's
+ *   contribution too (as moe_fused_v2 does), with the weights expanded to 16 bits in the
+ *   workspace.
  */
 size_t moe_int4_packed_size(int32_t num_experts, int32_t k_dim, int32_t n_dim, int32_t group_size,
                             uint32_t dtype, int32_t has_zeros);

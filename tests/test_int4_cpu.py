@@ -24,17 +24,18 @@ def test_sizes():
 
 
 def test_fused_refusals_without_a_gpu():
-    lib, p = cm.lib(), ctypes.c_void_p(256)
+    lib, p, q = cm.lib(), ctypes.c_void_p(256), ctypes.c_void_p(1 << 40)
 
-    def call(x=p, gate=p, down=p, T=4, H=256, I=128, E=8, k=2, dtype=1, G=64):
-        return lib.moe_fused_int4(x, gate, p, down, p, p, p, T, H, I, E, k, 0, dtype, G, 0, None, 0,
+    def call(x=p, gate=p, down=p, T=4, H=256, I=128, E=8, k=2, dtype=1, G=64, out=q):
+        return lib.moe_fused_int4(x, gate, p, down, p, p, out, T, H, I, E, k, 0, dtype, G, 0, None, 0,
                                   None)
     for kw in [dict(T=-1), dict(k=0), dict(H=0), dict(I=-64), dict(E=0), dict(dtype=4),
                dict(G=16), dict(G=0), dict(I=192, G=128), dict(x=None), dict(gate=None),
-               dict(down=None)]:
+               dict(down=None), dict(out=None), dict(out=p), dict(out=ctypes.c_void_p(256 + 2032))]:
         assert call(**kw) == 1, kw
     for kw in [dict(dtype=2), dict(H=96, G=32), dict(I=32, G=32), dict(E=4096), dict(T=2 ** 31),
-               dict(x=ctypes.c_void_p(264)), dict(gate=ctypes.c_void_p(264))]:
+               dict(x=ctypes.c_void_p(264)), dict(gate=ctypes.c_void_p(264)),
+               dict(out=ctypes.c_void_p((1 << 40) + 8))]:
         assert call(**kw) == 2, kw
     assert call(T=0) == 0
 

@@ -73,15 +73,16 @@ def test_zero_tokens():
     assert cm.fused_moe_int4(x, cm.Int4Experts(*mats), w, idx).shape == (0, 64)
 
 
-def test_infinities_stay_in_their_rows():
+@pytest.mark.parametrize("T", [12, 60, 900])
+def test_infinities_stay_in_their_rows(T):
     """A token of infinities or NaN does not reach the other tokens' rows."""
-    x, mats, w, idx = make(5, 12, 4, 2, 128, 128, 64, "bf16", False, False)
+    x, mats, w, idx = make(5, T, 4, 2, 128, 128, 64, "bf16", False, False)
     ex = cm.Int4Experts(*mats)
     clean = cm.fused_moe_int4(x, ex, w, idx)
     x[3] = float("inf")
     x[7] = float("nan")
     got = cm.fused_moe_int4(x, ex, w, idx)
-    keep = [t for t in range(12) if t not in (3, 7)]
+    keep = [t for t in range(T) if t not in (3, 7)]
     assert torch.equal(got[keep], clean[keep])
 
 
@@ -199,14 +200,18 @@ def test_refusals():
     odd = torch.empty(4 * 128 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(4, 128)
     with pytest.raises(cm.MoeError):
         cm.fused_moe_int4(odd, ex, w, idx)
+    with pytest.raises(cm.MoeError):
+        cm.fused_moe_int4(x, ex, w, idx, out=odd)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("zeros", [False, True])
-@pytest.mark.parametrize("T,E,k,H,I,G", [(300, 4, 2, 256, 384, 64), (129, 1, 1, 128, 256, 128),
-                                         (517, 7, 3, 384, 128, 32)])
+@pytest.mark.parametrize("T,E,k,H,I,G", [(300, 4, 2, 256, 384, 64), (517, 7, 3, 384, 128, 32),
+                                         (1500, 16, 3, 128, 192, 64), (400, 1, 1, 128, 256, 128),
+                                         (850, 2, 1, 384, 128, 32), (500, 1, 1, 192, 64, 64)])
 def test_many_rows(T, E, k, H, I, G, dtype, zeros):
-    """Calls whose weights are expanded to 16 bits (the bound counts those roundings)."""
+    """Hundreds of rows per expert, on both sides of the 384 from which the weights are expanded to
+    16 bits, more than 4096 rows, and a shape that stays packed."""
     for nomic in (False, True):
         x, mats, w, idx = make(T + E, T, E, k, H, I, G, dtype, zeros, nomic, skip=0.1)
         run(x, mats, w, idx, cm.Activation.Gelu if nomic else cm.Activation.Silu, rounded=True)
@@ -223,3 +228,33 @@ def test_some_rows_per_expert(T, E, k, H, I, G, dtype, zeros):
         x, mats, w, idx = make(T + E + G, T, E, k, H, I, G, dtype, zeros, nomic, skip=0.1)
         idx[: T // 2, 0] = 0
         run(x, mats, w, idx, cm.Activation.Gelu if nomic else cm.Activation.Silu, rounded=True)
+
+
+@pytest.mark.parametrize("T,E,k", [(6, 8, 8), (7, 8, 7), (24, 30, 2), (25, 30, 2), (48, 4, 1)])
+def test_around_the_table_limit(T, E, k):
+    """48 rows and the first calls beyond, tokens of one expert with more than a chunk of rows."""
+    x, mats, w, idx = make(T * k, T, E, k, 192, 128, 64, "f16", True, False)
+    run(x, mats, w, idx, 0, rounded=True)
+    idx[:, 0] = 1
+    run(x, mats, w, idx, 0, rounded=True)
+
+
+def test_wide_and_long_shapes():
+    """More columns than one wave of CTAs takes, and a long reduction with an odd number of blocks."""
+    for T in (2, 70):
+        x, mats, w, idx = make(T, T, 2, 2, 4416, 64, 64, "bf16", False, False)
+        run(x, mats, w, idx, 0, rounded=True)
+
+
+def test_output_over_the_input_is_refused():
+    x, mats, w, idx = make(5, 5, 2, 1, 128, 128, 32, "bf16", False, False)
+    ex = cm.Int4Experts(*mats)
+    both = torch.zeros(9, 128, dtype=torch.bfloat16, device="cuda")
+    for out in (x, both[4:]):
+        src = x if out is x else both[:5]
+        before = src.clone()
+        with pytest.raises(cm.MoeError):
+            cm.fused_moe_int4(src, ex, w, idx, out=out)
+        assert torch.equal(src, before)
+    assert torch.equal(cm.fused_moe_int4(both[:4], ex, w[:4], idx[:4], out=both[4:8]),
+                       cm.fused_moe_int4(both[:4], ex, w[:4], idx[:4]))
