@@ -52,12 +52,13 @@ def test_plain(dtype, T, E, k, scoring):
 @pytest.mark.parametrize("with_bias", [False, True])
 @pytest.mark.parametrize("E,n,kg,k", [(256, 8, 4, 8), (160, 8, 3, 6), (64, 4, 1, 3), (60, 5, 2, 4),
                                       (96, 32, 7, 12), (34, 17, 2, 3), (512, 2, 1, 32),
-                                      (32, 32, 5, 5), (66, 3, 3, 9)])
+                                      (32, 32, 5, 5), (66, 3, 3, 9), (256, 1, 1, 8), (60, 1, 1, 4),
+                                      (100, 1, 1, 12), (512, 16, 4, 8), (8, 2, 1, 2)])
 def test_groups(E, n, kg, k, group_score, with_bias, scoring):
     T = 61
     rng = np.random.default_rng(E + n)
     bias = np.round(rng.normal(size=E) * 0.1, 3) if with_bias else None
-    for dtype in ("f32", "bf16"):
+    for dtype in ("f32", "bf16", "f16"):
         x = make_logits(E * 7 + kg, T, E, dtype)
         check_route(x, k, bias=bias, scoring=cm.Scoring(scoring), num_groups=n, topk_groups=kg,
                     group_score=cm.GroupScore(group_score), renormalize=True, scaling=2.5)
@@ -270,3 +271,30 @@ def test_on_another_stream_and_in_a_graph():
         assert torch.equal(w2, w3) and torch.equal(i2, i3)
         assert torch.equal(d2, cm.route_experts_backward(g, x, w3, i3, renormalize=True))
     assert not torch.equal(d0, d2)
+
+
+@pytest.mark.parametrize("E,n,kg,k", [(128, 1, 1, 8), (256, 8, 4, 8), (60, 1, 1, 10), (40, 5, 2, 3),
+                                      (512, 1, 1, 32), (4, 1, 1, 4)])
+@pytest.mark.parametrize("scoring", [0, 1])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_constant_rows(E, n, kg, k, scoring, with_bias):
+    """Every logit the same (an untrained router, a padded batch): the first experts of the first
+    groups, at equal weights."""
+    x = torch.zeros(70, E, device="cuda", dtype=torch.bfloat16)
+    x[30:50] = 3.0
+    bias = np.zeros(E) if with_bias else None
+    w, idx = check_route(x, k, bias=bias, scoring=cm.Scoring(scoring), num_groups=n,
+                         topk_groups=kg, group_score=cm.GroupScore.Top2, renormalize=True)
+    assert (idx == torch.arange(k, device="cuda")).all()
+
+
+def test_few_distinct_logits():
+    """16-bit logits of a handful of values, with a bias of a handful: ties in every row."""
+    rng = np.random.default_rng(8)
+    x = torch.from_numpy(rng.integers(-3, 4, size=(300, 64)) * 0.5).bfloat16().cuda()
+    bias = rng.integers(-1, 2, size=64) * 0.125
+    for k in (4, 8, 20):
+        for kw in (dict(), dict(num_groups=4, topk_groups=2, group_score=cm.GroupScore.Top2)):
+            check_route(x, k, bias=bias, scoring=cm.Scoring.Sigmoid, renormalize=True, **kw)
+            check_route(x, k, bias=bias, scoring=cm.Scoring.Softmax, **kw)
+            check_route(x, k, scoring=cm.Scoring.Sigmoid, **kw)
