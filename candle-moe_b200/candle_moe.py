@@ -294,7 +294,7 @@ _NO_GUARD = contextlib.nullcontext()
 
 def _on(dev: torch.device):
     """Context with `dev` current; nothing to enter (and no time spent) when it already is."""
-    return _NO_GUARD if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return _NO_GUARD if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
 
 
 def _raw_stream(dev: torch.device) -> int:
@@ -303,6 +303,14 @@ def _raw_stream(dev: torch.device) -> int:
 
 def _addr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
+
+
+_DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def _dtype_code(dtype: torch.dtype) -> int:
+    code = _DTYPE_CODES.get(dtype)
+    return fused_moe_internal_dtype(dtype) if code is None else code  # raises for other types
 
 
 def _need_rows(t: torch.Tensor, name: str):
@@ -352,7 +360,7 @@ def route_experts(logits: torch.Tensor, top_k: int, scoring: Scoring = Scoring.S
     w = logits.new_empty(slots, dtype=torch.float32)
     idx = logits.new_empty(slots, dtype=torch.int32)
     with _on(dev):
-        st = lib().moe_route_experts(logits.data_ptr(), fused_moe_internal_dtype(logits.dtype),
+        st = lib().moe_route_experts(logits.data_ptr(), _dtype_code(logits.dtype),
                                      _row_stride(logits), None if bias is None else bias.data_ptr(),
                                      T, E, top_k, scoring, num_groups, topk_groups, group_score,
                                      renormalize, scaling, w.data_ptr(), idx.data_ptr(),
@@ -405,7 +413,7 @@ def route_experts_backward(grad_weights: torch.Tensor, logits: torch.Tensor,
     grad = logits.new_empty((T, E))
     with _on(dev):
         st = lib().moe_route_experts_backward(
-            grad_weights.data_ptr(), logits.data_ptr(), fused_moe_internal_dtype(logits.dtype),
+            grad_weights.data_ptr(), logits.data_ptr(), _dtype_code(logits.dtype),
             _row_stride(logits), weights.data_ptr(), indices.data_ptr(), T, E, shape[1], scoring,
             renormalize, scaling, grad.data_ptr(), _raw_stream(dev))
     if st != MOE_OK:
@@ -853,7 +861,7 @@ def fused_moe_int4(input: torch.Tensor, experts: Int4Experts, routing_weights: t
                                   _addr(experts.down), routing_weights.data_ptr(),
                                   expert_indices.data_ptr(), out.data_ptr(), T, H,
                                   experts.intermediate_dim, experts.num_experts, shape[1],
-                                  activation, fused_moe_internal_dtype(input.dtype),
+                                  activation, _dtype_code(input.dtype),
                                   experts.group_size, experts.has_zeros, _addr(workspace), ws_bytes,
                                   _raw_stream(dev))
     if st != MOE_OK:

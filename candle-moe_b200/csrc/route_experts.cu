@@ -550,7 +550,7 @@ constexpr int kRowWarps = 4;
 // four in turn (64 contiguous bytes of f32), with groups a lane holds one stretch of one group.
 // NaN needs no care where it is compared: it is never >= t nor > -inf.
 template <typename T, int LPR, int VPL, bool kBias>
-__global__ void __launch_bounds__(kRowWarps * 32, 6)
+__global__ void __launch_bounds__(kRowWarps * 32, VPL <= 16 ? 8 : 6)
     route_experts_rows_kernel(RouteExpertsParams p, int bs, int lpg, int vec) {
   extern __shared__ double smem_d[];
   constexpr int RPW = 32 / LPR;
@@ -1022,13 +1022,13 @@ void launch_rows(const RouteExpertsParams& p, int bs, int lpg, int num_sms, cuda
                                                                                        vec);
 }
 
-// Whether the kernel of LPR lanes per row and 32 experts per lane can take p.
-template <typename T, int LPR>
+// Whether the kernel of LPR lanes per row and VPL experts per lane can take p.
+template <typename T, int LPR, int VPL>
 bool try_rows(const RouteExpertsParams& p, int num_sms, cudaStream_t s) {
   if (LPR % p.num_groups != 0) return false;
   const int lpg = LPR / p.num_groups, bs = (p.E / p.num_groups + lpg - 1) / lpg;
-  if (p.num_groups == 1 ? p.E > 32 * LPR : bs > 32) return false;
-  launch_rows<T, LPR, 32>(p, bs, lpg, num_sms, s);
+  if (p.num_groups == 1 ? p.E > VPL * LPR : bs > VPL) return false;
+  launch_rows<T, LPR, VPL>(p, bs, lpg, num_sms, s);
   return true;
 }
 
@@ -1036,9 +1036,8 @@ template <typename T>
 void launch_route(const RouteExpertsParams& p, int num_sms, cudaStream_t s) {
   if (p.k <= 8) {
     if (p.num_groups == 1 && p.E <= 16) return launch_rows<T, 4, 4>(p, 4, 4, num_sms, s);
-    if (p.num_groups == 1 && p.E <= 64) return launch_rows<T, 4, 16>(p, 16, 4, num_sms, s);
-    if (try_rows<T, 4>(p, num_sms, s) || try_rows<T, 8>(p, num_sms, s) ||
-        try_rows<T, 16>(p, num_sms, s))
+    if (try_rows<T, 4, 16>(p, num_sms, s) || try_rows<T, 8, 16>(p, num_sms, s) ||
+        try_rows<T, 16, 16>(p, num_sms, s) || try_rows<T, 16, 32>(p, num_sms, s))
       return;
   }
   const int lpg = 32 / p.num_groups;
