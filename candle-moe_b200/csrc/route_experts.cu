@@ -199,7 +199,7 @@ __device__ __forceinline__ void store_row(const RouteExpertsParams& p, int64_t r
 
 // Every row in 64 bits: shapes whose rows do not fit the registers of the kernel below.
 template <typename T>
-__global__ void __launch_bounds__(kWarps * 32) route_experts64_kernel(RouteExpertsParams p) {
+__global__ void __launch_bounds__(kWarps * 32) route_experts64_kernel(const __grid_constant__ RouteExpertsParams p) {
   extern __shared__ double smem_d[];
   const int warp = threadIdx.x >> 5;
   double* key = smem_d + warp * row64_scratch(p.E);
@@ -236,7 +236,7 @@ __device__ __forceinline__ float redux_max(float v) {
 // 4e-6) of the largest score.
 template <typename T, int VPT, bool kBias, bool kGroups>
 __global__ void __launch_bounds__(kFastWarps * 32)
-    route_experts_kernel(RouteExpertsParams p, int bs, int lpg, int vec) {
+    route_experts_kernel(const __grid_constant__ RouteExpertsParams p, int bs, int lpg, int vec) {
   extern __shared__ double smem_d[];
   __shared__ alignas(16) float s_key[kFastWarps][kMaxCand];
   __shared__ uint16_t s_id[kFastWarps][kMaxCand];
@@ -551,7 +551,8 @@ constexpr int kRowWarps = 4;
 // NaN needs no care where it is compared: it is never >= t nor > -inf.
 template <typename T, int LPR, int VPL, bool kBias>
 __global__ void __launch_bounds__(kRowWarps * 32, VPL <= 16 ? 8 : 6)
-    route_experts_rows_kernel(RouteExpertsParams p, int bs, int lpg, int vec) {
+    route_experts_rows_kernel(const __grid_constant__ RouteExpertsParams p, int bs, int lpg,
+                              int vec) {
   extern __shared__ double smem_d[];
   constexpr int RPW = 32 / LPR;
   // (order-preserving key, ~id) of the candidates; then key and id by place
@@ -619,15 +620,33 @@ __global__ void __launch_bounds__(kRowWarps * 32, VPL <= 16 ? 8 : 6)
       // fast exponentials and quotients: their errors are inside delta (a sigmoid's exponential is
       // off by (2 + 1.16 |x|) ulp, times s (1 - s): under one ulp of 1)
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        const int off = (i / 4) * cs + i % 4;
-        float x = p.scoring == 0 ? __expf(v[i] - m) * inv : __fdividef(1.f, 1.f + __expf(-v[i]));
-        if (kBias && off < lim) x += __ldg(p.bias + base + off);
-        x = v[i] > kNone ? x : kNone;
-        if (kBias) v[i] = x;
-        if (sums) {
-          a2 = fmaxf(a2, fminf(a, x == x ? x : kNone));
-          a = fmaxf(a, x);
+      for (int c = 0; c < VPL / 4; ++c) {
+        float b[4] = {0.f, 0.f, 0.f, 0.f};
+        if (kBias) {
+          if (vec) {
+            if (c * cs < lim) {
+              const float4 b4 = __ldg(reinterpret_cast<const float4*>(p.bias + base + c * cs));
+              b[0] = b4.x;
+              b[1] = b4.y;
+              b[2] = b4.z;
+              b[3] = b4.w;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (c * cs + i < lim) b[i] = __ldg(p.bias + base + c * cs + i);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float at = v[4 * c + i];
+          float x = p.scoring == 0 ? __expf(at - m) * inv : __fdividef(1.f, 1.f + __expf(-at));
+          x = at > kNone ? x + b[i] : kNone;
+          if (kBias) v[4 * c + i] = x;
+          if (sums) {
+            a2 = fmaxf(a2, fminf(a, x == x ? x : kNone));
+            a = fmaxf(a, x);
+          }
         }
       }
       // score(m) = inv is the largest softmax score
@@ -1014,7 +1033,8 @@ void launch_rows(const RouteExpertsParams& p, int bs, int lpg, int num_sms, cuda
   const int per = p.E / p.num_groups;
   const int vec = (p.num_groups > 1 ? bs % 4 == 0 && per % bs == 0 : p.E % 4 == 0) &&
                   p.stride % 4 == 0 &&
-                  (reinterpret_cast<uintptr_t>(p.logits) & (4 * sizeof(T) - 1)) == 0;
+                  (reinterpret_cast<uintptr_t>(p.logits) & (4 * sizeof(T) - 1)) == 0 &&
+                  (reinterpret_cast<uintptr_t>(p.bias) & 15u) == 0;
   if (p.bias)
     route_experts_rows_kernel<T, LPR, VPL, true><<<grid, kRowWarps * 32, smem, s>>>(p, bs, lpg, vec);
   else
