@@ -37,6 +37,20 @@ __device__ __forceinline__ bool mbar_wait_parked(uint32_t bar, uint32_t parity,
   }
 }
 
+// Whether the phase is complete, without waiting.  The answer takes some hundred cycles on a busy
+// SM, so it is asked for ahead of the work before the wait.
+__device__ __forceinline__ uint32_t mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok;
+}
+
 constexpr int kMaxRecord = 608;  // int4_record_bytes(32, true)
 
 template <typename T> struct Nib;
@@ -105,6 +119,8 @@ struct WeightRing {
     mbar_wait_parked(bars + 8 * slot, phase, abort_flag, err, kErrWaitFull);
     return ring + slot * MATS * matrix_bytes;
   }
+  __device__ __forceinline__ uint32_t test() { return mbar_test(bars + 8 * slot, phase); }
+  __device__ __forceinline__ const char* stage() const { return ring + slot * MATS * matrix_bytes; }
   // After a wait that ran out: no copy may land once the CTA is gone (each wait again bounded).
   __device__ __forceinline__ void drain() {
     if (!*abort_flag) return;

@@ -70,35 +70,41 @@ template <typename T> __device__ __forceinline__ uint32_t zero_pair(uint32_t z) 
   return Nib<T>::kMagic | ((z << Nib<T>::kShift) * 0x10001u);
 }
 
-// The record's weights in the order of tmem_st_16x128b_x8.
+// A group's scales and zero points (as 16 + z) of a lane's two columns.
+template <typename T> struct Group {
+  typename Pair<T>::type scale[2], off[2];
+};
 template <typename T, bool kZeros>
-__device__ __forceinline__ void unpack_record(const char* record, int per, int lane,
-                                              uint32_t (&out)[16]) {
+__device__ __forceinline__ void load_group(const char* record, int per, int h, int lane,
+                                           Group<T>& g) {
   using T2 = typename Pair<T>::type;
   const int gid = lane >> 2;
+  const T2 s = *(reinterpret_cast<const T2*>(record + 512 + 32 * h) + gid);
+  g.scale[0].x = g.scale[0].y = s.x;
+  g.scale[1].x = g.scale[1].y = s.y;
+  uint32_t z = 0x0808u;
+  if (kZeros) z = *reinterpret_cast<const uint16_t*>(record + 512 + 32 * per + 16 * h + 2 * gid);
+  const uint32_t z0 = zero_pair<T>(z & 15u), z1 = zero_pair<T>((z >> 8) & 15u);
+  g.off[0] = *reinterpret_cast<const T2*>(&z0);
+  g.off[1] = *reinterpret_cast<const T2*>(&z1);
+}
+
+// The record's weights in the order of tmem_st_16x128b_x8; `g` holds its first group.
+template <typename T, bool kZeros>
+__device__ __forceinline__ void unpack_record(const char* record, int per, int lane, Group<T>& g,
+                                              uint32_t (&out)[16]) {
+  using T2 = typename Pair<T>::type;
   const uint4 wq = *(reinterpret_cast<const uint4*>(record) + lane);
   const uint32_t word[4] = {wq.x, wq.y, wq.z, wq.w};
-  T2 sc[2], off[2];
-  auto group = [&](int h) {
-    const T2 s = *(reinterpret_cast<const T2*>(record + 512 + 32 * h) + gid);
-    sc[0].x = sc[0].y = s.x;
-    sc[1].x = sc[1].y = s.y;
-    uint32_t z = 0x0808u;
-    if (kZeros) z = *reinterpret_cast<const uint16_t*>(record + 512 + 32 * per + 16 * h + 2 * gid);
-    const uint32_t z0 = zero_pair<T>(z & 15u), z1 = zero_pair<T>((z >> 8) & 15u);
-    off[0] = *reinterpret_cast<const T2*>(&z0);
-    off[1] = *reinterpret_cast<const T2*>(&z1);
-  };
-  group(0);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    if (h == 1 && per == 2) group(1);
+    if (h == 1 && per == 2) load_group<T, kZeros>(record, per, 1, lane, g);
 #pragma unroll
     for (int c = 0; c < 4; ++c)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const uint32_t u = nib_pair<T>(word[2 * h + (c >> 1)], 2 * (c & 1) + r);
-        const T2 v = __hmul2(__hsub2(*reinterpret_cast<const T2*>(&u), off[r]), sc[r]);
+        const T2 v = __hmul2(__hsub2(*reinterpret_cast<const T2*>(&u), g.off[r]), g.scale[r]);
         out[2 * (4 * h + c) + r] = *reinterpret_cast<const uint32_t*>(&v);
       }
   }
@@ -183,26 +189,35 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
                                       smem_addr(&s_ring[warp][0]), &s_abort, p.err, lane,
                                       matrix_bytes};
     int at = 0;
-    uint32_t phase = 0;
+    uint32_t phase = 0, landed = 0;
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
       for (int r = 0; r < kb; r += kRingBlocks) {
-        const char* stage = w.wait();
+        if (!landed) w.wait();
+        const char* stage = w.stage();
 #pragma unroll
         for (int b = 0; b < kRingBlocks; b += kStageBlocks) {
           if (r + b >= kb) break;
-          uint32_t regs[kStageBlocks][16];
-#pragma unroll
-          for (int i = 0; i < kStageBlocks; ++i)
-            if (r + b + i < kb)
-              unpack_record<T, kZeros>(stage + (b + i) * p.rec, per, lane, regs[i]);
-          // after a wait that ran out this goes on with what is there, to the end of the units
-          mbar_wait_parked(smem_addr(&s_empty[at]), phase ^ 1u, &s_abort, p.err, kErrWaitEmpty);
-          __syncwarp();
-          tc_fence_after();
+          const uint32_t empty = smem_addr(&s_empty[at]);
+          const uint32_t free_now = mbar_test(empty, phase ^ 1u);
           const uint32_t to = tmem_a + at * kStageBlocks * kACols + panel * 32 + lanes;
+          Group<T> g;
 #pragma unroll
-          for (int i = 0; i < kStageBlocks; ++i)
-            if (r + b + i < kb) tmem_st_16x128b_x8(to + i * kACols, regs[i]);
+          for (int i = 0; i < kStageBlocks; ++i) {
+            if (r + b + i >= kb) break;
+            const char* record = stage + (b + i) * p.rec;
+            // the two blocks of a stage are one group of 128
+            if (i == 0 || p.G != 128) load_group<T, kZeros>(record, per, 0, lane, g);
+            uint32_t regs[16];
+            unpack_record<T, kZeros>(record, per, lane, g, regs);
+            if (i == 0) {
+              // after a wait that ran out this goes on with what is there, to the end of the units
+              if (!free_now)
+                mbar_wait_parked(empty, phase ^ 1u, &s_abort, p.err, kErrWaitEmpty);
+              __syncwarp();
+              tc_fence_after();
+            }
+            tmem_st_16x128b_x8(to + i * kACols, regs);
+          }
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
@@ -212,6 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_many_kernel(Int4Params p) {
         }
         const int slot = w.slot;
         w.release();
+        landed = w.test();
         if (lane == 0) mbar_arrive(smem_addr(&s_free[warp][slot]));
       }
     }
