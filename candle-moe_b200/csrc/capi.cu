@@ -1163,7 +1163,7 @@ CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const vo
     g1.k = g2.k = topk;
     g1.sorted_w = g2.sorted_w = routing_weights;
     g2.out = output;
-    const int n = launch_int4_table_ffn(static_cast<int>(dtype), g1, g2, ds->num_sms, s);
+    const int n = launch_int4_table_ffn(static_cast<int>(dtype), g1, g2, gemm_sms(ds), s);
     if (n == 0) st = MOE_ERR_CUDA;
     g_launches += n;
     if (owned) cudaFreeAsync(ws, s);
@@ -1183,7 +1183,7 @@ CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const vo
     st = MOE_ERR_CUDA;
   if (st == MOE_OK) {
     const int n = launch_int4_ffn(static_cast<int>(dtype), g1, g2, expert_indices,
-                                  num_tokens, topk, output, ds->num_sms, s);
+                                  num_tokens, topk, output, gemm_sms(ds), s);
     if (n == 0) st = MOE_ERR_CUDA;
     g_launches += n + (small || !route_prep_scratch_bytes(rows, E) ? 1 : 3);
   }

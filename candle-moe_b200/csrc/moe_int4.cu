@@ -6,14 +6,20 @@
 // and the layer is y_t = sum_j w_tj (act(x_t Gate_e) * (x_t Up_e)) Down_e  (or act(x_t Gate_e)
 // Down_e without Up), e = idx[t,j], ids >= E skipped.
 //
-// The products run on mma.sync m16n8k16 with the weights as the 16-row operand: a call of few
-// tokens streams weights, and that fragment can be made from packed nibbles in registers, so the
-// weights go from memory to the tensor cores without touching shared memory.  For a group,
-//     sum_k W x = s * (sum_k (16 + q) x - (16 + z) * sum_k x)
-// where 16 + q is exact in bf16 and f16 and one LOP3 away from the nibble (the nibble is the top
-// of the mantissa of a number in [16, 32)); sum_k x comes from one more product with a matrix of
-// ones.  The products are exact, so the scales and zero points act on f32 sums: no weight is
-// ever rounded.
+// Three paths, by the rows (token, slot) of the call:
+//   - at most 48: the kernels below, on mma.sync m16n8k16 with the weights as the 16-row operand.
+//     Such a call streams weights, and that fragment is made from packed nibbles in registers:
+//         sum_k W x = s * (sum_k (16 + q) x - (16 + z) * sum_k x)      (k over a group)
+//     where 16 + q is exact in bf16 and f16 and one LOP3 away from the nibble (the top of the
+//     mantissa of a number in [16, 32)), and sum_k x comes from one more product with a matrix
+//     of ones.  The products are exact and the scales and zero points act on f32 sums: no
+//     weight is rounded.
+//   - more: moe_int4_mma.cu, tcgen05 with the unpacked weights in tensor memory.
+//   - from 384 rows per expert on: int4_expand_kernel writes the weights in 16 bits once, and the
+//     grouped GEMMs of the 16-bit experts run on them.
+// Measured (mean of a run of calls, inputs larger than L2): 128 experts of 2048 x 768, top 8: one
+// token 15 us (19 MB of weights and scales; floor 3), 8 tokens 50, 512 tokens 146 (316 MB; floor
+// 48), 2048 tokens 335; 8 experts of 4096 x 1536, top 2, 8 tokens 32 us (71 MB; floor 11).
 //
 // Packed layout: records [E][N/16][K/64], one per 16 n x 64 k: 512 bytes of nibbles, then for each
 // group (two with G = 32, else one) 8 x 2 scales (n = gid, gid + 8) and, with zero points, 8 x 2

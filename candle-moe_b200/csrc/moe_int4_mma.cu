@@ -3,17 +3,21 @@
 // A tile is two panels of 128 weight columns (the same columns of gate and up, or 256 columns of one
 // matrix) times at most 64 rows of one expert.  The weights are the MMA's 128-row operand and
 // come from tensor memory: sixteen warps, a strip of 16 columns each, stream their records
-// through rings in shared memory, unpack them in registers -- (q - z) exactly,
-// times the scale, one rounding to the 16-bit type -- and store them as they lie: the packed
-// fragment order is the 16x128b shape of tcgen05.st, so nothing is shuffled and shared memory
-// carries only the packed nibbles.  The rows are the other operand, gathered by cp.async into
-// the 128-byte swizzle.  The sums stay in tensor memory for all of K (two sets, so that the epilogue of a tile
-// runs under the next one) and leave it one weight column per thread.
+// through rings in shared memory, unpack them in registers -- (q - z) exactly, times the scale,
+// one rounding to the 16-bit type, as weights held in that type have -- and store them as they
+// lie: the packed fragment order is the 16x128b shape of tcgen05.st, so nothing is shuffled and
+// shared memory carries only the packed nibbles.  The rows are the other operand, gathered by
+// cp.async into the 128-byte swizzle.  The sums stay in tensor memory for all of K (two sets, so
+// that the epilogue of a tile runs under the next one) and leave it one weight column per thread.
 //
-// What bounds it: unpacking, 75 to 85 warp instructions for a record of 1024 weights, 20 to 25
-// cycles of an SM's issue slots against 24 cycles of its share of the memory rate; the MMAs of
-// 64 rows take 16 cycles.  With eight unpacking warps the chain from a record to tensor memory
-// (600 cycles) set the pace, hence sixteen.
+// What bounds it: issue slots.  A record of 1024 weights takes 60 warp instructions to unpack (for
+// a pair of weights a lane under two to place the nibbles, one to subtract, one to scale) and
+// 127 with copies, barriers and stores; at the 0.7 instructions a cycle that a scheduler reaches an SM
+// unpacks one in 45 cycles, against 24 cycles of its share of the memory rate.  The MMAs take 40
+// cycles each at 64 rows or fewer, 20 a record.  512 tokens of 128 experts (2048 x 768, top 8): 82 us
+// for gate and up (214 MB), 44 us for down.  What it took to get there: sixteen unpacking warps
+// instead of eight, hand-overs of two blocks, an issuer warp whose addresses are uniform (one
+// lane alone spent 1500 cycles a block), a warp that feeds all rings, barriers tested ahead.
 #include <stdint.h>
 
 #include "common.cuh"

@@ -199,7 +199,8 @@ __device__ __forceinline__ void store_row(const RouteExpertsParams& p, int64_t r
 
 // Every row in 64 bits: shapes whose rows do not fit the registers of the kernel below.
 template <typename T>
-__global__ void __launch_bounds__(kWarps * 32) route_experts64_kernel(const __grid_constant__ RouteExpertsParams p) {
+__global__ void __launch_bounds__(kWarps * 32)
+    route_experts64_kernel(const __grid_constant__ RouteExpertsParams p) {
   extern __shared__ double smem_d[];
   const int warp = threadIdx.x >> 5;
   double* key = smem_d + warp * row64_scratch(p.E);
@@ -230,7 +231,7 @@ __device__ __forceinline__ float redux_max(float v) {
 //
 // Keys that are logits are exact.  With a bias the key s + b is off by at most `delta`; two
 // candidates nearer than 2 delta that are not the same numbers, or two groups nearer than their
-// sums' error, send the row to route_row64, which decides in 64 bits (one row in some hundreds).
+// sums' error, send the row to route_row64, which decides in 64 bits (one row in thousands).
 // delta: a sigmoid is off by under 4 half-steps of 1 plus the sum's own rounding; a softmax score
 // by (expf 2 ulp, l - m: |l - m| 2^-24, 21 additions, one division, averaged over the row under
 // 4e-6) of the largest score.
@@ -549,6 +550,10 @@ constexpr int kRowWarps = 4;
 // Expert i of a lane is base + (i / 4) * cs + i % 4: without groups the row's lanes take pieces of
 // four in turn (64 contiguous bytes of f32), with groups a lane holds one stretch of one group.
 // NaN needs no care where it is compared: it is never >= t nor > -inf.
+//
+// Measured: 65536 x 128 f32 in 16.7 us (2.3 TB/s; 0.67 of the issue slots busy, 175 instructions a
+// row), 16384 x 256 with sigmoid scores 8.6 us, with a bias 12.0 us, with 8 groups as well 20 us
+// (the 64-bit check of a close pair of groups, one row in 20000, is 4 us of it).
 template <typename T, int LPR, int VPL, bool kBias>
 __global__ void __launch_bounds__(kRowWarps * 32, VPL <= 16 ? 8 : 6)
     route_experts_rows_kernel(const __grid_constant__ RouteExpertsParams p, int bs, int lpg,
@@ -847,8 +852,8 @@ template <int N> __device__ __forceinline__ void bulk_wait_read() {
 // so at most the picks' logits are read.  LPR lanes per row, a lane per slot (k <= LPR): a warp
 // reads the slots of 32 / LPR rows at once, drops their gradients into a tile of zeros in shared
 // memory and sends the tile out in one bulk copy; two tiles in turn, and the places written
-// are cleared once the copy has read them.  Bound by the T*E gradients written (a warp per row,
-// with its own stores, took 162 instructions a row and 3 times as long).
+// are cleared once the copy has read them.  Bound by the T*E gradients written: 65536 x 128 f32 in
+// 9.6 us, 4.2 TB/s (a warp per row, with its own stores, took 162 instructions a row and 33 us).
 template <typename T, int LPR>
 __global__ void __launch_bounds__(kRowWarps * 32)
     route_experts_backward_kernel(RouteExpertsBackwardParams p, int bulk) {
