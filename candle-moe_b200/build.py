@@ -11,6 +11,7 @@ import glob
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -36,7 +37,7 @@ def _newest_header() -> float:
 def build(verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     hdr_t = _newest_header()
-    objs, changed = [], False
+    objs, todo = [], []
     for src in SOURCES:
         s = os.path.join(CSRC, src)
         o = os.path.join(BUILD, src.replace(".cu", ".o"))
@@ -45,9 +46,10 @@ def build(verbose: bool = False) -> str:
             cmd = [NVCC] + COMMON + EXTRA.get(src, []) + ["-c", s, "-o", o]
             if verbose:
                 print(" ".join(cmd), flush=True)
-            subprocess.run(cmd, check=True)
-            changed = True
-    if changed or not os.path.exists(LIB):
+            todo.append(cmd)
+    with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+        list(pool.map(lambda cmd: subprocess.run(cmd, check=True), todo))
+    if todo or not os.path.exists(LIB):
         cmd = [NVCC] + ARCH + ["-shared", "-o", LIB] + objs + \
             ["-Xlinker", "--exclude-libs,ALL", "-Xlinker", "-Bsymbolic"]
         if verbose:
