@@ -130,7 +130,7 @@ int moe_router_project_topk(const void* input, const void* gate_proj, int64_t nu
  *                 holds num_experts (which moe_fused_v2 and the other expert calls skip) and
  *                 weight 0.
  * Any num_experts <= 512, num_groups <= 32 (a divisor of num_experts), topk <= 32 and <= the open
- * groups' experts; scaling positive and finite.
+ * groups' experts; scaling positive and finite.  The outputs must not overlap the inputs.
  */
 #define MOE_SCORING_SOFTMAX 0
 #define MOE_SCORING_SIGMOID 1
@@ -147,7 +147,8 @@ int moe_route_experts(const void* logits, uint32_t dtype, int64_t logits_stride,
  * topk] f32; logits, topk_weights, topk_indices, scoring, renormalize and scaling as in (and from)
  * the forward call; grad_logits [num_tokens, num_experts] of `dtype`, contiguous, written whole.
  * The picks are constants and the bias has no gradient.  Slots with ids outside [0, num_experts)
- * contribute nothing, an id that a token holds twice contributes both.  Deterministic.
+ * contribute nothing, an id that a token holds twice contributes both.  grad_logits must not overlap
+ * the inputs.  Deterministic.
  */
 int moe_route_experts_backward(const float* grad_weights, const void* logits, uint32_t dtype,
                                int64_t logits_stride, const float* topk_weights,
@@ -281,11 +282,11 @@ int moe_fused_v2(const void* input, const void* gate_weights, const void* up_wei
  *   act(x.Gate).Down (the Nomic form; its second matrix packed as [E, I, H]).  has_zeros tells
  *   whether all matrices were packed with zeros.  workspace as moe_fused_v2, of
  *   moe_fused_int4_workspace_size() bytes.  input, output and the packed matrices 16-byte
- *   aligned (else MOE_ERR_UNSUPPORTED); output must not overlap input (MOE_ERR_INVALID_ARG).  The intermediate is rounded to `dtype`.  Calls of at
- *   most 48 rows (num_tokens * topk) apply scales and zero points to f32 sums; larger ones
- *   round each weight to `dtype` once, and from 384 rows per expert on each slot's
- *   contribution too (as moe_fused_v2 does), with the weights expanded to 16 bits in the
- *   workspace.
+ *   aligned (else MOE_ERR_UNSUPPORTED); output must not overlap input (MOE_ERR_INVALID_ARG).
+ *   The intermediate is rounded to `dtype`.  Calls of at most 48 rows (num_tokens * topk) apply
+ *   scales and zero points to f32 sums; larger ones round each weight to `dtype` once, and from
+ *   384 rows per expert on each slot's contribution too (as moe_fused_v2 does), with the weights
+ *   expanded to 16 bits in the workspace.
  */
 size_t moe_int4_packed_size(int32_t num_experts, int32_t k_dim, int32_t n_dim, int32_t group_size,
                             uint32_t dtype, int32_t has_zeros);

@@ -258,3 +258,20 @@ def test_output_over_the_input_is_refused():
         assert torch.equal(src, before)
     assert torch.equal(cm.fused_moe_int4(both[:4], ex, w[:4], idx[:4], out=both[4:8]),
                        cm.fused_moe_int4(both[:4], ex, w[:4], idx[:4]))
+
+
+@pytest.mark.parametrize("T,E,k", [(3, 2048, 8), (300, 2048, 2), (150, 1501, 3), (1100, 513, 4)])
+def test_many_experts(T, E, k):
+    """Up to the most experts there may be, an odd number, and more than 4096 rows over them."""
+    x, mats, w, idx = make(E + T, T, E, k, 64, 64, 32, "bf16", True, False, skip=0.1)
+    idx[T - 1, 0] = E - 1
+    run(x, mats, w, idx, 0, rounded=True)
+
+
+def test_one_token_many_times_one_expert():
+    """More slots than experts: every slot of the tokens picks the same one or two."""
+    for T, k in ((1, 48), (1, 49), (3, 40)):
+        x, mats, w, idx = make(T, T, 64, k, 128, 64, 32, "bf16", False, False)
+        idx.fill_(63)
+        idx[:, ::3] = 0
+        run(x, mats, w, idx, 0, rounded=True)

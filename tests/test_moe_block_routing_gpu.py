@@ -124,3 +124,27 @@ def test_block_refusals():
     with pytest.raises(cm.MoeError):
         cm.SparseMoeBlock(r, None, None, None, 2, num_groups=3, int4_experts=b.int4_experts).forward(
             torch.zeros(2, 128, dtype=torch.bfloat16, device="cuda"))
+
+
+@pytest.mark.parametrize("E,kw", [(8, {}), (12, {"scoring": cm.Scoring.Sigmoid})])
+def test_zero_tokens_in_the_block(E, kw):
+    b, _ = block(4, E, 128, 64, 2, 32, "bf16", **kw)
+    out, logits = b.forward(torch.zeros(0, 128, dtype=torch.bfloat16, device="cuda"),
+                            return_router_logits=True)
+    assert out.shape == (0, 128) and logits.shape == (0, E)
+
+
+def test_4_bit_block_with_a_shared_expert():
+    """The shared expert's contribution is added to the 4-bit experts'."""
+    torch.manual_seed(5)
+    b, mats = block(6, 8, 128, 64, 2, 32, "bf16")
+    sg, su = [(torch.randn(1, 128, 192, device="cuda") * 0.05).bfloat16() for _ in range(2)]
+    sd = (torch.randn(1, 192, 128, device="cuda") * 0.05).bfloat16()
+    both = cm.SparseMoeBlock(b.router_weight, None, None, None, 2, int4_experts=b.int4_experts,
+                             shared_gate=sg, shared_up=su, shared_down=sd)
+    alone = cm.SparseMoeBlock(b.router_weight[:1], sg, su, sd, 1)
+    x = torch.randn(21, 128, device="cuda").bfloat16()
+    a, c, got = b.forward(x), alone.forward(x), both.forward(x)
+    # two sums, each rounded by half a step, against one of the rounded parts
+    size = a.abs().double() + c.abs().double()
+    assert ((got.double() - a.double() - c.double()).abs() <= 3 * 2.0 ** -8 * size).all()

@@ -298,3 +298,34 @@ def test_few_distinct_logits():
             check_route(x, k, bias=bias, scoring=cm.Scoring.Sigmoid, renormalize=True, **kw)
             check_route(x, k, bias=bias, scoring=cm.Scoring.Softmax, **kw)
             check_route(x, k, scoring=cm.Scoring.Sigmoid, **kw)
+
+
+@pytest.mark.parametrize("E,k", [(64, 4), (256, 8), (60, 3), (512, 32)])
+def test_bias_off_its_alignment(E, k):
+    x = make_logits(E, 50, E, "bf16")
+    long = torch.randn(E + 3, device="cuda") * 0.1
+    for lo in (1, 2, 3):
+        b = long[lo:lo + E]
+        w, idx = cm.route_experts(x, k, cm.Scoring.Sigmoid, bias=b)
+        w2, idx2 = cm.route_experts(x, k, cm.Scoring.Sigmoid, bias=b.clone())
+        assert torch.equal(idx, idx2) and torch.equal(w, w2)
+
+
+@pytest.mark.parametrize("E,k", [(512, 32), (511, 31), (300, 17)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_gradient_straight_from_the_library(E, k, dtype):
+    """The most experts and slots, and a gradient that does not start on 16 bytes."""
+    x = make_logits(E, 77, E, dtype)
+    for scoring, renorm in ((0, False), (0, True), (1, True)):
+        w, idx = cm.route_experts(x, k, cm.Scoring(scoring), renormalize=bool(renorm))
+        g = torch.randn_like(w)
+        ref = cm.route_experts_backward(g, x, w, idx, cm.Scoring(scoring), bool(renorm))
+        out = torch.full((77 * E + 2,), 7.0, dtype=x.dtype, device="cuda")
+        at = out[1:]
+        code = {"f16": 0, "bf16": 1, "f32": 2}[dtype]
+        st = cm.lib().moe_route_experts_backward(
+            g.data_ptr(), x.data_ptr(), code, E, w.data_ptr(), idx.data_ptr(), 77, E, k, scoring,
+            int(renorm), 1.0, at.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        assert st == 0
+        assert torch.equal(at[:77 * E].view(77, E), ref)
+        assert out[0] == 7 and out[-1] == 7
