@@ -124,8 +124,6 @@ def _logits(c, g):
 def prepare(case, seed):
     g = torch.Generator(device="cuda").manual_seed(seed)
     c = dict(case)
-    if own:
-        c["library"] = _library()  # imported once, as a program does
     if c["op"] == "int4":
         return _prepare_int4(c, g)
     s = dict(c, logits=_logits(c, g), bias_values=None)
@@ -165,7 +163,7 @@ def _prepare_int4(c, g):
     s = dict(c, x=x, weights=(top / top.sum(1, keepdim=True)).contiguous(),
              indices=idx.to(torch.int32).contiguous())
     if own:
-        m = s["library"]
+        m = _library()
         s["experts"] = m.Int4Experts(*[None if w is None else m.Int4Weights(*w, group_size=G)
                                        for w in (raw["gate"], raw["up"], raw["down"])])
         s["moe"] = m.FusedMoE(E, k, m.Activation.Gelu if c["nomic"] else m.Activation.Silu)
@@ -284,7 +282,7 @@ def _plain_int4(s):
 def run(state):
     s = state
     if own:
-        m = s["library"]
+        m = _library()
         scoring = m.Scoring.Sigmoid if s.get("scoring") == "sigmoid" else m.Scoring.Softmax
         if s["op"] == "int4":
             return s["moe"].forward_int4(s["x"], s["experts"], s["weights"], s["indices"])
