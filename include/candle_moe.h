@@ -118,7 +118,8 @@ int moe_router_project_topk(const void* input, const void* gate_proj, int64_t nu
  *                 for sigmoid scores only (softmax weights become NaN).
  *   bias          [num_experts] f32 or NULL: picks are made by score + bias, weights by the score
  *                 alone (NULL: picks by the logits, which order the scores).  A bias of -inf or
- *                 NaN makes the expert unavailable.
+ *                 NaN makes the expert unavailable; available experts with a bias of +inf are
+ *                 picked first, in the order of their ids.
  *   scoring       MOE_SCORING_SOFTMAX or MOE_SCORING_SIGMOID
  *   num_groups    consecutive groups of num_experts / num_groups experts (1: no groups), of which
  *                 the topk_groups with the largest value stay open: the largest key of the group
