@@ -183,17 +183,50 @@ __device__ __noinline__ void route_row64(const RouteExpertsParams& p, int64_t ro
     mine = static_cast<float>(score64(logit_of(l, mine_id), m, total, p.scoring));
 }
 
+// Scores below this, in a row whose picks' sum is below 1/2, send its renormalised weights to 64
+// bits: a sigmoid's exponential passes the largest f32 at a logit of -88.7 and a softmax score its
+// last subnormal 103 below the row's maximum, but a share of the sum does not depend on how small
+// its terms are.  (Next to a larger sum what is lost is under 2^-126, below any normal weight.)
+constexpr float kTinyScore = 0x1p-100f, kSmallSum = 0.5f;
+
+// The row's renormalised weights again, in 64 bits, from the ids its slots hold; by one warp.
+// 1 / (1 + e^-l) and e^(l - m) as in route_row64: what is 0 in 64 bits counts as 0.
+template <typename T>
+__device__ __noinline__ void renormalise_row64(const RouteExpertsParams& p, int64_t row) {
+  const int lane = threadIdx.x & 31;
+  const T* l = static_cast<const T*>(p.logits) + row * p.stride;
+  float m = -CUDART_INF_F;
+  if (p.scoring == 0) {
+#pragma unroll 1
+    for (int e = lane; e < p.E; e += 32) m = fmaxf(m, logit_of(l, e));
+    m = warp_max(m);
+  }
+  const int id = lane < p.k ? p.indices[row * p.k + lane] : p.E;
+  const double r = id < p.E ? score64(logit_of(l, id), m, 1.0, p.scoring) : 0.0;
+  const double sum = warp_sum(r);
+  if (lane < p.k)
+    p.weights[row * p.k + lane] =
+        sum > 0.0 ? static_cast<float>(r / sum * static_cast<double>(p.scaling)) : 0.f;
+}
+
 // Writes the row's k slots from the pick that each lane holds (slot `lane`).
+template <typename T>
 __device__ __forceinline__ void store_row(const RouteExpertsParams& p, int64_t row, float r,
                                           int id) {
   const int lane = threadIdx.x & 31;
+  bool tiny = false;
   if (p.renormalize) {
     const float sum = warp_sum(r);
+    tiny = sum < kSmallSum && id < p.E && r < kTinyScore;
     r = sum > 0.f ? r / sum : r;
   }
   if (lane < p.k) {
     p.weights[row * p.k + lane] = r * p.scaling;
     p.indices[row * p.k + lane] = id;
+  }
+  if (__any_sync(0xffffffffu, tiny)) {
+    __syncwarp();
+    renormalise_row64<T>(p, row);
   }
 }
 
@@ -209,7 +242,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     float r;
     int id;
     route_row64<T>(p, row, key, r, id);
-    store_row(p, row, r, id);
+    store_row<T>(p, row, r, id);
     __syncwarp();
   }
 }
@@ -465,7 +498,7 @@ __global__ void __launch_bounds__(kFastWarps * 32)
     }
     if ((kBias || sums) && __any_sync(0xffffffffu, unsure))
       route_row64<T>(p, row, smem_d + warp * row64_scratch(p.E), r, id);
-    store_row(p, row, r, id);
+    store_row<T>(p, row, r, id);
     __syncwarp();
   }
 }
@@ -811,9 +844,15 @@ __global__ void __launch_bounds__(kRowWarps * 32, VPL <= 16 ? 8 : 6)
       }
     }
     float scale = p.scaling;
+    bool tiny = false;
     if (p.renormalize) {
       sum = row_sum(sum);
       scale = sum > 0.f ? p.scaling / sum : scale;
+      if (sum < kSmallSum) {
+        tiny = isinf(scale);
+#pragma unroll
+        for (int h = 0; h < kSlots; ++h) tiny |= id[h] < p.E && r[h] < kTinyScore;
+      }
     }
     if (live) {
 #pragma unroll
@@ -823,15 +862,24 @@ __global__ void __launch_bounds__(kRowWarps * 32, VPL <= 16 ? 8 : 6)
           p.indices[row * p.k + q + h * LPR] = id[h];
         }
     }
+    // rows of tiny scores, one after the other (those of the next loop are stored again there)
+    unsigned left = __ballot_sync(0xffffffffu, tiny && live);
+    if (left) __syncwarp();  // reads the ids stored above
+    while (left) {
+      const int s = (__ffs(left) - 1) / LPR;
+      left &= ~(((1u << LPR) - 1u) << (s * LPR));
+      renormalise_row64<T>(p, row0 + s);
+      __syncwarp();
+    }
     // rows that 32 bits do not decide, or with many equal keys, one after the other
-    unsigned left = __ballot_sync(0xffffffffu, unsure && live);
+    left = __ballot_sync(0xffffffffu, unsure && live);
     while (left) {
       const int s = (__ffs(left) - 1) / LPR;
       left &= ~(((1u << LPR) - 1u) << (s * LPR));
       float r1;
       int id1;
       route_row64<T>(p, row0 + s, smem_d + warp * row64_scratch(p.E), r1, id1);
-      store_row(p, row0 + s, r1, id1);
+      store_row<T>(p, row0 + s, r1, id1);
       __syncwarp();
     }
     __syncwarp();

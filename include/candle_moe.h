@@ -125,7 +125,8 @@ int moe_router_project_topk(const void* input, const void* gate_proj, int64_t nu
  *                 the topk_groups with the largest value stay open: the largest key of the group
  *                 (MOE_GROUP_MAX) or the sum of its two largest score + bias (MOE_GROUP_TOP2)
  *   topk_weights  [num_tokens, topk] f32 out: scaling * score, divided by the sum of the token's
- *                 picked scores with renormalize (0 where that sum is 0)
+ *                 picked scores with renormalize, however small they are (0 where that sum is
+ *                 0 in 64 bits, e.g. sigmoids of logits below -709.8)
  *   topk_indices  [num_tokens, topk] i32 out, by descending key; every tie goes to the lower id,
  *                 decided on scores in 64 bits.  A slot for which no available expert is left
  *                 holds num_experts (which moe_fused_v2 and the other expert calls skip) and
