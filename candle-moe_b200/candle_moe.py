@@ -726,6 +726,9 @@ class Int4Weights:
                 _need_cuda(t, n)
                 _need_contig(t, n)
         _need_same_device(q.device, (scales, "scales"), (zeros, "zeros"))
+        # read back once, when weights are loaded: a larger one would count as its low four bits
+        if zeros is not None and int(zeros.max()) > 15:
+            raise ValueError("zeros must be in 0..15")
         self.q, self.scales, self.zeros, self.group_size = q, scales, zeros, group_size
         self.shape = (E, K, N)
 
@@ -764,7 +767,9 @@ def quantize_int4(weights: torch.Tensor, group_size: int = 128,
                                      _ptr(scales), _ptr(zeros), _stream(dev))
     if st != MOE_OK:
         raise MoeError(st, "moe_int4_quantize")
-    return Int4Weights(q, scales, zeros, group_size)
+    out = Int4Weights(q, scales, None, group_size)
+    out.zeros = zeros  # in range by construction, so not read back
+    return out
 
 
 class Int4Experts:

@@ -154,7 +154,8 @@ __global__ void int4_pack_kernel(const uint8_t* __restrict__ q, int E, int K, in
   }
 }
 
-// One thread per scale (and zero point) of a record.
+// One thread per scale (and zero point) of a record.  A zero point is its low four bits, so that
+// the kernels, which read them in different ways, see the same number.
 __global__ void int4_pack_groups_kernel(const uint16_t* __restrict__ scales,
                                         const uint8_t* __restrict__ zeros, int E, int K, int N,
                                         int G, int rec, char* __restrict__ out) {
@@ -170,7 +171,7 @@ __global__ void int4_pack_groups_kernel(const uint16_t* __restrict__ scales,
     const int64_t from = (e * (K / G) + (64 * b + 32 * h) / G) * N + n;
     char* o = out + t * rec + 512;
     reinterpret_cast<uint16_t*>(o + 32 * h)[r] = scales[from];
-    if (zeros) reinterpret_cast<uint8_t*>(o + 32 * per + 16 * h)[r] = zeros[from];
+    if (zeros) reinterpret_cast<uint8_t*>(o + 32 * per + 16 * h)[r] = zeros[from] & 15u;
   }
 }
 

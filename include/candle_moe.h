@@ -270,7 +270,8 @@ int moe_fused_v2(const void* input, const void* gate_weights, const void* up_wei
  *     W[e,k,n] = (q[e,k,n] - zero[e,k/group_size,n]) * scale[e,k/group_size,n]
  *   q       [num_experts, k_dim/2, n_dim] u8: the low nibble is even k, the high nibble k + 1
  *   scales  [num_experts, k_dim/group_size, n_dim] of `dtype` (0 f16, 1 bf16: the activations')
- *   zeros   the same shape, u8 in 0..15, or NULL: 8 everywhere
+ *   zeros   the same shape, u8 in 0..15 (of a larger one the low four bits count), or NULL: 8
+ *           everywhere
  * group_size 32, 64 or 128, a divisor of k_dim; k_dim and n_dim multiples of 64 (else
  * MOE_ERR_UNSUPPORTED).
  *
