@@ -1047,7 +1047,8 @@ def set_sm_reserve(sms: int) -> int:
 
 
 def last_gemm_path() -> int:
-    """Kernels of this thread's last fused call: 1 SIMT, 2 grouped GEMMs, 3 decode kernels."""
+    """Kernels of this thread's last fused call: 1 SIMT, 2 grouped GEMMs, 3 decode kernels, 4 the
+    4-bit kernels of few rows, 5 the 4-bit kernels on tcgen05."""
     return int(lib().moe_last_gemm_path())
 
 

@@ -1076,6 +1076,7 @@ CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const vo
                             int32_t group_size, int32_t has_zeros, void* workspace,
                             size_t workspace_bytes, void* stream) {
   const int H = hidden_dim, I = intermediate_dim, E = num_experts;
+  t_last_path = 0;
   if (num_tokens < 0 || topk <= 0) return MOE_ERR_INVALID_ARG;
   int st = int4_shape_status(E, H, I, group_size, dtype);
   if (st == MOE_OK) st = int4_shape_status(E, I, H, group_size, dtype);
@@ -1157,14 +1158,21 @@ CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const vo
   g2.G = group_size;
   g2.E = E;
   g2.act = activation_type;
+  cudaEvent_t* ev = timer_slots();
+  if (ev) cudaEventRecord(ev[0], s);
   if (rows <= int4_table_rows()) {
+    if (ev) cudaEventRecord(ev[1], s);
     g1.idx = g2.idx = expert_indices;
     g1.rows = g2.rows = static_cast<int>(rows);
     g1.k = g2.k = topk;
     g1.sorted_w = g2.sorted_w = routing_weights;
     g2.out = output;
-    const int n = launch_int4_table_ffn(static_cast<int>(dtype), g1, g2, gemm_sms(ds), s);
+    const int n = launch_int4_table_ffn(static_cast<int>(dtype), g1, g2, gemm_sms(ds),
+                                        ev ? ev[2] : nullptr, s);
     if (n == 0) st = MOE_ERR_CUDA;
+    if (ev) cudaEventRecord(ev[3], s);
+    if (ev) cudaEventRecord(ev[4], s);
+    t_last_path = 4;
     g_launches += n;
     if (owned) cudaFreeAsync(ws, s);
     return finish(st);
@@ -1181,12 +1189,16 @@ CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const vo
                                 int4_many_rows(), offsets, prefix, s_token, s_w, s_flat,
                                 ws + L.prep_scratch, s) != 0)
     st = MOE_ERR_CUDA;
+  if (ev) cudaEventRecord(ev[1], s);
   if (st == MOE_OK) {
     const int n = launch_int4_ffn(static_cast<int>(dtype), g1, g2, expert_indices,
-                                  num_tokens, topk, output, gemm_sms(ds), s);
+                                  num_tokens, topk, output, gemm_sms(ds), ev ? ev[2] : nullptr,
+                                  ev ? ev[3] : nullptr, s);
     if (n == 0) st = MOE_ERR_CUDA;
+    t_last_path = 5;
     g_launches += n + (small || !route_prep_scratch_bytes(rows, E) ? 1 : 3);
   }
+  if (ev) cudaEventRecord(ev[4], s);
   if (owned) cudaFreeAsync(ws, s);
   return finish(st);
 }

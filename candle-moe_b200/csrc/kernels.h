@@ -189,7 +189,7 @@ struct Int4Params {
 int int4_many_rows();
 bool int4_many_set_attributes();
 bool launch_int4_many(int dtype, const Int4Params& g1, const Int4Params& g2, int num_sms,
-                      cudaStream_t s);
+                      cudaEvent_t between, cudaStream_t s);
 int int4_table_rows();
 // The route preparation's tables (all but the scratch) for at most int4_sort_rows() rows.  False: the
 // launch failed.
@@ -198,8 +198,9 @@ bool launch_int4_sort(const uint32_t* idx, const float* weights, int64_t rows, i
                       int chunk, int32_t* offsets, int32_t* chunk_prefix, int32_t* sorted_token,
                       float* sorted_w, int32_t* sorted_flat, cudaStream_t s);
 // Both products of such a call; returns the number of kernels launched (0: a launch failed).
+// `between` (here and above; may be null) is recorded between the products.
 int launch_int4_table_ffn(int dtype, const Int4Params& g1, const Int4Params& g2, int num_sms,
-                          cudaStream_t s);
+                          cudaEvent_t between, cudaStream_t s);
 // Bytes of a packed record (16 columns x 64 k).
 int int4_record_bytes(int G, bool zeros);
 bool int4_set_attributes();
@@ -211,8 +212,10 @@ int launch_int4_pack(int dtype, const uint8_t* q, const void* scales, const uint
 // out [E,K,N], or [E,N,K] with trans, in 16 bits; N a multiple of 128.
 void launch_int4_expand(int dtype, const void* w, int E, int K, int N, int G, bool zeros,
                         bool trans, void* out, cudaStream_t s);
+// The products of launch_int4_many and the combine, with an event after each product (may be null).
 int launch_int4_ffn(int dtype, const Int4Params& g1, const Int4Params& g2, const uint32_t* idx,
-                    int64_t num_tokens, int k, void* out, int num_sms, cudaStream_t s);
+                    int64_t num_tokens, int k, void* out, int num_sms, cudaEvent_t after1,
+                    cudaEvent_t after2, cudaStream_t s);
 
 // ---- ep_kernels.cu -------------------------------------------------------------------------
 constexpr int kMaxEpBins = 12288;  // (chunk, rank) counters of ep_dest_groups (48 KB smem)

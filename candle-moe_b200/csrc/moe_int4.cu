@@ -799,22 +799,27 @@ template <typename T> bool few_attributes() {
 }
 
 template <typename T, int kG, bool kZeros>
-bool launch_table(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
-  return (g1.w[1] ? Few<T, 2, kG, kZeros>::launch(g1, num_sms, s)
-                  : Few<T, 1, kG, kZeros>::launch(g1, num_sms, s)) &&
+bool launch_table(const Int4Params& g1, const Int4Params& g2, int num_sms,
+                  cudaEvent_t between, cudaStream_t s) {
+  const bool ok = g1.w[1] ? Few<T, 2, kG, kZeros>::launch(g1, num_sms, s)
+                          : Few<T, 1, kG, kZeros>::launch(g1, num_sms, s);
+  if (between) cudaEventRecord(between, s);
+  return ok &&
          (g2.N / 16 <= num_sms ? FewDown<T, kG, kZeros, 16>::launch(g2, num_sms, s)
                                : FewDown<T, kG, kZeros, 8>::launch(g2, num_sms, s));
 }
 template <typename T, int kG>
-bool launch_table(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
-  return g1.zeros ? launch_table<T, kG, true>(g1, g2, num_sms, s)
-                  : launch_table<T, kG, false>(g1, g2, num_sms, s);
+bool launch_table(const Int4Params& g1, const Int4Params& g2, int num_sms,
+                  cudaEvent_t between, cudaStream_t s) {
+  return g1.zeros ? launch_table<T, kG, true>(g1, g2, num_sms, between, s)
+                  : launch_table<T, kG, false>(g1, g2, num_sms, between, s);
 }
 template <typename T>
-bool launch_table(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
-  return g1.G == 32   ? launch_table<T, 32>(g1, g2, num_sms, s)
-         : g1.G == 64 ? launch_table<T, 64>(g1, g2, num_sms, s)
-                      : launch_table<T, 128>(g1, g2, num_sms, s);
+bool launch_table(const Int4Params& g1, const Int4Params& g2, int num_sms,
+                  cudaEvent_t between, cudaStream_t s) {
+  return g1.G == 32   ? launch_table<T, 32>(g1, g2, num_sms, between, s)
+         : g1.G == 64 ? launch_table<T, 64>(g1, g2, num_sms, between, s)
+                      : launch_table<T, 128>(g1, g2, num_sms, between, s);
 }
 
 template <typename T>
@@ -899,18 +904,20 @@ bool launch_int4_sort(const uint32_t* idx, const float* weights, int64_t rows, i
 int64_t int4_sort_rows() { return kSortThreads * kSortPer; }
 
 int launch_int4_table_ffn(int dtype, const Int4Params& g1, const Int4Params& g2, int num_sms,
-                          cudaStream_t s) {
-  const bool ok = dtype == kBF16 ? launch_table<__nv_bfloat16>(g1, g2, num_sms, s)
-                                 : launch_table<__half>(g1, g2, num_sms, s);
+                          cudaEvent_t between, cudaStream_t s) {
+  const bool ok = dtype == kBF16 ? launch_table<__nv_bfloat16>(g1, g2, num_sms, between, s)
+                                 : launch_table<__half>(g1, g2, num_sms, between, s);
   return ok ? 2 : 0;
 }
 
 int launch_int4_ffn(int dtype, const Int4Params& g1, const Int4Params& g2, const uint32_t* idx,
-                    int64_t num_tokens, int k, void* out, int num_sms, cudaStream_t s) {
-  const bool ok = launch_int4_many(dtype, g1, g2, num_sms, s) &&
-                  (dtype == kBF16
-                       ? launch_combine<__nv_bfloat16>(g2, idx, num_tokens, k, out, num_sms, s)
-                       : launch_combine<__half>(g2, idx, num_tokens, k, out, num_sms, s));
+                    int64_t num_tokens, int k, void* out, int num_sms, cudaEvent_t after1,
+                    cudaEvent_t after2, cudaStream_t s) {
+  bool ok = launch_int4_many(dtype, g1, g2, num_sms, after1, s);
+  if (after2) cudaEventRecord(after2, s);
+  ok = ok && (dtype == kBF16
+                  ? launch_combine<__nv_bfloat16>(g2, idx, num_tokens, k, out, num_sms, s)
+                  : launch_combine<__half>(g2, idx, num_tokens, k, out, num_sms, s));
   return ok ? 3 : 0;
 }
 

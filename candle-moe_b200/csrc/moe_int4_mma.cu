@@ -460,13 +460,15 @@ bool attribute() {
 }
 
 template <typename T, bool kZeros>
-bool launch(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaStream_t s) {
+bool launch(const Int4Params& g1, const Int4Params& g2, int num_sms, cudaEvent_t between,
+            cudaStream_t s) {
   const size_t smem = smem_bytes(g1.rec, g1.E);
   const bool ok =
       g1.w[1] ? launch_dependent(int4_many_kernel<T, true, false, kZeros>, num_sms, kThreads, smem, s,
                                  g1)
               : launch_dependent(int4_many_kernel<T, false, false, kZeros>, num_sms, kThreads, smem,
                                  s, g1);
+  if (between) cudaEventRecord(between, s);
   return ok && launch_dependent(int4_many_kernel<T, false, true, kZeros>, num_sms, kThreads, smem, s,
                                 g2);
 }
@@ -486,12 +488,12 @@ bool int4_many_set_attributes() {
 }
 
 bool launch_int4_many(int dtype, const Int4Params& g1, const Int4Params& g2, int num_sms,
-                      cudaStream_t s) {
+                      cudaEvent_t between, cudaStream_t s) {
   if (dtype == kBF16)
-    return g1.zeros ? launch<__nv_bfloat16, true>(g1, g2, num_sms, s)
-                    : launch<__nv_bfloat16, false>(g1, g2, num_sms, s);
-  return g1.zeros ? launch<__half, true>(g1, g2, num_sms, s)
-                  : launch<__half, false>(g1, g2, num_sms, s);
+    return g1.zeros ? launch<__nv_bfloat16, true>(g1, g2, num_sms, between, s)
+                    : launch<__nv_bfloat16, false>(g1, g2, num_sms, between, s);
+  return g1.zeros ? launch<__half, true>(g1, g2, num_sms, between, s)
+                  : launch<__half, false>(g1, g2, num_sms, between, s);
 }
 
 }  // namespace cmoe

@@ -349,8 +349,10 @@ int32_t moe_set_gemm_path(int32_t path);
  */
 int32_t moe_set_sm_reserve(int32_t sms);
 
-/* Which family served the last moe_fused_v2 / fused_moe call of this thread: 1 SIMT, 2 tensor-core
- * grouped GEMMs, 3 tensor-core decode kernels, 0 none. */
+/* Which family served the last moe_fused_v2 / fused_moe / moe_fused_int4 call of this thread: 1 SIMT,
+ * 2 tensor-core grouped GEMMs, 3 tensor-core decode kernels, 4 the 4-bit kernels of few rows, 5 the
+ * 4-bit kernels on tcgen05, 0 none (a moe_fused_int4 call that expanded its weights: the family
+ * that ran on them). */
 int32_t moe_last_gemm_path(void);
 
 /*
@@ -358,9 +360,10 @@ int32_t moe_last_gemm_path(void);
  * puts around each forward, src/bin/profile_fused_moe.rs:109-127).
  *
  * moe_kernel_launches: kernels this library has launched so far in this process.
- * moe_phase_timing(1): from now on every moe_fused_v2 / fused_moe call records CUDA events on
- *   its stream around route preparation, GEMM-1, GEMM-2 and the combine (resets the totals);
- *   moe_phase_timing(0) stops recording.
+ * moe_phase_timing(1): from now on every moe_fused_v2 / fused_moe / moe_fused_int4 call records
+ *   CUDA events on its stream around route preparation, GEMM-1, GEMM-2 and the combine (resets the
+ *   totals); moe_phase_timing(0) stops recording.  The 4-bit kernels of few rows have nothing to
+ *   show for the first and the last, and an expansion of 4-bit weights comes before the first.
  * moe_phase_times: waits for the recorded events and writes the summed milliseconds of the four
  *   phases to ms[0..3] and the number of recorded calls to *calls.
  */
