@@ -1100,9 +1100,16 @@ CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const vo
   const size_t need = moe_fused_int4_workspace_size(num_tokens, H, I, E, topk);
   char* ws = static_cast<char*>(workspace);
   const bool owned = ws == nullptr;
+  bool expand = int4_expands(num_tokens, H, I, E, topk);
   if (owned) {
     void* p = nullptr;
-    if (cudaMallocFromPoolAsync(&p, need, ds->pool, s) != cudaSuccess) {
+    bool got = cudaMallocFromPoolAsync(&p, need, ds->pool, s) == cudaSuccess;
+    if (!got && expand) {  // no room for the weights in 16 bits: the packed kernels take any size
+      cudaGetLastError();
+      expand = false;
+      got = cudaMallocFromPoolAsync(&p, L.total, ds->pool, s) == cudaSuccess;
+    }
+    if (!got) {
       cudaGetLastError();
       return MOE_ERR_NO_MEMORY;
     }
@@ -1118,7 +1125,7 @@ CMOE_API int moe_fused_int4(const void* input, const void* gate_packed, const vo
   g1.err = g2.err = ds->err_word;
   g1.zeros = g2.zeros = has_zeros != 0;
   g1.rec = g2.rec = int4_record_bytes(group_size, has_zeros != 0);
-  if (int4_expands(num_tokens, H, I, E, topk)) {
+  if (expand) {
     // two-matrix experts: the grouped GEMMs read the second matrix as [E, H, I]
     const size_t size = align256(2 * static_cast<size_t>(E) * H * I);
     const int dt = static_cast<int>(dtype);

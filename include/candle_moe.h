@@ -289,7 +289,8 @@ int moe_fused_v2(const void* input, const void* gate_weights, const void* up_wei
  *   The intermediate is rounded to `dtype`.  Calls of at most 48 rows (num_tokens * topk) apply
  *   scales and zero points to f32 sums; larger ones round each weight to `dtype` once, and from
  *   384 rows per expert on each slot's contribution too (as moe_fused_v2 does), with the weights
- *   expanded to 16 bits in the workspace.
+ *   expanded to 16 bits in the workspace (without a caller's workspace they stay packed where the
+ *   library's pool cannot hold them).
  */
 size_t moe_int4_packed_size(int32_t num_experts, int32_t k_dim, int32_t n_dim, int32_t group_size,
                             uint32_t dtype, int32_t has_zeros);

@@ -48,3 +48,38 @@ def test_path_and_phases_are_those_of_the_call(T, E, path):
     with pytest.raises(cm.MoeError):
         cm.fused_moe_int4(x, ex, w, idx, out=x)
     assert cm.last_gemm_path() == 0
+
+
+def test_weights_stay_packed_where_their_expansion_does_not_fit():
+    """Four experts of 90112 x 90112, all matrices one buffer of 17 GB, so that 16-bit copies of
+    the three do not fit the GPU.  A matrix is one number s_e (a power of two) and a token one
+    number c, so that g = s_e H c is a sum of H small integers, exact in f32, and the output is
+    s_e I h.  The bound: h and the output rounded to bf16 (2^-8 each), 2^-17 for the activation,
+    and 2^-23 for each of the 5632 additions of 16 products."""
+    E, H, T = 4, 90112, 1536
+    if 6 * E * H * H < torch.cuda.get_device_properties(0).total_memory:
+        pytest.skip("the expansion fits this GPU")
+    ex = object.__new__(cm.Int4Experts)
+    ex.num_experts, ex.hidden_dim, ex.intermediate_dim = E, H, H
+    ex.group_size, ex.dtype, ex.has_zeros, ex.device = 128, torch.bfloat16, False, torch.device(
+        "cuda", torch.cuda.current_device())
+    scale = 2.0 ** -torch.arange(6.0, 6.0 + E)
+    packed = torch.empty(E, H // 16 * (H // 64), 544, dtype=torch.uint8, device="cuda")
+    for e in range(E):
+        q = torch.full((1, 64, 64), 0x99, dtype=torch.uint8, device="cuda")  # 9 - 8 = 1
+        s = torch.full((1, 1, 64), float(scale[e]), dtype=torch.bfloat16, device="cuda")
+        packed[e] = cm.Int4Weights(q, s, None, 128)._pack()[:544]
+    ex.gate = ex.up = ex.down = packed
+    c = 2.0 ** -12 * (1 + torch.arange(T) % 3)
+    x = c[:, None].repeat(1, H).to(torch.bfloat16).cuda()
+    idx = (torch.arange(T) % E).int()[:, None].cuda()
+    w = torch.ones(T, 1, device="cuda")
+    got = cm.fused_moe_int4(x, ex, w, idx)
+    assert cm.last_gemm_path() == 5
+    g = scale[torch.arange(T) % E].double() * H * c.double()
+    y = scale[torch.arange(T) % E].double() * H * (g * g / (1 + torch.exp(-g)))
+    tol = 2 * 2.0 ** -8 + 2.0 ** -17 + 5632 * 2.0 ** -23
+    err = (got.double() - y.cuda()[:, None]).abs().amax(1).cpu()
+    assert (err <= tol * y).all()
+    del packed, ex, got, x
+    torch.cuda.empty_cache()
