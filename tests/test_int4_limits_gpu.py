@@ -5,7 +5,7 @@ import torch
 
 import candle_moe as cm
 from int4_testlib import random_weights
-from test_int4_gpu import make
+from test_int4_gpu import make, run
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,49 @@ def test_weights_stay_packed_where_their_expansion_does_not_fit():
     assert (err <= tol * y).all()
     del packed, ex, got, x
     torch.cuda.empty_cache()
+
+
+# ---- calls of few rows: at most 48 rows scale f32 sums, so no weight is rounded ---------------------
+
+FEW_ROWS = 48
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("T,E,k,H,I,G", [
+    # chunks of several rows of an expert
+    (9, 2, 1, 128, 64, 32), (16, 4, 2, 320, 64, 64), (33, 5, 1, 256, 256, 128),
+    (24, 2, 2, 256, 128, 64), (16, 3, 3, 192, 320, 32), (48, 4, 1, 192, 128, 64),
+    # K in pieces of which the last ones are empty
+    (1, 1, 1, 1536, 768, 128), (1, 4, 2, 1536, 768, 128), (2, 2, 1, 768, 1536, 128),
+    (3, 4, 2, 1536, 1536, 128), (1, 2, 1, 640, 896, 128), (2, 3, 2, 1600, 832, 64),
+    (1, 1, 1, 1600, 832, 32)])
+def test_few_rows_round_no_weight(T, E, k, H, I, G, dtype, zeros):
+    assert T * k <= FEW_ROWS
+    for nomic in (False, True):
+        x, mats, w, idx = make(T + E + I, T, E, k, H, I, G, dtype, zeros, nomic)
+        run(x, mats, w, idx, cm.Activation.Gelu if nomic else cm.Activation.Silu, rounded=False)
+
+
+@pytest.mark.parametrize("T,E,k", [(4, 6, 3), (16, 6, 3), (6, 8, 8), (48, 4, 1), (1, 64, 48),
+                                   (3, 64, 16)])
+def test_few_rows_of_skipped_and_repeated_experts(T, E, k):
+    x, mats, w, idx = make(T * k, T, E, k, 192, 128, 64, "f16", True, False, skip=0.3)
+    run(x, mats, w, idx, 0, rounded=False)
+    idx[:, 0] = 1
+    idx[:, ::3] = E - 1
+    idx[T - 1, k - 1] = -1
+    run(x, mats, w, idx, 0, rounded=False)
+    idx.fill_(E - 1)
+    run(x, mats, w, idx, 0, rounded=False)
+
+
+@pytest.mark.parametrize("T,E,k", [(49, 4, 1), (25, 30, 2), (7, 8, 7)])
+def test_the_first_calls_beyond_round_each_weight_once(T, E, k):
+    x, mats, w, idx = make(T * k, T, E, k, 192, 128, 64, "bf16", True, False)
+    assert T * k == FEW_ROWS + 1 or T * k == 50
+    run(x, mats, w, idx, 0, rounded=True)
+    assert cm.last_gemm_path() == 5
+    run(x[: FEW_ROWS // k].contiguous(), mats, w[: FEW_ROWS // k].contiguous(),
+        idx[: FEW_ROWS // k].contiguous(), 0, rounded=False)
+    assert cm.last_gemm_path() == 4

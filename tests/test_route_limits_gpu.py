@@ -79,3 +79,106 @@ def test_small_scores_between_ordinary_rows():
     w, idx = check_route(low, 8, scoring=cm.Scoring.Sigmoid, renormalize=True)
     keep = [t for t in range(333) if t % 7]
     assert torch.equal(w[keep], ordinary[keep])
+
+
+# ---- batches of which every warp takes several groups of rows ------------------------------------
+# One pass of the gradient covers at most num_sms x 16 blocks x 4 warps x 32 / LPR rows, LPR the
+# lanes of a row (8, 16 or 32 by k): 37888, 18944 and 9472 on 148 SMs; the dense one and the
+# 64-bit kernel 9472 and 4736, the forward one with 4 lanes a row 75776.
+
+def scores64(x, scoring):
+    """Scores in 64 bits; logits of -inf score 0."""
+    return torch.sigmoid(x) if scoring == 1 else torch.softmax(x, 1)
+
+
+def route64(x, k, scoring, renormalize, scaling, bias=None):
+    """Stable sorts of a 64-bit key: ties go to the lower id, as everywhere."""
+    s = scores64(x.double(), scoring)
+    key = x.double() if bias is None else s + bias.double()
+    idx = torch.sort(key, dim=1, descending=True, stable=True).indices[:, :k]
+    r = s.gather(1, idx)
+    if renormalize:
+        r = r / r.sum(1, keepdim=True)
+    return r * scaling, idx.int()
+
+
+def backward64(g, x, idx, scoring, renormalize, scaling):
+    s = scores64(x.double(), scoring)
+    at = idx.long()
+    r, d = s.gather(1, at), g.double() * scaling
+    if renormalize:
+        R = r.sum(1, keepdim=True)
+        d = (d - (d * r).sum(1, keepdim=True) / R) / R
+    ds = torch.zeros_like(s).scatter_add_(1, at, d)
+    return ds * s * (1 - s) if scoring == 1 else s * (ds - (ds * s).sum(1, keepdim=True))
+
+
+def spread(seed, T, E, dtype):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(T, E, generator=g, device="cuda") * 1.5
+    return (x + torch.randn(E, generator=g, device="cuda") * 0.5).to(DT[dtype])
+
+
+# E: rows of whole 16-byte pieces, tiles of whole pieces only, neither
+@pytest.mark.parametrize("T,E,k", [(80001, 64, 8), (80003, 36, 5), (80001, 33, 3), (40001, 64, 12),
+                                   (40003, 23, 10), (20011, 72, 20), (20011, 61, 17)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("scoring,renormalize", [(0, True), (1, True), (1, False), (0, False)])
+def test_gradients_of_several_passes(T, E, k, dtype, scoring, renormalize):
+    """Zeros of the second tile, places cleared between passes, picks loaded a pass ahead, a short
+    last tile behind full ones: all rows against the formula."""
+    x = spread(E, T, E, dtype)
+    w, idx = cm.route_experts(x, k, cm.Scoring(scoring), renormalize=renormalize, scaling=1.5)
+    g = torch.randn(w.shape, generator=torch.Generator(device="cuda").manual_seed(k), device="cuda")
+    d = cm.route_experts_backward(g, x, w, idx, cm.Scoring(scoring), renormalize, 1.5)
+    ref = backward64(g, x, idx, scoring, renormalize, 1.5)
+    tol = 2 * REL * 2 * 1.5 * g.abs().amax(1, keepdim=True).double()
+    if dtype != "f32":
+        tol = tol + torch.finfo(x.dtype).eps / 2 * ref.abs() + 2.0 ** -25
+    assert ((d.double() - ref).abs() <= tol).all()
+    if scoring == 1 or renormalize:  # zero but at the picks
+        rest = torch.ones_like(d, dtype=torch.bool).scatter_(1, idx.long(), False)
+        assert (d[rest] == 0).all()
+
+
+@pytest.mark.parametrize("T,E,k,n,kg", [(160001, 64, 8, 1, 1), (160003, 30, 4, 1, 1),
+                                        (80001, 128, 8, 1, 1), (80001, 16, 3, 1, 1),
+                                        (40003, 256, 8, 1, 1), (40001, 100, 12, 1, 1),
+                                        (20001, 480, 7, 12, 12)])
+@pytest.mark.parametrize("scoring,with_bias", [(0, False), (1, False), (1, True), (0, True)])
+def test_routing_of_several_passes(T, E, k, n, kg, scoring, with_bias):
+    """All rows against stable 64-bit sorts (every group stays open where there are groups)."""
+    x = spread(E + k, T, E, "f32" if E % 4 == 0 else "bf16")
+    bias = None
+    if with_bias:
+        gen = torch.Generator(device="cuda").manual_seed(5)
+        bias = torch.round(torch.randn(E, generator=gen, device="cuda") * 100) / 1000
+    w, idx = cm.route_experts(x, k, cm.Scoring(scoring), bias=bias, num_groups=n, topk_groups=kg,
+                              renormalize=True, scaling=2.5)
+    w_ref, i_ref = route64(x, k, scoring, True, 2.5, bias)
+    assert torch.equal(idx, i_ref)
+    assert ((w.double() - w_ref).abs() <= REL * w_ref).all()
+
+
+# ---- shapes that are ranked with 64-bit keys: more than 16 experts of a group to a lane -----------
+
+@pytest.mark.parametrize("E,n,kg,k", [(510, 5, 2, 4), (510, 5, 3, 20), (480, 12, 5, 8), (480, 12, 1, 9),
+                                      (510, 17, 4, 6), (511, 7, 2, 32), (510, 3, 1, 8),
+                                      (510, 30, 30, 11)])
+@pytest.mark.parametrize("scoring", [0, 1])
+@pytest.mark.parametrize("group_score", [0, 1])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_groups_ranked_in_64_bits(E, n, kg, k, group_score, with_bias, scoring):
+    bias = None
+    if with_bias:
+        bias = np.round(np.random.default_rng(E + n).normal(size=E) * 0.1, 3)
+        bias[7], bias[8] = -np.inf, np.nan
+    for dtype in ("f32", "bf16", "f16"):
+        x = make_logits(E * 7 + kg, 29, E, dtype)
+        x[:, 6::7] = float("-inf")          # out of service
+        x[3] = float("-inf")                # padding
+        x[4, 2:] = float("nan")
+        x[5] = 0.25                         # all equal
+        x[6, : E // n] = float("-inf")      # a whole group
+        check_route(x, k, bias=bias, scoring=cm.Scoring(scoring), num_groups=n, topk_groups=kg,
+                    group_score=cm.GroupScore(group_score), renormalize=(E % 2 == 0), scaling=2.5)
