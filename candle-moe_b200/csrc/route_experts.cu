@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(kFastWarps * 32)
     if (kBias) {
       delta += 1.2e-7f * fmaxf(fabsf(best), t > kNone ? fabsf(t) : 0.f);
       t -= 4.f * delta;
-      if (!(delta < CUDART_INF_F)) {  // a bias of +inf: no candidates here, all in 64 bits
+      if (best == CUDART_INF_F) {  // a bias of +inf: no candidates here, all in 64 bits
         unsure = true;
         t = CUDART_NAN_F;
       }
