@@ -342,7 +342,8 @@ def route_experts(logits: torch.Tensor, top_k: int, scoring: Scoring = Scoring.S
 
     logits [T,E] f32/f16/bf16, E <= 512; rows may be strided.  Returns (weights [T,k] f32, indices
     [T,k] int32); a slot without an available expert (logit -inf or NaN) holds index E and
-    weight 0, which the expert calls skip."""
+    weight 0, which the expert calls skip.  The weights carry no autograd graph, whether or not
+    the logits need a gradient: route_experts_backward is called explicitly."""
     # one test for the ordinary call; what fails it is looked at argument by argument
     if not (logits.is_cuda and logits.dim() == 2 and logits.is_contiguous()):
         _need_cuda(logits, "logits")

@@ -10,8 +10,8 @@
 namespace cmoe {
 namespace {
 
-// mbar_wait_bounded that parks the warp in each try (up to 10 us) instead of polling: with 25 warps
-// on an SM, most of them waiting, the polls take the issue slots of those that work.
+// mbar_wait_bounded that parks the warp in each try (up to 10 us) instead of polling, so that the
+// waiting ones of an SM's 26 warps take no issue slots.  (No faster than polling when measured.)
 __device__ __forceinline__ bool mbar_wait_parked(uint32_t bar, uint32_t parity,
                                                  volatile int* abort_flag, uint32_t* err,
                                                  uint32_t code) {

@@ -19,7 +19,7 @@
 //     grouped GEMMs of the 16-bit experts run on them.
 // Measured (mean of a run of calls, inputs larger than L2): 128 experts of 2048 x 768, top 8: one
 // token 15 us (19 MB of weights and scales; floor 3), 8 tokens 50, 512 tokens 146 (316 MB; floor
-// 48), 2048 tokens 335; 8 experts of 4096 x 1536, top 2, 8 tokens 32 us (71 MB; floor 11).
+// 48), 2048 tokens 339; 8 experts of 4096 x 1536, top 2, 8 tokens 32 us (71 MB; floor 11).
 //
 // Packed layout: records [E][N/16][K/64], one per 16 n x 64 k: 512 bytes of nibbles, then for each
 // group (two with G = 32, else one) 8 x 2 scales (n = gid, gid + 8) and, with zero points, 8 x 2
@@ -377,9 +377,13 @@ __device__ __forceinline__ void init_rings(uint64_t (&bar)[kCount][kSlots], int*
   __syncthreads();
 }
 
-// Calls of at most kTableRows rows need no route preparation: every CTA sorts the rows by expert
-// itself (stable, as the route preparation does).
+// Calls of at most kTableLimit rows need no route preparation: every CTA sorts the rows by expert
+// itself (stable, as the route preparation does), in tables for kTableRows.  Up to the limit the
+// kernels with a table win, by one measurement on each side of it: 48 rows of 128 experts (2048 x
+// 768) take 42 us against 49, 64 rows of 8 experts (4096 x 1536) 58 against 46.
+constexpr int kTableLimit = 48;
 constexpr int kTableRows = 64;
+static_assert(kTableLimit <= kTableRows, "rows of the table");
 struct RowTable {
   int row[kTableRows];               // flat row t*k + j of each sorted position
   int place[kTableRows];             // sorted position of each flat row, -1: id >= E
@@ -533,7 +537,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) int4_few_kernel(Int4Params p) 
   w.drain();
 }
 
-// The second product of a call of at most kTableRows rows, with the combine: a CTA takes a strip of
+// The second product of a call of at most kTableLimit rows, with the combine: a CTA takes a strip of
 // 16 output columns of every token.  A warp's task is (chunk, piece of K); the partial results
 // of all tasks meet in shared memory, where the strip's outputs are summed in slot order.
 template <typename T, int kG, bool kZeros, int kDownWarps>
@@ -886,9 +890,7 @@ int launch_int4_pack(int dtype, const uint8_t* q, const void* scales, const uint
   return 2;
 }
 
-// Up to here the kernels with a table win: 48 rows of 128 experts (2048 x 768) take 42 us against 49,
-// 64 rows of 8 experts (4096 x 1536) 58 against 46.
-int int4_table_rows() { return 48; }
+int int4_table_rows() { return kTableLimit; }
 
 static size_t sort_smem(int E) {
   return sizeof(int) * E + sizeof(uint16_t) * kSortWarps * static_cast<size_t>(E);

@@ -230,7 +230,8 @@ __device__ __forceinline__ void store_row(const RouteExpertsParams& p, int64_t r
   }
 }
 
-// Every row in 64 bits: shapes whose rows do not fit the registers of the kernel below.
+// Every row in 64 bits: groups so uneven to the lanes that one would hold more than the 16 experts
+// the kernel below keeps in registers.  16384 rows of 510 experts in 5 groups: 141 us.
 template <typename T>
 __global__ void __launch_bounds__(kWarps * 32)
     route_experts64_kernel(const __grid_constant__ RouteExpertsParams p) {
@@ -265,9 +266,25 @@ __device__ __forceinline__ float redux_max(float v) {
 // Keys that are logits are exact.  With a bias the key s + b is off by at most `delta`; two
 // candidates nearer than 2 delta that are not the same numbers, or two groups nearer than their
 // sums' error, send the row to route_row64, which decides in 64 bits (one row in thousands).
-// delta: a sigmoid is off by under 4 half-steps of 1 plus the sum's own rounding; a softmax score
-// by (expf 2 ulp, l - m: |l - m| 2^-24, 21 additions, one division, averaged over the row under
-// 4e-6) of the largest score.
+//
+// delta, here and in the kernel below, with h = 2^-24 and CUDA's stated bounds (expf 2 ulp, __expf
+// 2 + 1.173 |x| ulp, __fdividef 2 ulp, an ulp being at most 2 h):
+//   sigmoid 1 / (1 + e), e = exp(-x): the relative error of e, at most (4 + 2.35 |x|) h, counts
+//     s (1 - s) times, h for 1 + e and 4 h for the quotient s times.  s (1 - s) (4 + 2.35 |x|) + 5 s
+//     is below 5.6 for every x: under 3.4e-7 of the 4e-7 taken.
+//   softmax exp(-d) / S, d = m - x: a key's own part is d h for the difference, (4 + 2.35 d) h for
+//     the exponential and h for the product, exp(-d) (5 + 3.35 d) <= 5 times h / S.  What all keys
+//     of a row share is the error of 1 / S: the terms' (d + 4) h weighted by exp(-d) / S, where the
+//     mean of d is at most ln 512 = 6.3 (it is the entropy less ln S), up to 36 additions of a
+//     term (32 in a lane, 4 across) and the division, under 48 h.  Together 53 h / S = 3.2e-6 of
+//     the largest score 1 / S; 6e-6 is taken.
+//   the sum s + b: one rounding, h |s + b|; 1.2e-7 of the largest candidate is twice that.
+// The bound t lies 4 delta below the k-th block maximum: a true pick is above the k-th true key,
+// so its computed key is at most 2 delta below the k-th computed one.  A group's sum of two keys
+// is off by 2 delta and four roundings, so two groups by 4 delta + 8 h of the larger key.
+//
+// Measured, 16384 rows, eight sets of inputs in turn: 512 experts top 10 17.2 us, 256 top 16 18.4
+// us (0.9 TB/s), with sigmoid scores and a bias 39 us, 60 experts in 5 groups top 8 17 us.
 template <typename T, int VPT, bool kBias, bool kGroups>
 __global__ void __launch_bounds__(kFastWarps * 32)
     route_experts_kernel(const __grid_constant__ RouteExpertsParams p, int bs, int lpg, int vec) {
@@ -588,9 +605,11 @@ constexpr int kRowWarps = 4;
 // four in turn (64 contiguous bytes of f32), with groups a lane holds one stretch of one group.
 // NaN needs no care where it is compared: it is never >= t nor > -inf.
 //
-// Measured: 65536 x 128 f32 in 16.7 us (2.3 TB/s; 0.67 of the issue slots busy, 175 instructions a
-// row), 16384 x 256 with sigmoid scores 8.6 us, with a bias 12.0 us, with 8 groups as well 20 us
-// (the 64-bit check of a close pair of groups, one row in 20000, is 4 us of it).
+// Measured, eight sets of inputs in turn: 65536 x 128 f32 in 16.6 us (2.3 TB/s; 0.66 of the issue
+// slots busy, 176 instructions a row), 16384 x 256 with sigmoid scores 10.2 us, with a bias 13.5
+// us, with 8 groups as well 21.3 us (the 64-bit check of a close pair of groups, one row in 20000,
+// is 4 us of it).  Rows with more than 16 keys at the bound go to route_row64 too, one after the
+// other: 65536 x 128 with every other row constant takes 88 us.
 template <typename T, int LPR, int VPL, bool kBias>
 __global__ void __launch_bounds__(kRowWarps * 32, VPL <= 16 ? 8 : 6)
     route_experts_rows_kernel(const __grid_constant__ RouteExpertsParams p, int bs, int lpg,
@@ -904,8 +923,10 @@ template <int N> __device__ __forceinline__ void bulk_wait_read() {
 // so at most the picks' logits are read.  LPR lanes per row, a lane per slot (k <= LPR): a warp
 // reads the slots of 32 / LPR rows at once, drops their gradients into a tile of zeros in shared
 // memory and sends the tile out in one bulk copy; two tiles in turn, and the places written
-// are cleared once the copy has read them.  Bound by the T*E gradients written: 65536 x 128 f32 in
-// 9.6 us, 4.2 TB/s (a warp per row, with its own stores, took 162 instructions a row and 33 us).
+// are cleared once the copy has read them.  65536 x 128 f32 in 8.3 us, 4.8 TB/s of slots read and
+// gradients written; held by shared memory, the match over the warp and the shuffles (short
+// scoreboard and MIO stalls), not yet by the bytes (a warp per row, with its own stores, took 162
+// instructions a row and 33 us).
 template <typename T, int LPR>
 __global__ void __launch_bounds__(kRowWarps * 32)
     route_experts_backward_kernel(RouteExpertsBackwardParams p, int bulk) {
